@@ -30,6 +30,10 @@ extern "C" {
                                * held CUs. The launch still finishes; its outputs are not valid. Also raised when a call's
                                * wait for the launches before it on another stream ran out (about 20 s): it then
                                * goes ahead. */
+#define SSMOE_ERR_PAGE 32     /* a page id outside [0, n_pages) where a cache token is read, written or moved: read as not
+                               * there, not written */
+#define SSMOE_ERR_BATCH 64    /* cu_rows or kv_len contradict the call (rows outside [0, rows), more than max_rows of a
+                               * sequence, a length below 0 or beyond the table): cut to what the call's shapes allow */
 
 /* Text of the last error on this host thread ("" if none). */
 const char* ssmoe_last_error(void);
@@ -512,6 +516,80 @@ int ssmoe_hc_inject(const uint16_t* hyp, const uint16_t* y, const uint16_t* inj,
  * and raises SSMOE_ERR_TOKEN in the device status. */
 int ssmoe_gather_rows(const void* src, int64_t n_src, int64_t row_bytes, const int32_t* idx, int n, int idx_add,
                       void* dst, void* stream);
+
+/* ---------------------------------------------------------------- attention over a paged key-value cache */
+
+/* No reference counterpart by interface: the reference's attention (QSA over its own caches, kernels/vendored.py:105-118,
+ * and the head's, engine/mtp.py:209-227) is not on the path of this library; these are the operators that a model with
+ * plain causal attention needs at the same places.
+ *
+ * Cache of a layer: keys [n_pages][kv_heads][page][dim], values [n_pages][kv_heads][dim][page] (each dimension's tokens
+ * side by side: the form in which the product with the probabilities reads them), 16-bit elements of one type
+ * (SSMOE_BF16 or SSMOE_FP16). page is 16, 32, 64, 128 or 256 tokens, dim 64, 128 or 256.
+ * Batch: cu_rows int32 [seqs + 1], ascending, the rows of sequence s are cu_rows[s] .. cu_rows[s + 1] of the call's
+ * `rows` (rows past cu_rows[seqs] belong to none and are left as they were); kv_len int32 [seqs], the tokens of a sequence
+ * with the call's rows as the last ones, so row i of n has the position kv_len - n + i; table int32 [seqs][width],
+ * the page of tokens page * w .. page * w + page - 1 of a sequence in entry w. All three are read on the device: a captured
+ * call follows their contents. max_rows bounds the rows of one sequence (the launch covers so many). Entries of pages that
+ * no visible token needs are not looked at (-1 where none is held). */
+#define SSMOE_BF16 0
+#define SSMOE_FP16 1
+
+/* Turns query and key rows by their positions and writes the key and value rows into the cache at their sequence's
+ * places. q [rows][heads][dim], k and v [rows][kv_heads][dim] with the given strides (elements, multiples of 8), e.g. the
+ * parts of one fused projection; q_out [rows][heads][dim] contiguous (may be q where that is contiguous). For
+ * frequency i of rot / 2 the angle is positions[axis[i] * pos_stride + row] * inv_freq[i] (fp64, reduced to a
+ * fraction of a turn in fp64); axis NULL means axis 0 (text), 3 axes with an axis per frequency are the (time,
+ * height, width) positions of images and video. The pair turned is (i, i + rot / 2), or (2 i, 2 i + 1) with adjacent;
+ * elements from rot on are copied. cos and sin are multiplied by factor. One rounding to 16 bits at the end. Rows with
+ * a position below 0 are turned but not written. Two rows that share a place (a page in two sequences' tables) race. */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  void* q_out;
+  const int32_t* positions; /* [axes][rows], pos_stride apart */
+  int64_t pos_stride;
+  const double* inv_freq; /* [rot / 2] */
+  const int32_t* axis;    /* [rot / 2] or NULL */
+  void *k_pages, *v_pages;
+  const int32_t *cu_rows, *kv_len, *table;
+  int64_t n_pages;
+  int rows, seqs, max_rows, heads, kv_heads, dim, page, width, rot, axes, adjacent, type;
+  float factor;
+} ssmoe_rope_append_args;
+int ssmoe_rope_append(const ssmoe_rope_append_args* a, void* stream);
+
+/* out row i = sum_j softmax_j(scale * q_i . k_j) v_j over the tokens j <= p of its sequence (p its position), under
+ * window > 0 only those with p - j < window or j < sinks (the first tokens that stay visible); lse (fp32 [rows][heads], or
+ * NULL) = ln sum_j exp(scale * q_i . k_j). Head h reads key head h / (heads / kv_heads). A row that sees nothing is 0 with
+ * lse -inf. q [rows][heads][dim] with the given strides (elements, multiples of 8), out contiguous. Scores, maxima, sums and
+ * partial results are fp32; a probability is rounded to the element type before its product with the values. What the
+ * cache holds at tokens that a row does not see does not reach it, infinities and NaN included.
+ * Calls with max_rows <= 8 (decoding, verification): the bits of a row depend on its sequence's tokens, seqs, kv_heads and
+ * the width of the table, not on the other rows of the call.
+ * ws: at least ssmoe_paged_attention_workspace_bytes(a) bytes, 256-byte aligned (may be NULL when that is 0); nothing
+ * is kept in it between calls, and calls that may run at the same time need one each. */
+typedef struct {
+  const void* q;
+  int64_t q_row, q_head;
+  const void *k_pages, *v_pages;
+  const int32_t *cu_rows, *kv_len, *table;
+  void* out;
+  float* lse;
+  void* ws;
+  int64_t ws_bytes, n_pages;
+  int rows, seqs, max_rows, heads, kv_heads, dim, page, width, window, sinks, type;
+  float scale;
+} ssmoe_paged_attention_args;
+int64_t ssmoe_paged_attention_workspace_bytes(const ssmoe_paged_attention_args* a); /* -1: arguments refused */
+int ssmoe_paged_attention(const ssmoe_paged_attention_args* a, void* stream);
+
+/* Page dst[i] := page src[i] for i < n, keys and values of every layer ([layers][n_pages][page_bytes] each), and table
+ * entries (int32 [entries], or NULL) equal to src[i] become dst[i] (the lowest such i): the copies of a fork, the moves of a
+ * compaction. src and dst int32 [n] on the device; no page may be in dst twice, or in src and dst (the result of such a
+ * page is undefined, nothing else is touched). page_bytes a multiple of 2048. */
+int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page_bytes, const int32_t* src,
+                     const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream);
 
 /* ---------------------------------------------------------------- expert slot pool */
 

@@ -1,0 +1,414 @@
+// Attention of a batch's few new rows (a decoded token, the rows of a verify round) over a paged cache.
+//
+// For row i at position p, o_i = sum_j softmax_j(scale q_i k_j) v_j over the tokens j <= p, under a window those with
+// p - j < window or j < sinks. Every key and value is used by the few rows of a sequence and the heads that share its key
+// head, so the work is reading the cache once: 4 dim bytes per token and key head.
+//
+// The rows of a sequence times the heads of a key head are one "packed" axis: NT tiles of 16, the columns of
+// v_mfma_f32_16x16x32. A workgroup takes one chunk of the tokens of one (sequence, key head, NT tiles); its four waves
+// take the chunk's 32-token tiles in turn, each straight from memory into MFMA operands, no LDS:
+//   S^T = K Q^T: A row m of S tile t (0, 1) is token 8 (m / 4) + 4 t + m % 4, so lane (c, g) = (lane % 16, lane / 16) ends
+//     with the scores of column c at tokens 8 g + 0..7: its probabilities are, as they are, the B operand of
+//   O^T = V^T P^T, whose A operand is 8 consecutive tokens 8 g.. of dimension 16 d + c.
+// The running maximum is one value per column, equal in its four lanes; the sum of the weights stays per lane to the end.
+//
+// A chunk begins at a multiple of its size from the sequence's first token and its tiles go to waves by their place in
+// it, and masked tokens add exact zeros: the bits of a row do not depend on the other rows of the call. The
+// chunks' partial sums are joined by a second launch (attn_join_kernel); a grid of one chunk writes the result itself.
+//
+// Values at places that a row does not see must not reach it, whatever they hold: a probability of 0 times an infinity is
+// not 0. Only tiles that some row does not see whole can hold such places. There the operand is searched for non-finite
+// values; where any are, they are taken out of the product and added back, by three more products with ones in their
+// places and ones for the tokens seen, to the rows that see them.
+#include <hip/hip_runtime.h>
+
+#include "ss_attn.hpp"
+#include "ss_launch.hpp"
+
+namespace ss {
+
+namespace {
+
+constexpr float kNegInf = -__builtin_inff();
+
+SS_DEV float max_over_quads(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+  uint32_t lo, hi;
+  ss_pair<16>(ss_fu(v), lo, hi);
+  v = fmaxf(ss_uf(lo), ss_uf(hi));
+  ss_pair<32>(ss_fu(v), lo, hi);
+  return fmaxf(ss_uf(lo), ss_uf(hi));
+}
+
+// Whether either half of a word is an infinity or NaN.
+template <class T>
+SS_DEV bool nonfinite2(uint32_t w) {
+  return (w & T::kExp) == T::kExp || (w & (T::kExp << 16)) == (T::kExp << 16);
+}
+// One 16-bit value: the value to multiply with, or with `kind` 0, 1, 2 a one where it is +inf, -inf, NaN.
+template <class T>
+SS_DEV uint32_t part_of(uint32_t x, int kind) {
+  const bool nf = (x & T::kExp) == T::kExp, nan = nf && (x & (T::kExp ^ 0x7FFFu)) != 0;
+  if (kind < 0) return nf ? 0u : x;
+  const bool hit = kind == 2 ? nan : (nf && !nan && (x >> 15) == (uint32_t)kind);
+  return hit ? T::kOne : 0u;
+}
+template <class T>
+SS_DEV ss_u32x4 parts_of(const ss_u32x4& v, int kind) {
+  ss_u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = part_of<T>(v[i] & 0xFFFFu, kind) | (part_of<T>(v[i] >> 16, kind) << 16);
+  return r;
+}
+
+template <class T, int D, int NT>
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
+  constexpr int KS = D / 32, DT = D / 16;
+  constexpr bool kQLds = NT * KS > 8;  // more than 32 registers of queries stay in LDS, one copy for the four waves
+  __shared__ ss_u32x4 q_lds[kQLds ? NT * KS : 1][64];
+  __shared__ int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
+  __shared__ __attribute__((aligned(16))) float join_o[4][16][D + 4];
+  __shared__ float join_m[4][NT][16], join_l[4][NT][16];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  int b = blockIdx.x;
+  const int slot = b % a.slots;
+  b /= a.slots;
+  const int tile = b % a.tiles;
+  b /= a.tiles;
+  const int h = b % a.kv_heads, s = b / a.kv_heads;
+  const int page = 1 << a.page_shift;
+  const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width * page, a.err);
+  const int p0 = tile * NT * 16, np = sr.n * a.group;  // packed rows [p0, min(p0 + 16 NT, np))
+  if (p0 >= np) return;                                // whole workgroup, before any barrier
+  const int i0 = p0 / a.group, i1 = (min(p0 + NT * 16, np) - 1) / a.group;
+  const Seen sn = seen_tokens(sr.pos0 + i0, sr.pos0 + i1, sr.end, a.window, a.sinks);
+  // Slots cover the chunks that hold first tokens, then those from the window's on.
+  const int sc = (sn.s_end + a.chunk - 1) / a.chunk;
+  const int wc = max(sn.w_begin / a.chunk, sc);
+  const int ch = slot < sc ? slot : wc + slot - sc;
+  const int t_begin = ch * a.chunk, t_end = min(t_begin + a.chunk, sn.end);
+  const bool empty = t_begin >= t_end;
+  if (empty && a.slots > 1) return;  // the join reads no further than the last token's chunk
+
+  for (int j = tid; j < a.chunk / 8; j += 256) {
+    const int t = t_begin + 8 * j, at = t >> a.page_shift;
+    int id = -1;
+    if (t < t_end) {
+      id = gp(a.table)[(int64_t)s * a.width + at];
+      if ((uint32_t)id >= (uint64_t)a.n_pages) {
+        id = -1;
+        if (t < sn.s_end || t + 8 > sn.w_begin) ss_raise(a.err, SS_ERR_PAGE);
+      }
+    }
+    page_of[j] = id;
+  }
+  ss_u32x4 qf[kQLds ? 1 : NT][KS];
+  int qpos[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int p = p0 + 16 * n + c, i = p / a.group;
+    const bool in = p < np;
+    qpos[n] = in ? sr.pos0 + i : -1;
+    const uint16_t* qp = a.q + (int64_t)(sr.r0 + (in ? i : 0)) * a.q_row +
+                         (int64_t)(h * a.group + (in ? p - i * a.group : 0)) * a.q_head + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if constexpr (kQLds) {
+        if (((n * KS + ks) & 3) == w) q_lds[n * KS + ks][lane] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
+      } else {
+        qf[n][ks] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
+      }
+    }
+  }
+  ss_f32x4 acc[NT][DT];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n] = kNegInf;
+    l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[n][d] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int pos_lo = sr.pos0 + i0, pos_hi = sr.pos0 + i1;
+  __syncthreads();
+
+  const int nt = (t_end - t_begin + 31) / 32;
+#pragma unroll 1
+  for (int tt = w; tt < nt; tt += 4) {
+    const int t0 = t_begin + 32 * tt;
+    if (t0 >= sn.s_end && t0 + 32 <= sn.w_begin) continue;  // no row sees any of it
+    const int idk = page_of[4 * tt + (c >> 2)], idv = page_of[4 * tt + g];
+    const int tk = (t0 + 8 * (c >> 2)) & (page - 1), tv = (t0 + 8 * g) & (page - 1);
+    const uint16_t* kp = a.k + (((int64_t)max(idk, 0) * a.kv_heads + h) * page + tk + (c & 3)) * D + 8 * g;
+    const uint16_t* vp = a.v + ((int64_t)max(idv, 0) * a.kv_heads + h) * page * D + (int64_t)c * page + tv;
+    ss_u32x4 kf[2][KS], vf[DT];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *(const SS_G ss_u32x4*)(kp + 4 * t * D + 32 * ks);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vf[d] = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * d * page);
+    // Whether every row of the workgroup sees all 32 tokens.
+    const bool whole = t0 + 31 <= pos_lo && (t0 > pos_hi - a.window || t0 + 32 <= a.sinks) && __all(idv >= 0);
+    ss_u32x4 pf[NT];
+    uint32_t vis[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        ss_f32x4 sv = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sv = T::mfma16(kf[t][ks], kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * t + i] = sv[i];
+      }
+      vis[n] = 0xFFu;
+      if (!whole) {
+        vis[n] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int tok = t0 + 8 * g + e;
+          const bool see = idv >= 0 && tok <= qpos[n] && (tok > qpos[n] - a.window || tok < a.sinks);
+          vis[n] |= see ? 1u << e : 0u;
+          x[e] = see ? x[e] : kNegInf;
+        }
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+      mx = max_over_quads(mx) * a.scale - T::kShift;
+      const float mn = fmaxf(m[n], mx);
+      const float mu = mn == kNegInf ? 0.f : mn;
+      if (__any(mn > m[n])) {
+        const float f = __builtin_amdgcn_exp2f(m[n] - mu);
+        l[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[n][d][i] *= f;
+      }
+      m[n] = mn;
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -mu));
+        l[n] += p[e];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[n][i] = T::pack(p[2 * i], p[2 * i + 1]);
+    }
+    bool odd = false;
+    if (!whole) {
+      bool mine = false;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine |= nonfinite2<T>(vf[d][i]);
+      odd = __any(mine);
+    }
+    if (odd) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {
+          const ss_u32x4 at = parts_of<T>(vf[d], kind);
+          const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            ss_u32x4 ones;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              ones[i] = ((vis[n] >> (2 * i)) & 1u) * T::kOne | (((vis[n] >> (2 * i + 1)) & 1u) * T::kOne) << 16;
+            const ss_f32x4 hits = T::mfma16(at, ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][d][i] += hits[i] > 0.f ? add : 0.f;
+          }
+        }
+        vf[d] = parts_of<T>(vf[d], -1);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[n][d] = T::mfma16(vf[d], pf[n], acc[n][d]);
+  }
+
+  // The four waves' sums, weighted by how far each wave's maximum is below the largest.
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    l[n] = ss_rows_sum(l[n]);
+    if (g == 0) {
+      join_m[w][n][c] = m[n];
+      join_l[w][n][c] = l[n];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float top = kNegInf;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, join_m[k][n][c]);
+    const float f = m[n] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      ss_f32x4 o = acc[n][d];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = m[n] == kNegInf ? o[i] : o[i] * f;
+      *reinterpret_cast<ss_f32x4*>(&join_o[w][c][16 * d + 4 * g]) = o;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int j = tid; j < 16 * (D / 4); j += 256) {
+      const int col = j / (D / 4), d4 = 4 * (j % (D / 4));
+      const int p = p0 + 16 * n + col;
+      if (p < np) {
+        float big = kNegInf, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) big = fmaxf(big, join_m[k][n][col]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float mk = join_m[k][n][col];
+          sum += mk == kNegInf ? join_l[k][n][col] : join_l[k][n][col] * __builtin_amdgcn_exp2f(mk - big);
+        }
+        ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[0][col][d4]);
+#pragma unroll
+        for (int k = 1; k < 4; ++k) {
+          const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[k][col][d4]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] += x[i];
+        }
+        const int i = p / a.group;
+        const int64_t at = (int64_t)(sr.r0 + i) * a.heads + h * a.group + (p - i * a.group);
+        if (a.slots > 1) {
+          const int64_t pa = (int64_t)slot * a.rows * a.heads + at;
+          *reinterpret_cast<SS_G ss_f32x4*>(gp(a.po) + pa * D + d4) = o;
+          if (d4 == 0) {
+            gp(a.pml)[2 * pa] = big;
+            gp(a.pml)[2 * pa + 1] = sum;
+          }
+        } else {
+          const float r = sum == 0.f ? 0.f : 1.f / sum;
+          uint2 word;
+          word.x = T::pack(o[0] * r, o[1] * r);
+          word.y = T::pack(o[2] * r, o[3] * r);
+          *reinterpret_cast<uint2*>(a.out + at * D + d4) = word;
+          if (a.lse && d4 == 0) a.lse[at] = sum == 0.f ? kNegInf : (big + __log2f(sum)) * 0.693147180559945309f;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the chunks of a row: o = sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), m the largest m_k. One workgroup per row and
+// head; its groups of dim / 4 threads take the chunks by their number modulo the number of groups, each with a running
+// maximum, and the groups' sums are added in order.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  constexpr int TD = D / 4, GROUPS = 256 / TD;
+  __shared__ __attribute__((aligned(16))) float part[GROUPS][D];
+  __shared__ float part_l[GROUPS], part_m[GROUPS];
+  const int tid = threadIdx.x, d4 = 4 * (tid % TD), k = tid / TD;
+  int b = blockIdx.x;
+  const int head = b % a.heads;
+  b /= a.heads;
+  const int i = b % a.max_rows, s = b / a.max_rows;
+  const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width << a.page_shift, nullptr);
+  if (i >= sr.n) return;
+  // The slots of the workgroup that had this row, as it counted them.
+  const int tile = (i * a.group + head % a.group) / a.packed, p0 = tile * a.packed, np = sr.n * a.group;
+  const Seen sn = seen_tokens(sr.pos0 + p0 / a.group, sr.pos0 + (min(p0 + a.packed, np) - 1) / a.group, sr.end, a.window,
+                              a.sinks);
+  const int sc = (sn.s_end + a.chunk - 1) / a.chunk, wc = max(sn.w_begin / a.chunk, sc);
+  const int used = sc + max((sn.end + a.chunk - 1) / a.chunk - wc, 0);
+  const int64_t row = (int64_t)(sr.r0 + i) * a.heads + head, rows = (int64_t)a.rows * a.heads;
+  ss_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float m = kNegInf, l = 0.f;
+  auto add = [&](const ss_f32x4& x, float mk, float lk) {
+    const float mn = fmaxf(m, mk), mu = mn == kNegInf ? 0.f : mn;
+    const float f = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mu), fk = mk == kNegInf ? 1.f : __builtin_amdgcn_exp2f(mk - mu);
+    m = mn;
+    l = l * f + lk * fk;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * fk;
+  };
+  // Slot j holds chunk j (first tokens) or chunk wc + j - sc: group k takes the chunks k, k + GROUPS, ...
+  const int j1 = sc + (k + GROUPS - wc % GROUPS) % GROUPS;
+  auto take = [&](int from, int to) {
+#pragma unroll 4
+    for (int j = from; j < to; j += GROUPS) {
+      const int64_t at = j * rows + row;
+      const float mk = gp(a.pml)[2 * at], lk = gp(a.pml)[2 * at + 1];
+      const ss_f32x4 x = *reinterpret_cast<const SS_G ss_f32x4*>(gp(a.po) + at * D + d4);
+      add(x, mk, lk);
+    }
+  };
+  take(k, sc);
+  take(j1, used);
+  *reinterpret_cast<ss_f32x4*>(&part[k][d4]) = o;
+  if (d4 == 0) {
+    part_m[k] = m;
+    part_l[k] = l;
+  }
+  __syncthreads();
+  if (k > 0) return;
+  m = kNegInf;
+  l = 0.f;
+  o = ss_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) add(*reinterpret_cast<const ss_f32x4*>(&part[j][d4]), part_m[j], part_l[j]);
+  const float r = l == 0.f ? 0.f : 1.f / l;
+  uint2 word;
+  word.x = T::pack(o[0] * r, o[1] * r);
+  word.y = T::pack(o[2] * r, o[3] * r);
+  *reinterpret_cast<uint2*>(a.out + row * D + d4) = word;
+  if (a.lse && d4 == 0) a.lse[row] = l == 0.f ? kNegInf : (m + __log2f(l)) * 0.693147180559945309f;
+}
+
+template <class T, int D, int NT>
+hipError_t launch_few(const AttnArgs& a, hipStream_t st) {
+  const unsigned grid = (unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs);
+  hipLaunchKernelGGL((attn_few_kernel<T, D, NT>), dim3(grid), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_few_of(const AttnArgs& a, int dim, hipStream_t st) {
+  const int nt = a.packed / 16;
+  if (dim == 64) return nt == 1 ? launch_few<T, 64, 1>(a, st) : nt == 2 ? launch_few<T, 64, 2>(a, st) : launch_few<T, 64, 4>(a, st);
+  if (dim == 128)
+    return nt == 1 ? launch_few<T, 128, 1>(a, st) : launch_few<T, 128, 2>(a, st);
+  return launch_few<T, 256, 1>(a, st);
+}
+
+template <class T>
+hipError_t launch_join_of(const AttnArgs& a, int dim, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.seqs * a.max_rows * a.heads));
+  if (dim == 64)
+    hipLaunchKernelGGL((attn_join_kernel<T, 64>), grid, dim3(256), 0, st, a);
+  else if (dim == 128)
+    hipLaunchKernelGGL((attn_join_kernel<T, 128>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<T, 256>), grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Packed rows of a workgroup: as few tiles of 16 as hold them all, as far as two waves of a SIMD have the registers: up
+// to 4 tiles of 64 dimensions, 2 of 128, 1 of 256.
+int attn_few_packed(int dim, int packed) {
+  if (packed <= 16 || dim == 256) return 16;
+  return packed <= 32 || dim == 128 ? 32 : 64;
+}
+
+hipError_t launch_attn_few(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {
+  return fp16 ? launch_few_of<Fp16>(a, dim, st) : launch_few_of<Bf16>(a, dim, st);
+}
+
+hipError_t launch_attn_join(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {
+  return fp16 ? launch_join_of<Fp16>(a, dim, st) : launch_join_of<Bf16>(a, dim, st);
+}
+
+}  // namespace ss

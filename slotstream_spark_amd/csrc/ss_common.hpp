@@ -20,6 +20,8 @@ enum {
   SS_ERR_TOKEN = 4,        // a draft token outside [0, V)
   SS_ERR_NONFINITE = 8,    // non-finite logits reached a p/q decision
   SS_ERR_TIMEOUT = 16,     // a persistent launch's bounded wait for other workgroups ran out
+  SS_ERR_PAGE = 32,        // a page id outside the cache where a token is read or written
+  SS_ERR_BATCH = 64,       // a batch's row counts or lengths contradict the call's shapes
 };
 
 // ---------------------------------------------------------------- global-space access

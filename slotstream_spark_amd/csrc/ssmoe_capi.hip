@@ -2,6 +2,7 @@
 // launches. No entry point allocates device memory or synchronises, except ssmoe_device_error.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -9,8 +10,10 @@
 #include <string>
 
 #include "../../include/ssmoe.h"
+#include "ss_attn.hpp"
 #include "ss_common.hpp"
 #include "ss_launch.hpp"
+#include "ss_rope.hpp"
 
 // Per-device status word raised by kernels on bad input.
 __device__ int ss_status_storage;
@@ -191,6 +194,71 @@ class PersistentOrder {
 };
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+// ---------------------------------------------------------------- attention over a paged cache
+// Checks that the calls on a paged cache share; *shift becomes log2(page).
+int check_paged(int rows, int seqs, int max_rows, int heads, int kv_heads, int dim, int page, int width, int64_t n_pages,
+                int type, int* shift) {
+  if (rows < 0 || seqs < 0 || max_rows < 1) return fail(SSMOE_EINVAL, "need rows >= 0, seqs >= 0 and max_rows >= 1");
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65536)
+    return fail(SSMOE_EINVAL, "heads must be a positive multiple of kv_heads, got %d and %d", heads, kv_heads);
+  if (dim != 64 && dim != 128 && dim != 256) return fail(SSMOE_EINVAL, "dim must be 64, 128 or 256, got %d", dim);
+  *shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : page == 256 ? 8 : 0;
+  if (!*shift) return fail(SSMOE_EINVAL, "page must be 16, 32, 64, 128 or 256 tokens, got %d", page);
+  if (width < 1 || (int64_t)width * page > (1 << 30))
+    return fail(SSMOE_EINVAL, "a table row must cover 1 .. 2^30 tokens, got %d pages of %d", width, page);
+  if (n_pages < 1 || n_pages > INT32_MAX) return fail(SSMOE_EINVAL, "need 1 <= n_pages < 2^31");
+  if (type != SSMOE_BF16 && type != SSMOE_FP16) return fail(SSMOE_EINVAL, "type must be SSMOE_BF16 or SSMOE_FP16, got %d", type);
+  return ok();
+}
+
+// How a call of ssmoe_paged_attention is laid out (its checks included).
+//
+// Chunk: the tokens of one workgroup, so that a batch of full tables makes about 2048 workgroups, but none of fewer
+// than 128 tokens (a tile for each wave) or more than 4096. It goes by seqs, kv_heads and the table's width alone, so a
+// row's chunks, and with them its bits, do not depend on the other rows of a call.
+int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64_t* ws) {
+  if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
+  int shift = 0;
+  if (int rc = check_paged(p->rows, p->seqs, p->max_rows, p->heads, p->kv_heads, p->dim, p->page, p->width, p->n_pages,
+                           p->type, &shift))
+    return rc;
+  if (p->window < 0 || p->sinks < 0) return fail(SSMOE_EINVAL, "window and sinks must be >= 0");
+  if (!(p->scale > 0) || !std::isfinite(p->scale)) return fail(SSMOE_EINVAL, "scale must be positive and finite");
+  ss::AttnArgs a{};
+  const int max_rows = p->max_rows < p->rows ? p->max_rows : (p->rows > 0 ? p->rows : 1);
+  const int64_t cap = (int64_t)p->width * p->page;
+  a.rows = p->rows;
+  a.seqs = p->seqs;
+  a.max_rows = max_rows;
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.group = p->heads / p->kv_heads;
+  a.page_shift = shift;
+  a.width = p->width;
+  a.window = p->window > 0 && p->window < (1 << 30) ? p->window : (1 << 30);
+  a.sinks = a.window < (1 << 30) ? p->sinks : 0;
+  a.scale = p->scale * 1.44269504088896340736f;
+  if ((int64_t)max_rows * a.group > (1 << 30)) return fail(SSMOE_EINVAL, "max_rows * heads / kv_heads must be at most 2^30");
+  a.packed = ss::attn_few_packed(p->dim, max_rows * a.group);
+  a.tiles = (max_rows * a.group + a.packed - 1) / a.packed;
+  // tokens of a sequence that the call may read
+  int64_t seen = cap;
+  if (a.window < (1 << 30)) seen = std::min<int64_t>(cap, (int64_t)a.window + max_rows + a.sinks);
+  int64_t chunk = (seen * p->seqs * p->kv_heads + 2047) / 2048;
+  chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), 4096);
+  a.chunk = (int)chunk;
+  int64_t slots = (cap + chunk - 1) / chunk;
+  if (a.window < (1 << 30))
+    slots = std::min(slots, (std::min<int64_t>(a.sinks, cap) + chunk - 1) / chunk + (a.window + max_rows + chunk - 2) / chunk + 1);
+  a.slots = (int)slots;
+  if (slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
+    return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
+  const int64_t parts = slots > 1 ? slots * p->rows * p->heads : 0;
+  *ws = (parts * p->dim * 4 + 255) / 256 * 256 + parts * 8;
+  *out = a;
+  return ok();
+}
 
 int check_moe_shape(int R, int H, int I, int K, int E) {
   if (R < 1) return fail(SSMOE_EINVAL, "R must be >= 1, got %d", R);
@@ -1263,6 +1331,131 @@ int ssmoe_gather_rows(const void* src, int64_t n_src, int64_t row_bytes, const i
   return hip_check(ss::launch_gather_rows(src, n_src, row_bytes, idx, n, idx_add, dst, st,
                                           static_cast<hipStream_t>(stream)),
                    "gather launch");
+}
+
+int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
+  if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
+  ss::RopeArgs a{};
+  if (int rc = check_paged(p->rows, p->seqs, p->max_rows, p->heads, p->kv_heads, p->dim, p->page, p->width, p->n_pages,
+                           p->type, &a.page_shift))
+    return rc;
+  if (p->rot < 16 || p->rot % 16 || p->rot > p->dim)
+    return fail(SSMOE_EINVAL, "rot must be a multiple of 16 in [16, dim], got %d of %d", p->rot, p->dim);
+  if (p->axes < 1) return fail(SSMOE_EINVAL, "need axes >= 1");
+  if (!std::isfinite(p->factor)) return fail(SSMOE_EINVAL, "factor must be finite");
+  if (p->rows == 0 || p->seqs == 0) return ok();
+  if (!p->q || !p->k || !p->v || !p->q_out || !p->positions || !p->inv_freq || !p->k_pages || !p->v_pages || !p->cu_rows ||
+      !p->kv_len || !p->table)
+    return fail(SSMOE_EINVAL, "q, k, v, q_out, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len and table must be non-null");
+  for (int64_t st : {p->q_row, p->q_head, p->k_row, p->k_head, p->v_row, p->v_head})
+    if (st < 0 || st % 8) return fail(SSMOE_EINVAL, "strides must be multiples of 8 elements");
+  for (const void* t : {p->q, p->k, p->v, (const void*)p->q_out, (const void*)p->k_pages, (const void*)p->v_pages})
+    if (!aligned(t, 16)) return fail(SSMOE_EINVAL, "q, k, v, q_out and the pages must be 16-byte aligned");
+  if (!aligned(p->inv_freq, 8)) return fail(SSMOE_EINVAL, "inv_freq must be 8-byte aligned");
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.k = static_cast<const uint16_t*>(p->k);
+  a.v = static_cast<const uint16_t*>(p->v);
+  a.q_row = p->q_row;
+  a.q_head = p->q_head;
+  a.k_row = p->k_row;
+  a.k_head = p->k_head;
+  a.v_row = p->v_row;
+  a.v_head = p->v_head;
+  a.out = static_cast<uint16_t*>(p->q_out);
+  a.positions = p->positions;
+  a.pos_stride = p->pos_stride;
+  a.inv_freq = p->inv_freq;
+  a.axis = p->axis;
+  a.k_pages = static_cast<uint16_t*>(p->k_pages);
+  a.v_pages = static_cast<uint16_t*>(p->v_pages);
+  a.cu = p->cu_rows;
+  a.kv_len = p->kv_len;
+  a.table = p->table;
+  if (int rc = status_ptr(&a.err)) return rc;
+  a.n_pages = p->n_pages;
+  a.rows = p->rows;
+  a.seqs = p->seqs;
+  a.max_rows = p->max_rows < p->rows ? p->max_rows : p->rows;
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.dim = p->dim;
+  a.rot = p->rot;
+  a.axes = p->axes;
+  a.width = p->width;
+  a.adjacent = p->adjacent != 0;
+  a.factor = p->factor;
+  a.tiles = (int)(((int64_t)a.max_rows + 14) / 8);
+  a.head_groups = 1;
+  if ((int64_t)a.tiles * a.head_groups * p->seqs > INT32_MAX)
+    return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
+  return hip_check(ss::launch_rope_append(a, p->type == SSMOE_FP16, static_cast<hipStream_t>(stream)), "rope launch");
+}
+
+int64_t ssmoe_paged_attention_workspace_bytes(const ssmoe_paged_attention_args* p) {
+  ss::AttnArgs a{};
+  int64_t ws = 0;
+  return plan_attention(p, &a, &ws) ? -1 : ws;
+}
+
+int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
+  ss::AttnArgs a{};
+  int64_t ws = 0;
+  if (int rc = plan_attention(p, &a, &ws)) return rc;
+  if (p->rows == 0 || p->seqs == 0) return ok();
+  if (!p->q || !p->k_pages || !p->v_pages || !p->cu_rows || !p->kv_len || !p->table || !p->out)
+    return fail(SSMOE_EINVAL, "q, k_pages, v_pages, cu_rows, kv_len, table and out must be non-null");
+  if (p->q_row < 0 || p->q_head < 0 || p->q_row % 8 || p->q_head % 8)
+    return fail(SSMOE_EINVAL, "strides must be multiples of 8 elements");
+  if (!aligned(p->q, 16) || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16) || !aligned(p->out, 16))
+    return fail(SSMOE_EINVAL, "q, out and the pages must be 16-byte aligned");
+  if (ws > 0 && (!p->ws || p->ws_bytes < ws || !aligned(p->ws, 256)))
+    return fail(SSMOE_EINVAL, "workspace holds %lld bytes, the call needs %lld (256-byte aligned)",
+                (long long)(p->ws ? p->ws_bytes : 0), (long long)ws);
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.q_row = p->q_row;
+  a.q_head = p->q_head;
+  a.k = static_cast<const uint16_t*>(p->k_pages);
+  a.v = static_cast<const uint16_t*>(p->v_pages);
+  a.cu = p->cu_rows;
+  a.kv_len = p->kv_len;
+  a.table = p->table;
+  a.out = static_cast<uint16_t*>(p->out);
+  a.lse = p->lse;
+  a.n_pages = p->n_pages;
+  if (int rc = status_ptr(&a.err)) return rc;
+  if (ws > 0) {
+    const int64_t parts = (int64_t)a.slots * p->rows * p->heads;
+    a.po = static_cast<float*>(p->ws);
+    a.pml = reinterpret_cast<float*>(static_cast<char*>(p->ws) + (parts * p->dim * 4 + 255) / 256 * 256);
+  }
+  const bool fp16 = p->type == SSMOE_FP16;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (int rc = hip_check(ss::launch_attn_few(a, p->dim, fp16, st), "attention launch")) return rc;
+  return a.slots > 1 ? hip_check(ss::launch_attn_join(a, p->dim, fp16, st), "attention join launch") : ok();
+}
+
+int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page_bytes, const int32_t* src,
+                     const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream) {
+  if (layers < 1 || n_pages < 1 || n_pages > INT32_MAX || page_bytes < 2048 || page_bytes % 2048)
+    return fail(SSMOE_EINVAL, "need layers >= 1, 1 <= n_pages < 2^31 and page_bytes a positive multiple of 2048");
+  if (n < 0 || entries < 0 || entries > INT32_MAX) return fail(SSMOE_EINVAL, "need n >= 0 and 0 <= entries < 2^31");
+  if (n == 0) return ok();
+  if (!k || !v || !src || !dst) return fail(SSMOE_EINVAL, "k, v, src and dst must be non-null");
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(SSMOE_EINVAL, "k and v must be 16-byte aligned");
+  if (2 * (page_bytes / 2048) * n > ((int64_t)1 << 34) / layers) return fail(SSMOE_EINVAL, "too many bytes for one call");
+  ss::MoveArgs a{};
+  a.k = static_cast<uint8_t*>(k);
+  a.v = static_cast<uint8_t*>(v);
+  a.src = src;
+  a.dst = dst;
+  a.table = entries > 0 ? table : nullptr;
+  if (int rc = status_ptr(&a.err)) return rc;
+  a.n_pages = n_pages;
+  a.page_bytes = page_bytes;
+  a.entries = entries;
+  a.layers = layers;
+  a.n = n;
+  return hip_check(ss::launch_move_pages(a, static_cast<hipStream_t>(stream)), "page move launch");
 }
 
 int ssmoe_pool_open(const char* experts_path, int layers, int experts, int64_t record_bytes, int max_slots,

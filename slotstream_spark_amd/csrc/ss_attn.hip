@@ -39,27 +39,6 @@ SS_DEV float max_over_quads(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^
   return fmaxf(ss_uf(lo), ss_uf(hi));
 }
 
-// Whether either half of a word is an infinity or NaN.
-template <class T>
-SS_DEV bool nonfinite2(uint32_t w) {
-  return (w & T::kExp) == T::kExp || (w & (T::kExp << 16)) == (T::kExp << 16);
-}
-// One 16-bit value: the value to multiply with, or with `kind` 0, 1, 2 a one where it is +inf, -inf, NaN.
-template <class T>
-SS_DEV uint32_t part_of(uint32_t x, int kind) {
-  const bool nf = (x & T::kExp) == T::kExp, nan = nf && (x & (T::kExp ^ 0x7FFFu)) != 0;
-  if (kind < 0) return nf ? 0u : x;
-  const bool hit = kind == 2 ? nan : (nf && !nan && (x >> 15) == (uint32_t)kind);
-  return hit ? T::kOne : 0u;
-}
-template <class T>
-SS_DEV ss_u32x4 parts_of(const ss_u32x4& v, int kind) {
-  ss_u32x4 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = part_of<T>(v[i] & 0xFFFFu, kind) | (part_of<T>(v[i] >> 16, kind) << 16);
-  return r;
-}
-
 template <class T, int D, int NT>
 __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16;

@@ -59,6 +59,27 @@ struct Fp16 {
   SS_DEV static float widen(uint32_t u) { return (float)__builtin_bit_cast(_Float16, (uint16_t)u); }
 };
 
+// Whether either half of a word is an infinity or NaN.
+template <class T>
+SS_DEV bool nonfinite2(uint32_t w) {
+  return (w & T::kExp) == T::kExp || (w & (T::kExp << 16)) == (T::kExp << 16);
+}
+// One 16-bit value: the value to multiply with, or with `kind` 0, 1, 2 a one where it is +inf, -inf, NaN.
+template <class T>
+SS_DEV uint32_t part_of(uint32_t x, int kind) {
+  const bool nf = (x & T::kExp) == T::kExp, nan = nf && (x & (T::kExp ^ 0x7FFFu)) != 0;
+  if (kind < 0) return nf ? 0u : x;
+  const bool hit = kind == 2 ? nan : (nf && !nan && (x >> 15) == (uint32_t)kind);
+  return hit ? T::kOne : 0u;
+}
+template <class T>
+SS_DEV ss_u32x4 parts_of(const ss_u32x4& v, int kind) {
+  ss_u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = part_of<T>(v[i] & 0xFFFFu, kind) | (part_of<T>(v[i] >> 16, kind) << 16);
+  return r;
+}
+
 // Rows [r0, r0 + n) of sequence s, the position of its first row (negative where the cache is said to hold fewer tokens
 // than the call has rows) and the end of its tokens. What contradicts the arguments is cut to them and raised.
 struct SeqRows {
@@ -96,6 +117,7 @@ SS_DEV Seen seen_tokens(int pos_a, int pos_b, int end, int window, int sinks) {
   return r;
 }
 
+hipError_t launch_attn_prompt(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 hipError_t launch_attn_few(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 int attn_few_packed(int dim, int packed);
 hipError_t launch_attn_join(const AttnArgs& a, int dim, bool fp16, hipStream_t st);

@@ -1,0 +1,404 @@
+// Attention of prompt chunks over a paged cache: many rows of a sequence, so that the work is the two matrix products,
+// 4 dim FLOP per (row, token) and head.
+//
+// The rows of a sequence times the heads of a key head are one packed axis, as in ss_attn.hip: a chunk's tiles hold
+// rows of nearly one position, and a key head's tokens are read once for all its heads. A workgroup has 128 packed rows,
+// 32 a wave as the columns of v_mfma_f32_32x32x16, and goes over the tokens in tiles of TK:
+//   S^T = K Q^T, queries in registers; A row m = 8 b + 4 h + r of a 32-token tile is token 16 (b / 2) + 8 h + 4 (b % 2) + r, so
+//     lane (c, h) = (lane % 32, lane / 32) ends with column c's scores at tokens 16 s + 8 h + 0..7 (s = 0, 1), and its
+//     probabilities are, as they are, the B operands of
+//   O^T = V^T P^T, whose A operand is 8 consecutive tokens of a dimension: the cache's own order.
+// A column's maximum and weight need one exchange between lanes c and c + 32.
+//
+// Keys and values go from memory to LDS without registers, two stages, the next tile's loads issued before the present
+// tile's products. In LDS the 16-byte piece c of a row lies at c ^ swizzle(row), so that 16 rows read at one place
+// touch all banks; the loads put it there by which piece each lane fetches.
+//
+// The running maximum is raised only when a score passes it by 2^kLazy: until then probabilities are up to 2^kLazy, exact
+// all the same, and the sums are not touched. Masks are worked out only in tiles that some row of the wave does not see
+// whole, where values at unseen places are also kept out of the products (as in ss_attn.hip).
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "ss_attn.hpp"
+#include "ss_launch.hpp"
+
+namespace ss {
+
+namespace {
+
+constexpr float kNegInf = -__builtin_inff();
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+SS_DEV void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, 0, 0); }
+
+template <class T>
+SS_DEV f32x16 mfma32(const ss_u32x4& a, const ss_u32x4& b, const f32x16& c) {
+  if constexpr (std::is_same<T, Bf16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ss_bf16x8, a), __builtin_bit_cast(ss_bf16x8, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ss_f16x8, a), __builtin_bit_cast(ss_f16x8, b), c, 0,
+                                                  0, 0);
+}
+
+SS_DEV void local_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+SS_DEV float other_half(float v, bool upper) {
+  uint32_t lo, hi;
+  ss_pair<32>(ss_fu(v), lo, hi);
+  return ss_uf(upper ? lo : hi);
+}
+
+// D: dimensions; DV: those of the output that one workgroup has (of 256 it has half, and its scores are computed twice: the
+// sums of all of them beside the queries would leave no registers).
+template <class T, int D, int DV, int TK>
+__global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
+  constexpr int KS = D / 16, DT = DV / 32, ST = TK / 32;        // products per score tile, output tiles, score tiles
+  constexpr int KROW = D * 2, VROW = TK * 2;                   // bytes of a row in LDS
+  constexpr int KC = D / 8, VC = TK / 8;                       // 16-byte pieces of a row
+  constexpr int KI = TK * KROW / 4096, VI = DV * VROW / 4096;   // 1 KB load instructions a wave
+  constexpr float kLazy = std::is_same<T, Bf16>::value ? 8.f : 4.f;
+  __shared__ __attribute__((aligned(1024))) uint8_t k0[TK * KROW];
+  __shared__ __attribute__((aligned(1024))) uint8_t k1[TK * KROW];
+  __shared__ __attribute__((aligned(1024))) uint8_t v0[DV * VROW];
+  __shared__ __attribute__((aligned(1024))) uint8_t v1[DV * VROW];
+  __shared__ int odd;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  int b = blockIdx.x;
+  const int dv = b % (D / DV) * DV;  // first output dimension
+  b /= D / DV;
+  const int kh = b % a.kv_heads;
+  b /= a.kv_heads;
+  const int slot = b % a.slots;
+  b /= a.slots;
+  const int tile = a.tiles - 1 - b % a.tiles, s = b / a.tiles;  // the rows that see most first
+  const int page = 1 << a.page_shift;
+  SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width * page, a.err);
+  sr.r0 = __builtin_amdgcn_readfirstlane(sr.r0);
+  sr.n = __builtin_amdgcn_readfirstlane(sr.n);
+  sr.pos0 = __builtin_amdgcn_readfirstlane(sr.pos0);
+  sr.end = __builtin_amdgcn_readfirstlane(sr.end);
+  const int p0 = tile * 128, np = sr.n * a.group;
+  if (p0 >= np) return;
+  const Seen sn = seen_tokens(sr.pos0 + p0 / a.group, sr.pos0 + (min(p0 + 128, np) - 1) / a.group, sr.end, a.window,
+                              a.sinks);
+  const int sc = (sn.s_end + a.chunk - 1) / a.chunk, wc = max(sn.w_begin / a.chunk, sc);
+  int t_begin = 0, t_end = sn.end;
+  if (a.slots > 1) {
+    const int ch = slot < sc ? slot : wc + slot - sc;
+    t_begin = ch * a.chunk;
+    t_end = min(t_begin + a.chunk, sn.end);
+    if (t_begin >= t_end) return;
+  }
+  // The tiles of [t_begin, t_end) that some row sees: up to the first tokens' end, then from the window's begin on.
+  const int gap_a = (sn.s_end + TK - 1) / TK * TK, gap_b = max(sn.w_begin / TK * TK, gap_a);
+  auto next_tile = [&](int t) { return t >= gap_a && t < gap_b ? gap_b : t; };
+
+  // This lane's column.
+  const int p = p0 + 32 * w + c, i = p / a.group;
+  const bool in = p < np;
+  const int qpos = in ? sr.pos0 + i : -1;
+  // positions of the wave's first and last row; a wave past the rows has none and skips the products
+  const int wp0 = p0 + 32 * w;
+  const bool work = wp0 < np;
+  const int pos_lo = sr.pos0 + wp0 / a.group, pos_hi = sr.pos0 + (min(wp0 + 32, np) - 1) / a.group;
+  ss_u32x4 qf[KS];
+  {
+    const uint16_t* qp = a.q + (int64_t)(sr.r0 + (in ? i : 0)) * a.q_row +
+                         (int64_t)(kh * a.group + (in ? p - i * a.group : 0)) * a.q_head + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const SS_G ss_u32x4*)(qp + 16 * ks);
+  }
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  float m = kNegInf, l = 0.f;
+
+  const int32_t* tab = a.table + (int64_t)s * a.width;
+  const int64_t page_elems = (int64_t)a.kv_heads * page * D;
+  const uint16_t* kbase = a.k + (int64_t)kh * page * D;
+  const uint16_t* vbase = a.v + (int64_t)(kh * D + dv) * page;
+  // Page of 16-token group j of a tile, -1 where there is none. The kernel does not write the table, so these are scalar
+  // loads, which do not stand behind the stages' loads in the vector memory queue.
+  auto page_id = [&](int t, int j) {
+    const int at = (t + 16 * j) >> a.page_shift;
+    const int id = ((const __attribute__((address_space(4))) int32_t*)tab)[min(at, a.width - 1)];
+    return at < a.width && (uint32_t)id < (uint64_t)a.n_pages ? id : -1;
+  };
+  // Issues the loads of the tile at t into a stage; bit j of the result: its 16-token group j has a page.
+  auto load = [&](int t, uint8_t* kl, uint8_t* vl) {
+    int ids[TK / 16];
+#pragma unroll
+    for (int j = 0; j < TK / 16; ++j) ids[j] = page_id(t, j);
+#pragma unroll
+    for (int n = 0; n < KI; ++n) {
+      const int at = (w * KI + n) * 64 + lane, row = at / KC, pos = at % KC;
+      const int piece = D == 64 ? pos ^ ((row >> 1) & 7) : pos ^ (row & 15);
+      int id = ids[0];
+#pragma unroll
+      for (int j = 1; j < TK / 16; ++j) id = row / 16 == j ? ids[j] : id;
+      const int off = (t + row) & (page - 1);
+      dma16(kbase + max(id, 0) * page_elems + off * D + 8 * piece, kl + (w * KI + n) * 1024);
+    }
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int at = (w * VI + n) * 64 + lane, row = at / VC, pos = at % VC;
+      const int piece = TK == 64 ? pos ^ ((row >> 1) & 7) : pos ^ ((row >> 2) & 3);
+      int id = ids[0];
+#pragma unroll
+      for (int j = 1; j < TK / 16; ++j) id = piece / 2 == j ? ids[j] : id;
+      const int off = (t + 8 * piece) & (page - 1);
+      dma16(vbase + max(id, 0) * page_elems + row * page + off, vl + (w * VI + n) * 1024);
+    }
+    uint32_t held = 0;
+#pragma unroll
+    for (int j = 0; j < TK / 16; ++j) held |= ids[j] >= 0 ? 1u << j : 0u;
+    return held;
+  };
+
+  // Where this lane reads: K row of score row c, V row of dimension c.
+  const int krow = 16 * (c / 16) + 8 * ((c / 4) % 2) + 4 * ((c / 8) % 2) + c % 4;
+  const int kswz = D == 64 ? (krow >> 1) & 7 : krow & 15;
+  const int vswz = TK == 64 ? (c >> 1) & 7 : (c >> 2) & 3;
+
+  auto sees = [&](int tok, bool held) { return held && tok <= qpos && (tok > qpos - a.window || tok < a.sinks); };
+  // Whether rows at positions [lo, hi] all see the whole tile, and every page of it is there.
+  auto whole_tile = [&](int t, int lo, int hi, uint32_t held) {
+    return t + TK - 1 <= lo && (t > hi - a.window || t + TK <= a.sinks) && held == (1u << (TK / 16)) - 1;
+  };
+  const int blk_lo = sr.pos0 + p0 / a.group, blk_hi = sr.pos0 + (min(p0 + 128, np) - 1) / a.group;
+  auto step = [&](int t, uint32_t held, const uint8_t* kl, const uint8_t* vl) {
+    if (!work || t > pos_hi) return;                                           // no row of the wave sees any of it
+    if (t >= a.sinks && t + TK - 1 <= pos_lo - a.window) return;
+    // Operands are read four at a time, one group ahead of the products (more in flight take registers that the sums need).
+    auto kread = [&](int f) {
+      return *reinterpret_cast<const ss_u32x4*>(kl + (krow + 32 * (f / KS)) * KROW + 16 * ((2 * (f % KS) + h) ^ kswz));
+    };
+    auto vread = [&](int d, int nk) {
+      return *reinterpret_cast<const ss_u32x4*>(vl + (c + 32 * d) * VROW + 16 * ((2 * nk + h) ^ vswz));
+    };
+    f32x16 x[ST];
+    ss_u32x4 fr[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fr[0][j] = kread(j);
+#pragma unroll
+    for (int n = 0; n < ST; ++n) x[n] = f32x16{};
+#pragma unroll
+    for (int g = 0; g < ST * KS / 4; ++g) {
+      if (g + 1 < ST * KS / 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fr[(g + 1) % 2][j] = kread(4 * g + 4 + j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[(4 * g + j) / KS] = mfma32<T>(fr[g % 2][j], qf[(4 * g + j) % KS], x[(4 * g + j) / KS]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const bool whole = whole_tile(t, pos_lo, pos_hi, held);
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < ST; ++n) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          x[n][e] = sees(t + 32 * n + 16 * (e / 8) + 8 * h + e % 8, (held >> (2 * n + e / 8)) & 1u) ? x[n][e] : kNegInf;
+        }
+      }
+      // a page that is missing where a row of the wave sees a token
+      bool miss = false;
+#pragma unroll
+      for (int j = 0; j < TK / 16; ++j) {
+        const int lo = t + 16 * j;
+        miss |= !((held >> j) & 1u) && lo <= qpos && (lo + 15 > qpos - a.window || lo < a.sinks);
+      }
+      if (miss) ss_raise(a.err, SS_ERR_PAGE);
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int n = 0; n < ST; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[n][e]);
+    mx = fmaxf(mx, other_half(mx, h)) * a.scale - T::kShift;
+    if (__any(mx > m + kLazy || (m == kNegInf && mx > kNegInf))) {
+      const float mn = fmaxf(m, mx);
+      const float f = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);  // nothing summed yet (or NaN) where m is -inf
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] *= f;
+      m = mn;
+    }
+    const float mu = m == kNegInf ? 0.f : m;
+    ss_u32x4 pf[ST][2];
+#pragma unroll
+    for (int n = 0; n < ST; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float q0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], a.scale, -mu));
+        const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e + 1], a.scale, -mu));
+        l += q0;
+        l += q1;
+        pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
+      }
+    constexpr int NV = DT * 2 * ST;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fr[0][j] = vread(j / (2 * ST), j % (2 * ST));
+#pragma unroll
+    for (int g = 0; g < NV / 4; ++g) {
+      if (g + 1 < NV / 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fr[(g + 1) % 2][j] = vread((4 * g + 4 + j) / (2 * ST), (4 * g + 4 + j) % (2 * ST));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = (4 * g + j) / (2 * ST), nk = (4 * g + j) % (2 * ST);
+        acc[d] = mfma32<T>(fr[g % 2][j], pf[nk / 2][nk % 2], acc[d]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // In a tile that some row of the workgroup does not see whole, non-finite values are taken out of the stage before any
+  // wave uses it; `odd` says that there were any, and they are dealt with after the last tile.
+  auto clean = [&](int t, uint32_t held, uint8_t* vl) {
+    if (whole_tile(t, blk_lo, blk_hi, held)) return;
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      ss_u32x4* at = reinterpret_cast<ss_u32x4*>(vl + (n * 256 + tid) * 16);
+      const ss_u32x4 x = *at;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bad |= nonfinite2<T>(x[j]);
+      if (bad) {
+        *at = parts_of<T>(x, -1);
+        odd = 1;
+      }
+    }
+    local_barrier();
+  };
+  auto sync = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of the stage have landed
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  if (tid == 0) odd = 0;  // before the first tile's barrier
+  int t = next_tile(t_begin);
+  uint32_t held = t < t_end ? load(t, k0, v0) : 0;
+  while (t < t_end) {
+    int u = next_tile(t + TK);
+    uint32_t next = 0;
+    sync();  // the tile at t is in stage 0, and stage 1 is free: every wave has finished with it
+    if (u < t_end) next = load(u, k1, v1);
+    clean(t, held, v0);
+    step(t, held, k0, v0);
+    t = u;
+    held = next;
+    if (t >= t_end) break;
+    u = next_tile(t + TK);
+    sync();
+    if (u < t_end) next = load(u, k0, v0);
+    clean(t, held, v1);
+    step(t, held, k1, v1);
+    t = u;
+    held = next;
+  }
+  __syncthreads();
+  const bool fix = work && odd;
+  l += other_half(l, h);
+  const int64_t at = (int64_t)(sr.r0 + i) * a.heads + kh * a.group + (p - i * a.group);
+  const int64_t pa = (int64_t)slot * a.rows * a.heads + at;
+  if (in && a.slots > 1) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int b4 = 0; b4 < 4; ++b4) {
+        ss_f32x4 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = acc[d][4 * b4 + r];
+        *reinterpret_cast<SS_G ss_f32x4*>(gp(a.po) + pa * D + dv + 32 * d + 8 * b4 + 4 * h) = o;
+      }
+    if (h == 0 && dv == 0) {
+      gp(a.pml)[2 * pa] = m;
+      gp(a.pml)[2 * pa + 1] = l;
+    }
+  } else if (in) {
+    const float r = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int b4 = 0; b4 < 4; ++b4) {
+        uint2 word;
+        word.x = T::pack(acc[d][4 * b4] * r, acc[d][4 * b4 + 1] * r);
+        word.y = T::pack(acc[d][4 * b4 + 2] * r, acc[d][4 * b4 + 3] * r);
+        *reinterpret_cast<uint2*>(a.out + at * D + dv + 32 * d + 8 * b4 + 4 * h) = word;
+      }
+    if (a.lse && h == 0 && dv == 0) a.lse[at] = l == 0.f ? kNegInf : (m + __log2f(l)) * 0.693147180559945309f;
+  }
+  if (!fix) return;
+  // Infinities and NaN that were taken out go to the columns that see them, by a product of ones in their places with ones
+  // for the tokens seen; each lane adds to what it wrote itself.
+#pragma unroll 1
+  for (t = next_tile(t_begin); t < t_end; t = next_tile(t + TK)) {
+    held = 0;
+#pragma unroll
+    for (int j = 0; j < TK / 16; ++j) held |= page_id(t, j) >= 0 ? 1u << j : 0u;
+    if (whole_tile(t, blk_lo, blk_hi, held)) continue;
+#pragma unroll 1
+    for (int nk = 0; nk < 2 * ST; ++nk) {
+      const int first = t + 16 * nk + 8 * h, id = page_id(t, nk);
+      const uint16_t* vp = vbase + max(id, 0) * page_elems + (int64_t)c * page + (first & (page - 1));
+      ss_u32x4 ones;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        ones[j] = (sees(first + 2 * j, id >= 0) ? T::kOne : 0u) | (sees(first + 2 * j + 1, id >= 0) ? T::kOne << 16 : 0u);
+#pragma unroll 1
+      for (int d = 0; d < DT; ++d) {
+        const ss_u32x4 vf = *(const SS_G ss_u32x4*)(vp + (int64_t)32 * d * page);
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {
+          const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+          const f32x16 hits = mfma32<T>(parts_of<T>(vf, kind), ones, f32x16{});
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (!in || !(hits[e] > 0.f)) continue;
+            const int od = dv + 32 * d + 8 * (e / 4) + 4 * h + e % 4;
+            if (a.slots > 1)
+              gp(a.po)[pa * D + od] += add;
+            else
+              a.out[at * D + od] = (uint16_t)T::pack(T::widen(a.out[at * D + od]) + add, 0.f);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <class T>
+hipError_t launch_prompt_of(const AttnArgs& a, int dim, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs * (dim == 256 ? 2 : 1)));
+  if (dim == 64)
+    hipLaunchKernelGGL((attn_prompt_kernel<T, 64, 64, 64>), grid, dim3(256), 0, st, a);
+  else if (dim == 128)
+    hipLaunchKernelGGL((attn_prompt_kernel<T, 128, 128, 64>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_prompt_kernel<T, 256, 128, 32>), grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attn_prompt(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {
+  return fp16 ? launch_prompt_of<Fp16>(a, dim, st) : launch_prompt_of<Bf16>(a, dim, st);
+}
+
+}  // namespace ss

@@ -212,12 +212,14 @@ int check_paged(int rows, int seqs, int max_rows, int heads, int kv_heads, int d
   return ok();
 }
 
-// How a call of ssmoe_paged_attention is laid out (its checks included).
+// How a call of ssmoe_paged_attention is laid out (its checks included). `prompt`: the kernel for many rows of a sequence.
 //
-// Chunk: the tokens of one workgroup, so that a batch of full tables makes about 2048 workgroups, but none of fewer
-// than 128 tokens (a tile for each wave) or more than 4096. It goes by seqs, kv_heads and the table's width alone, so a
-// row's chunks, and with them its bits, do not depend on the other rows of a call.
-int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64_t* ws) {
+// Few rows (up to kFewRows): chunk is the tokens of one workgroup, so that a batch of full tables makes about 2048
+// workgroups, but none of fewer than 128 tokens (a tile for each wave) or more than 4096. It goes by seqs, kv_heads and the
+// table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call.
+// Many rows: the tokens are split only where the row tiles alone would leave CUs without work.
+constexpr int kFewRows = 8;
+int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
   if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
   int shift = 0;
   if (int rc = check_paged(p->rows, p->seqs, p->max_rows, p->heads, p->kv_heads, p->dim, p->page, p->width, p->n_pages,
@@ -240,19 +242,29 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
   a.sinks = a.window < (1 << 30) ? p->sinks : 0;
   a.scale = p->scale * 1.44269504088896340736f;
   if ((int64_t)max_rows * a.group > (1 << 30)) return fail(SSMOE_EINVAL, "max_rows * heads / kv_heads must be at most 2^30");
-  a.packed = ss::attn_few_packed(p->dim, max_rows * a.group);
+  *prompt = p->max_rows > kFewRows;
+  a.packed = *prompt ? 128 : ss::attn_few_packed(p->dim, max_rows * a.group);
   a.tiles = (max_rows * a.group + a.packed - 1) / a.packed;
   // tokens of a sequence that the call may read
   int64_t seen = cap;
   if (a.window < (1 << 30)) seen = std::min<int64_t>(cap, (int64_t)a.window + max_rows + a.sinks);
-  int64_t chunk = (seen * p->seqs * p->kv_heads + 2047) / 2048;
-  chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), 4096);
+  int64_t chunk = cap, slots = 1;
+  const int64_t units = (int64_t)p->seqs * p->kv_heads;
+  if (*prompt) {
+    const int64_t want = 512 / std::max<int64_t>(units * a.tiles * (p->dim == 256 ? 2 : 1), 1);
+    if (want > 1 && seen > 512) chunk = std::max<int64_t>((seen + want - 1) / want, 512);
+    chunk = (chunk + 127) / 128 * 128;
+  } else {
+    chunk = (seen * units + 2047) / 2048;
+    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), 4096);
+  }
   a.chunk = (int)chunk;
-  int64_t slots = (cap + chunk - 1) / chunk;
+  slots = (cap + chunk - 1) / chunk;
   if (a.window < (1 << 30))
     slots = std::min(slots, (std::min<int64_t>(a.sinks, cap) + chunk - 1) / chunk + (a.window + max_rows + chunk - 2) / chunk + 1);
+  if (*prompt && chunk >= seen) slots = 1;
   a.slots = (int)slots;
-  if (slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
+  if (2 * slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
     return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
   const int64_t parts = slots > 1 ? slots * p->rows * p->heads : 0;
   *ws = (parts * p->dim * 4 + 255) / 256 * 256 + parts * 8;
@@ -1394,13 +1406,15 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
 int64_t ssmoe_paged_attention_workspace_bytes(const ssmoe_paged_attention_args* p) {
   ss::AttnArgs a{};
   int64_t ws = 0;
-  return plan_attention(p, &a, &ws) ? -1 : ws;
+  bool prompt = false;
+  return plan_attention(p, &a, &ws, &prompt) ? -1 : ws;
 }
 
 int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
   ss::AttnArgs a{};
   int64_t ws = 0;
-  if (int rc = plan_attention(p, &a, &ws)) return rc;
+  bool prompt = false;
+  if (int rc = plan_attention(p, &a, &ws, &prompt)) return rc;
   if (p->rows == 0 || p->seqs == 0) return ok();
   if (!p->q || !p->k_pages || !p->v_pages || !p->cu_rows || !p->kv_len || !p->table || !p->out)
     return fail(SSMOE_EINVAL, "q, k_pages, v_pages, cu_rows, kv_len, table and out must be non-null");
@@ -1430,7 +1444,9 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
   }
   const bool fp16 = p->type == SSMOE_FP16;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (int rc = hip_check(ss::launch_attn_few(a, p->dim, fp16, st), "attention launch")) return rc;
+  if (int rc = hip_check(prompt ? ss::launch_attn_prompt(a, p->dim, fp16, st) : ss::launch_attn_few(a, p->dim, fp16, st),
+                         "attention launch"))
+    return rc;
   return a.slots > 1 ? hip_check(ss::launch_attn_join(a, p->dim, fp16, st), "attention join launch") : ok();
 }
 

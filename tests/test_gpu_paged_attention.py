@@ -211,3 +211,80 @@ def test_other_stream_and_captured_graph():
         torch.cuda.synchronize()
         assert torch.equal(out.view(torch.int16), want.view(torch.int16)), step
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [
+    (1, 1, 64, 16, torch.bfloat16), (4, 1, 64, 64, torch.float16), (5, 1, 128, 32, torch.bfloat16), (8, 4, 128, 64, torch.float16),
+    (3, 1, 256, 16, torch.bfloat16), (2, 2, 256, 128, torch.float16), (16, 1, 64, 256, torch.bfloat16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (50, 3), (64, 64), (130, 17)])
+def test_prompt_chunks(heads, kv_heads, dim, page, dtype, window, sinks):
+    """Chunks of many rows, from an empty cache and behind one, of mixed sizes, with lengths at the edges of tiles."""
+    check(Batch([130, 9, 1, 0, 64, 65], [130, 200, 77, 50, 64, 129], heads, kv_heads, dim, page, dtype, seed=heads + dim),
+          window, sinks)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_split_over_its_length(dim):
+    """Few row tiles behind a long context: the tokens are shared out and joined."""
+    b = Batch([20, 33], [2100, 3333], 4, 2, dim, 64, seed=dim)
+    check(b)
+    check(b, window=1500, sinks=40)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("long", [False, True])
+def test_prompt_unseen_places_do_not_matter(dim, bad, long):
+    """As for few rows: past the tokens, before the window, in pages not held, at later rows' tokens; with and without the
+    split over the length."""
+    n = 2500 if long else 150
+    b = Batch([40, 12], [n, 205], 4, 2, dim, 16, tail=bad, seed=3)
+    b.table[1, 1:6] = -1                                  # tokens 16 .. 95 are not held: the windows begin at 134 and later
+    check(b, window=60, sinks=16)
+    b = Batch([40], [n], 4, 2, dim, 16, seed=4)
+    want = check(b)
+    at = n - 10                                           # the token of row 30: seen by it and the rows behind it
+    page, off = int(b.table[0, at // 16]), at % 16
+    b.k[page, :, off] = bad
+    got = paged_attention(*b.args())
+    assert torch.equal(got[:30].view(torch.int16), want[:30].view(torch.int16)) and torch.isnan(got[30:]).all()
+    b = Batch([40], [n], 4, 2, dim, 16, seed=4)
+    b.v[page, 1, 7, off] = bad
+    got = paged_attention(*b.args())
+    keep = torch.ones(4, dim, dtype=torch.bool, device="cuda")
+    keep[2:, 7] = False
+    assert torch.equal(got[:30].view(torch.int16), want[:30].view(torch.int16))
+    assert torch.equal(got[30:][:, keep].view(torch.int16), want[30:][:, keep].view(torch.int16))
+    seen = got[30:, 2:, 7].float()
+    assert torch.isnan(seen).all() if math.isnan(bad) else (seen == bad).all()
+
+
+def test_prompt_bad_pages_are_raised():
+    b = Batch([100], [400], 4, 2, 64, 16, seed=12)
+    b.table[0, 2] = -1
+    b.table[0, 22] = b.k.shape[0]
+    got = paged_attention(*b.args())
+    assert _lib.device_error() == ERR_PAGE
+    assert ((got.double().cpu() - attention64(b)[0]).abs() <= attention_bound(b)).all()
+
+
+def test_prompt_strides_padding_rows_and_graph():
+    b = Batch([70, 20], [70, 300], 8, 2, 128, 32, seed=8)
+    q, k, v, cu, kv_len, table, n = b.args()
+    fused = torch.zeros(95, 13, 128, dtype=q.dtype, device="cuda")
+    fused[:90, 2:10] = q
+    out = torch.full((95, 8, 128), 5.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((95, 8), 5.0, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    paged_attention(fused[:, 2:10], k, v, cu, kv_len, table, n, out=out, lse=lse)
+    assert (out[90:] == 5).all() and (lse[90:] == 5).all()
+    want = paged_attention(q, k, v, cu, kv_len, table, n)
+    assert torch.equal(out[:90].view(torch.int16), want.view(torch.int16))
+    with torch.cuda.graph(graph):
+        paged_attention(fused[:, 2:10], k, v, cu, kv_len, table, n, out=out)
+    for step in range(3):
+        fused.normal_()
+        kv_len[1] -= step
+        graph.replay()
+        want = paged_attention(fused[:90, 2:10], k, v, cu, kv_len, table, n)
+        assert torch.equal(out[:90].view(torch.int16), want.view(torch.int16)), step

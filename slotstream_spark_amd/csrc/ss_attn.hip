@@ -280,19 +280,22 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   }
 }
 
-// Joins the chunks of a row: o = sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), m the largest m_k. One workgroup per row and
-// head; its groups of dim / 4 threads take the chunks by their number modulo the number of groups, each with a running
-// maximum, and the groups' sums are added in order.
-template <class T, int D>
+// Joins the chunks of a row: o = sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), m the largest m_k. A row and head is read by
+// groups of dim / 4 threads, 16 bytes each. WIDE: its workgroup's groups take the chunks by their number modulo the
+// number of groups, each with a running maximum, and the groups' sums are added in order; else one group takes all its
+// chunks and a workgroup has as many rows. Either way the order goes by the chunks' numbers alone.
+template <class T, int D, bool WIDE>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-  constexpr int TD = D / 4, GROUPS = 256 / TD;
-  __shared__ __attribute__((aligned(16))) float part[GROUPS][D];
+  constexpr int TD = D / 4, GROUPS = 256 / TD, STEP = WIDE ? GROUPS : 1;
+  __shared__ __attribute__((aligned(16))) float part[WIDE ? GROUPS : 1][D];
   __shared__ float part_l[GROUPS], part_m[GROUPS];
   const int tid = threadIdx.x, d4 = 4 * (tid % TD), k = tid / TD;
-  int b = blockIdx.x;
-  const int head = b % a.heads;
+  const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
+  int64_t b = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * GROUPS + k;
+  if (b >= all) return;
+  const int head = (int)(b % a.heads);
   b /= a.heads;
-  const int i = b % a.max_rows, s = b / a.max_rows;
+  const int i = (int)(b % a.max_rows), s = (int)(b / a.max_rows);
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width << a.page_shift, nullptr);
   if (i >= sr.n) return;
   // The slots of the workgroup that had this row, as it counted them.
@@ -312,31 +315,34 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * fk;
   };
-  // Slot j holds chunk j (first tokens) or chunk wc + j - sc: group k takes the chunks k, k + GROUPS, ...
-  const int j1 = sc + (k + GROUPS - wc % GROUPS) % GROUPS;
   auto take = [&](int from, int to) {
 #pragma unroll 4
-    for (int j = from; j < to; j += GROUPS) {
+    for (int j = from; j < to; j += STEP) {
       const int64_t at = j * rows + row;
       const float mk = gp(a.pml)[2 * at], lk = gp(a.pml)[2 * at + 1];
       const ss_f32x4 x = *reinterpret_cast<const SS_G ss_f32x4*>(gp(a.po) + at * D + d4);
       add(x, mk, lk);
     }
   };
-  take(k, sc);
-  take(j1, used);
-  *reinterpret_cast<ss_f32x4*>(&part[k][d4]) = o;
-  if (d4 == 0) {
-    part_m[k] = m;
-    part_l[k] = l;
-  }
-  __syncthreads();
-  if (k > 0) return;
-  m = kNegInf;
-  l = 0.f;
-  o = ss_f32x4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (WIDE) {
+    // Slot j holds chunk j (first tokens) or chunk wc + j - sc: group k takes the chunks k, k + GROUPS, ...
+    take(k, sc);
+    take(sc + (k + GROUPS - wc % GROUPS) % GROUPS, used);
+    *reinterpret_cast<ss_f32x4*>(&part[k][d4]) = o;
+    if (d4 == 0) {
+      part_m[k] = m;
+      part_l[k] = l;
+    }
+    __syncthreads();
+    if (k > 0) return;
+    m = kNegInf;
+    l = 0.f;
+    o = ss_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < GROUPS; ++j) add(*reinterpret_cast<const ss_f32x4*>(&part[j][d4]), part_m[j], part_l[j]);
+    for (int j = 0; j < GROUPS; ++j) add(*reinterpret_cast<const ss_f32x4*>(&part[j][d4]), part_m[j], part_l[j]);
+  } else {
+    take(0, used);
+  }
   const float r = l == 0.f ? 0.f : 1.f / l;
   uint2 word;
   word.x = T::pack(o[0] * r, o[1] * r);
@@ -361,16 +367,20 @@ hipError_t launch_few_of(const AttnArgs& a, int dim, hipStream_t st) {
   return launch_few<T, 256, 1>(a, st);
 }
 
+template <class T, int D>
+hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
+  const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
+  constexpr int GROUPS = 256 / (D / 4);
+  if (a.slots > 16)
+    hipLaunchKernelGGL((attn_join_kernel<T, D, true>), dim3((unsigned)all), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<T, D, false>), dim3((unsigned)((all + GROUPS - 1) / GROUPS)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
 template <class T>
 hipError_t launch_join_of(const AttnArgs& a, int dim, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.seqs * a.max_rows * a.heads));
-  if (dim == 64)
-    hipLaunchKernelGGL((attn_join_kernel<T, 64>), grid, dim3(256), 0, st, a);
-  else if (dim == 128)
-    hipLaunchKernelGGL((attn_join_kernel<T, 128>), grid, dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((attn_join_kernel<T, 256>), grid, dim3(256), 0, st, a);
-  return hipGetLastError();
+  return dim == 64 ? launch_join<T, 64>(a, st) : dim == 128 ? launch_join<T, 128>(a, st) : launch_join<T, 256>(a, st);
 }
 
 }  // namespace

@@ -30,6 +30,7 @@ struct AttnArgs {
   int chunk;   // tokens of a chunk, a multiple of 128, at most 4096
   int packed;  // packed rows (rows times heads of a key head) of a workgroup
   int tiles;   // workgroups over the packed rows of one sequence and key head
+  int rising;  // many rows: the tiles at the end of the launch that go up
   float scale; // of the scores, times log2(e)
 };
 
@@ -42,7 +43,12 @@ struct Bf16 {
   static constexpr float kShift = 0.f;
   static constexpr uint32_t kExp = 0x7F80u, kOne = 0x3F80u;
   SS_DEV static ss_f32x4 mfma16(const ss_u32x4& a, const ss_u32x4& b, const ss_f32x4& c) { return ss_mfma(a, b, c); }
-  SS_DEV static uint32_t pack(float lo, float hi) { return ss_pack_bf16(lo, hi); }
+  // One v_cvt_pk_bf16_f32 (of two conversions and an or, the compiler makes four instructions).
+  SS_DEV static uint32_t pack(float lo, float hi) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
+  }
   SS_DEV static float widen(uint32_t u) { return ss_bf16_to_f32(u); }
 };
 struct Fp16 {

@@ -58,7 +58,8 @@ SS_DEV float other_half(float v, bool upper) {
 
 // D: dimensions; DV: those of the output that one workgroup has (of 256 it has half, and its scores are computed twice: the
 // sums of all of them beside the queries would leave no registers).
-template <class T, int D, int DV, int TK>
+// ONE: a tile lies in one page (page >= TK).
+template <class T, int D, int DV, int TK, bool ONE>
 __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int KS = D / 16, DT = DV / 32, ST = TK / 32;        // products per score tile, output tiles, score tiles
   constexpr int KROW = D * 2, VROW = TK * 2;                   // bytes of a row in LDS
@@ -79,7 +80,9 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   b /= a.kv_heads;
   const int slot = b % a.slots;
   b /= a.slots;
-  const int tile = a.tiles - 1 - b % a.tiles, s = b / a.tiles;  // the rows that see most first
+  const int s = b % a.seqs, turn = b / a.seqs;
+  // The tiles that see most first; the last `a.rising` turns, which share CUs with the first ones, from the other end.
+  const int tile = turn < a.tiles - a.rising ? a.tiles - 1 - turn : turn - (a.tiles - a.rising);
   const int page = 1 << a.page_shift;
   SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width * page, a.err);
   sr.r0 = __builtin_amdgcn_readfirstlane(sr.r0);
@@ -122,47 +125,76 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float m = kNegInf, l = 0.f;
 
-  const int32_t* tab = a.table + (int64_t)s * a.width;
-  const int64_t page_elems = (int64_t)a.kv_heads * page * D;
-  const uint16_t* kbase = a.k + (int64_t)kh * page * D;
-  const uint16_t* vbase = a.v + (int64_t)(kh * D + dv) * page;
-  // Page of 16-token group j of a tile, -1 where there is none. The kernel does not write the table, so these are scalar
-  // loads, which do not stand behind the stages' loads in the vector memory queue.
+  // Pages of a tile's 16-token groups (one where the tile lies in one page), -1 where there is none. The kernel does not write
+  // the table, so these are scalar loads, which do not stand behind the stages' loads in the vector memory queue.
+  constexpr int NP = ONE ? 1 : TK / 16;
+  const __attribute__((address_space(4))) int32_t* tab =
+      (const __attribute__((address_space(4))) int32_t*)(a.table + (int64_t)s * a.width);
+  const uint32_t n_pages = (uint32_t)a.n_pages;
   auto page_id = [&](int t, int j) {
     const int at = (t + 16 * j) >> a.page_shift;
-    const int id = ((const __attribute__((address_space(4))) int32_t*)tab)[min(at, a.width - 1)];
-    return at < a.width && (uint32_t)id < (uint64_t)a.n_pages ? id : -1;
+    const int id = tab[min(at, a.width - 1)];
+    return at < a.width && (uint32_t)id < n_pages ? id : -1;
   };
-  // Issues the loads of the tile at t into a stage; bit j of the result: its 16-token group j has a page.
+  const int64_t page_bytes = (int64_t)a.kv_heads * page * D * 2;
+  const char* kbase = reinterpret_cast<const char*>(a.k) + (int64_t)kh * page * D * 2;
+  const char* vbase = reinterpret_cast<const char*>(a.v) + (int64_t)(kh * D + dv) * page * 2;
+  // What this lane fetches in each load, as bytes from the place of the tile in its page: K rows are tokens (a load's rows
+  // are of one 16-token group), V rows dimensions.
+  uint32_t koff[KI], voff[VI];
+  int vpiece[VI];
+#pragma unroll
+  for (int n = 0; n < KI; ++n) {
+    const int at = (w * KI + n) * 64 + lane, row = at / KC, pos = at % KC;
+    const int piece = D == 64 ? pos ^ ((row >> 1) & 7) : pos ^ (row & 15);
+    koff[n] = (ONE ? row : row % 16) * KROW + 16 * piece;
+  }
+#pragma unroll
+  for (int n = 0; n < VI; ++n) {
+    const int at = (w * VI + n) * 64 + lane, row = at / VC, pos = at % VC;
+    vpiece[n] = TK == 64 ? pos ^ ((row >> 1) & 7) : pos ^ ((row >> 2) & 3);
+    voff[n] = (uint32_t)row * page * 2 + (ONE ? 16 * vpiece[n] : 16 * (vpiece[n] & 1));
+  }
+  // Issues the loads of the tile at t into a stage; bit j of the result: its j-th page is there.
   auto load = [&](int t, uint8_t* kl, uint8_t* vl) {
-    int ids[TK / 16];
-#pragma unroll
-    for (int j = 0; j < TK / 16; ++j) ids[j] = page_id(t, j);
-#pragma unroll
-    for (int n = 0; n < KI; ++n) {
-      const int at = (w * KI + n) * 64 + lane, row = at / KC, pos = at % KC;
-      const int piece = D == 64 ? pos ^ ((row >> 1) & 7) : pos ^ (row & 15);
-      int id = ids[0];
-#pragma unroll
-      for (int j = 1; j < TK / 16; ++j) id = row / 16 == j ? ids[j] : id;
-      const int off = (t + row) & (page - 1);
-      dma16(kbase + max(id, 0) * page_elems + off * D + 8 * piece, kl + (w * KI + n) * 1024);
-    }
-#pragma unroll
-    for (int n = 0; n < VI; ++n) {
-      const int at = (w * VI + n) * 64 + lane, row = at / VC, pos = at % VC;
-      const int piece = TK == 64 ? pos ^ ((row >> 1) & 7) : pos ^ ((row >> 2) & 3);
-      int id = ids[0];
-#pragma unroll
-      for (int j = 1; j < TK / 16; ++j) id = piece / 2 == j ? ids[j] : id;
-      const int off = (t + 8 * piece) & (page - 1);
-      dma16(vbase + max(id, 0) * page_elems + row * page + off, vl + (w * VI + n) * 1024);
-    }
+    int ids[NP];
     uint32_t held = 0;
 #pragma unroll
-    for (int j = 0; j < TK / 16; ++j) held |= ids[j] >= 0 ? 1u << j : 0u;
+    for (int j = 0; j < NP; ++j) {
+      ids[j] = page_id(t, j);
+      held |= ids[j] >= 0 ? 1u << j : 0u;
+      ids[j] = max(ids[j], 0);
+    }
+    if constexpr (ONE) {
+      const int off = t & (page - 1);
+      const char* kp = kbase + ids[0] * page_bytes + off * KROW;
+      const char* vp = vbase + ids[0] * page_bytes + off * 2;
+#pragma unroll
+      for (int n = 0; n < KI; ++n) dma16(kp + koff[n], kl + (w * KI + n) * 1024);
+#pragma unroll
+      for (int n = 0; n < VI; ++n) dma16(vp + voff[n], vl + (w * VI + n) * 1024);
+    } else {
+#pragma unroll
+      for (int n = 0; n < KI; ++n) {
+        const int j = (w * KI + n) * (64 / KC) / 16;  // the load's 16-token group
+        int id = ids[0];
+#pragma unroll
+        for (int q = 1; q < NP; ++q) id = j == q ? ids[q] : id;
+        dma16(kbase + id * page_bytes + ((t + 16 * j) & (page - 1)) * KROW + koff[n], kl + (w * KI + n) * 1024);
+      }
+#pragma unroll
+      for (int n = 0; n < VI; ++n) {
+        const int j = vpiece[n] / 2;
+        int id = ids[0];
+#pragma unroll
+        for (int q = 1; q < NP; ++q) id = j == q ? ids[q] : id;
+        dma16(vbase + id * page_bytes + ((t + 16 * j) & (page - 1)) * 2 + voff[n], vl + (w * VI + n) * 1024);
+      }
+    }
     return held;
   };
+  constexpr uint32_t kAll = (1u << NP) - 1;
+  auto has = [&](uint32_t held, int group) { return ((held >> (ONE ? 0 : group)) & 1u) != 0; };
 
   // Where this lane reads: K row of score row c, V row of dimension c.
   const int krow = 16 * (c / 16) + 8 * ((c / 4) % 2) + 4 * ((c / 8) % 2) + c % 4;
@@ -172,7 +204,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   auto sees = [&](int tok, bool held) { return held && tok <= qpos && (tok > qpos - a.window || tok < a.sinks); };
   // Whether rows at positions [lo, hi] all see the whole tile, and every page of it is there.
   auto whole_tile = [&](int t, int lo, int hi, uint32_t held) {
-    return t + TK - 1 <= lo && (t > hi - a.window || t + TK <= a.sinks) && held == (1u << (TK / 16)) - 1;
+    return t + TK - 1 <= lo && (t > hi - a.window || t + TK <= a.sinks) && held == kAll;
   };
   const int blk_lo = sr.pos0 + p0 / a.group, blk_hi = sr.pos0 + (min(p0 + 128, np) - 1) / a.group;
   auto step = [&](int t, uint32_t held, const uint8_t* kl, const uint8_t* vl) {
@@ -204,21 +236,39 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     }
     const bool whole = whole_tile(t, pos_lo, pos_hi, held);
     if (!whole) {
+      // This lane's token e of score tile n is seen where lo < 32 n + 16 (e / 8) + e % 8 <= hi. The comparisons are kept in
+      // small groups: all at once they would take more scalar registers than there are.
+      const int hi = qpos - t - 8 * h, lo = hi - a.window;
+      if (t >= a.sinks && held == kAll) {
 #pragma unroll
-      for (int n = 0; n < ST; ++n) {
+        for (int n = 0; n < ST; ++n)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          x[n][e] = sees(t + 32 * n + 16 * (e / 8) + 8 * h + e % 8, (held >> (2 * n + e / 8)) & 1u) ? x[n][e] : kNegInf;
+          for (int e = 0; e < 16; ++e) {
+            const int off = 32 * n + 16 * (e / 8) + e % 8;
+            x[n][e] = off <= hi && off > lo ? x[n][e] : kNegInf;
+            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < ST; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int off = 32 * n + 16 * (e / 8) + e % 8;
+            const bool see = has(held, 2 * n + e / 8) && off <= hi && (off > lo || off < a.sinks - t - 8 * h);
+            x[n][e] = see ? x[n][e] : kNegInf;
+            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      if (held != kAll) {
+        // a page that is missing where a row of the wave sees a token
+        bool miss = false;
+#pragma unroll
+        for (int j = 0; j < TK / 16; ++j) {
+          const int first = t + 16 * j;
+          miss |= !has(held, j) && first <= qpos && (first + 15 > qpos - a.window || first < a.sinks);
         }
+        if (miss) ss_raise(a.err, SS_ERR_PAGE);
       }
-      // a page that is missing where a row of the wave sees a token
-      bool miss = false;
-#pragma unroll
-      for (int j = 0; j < TK / 16; ++j) {
-        const int lo = t + 16 * j;
-        miss |= !((held >> j) & 1u) && lo <= qpos && (lo + 15 > qpos - a.window || lo < a.sinks);
-      }
-      if (miss) ss_raise(a.err, SS_ERR_PAGE);
     }
     float mx = x[0][0];
 #pragma unroll
@@ -238,16 +288,18 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     }
     const float mu = m == kNegInf ? 0.f : m;
     ss_u32x4 pf[ST][2];
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < ST; ++n)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const float q0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], a.scale, -mu));
         const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e + 1], a.scale, -mu));
-        l += q0;
-        l += q1;
+        part[e % 4] += q0;
+        part[e % 4 + 1] += q1;
         pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
       }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
     constexpr int NV = DT * 2 * ST;
 #pragma unroll
     for (int j = 0; j < 4; ++j) fr[0][j] = vread(j / (2 * ST), j % (2 * ST));
@@ -351,12 +403,13 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   for (t = next_tile(t_begin); t < t_end; t = next_tile(t + TK)) {
     held = 0;
 #pragma unroll
-    for (int j = 0; j < TK / 16; ++j) held |= page_id(t, j) >= 0 ? 1u << j : 0u;
+    for (int j = 0; j < NP; ++j) held |= page_id(t, j) >= 0 ? 1u << j : 0u;
     if (whole_tile(t, blk_lo, blk_hi, held)) continue;
 #pragma unroll 1
     for (int nk = 0; nk < 2 * ST; ++nk) {
       const int first = t + 16 * nk + 8 * h, id = page_id(t, nk);
-      const uint16_t* vp = vbase + max(id, 0) * page_elems + (int64_t)c * page + (first & (page - 1));
+      const uint16_t* vp = reinterpret_cast<const uint16_t*>(vbase + max(id, 0) * page_bytes) + (int64_t)c * page +
+                           (first & (page - 1));
       ss_u32x4 ones;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -383,15 +436,23 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   }
 }
 
+template <class T, int D, int DV, int TK>
+void launch_prompt(const AttnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs * (D / DV)));
+  if ((1 << a.page_shift) >= TK)
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, TK, true>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, TK, false>), grid, dim3(256), 0, st, a);
+}
+
 template <class T>
 hipError_t launch_prompt_of(const AttnArgs& a, int dim, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs * (dim == 256 ? 2 : 1)));
   if (dim == 64)
-    hipLaunchKernelGGL((attn_prompt_kernel<T, 64, 64, 64>), grid, dim3(256), 0, st, a);
+    launch_prompt<T, 64, 64, 64>(a, st);
   else if (dim == 128)
-    hipLaunchKernelGGL((attn_prompt_kernel<T, 128, 128, 64>), grid, dim3(256), 0, st, a);
+    launch_prompt<T, 128, 128, 64>(a, st);
   else
-    hipLaunchKernelGGL((attn_prompt_kernel<T, 256, 128, 32>), grid, dim3(256), 0, st, a);
+    launch_prompt<T, 256, 128, 32>(a, st);
   return hipGetLastError();
 }
 

@@ -261,8 +261,12 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
   a.chunk = (int)chunk;
   slots = (cap + chunk - 1) / chunk;
   if (a.window < (1 << 30))
-    slots = std::min(slots, (std::min<int64_t>(a.sinks, cap) + chunk - 1) / chunk + (a.window + max_rows + chunk - 2) / chunk + 1);
+    slots = std::min(slots, (std::min<int64_t>(a.sinks, cap) + chunk - 1) / chunk +
+                                (a.window + std::max(max_rows, kFewRows) + chunk - 2) / chunk + 1);
   if (*prompt && chunk >= seen) slots = 1;
+  // Two workgroups fit a CU: of at most 512, the second 256 go to the CUs of the first, the lightest to the heaviest.
+  const int64_t per_tile = units * slots * (p->dim == 256 ? 2 : 1), all = per_tile * a.tiles;
+  a.rising = *prompt && all > 256 && all <= 512 ? (int)((all - 256) / per_tile) : 0;
   a.slots = (int)slots;
   if (2 * slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
     return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       id = gp(a.table)[(int64_t)s * a.width + at];
       if ((uint32_t)id >= (uint64_t)a.n_pages) {
         id = -1;
-        if (t < sn.s_end || t + 8 > sn.w_begin) ss_raise(a.err, SS_ERR_PAGE);
+        if (t < sn.s_end || t + 8 > sn.w_begin) raise_bit(a.err, SS_ERR_PAGE);
       }
     }
     page_of[j] = id;

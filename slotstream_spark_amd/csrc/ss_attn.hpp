@@ -34,6 +34,11 @@ struct AttnArgs {
   float scale; // of the scores, times log2(e)
 };
 
+// ss_raise through a global pointer (a flat atomic would make every later wait of the wave one for all its LDS reads).
+SS_DEV void raise_bit(int* err, int bit) {
+  if (err) __hip_atomic_fetch_or(gp(err), bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 typedef _Float16 ss_f16x8 __attribute__((ext_vector_type(8)));
 
 // The element types. kShift: probabilities are kept 2^kShift times as large, the running maximum that much lower. fp16
@@ -104,7 +109,7 @@ SS_DEV SeqRows seq_rows(const int32_t* cu, const int32_t* kv_len, int s, int row
   const int64_t p0 = (int64_t)len - (b > a ? (int64_t)b - a : 0) + (r.r0 - a);
   r.pos0 = (int)(p0 < -(1 << 30) ? -(1 << 30) : p0);
   r.end = (int64_t)len > cap ? (int)cap : len;
-  if (bad && (threadIdx.x & 63) == 0) ss_raise(err, SS_ERR_BATCH);
+  if (bad && (threadIdx.x & 63) == 0) raise_bit(err, SS_ERR_BATCH);
   return r;
 }
 
@@ -123,6 +128,7 @@ SS_DEV Seen seen_tokens(int pos_a, int pos_b, int end, int window, int sinks) {
   return r;
 }
 
+int attn_prompt_parts(int dim, int page_shift);
 hipError_t launch_attn_prompt(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 hipError_t launch_attn_few(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 int attn_few_packed(int dim, int packed);

@@ -56,6 +56,17 @@ SS_DEV float other_half(float v, bool upper) {
   return ss_uf(upper ? lo : hi);
 }
 
+// Where the 16-byte piece c of row r lies in LDS: at c ^ swizzle(r). A row has D / 8 pieces (keys) or TK / 8 (values), and 16
+// rows that one read touches at the same piece fall on 16 different places of the 256 bytes that the banks cover.
+template <int D>
+SS_DEV constexpr int kswizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+template <int TK>
+SS_DEV constexpr int vswizzle(int row) {
+  return TK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
 // D: dimensions; DV: those of the output that one workgroup has (of 256 it has half, and its scores are computed twice: the
 // sums of all of them beside the queries would leave no registers).
 // ONE: a tile lies in one page (page >= TK).
@@ -139,67 +150,66 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int64_t page_bytes = (int64_t)a.kv_heads * page * D * 2;
   const char* kbase = reinterpret_cast<const char*>(a.k) + (int64_t)kh * page * D * 2;
   const char* vbase = reinterpret_cast<const char*>(a.v) + (int64_t)(kh * D + dv) * page * 2;
-  // What this lane fetches in each load, as bytes from the place of the tile in its page: K rows are tokens (a load's rows
-  // are of one 16-token group), V rows dimensions.
-  uint32_t koff[KI], voff[VI];
-  int vpiece[VI];
-#pragma unroll
-  for (int n = 0; n < KI; ++n) {
-    const int at = (w * KI + n) * 64 + lane, row = at / KC, pos = at % KC;
-    const int piece = D == 64 ? pos ^ ((row >> 1) & 7) : pos ^ (row & 15);
-    koff[n] = (ONE ? row : row % 16) * KROW + 16 * piece;
-  }
-#pragma unroll
-  for (int n = 0; n < VI; ++n) {
-    const int at = (w * VI + n) * 64 + lane, row = at / VC, pos = at % VC;
-    vpiece[n] = TK == 64 ? pos ^ ((row >> 1) & 7) : pos ^ ((row >> 2) & 3);
-    voff[n] = (uint32_t)row * page * 2 + (ONE ? 16 * vpiece[n] : 16 * (vpiece[n] & 1));
-  }
-  // Issues the loads of the tile at t into a stage; bit j of the result: its j-th page is there.
-  auto load = [&](int t, uint8_t* kl, uint8_t* vl) {
-    int ids[NP];
-    uint32_t held = 0;
+  // What this lane fetches in its first load of a stage, as bytes from the place of the tile (K without ONE: of the load's
+  // 16-token group) in its page; K rows are tokens, V rows dimensions. Load n is RK (RV) rows on, and its piece differs in
+  // the swizzle bits of those rows.
+  constexpr int RK = 64 / KC, RV = 64 / VC;
+  const int krow0 = w * KI * RK + lane / KC, vrow0 = w * VI * RV + lane / VC;
+  const uint32_t koff0 = (ONE ? krow0 : krow0 % 16) * KROW + 16 * ((lane % KC) ^ kswizzle<D>(krow0));
+  const int vpiece0 = (lane % VC) ^ vswizzle<TK>(vrow0);
+  const uint32_t voff0 = (uint32_t)vrow0 * page * 2 + 16 * (ONE ? vpiece0 : vpiece0 & 1);
+  struct Tile {
+    int t;          // its first token
+    int ids[NP];    // its pages, 0 where there is none
+    uint32_t held;  // bit j: page j is there
+  };
+  auto tile_at = [&](int t) {
+    Tile r;
+    r.t = t;
+    r.held = 0;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      ids[j] = page_id(t, j);
-      held |= ids[j] >= 0 ? 1u << j : 0u;
-      ids[j] = max(ids[j], 0);
+      const int id = page_id(t, j);
+      r.held |= id >= 0 ? 1u << j : 0u;
+      r.ids[j] = max(id, 0);
     }
-    if constexpr (ONE) {
-      const int off = t & (page - 1);
-      const char* kp = kbase + ids[0] * page_bytes + off * KROW;
-      const char* vp = vbase + ids[0] * page_bytes + off * 2;
+    return r;
+  };
+  auto load_k = [&](const Tile& r, uint8_t* kl) {
 #pragma unroll
-      for (int n = 0; n < KI; ++n) dma16(kp + koff[n], kl + (w * KI + n) * 1024);
+    for (int n = 0; n < KI; ++n) {
+      const int j = ONE ? 0 : (w * KI + n) * (64 / KC) / 16;  // the load's 16-token group
+      int id = r.ids[0];
 #pragma unroll
-      for (int n = 0; n < VI; ++n) dma16(vp + voff[n], vl + (w * VI + n) * 1024);
-    } else {
+      for (int q = 1; q < NP; ++q) id = j == q ? r.ids[q] : id;
+      dma16(kbase + id * page_bytes + ((r.t + 16 * j) & (page - 1)) * KROW + n * RK * KROW +
+                (koff0 ^ (16 * kswizzle<D>(n * RK))),
+            kl + (w * KI + n) * 1024);
+    }
+  };
+  auto load_v = [&](const Tile& r, uint8_t* vl) {
 #pragma unroll
-      for (int n = 0; n < KI; ++n) {
-        const int j = (w * KI + n) * (64 / KC) / 16;  // the load's 16-token group
-        int id = ids[0];
+    for (int n = 0; n < VI; ++n) {
+      if constexpr (ONE) {
+        dma16(vbase + r.ids[0] * page_bytes + (r.t & (page - 1)) * 2 + n * RV * page * 2 +
+                  (voff0 ^ (16 * vswizzle<TK>(n * RV))),
+              vl + (w * VI + n) * 1024);
+      } else {
+        const int j = (vpiece0 ^ vswizzle<TK>(n * RV)) / 2;
+        int id = r.ids[0];
 #pragma unroll
-        for (int q = 1; q < NP; ++q) id = j == q ? ids[q] : id;
-        dma16(kbase + id * page_bytes + ((t + 16 * j) & (page - 1)) * KROW + koff[n], kl + (w * KI + n) * 1024);
-      }
-#pragma unroll
-      for (int n = 0; n < VI; ++n) {
-        const int j = vpiece[n] / 2;
-        int id = ids[0];
-#pragma unroll
-        for (int q = 1; q < NP; ++q) id = j == q ? ids[q] : id;
-        dma16(vbase + id * page_bytes + ((t + 16 * j) & (page - 1)) * 2 + voff[n], vl + (w * VI + n) * 1024);
+        for (int q = 1; q < NP; ++q) id = j == q ? r.ids[q] : id;
+        dma16(vbase + id * page_bytes + ((r.t + 16 * j) & (page - 1)) * 2 + n * RV * page * 2 + voff0,
+              vl + (w * VI + n) * 1024);
       }
     }
-    return held;
   };
   constexpr uint32_t kAll = (1u << NP) - 1;
   auto has = [&](uint32_t held, int group) { return ((held >> (ONE ? 0 : group)) & 1u) != 0; };
 
   // Where this lane reads: K row of score row c, V row of dimension c.
   const int krow = 16 * (c / 16) + 8 * ((c / 4) % 2) + 4 * ((c / 8) % 2) + c % 4;
-  const int kswz = D == 64 ? (krow >> 1) & 7 : krow & 15;
-  const int vswz = TK == 64 ? (c >> 1) & 7 : (c >> 2) & 3;
+  const int kswz = kswizzle<D>(krow), vswz = vswizzle<TK>(c);
 
   auto sees = [&](int tok, bool held) { return held && tok <= qpos && (tok > qpos - a.window || tok < a.sinks); };
   // Whether rows at positions [lo, hi] all see the whole tile, and every page of it is there.
@@ -207,69 +217,66 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     return t + TK - 1 <= lo && (t > hi - a.window || t + TK <= a.sinks) && held == kAll;
   };
   const int blk_lo = sr.pos0 + p0 / a.group, blk_hi = sr.pos0 + (min(p0 + 128, np) - 1) / a.group;
-  auto step = [&](int t, uint32_t held, const uint8_t* kl, const uint8_t* vl) {
-    if (!work || t > pos_hi) return;                                           // no row of the wave sees any of it
-    if (t >= a.sinks && t + TK - 1 <= pos_lo - a.window) return;
-    // Operands are read four at a time, one group ahead of the products (more in flight take registers that the sums need).
-    auto kread = [&](int f) {
-      return *reinterpret_cast<const ss_u32x4*>(kl + (krow + 32 * (f / KS)) * KROW + 16 * ((2 * (f % KS) + h) ^ kswz));
-    };
-    auto vread = [&](int d, int nk) {
-      return *reinterpret_cast<const ss_u32x4*>(vl + (c + 32 * d) * VROW + 16 * ((2 * nk + h) ^ vswz));
-    };
-    f32x16 x[ST];
-    ss_u32x4 fr[2][4];
+  auto kread = [&](const uint8_t* kl, int f) {
+    return *reinterpret_cast<const ss_u32x4*>(kl + (krow + 32 * (f / KS)) * KROW + 16 * ((2 * (f % KS) + h) ^ kswz));
+  };
+  auto vread = [&](const uint8_t* vl, int d, int nk) {
+    return *reinterpret_cast<const ss_u32x4*>(vl + (c + 32 * d) * VROW + 16 * ((2 * nk + h) ^ vswz));
+  };
+  // Whether the wave has a row that sees some of the tile.
+  auto active = [&](int t) { return work && t <= pos_hi && (t < a.sinks || t + TK - 1 > pos_lo - a.window); };
+  auto scores = [&](const uint8_t* kl, f32x16 (&y)[ST]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fr[0][j] = kread(j);
+    for (int n = 0; n < ST; ++n) y[n] = f32x16{};
 #pragma unroll
-    for (int n = 0; n < ST; ++n) x[n] = f32x16{};
+    for (int f = 0; f < ST * KS; ++f) y[f / KS] = mfma32<T>(kread(kl, f), qf[f % KS], y[f / KS]);
+  };
+  auto mask = [&](const Tile& r, f32x16 (&x)[ST]) {
+    const int t = r.t;
+    const uint32_t held = r.held;
+    if (whole_tile(t, pos_lo, pos_hi, held)) return;
+    // This lane's token e of score tile n is seen where lo < 32 n + 16 (e / 8) + e % 8 <= hi. The comparisons are kept in
+    // small groups: all at once they would take more scalar registers than there are.
+    const int hi = qpos - t - 8 * h, lo = hi - a.window;
+    if (t >= a.sinks && held == kAll) {
 #pragma unroll
-    for (int g = 0; g < ST * KS / 4; ++g) {
-      if (g + 1 < ST * KS / 4) {
+      for (int n = 0; n < ST; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) fr[(g + 1) % 2][j] = kread(4 * g + 4 + j);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[(4 * g + j) / KS] = mfma32<T>(fr[g % 2][j], qf[(4 * g + j) % KS], x[(4 * g + j) / KS]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    const bool whole = whole_tile(t, pos_lo, pos_hi, held);
-    if (!whole) {
-      // This lane's token e of score tile n is seen where lo < 32 n + 16 (e / 8) + e % 8 <= hi. The comparisons are kept in
-      // small groups: all at once they would take more scalar registers than there are.
-      const int hi = qpos - t - 8 * h, lo = hi - a.window;
-      if (t >= a.sinks && held == kAll) {
-#pragma unroll
-        for (int n = 0; n < ST; ++n)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int off = 32 * n + 16 * (e / 8) + e % 8;
-            x[n][e] = off <= hi && off > lo ? x[n][e] : kNegInf;
-            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-          }
-      } else {
-#pragma unroll
-        for (int n = 0; n < ST; ++n)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int off = 32 * n + 16 * (e / 8) + e % 8;
-            const bool see = has(held, 2 * n + e / 8) && off <= hi && (off > lo || off < a.sinks - t - 8 * h);
-            x[n][e] = see ? x[n][e] : kNegInf;
-            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-          }
-      }
-      if (held != kAll) {
-        // a page that is missing where a row of the wave sees a token
-        bool miss = false;
-#pragma unroll
-        for (int j = 0; j < TK / 16; ++j) {
-          const int first = t + 16 * j;
-          miss |= !has(held, j) && first <= qpos && (first + 15 > qpos - a.window || first < a.sinks);
+        for (int e = 0; e < 16; ++e) {
+          const int off = 32 * n + 16 * (e / 8) + e % 8;
+          x[n][e] = off <= hi && off > lo ? x[n][e] : kNegInf;
+          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
-        if (miss) ss_raise(a.err, SS_ERR_PAGE);
-      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < ST; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int off = 32 * n + 16 * (e / 8) + e % 8;
+          const bool see = has(held, 2 * n + e / 8) && off <= hi && (off > lo || off < a.sinks - t - 8 * h);
+          x[n][e] = see ? x[n][e] : kNegInf;
+          if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
     }
+    if (held != kAll) {
+      // a page that is missing where a row of the wave sees a token
+      bool miss = false;
+#pragma unroll
+      for (int j = 0; j < TK / 16; ++j) {
+        const int first = t + 16 * j;
+        miss |= !has(held, j) && first <= qpos && (first + 15 > qpos - a.window || first < a.sinks);
+      }
+      if (miss) raise_bit(a.err, SS_ERR_PAGE);
+    }
+  };
+  // The softmax and value product of tile r, whose scores are x, with the scores of the next tile (in kl) worked out
+  // between into y: the matrix unit has them while the exponentials take the vector unit.
+  auto step = [&](const Tile& r, const uint8_t* kl, const uint8_t* vl, f32x16 (&x)[ST], f32x16 (&y)[ST]) {
+    if (!active(r.t)) {
+      scores(kl, y);
+      return;
+    }
+    mask(r, x);
     float mx = x[0][0];
 #pragma unroll
     for (int n = 0; n < ST; ++n)
@@ -288,34 +295,47 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     }
     const float mu = m == kNegInf ? 0.f : m;
     ss_u32x4 pf[ST][2];
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    float part[2] = {0.f, 0.f};
+    // The operands of a product are read AHEAD products before it, those of the first value products beside the last of
+    // the scores; PER scores of x are worked on beside each product of y.
+    constexpr int NK = ST * KS, PER = 16 * ST / NK, NV = DT * 2 * ST, AHEAD = 4, RING = AHEAD + 1;
+    ss_u32x4 fr[RING];
+    auto fetch = [&](int f) {
+      if (f < NK)
+        fr[f % RING] = kread(kl, f);
+      else if (f < NK + NV)
+        fr[f % RING] = vread(vl, (f - NK) / (2 * ST), (f - NK) % (2 * ST));
+    };
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): no scalar load is in flight, so the reads below are waited for by count
 #pragma unroll
-    for (int n = 0; n < ST; ++n)
+    for (int f = 0; f < AHEAD; ++f) fetch(f);
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float q0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], a.scale, -mu));
-        const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e + 1], a.scale, -mu));
-        part[e % 4] += q0;
-        part[e % 4 + 1] += q1;
-        pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
+    for (int n = 0; n < ST; ++n) y[n] = f32x16{};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < NK; ++f) {
+      fetch(f + AHEAD);
+      y[f / KS] = mfma32<T>(fr[f % RING], qf[f % KS], y[f / KS]);
+      if (PER > 1 || f % 2 == 0) {
+#pragma unroll
+        for (int q = f * PER; q < f * PER + (PER > 1 ? PER : 2); q += 2) {
+          const int n = q / 16, e = q % 16;
+          const float q0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], a.scale, -mu));
+          const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e + 1], a.scale, -mu));
+          part[q / 2 % 2] += q0;
+          part[q / 2 % 2] += q1;
+          pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
+        }
       }
-    l += (part[0] + part[1]) + (part[2] + part[3]);
-    constexpr int NV = DT * 2 * ST;
+      if (f % 2) __builtin_amdgcn_sched_barrier(0);
+    }
+    l += part[0] + part[1];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fr[0][j] = vread(j / (2 * ST), j % (2 * ST));
-#pragma unroll
-    for (int g = 0; g < NV / 4; ++g) {
-      if (g + 1 < NV / 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) fr[(g + 1) % 2][j] = vread((4 * g + 4 + j) / (2 * ST), (4 * g + 4 + j) % (2 * ST));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = (4 * g + j) / (2 * ST), nk = (4 * g + j) % (2 * ST);
-        acc[d] = mfma32<T>(fr[g % 2][j], pf[nk / 2][nk % 2], acc[d]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int f = NK; f < NK + NV; ++f) {
+      const int d = (f - NK) / (2 * ST), nk = (f - NK) % (2 * ST);
+      fetch(f + AHEAD);
+      acc[d] = mfma32<T>(fr[f % RING], pf[nk / 2][nk % 2], acc[d]);
+      if (f % 2) __builtin_amdgcn_sched_barrier(0);
     }
   };
   // In a tile that some row of the workgroup does not see whole, non-finite values are taken out of the stage before any
@@ -344,25 +364,32 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   };
 
   if (tid == 0) odd = 0;  // before the first tile's barrier
-  int t = next_tile(t_begin);
-  uint32_t held = t < t_end ? load(t, k0, v0) : 0;
-  while (t < t_end) {
-    int u = next_tile(t + TK);
-    uint32_t next = 0;
-    sync();  // the tile at t is in stage 0, and stage 1 is free: every wave has finished with it
-    if (u < t_end) next = load(u, k1, v1);
-    clean(t, held, v0);
-    step(t, held, k0, v0);
-    t = u;
-    held = next;
-    if (t >= t_end) break;
-    u = next_tile(t + TK);
+  // Tile i: keys in stage i % 2 from two steps before its softmax, values from one.
+  f32x16 x[ST], y[ST];
+  Tile r0 = tile_at(next_tile(t_begin)), r1 = tile_at(next_tile(r0.t + TK));
+  if (r0.t < t_end) {
+    load_k(r0, k0);
+    if (r1.t < t_end) load_k(r1, k1);
+    load_v(r0, v0);
     sync();
-    if (u < t_end) next = load(u, k0, v0);
-    clean(t, held, v1);
-    step(t, held, k1, v1);
-    t = u;
-    held = next;
+    scores(k0, x);
+  }
+  while (r0.t < t_end) {
+    sync();  // keys of r1 and values of r0 are there, the other stages free: every wave has finished with them
+    Tile r2 = tile_at(next_tile(r1.t + TK));
+    if (r2.t < t_end) load_k(r2, k0);
+    if (r1.t < t_end) load_v(r1, v1);
+    clean(r0.t, r0.held, v0);
+    step(r0, k1, v0, x, y);
+    if (r1.t >= t_end) break;
+    sync();
+    r0 = tile_at(next_tile(r2.t + TK));
+    if (r0.t < t_end) load_k(r0, k1);
+    if (r2.t < t_end) load_v(r2, v0);
+    clean(r1.t, r1.held, v1);
+    step(r1, k0, v1, y, x);
+    r1 = r0;
+    r0 = r2;
   }
   __syncthreads();
   const bool fix = work && odd;
@@ -400,11 +427,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   // Infinities and NaN that were taken out go to the columns that see them, by a product of ones in their places with ones
   // for the tokens seen; each lane adds to what it wrote itself.
 #pragma unroll 1
-  for (t = next_tile(t_begin); t < t_end; t = next_tile(t + TK)) {
-    held = 0;
-#pragma unroll
-    for (int j = 0; j < NP; ++j) held |= page_id(t, j) >= 0 ? 1u << j : 0u;
-    if (whole_tile(t, blk_lo, blk_hi, held)) continue;
+  for (int t = next_tile(t_begin); t < t_end; t = next_tile(t + TK)) {
+    if (whole_tile(t, blk_lo, blk_hi, tile_at(t).held)) continue;
 #pragma unroll 1
     for (int nk = 0; nk < 2 * ST; ++nk) {
       const int first = t + 16 * nk + 8 * h, id = page_id(t, nk);
@@ -436,27 +460,33 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   }
 }
 
-template <class T, int D, int DV, int TK>
+// Tiles of 64 tokens where a page holds them, else of 32 (and of 256 dimensions always: registers).
+template <class T, int D, int DV>
 void launch_prompt(const AttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs * (D / DV)));
-  if ((1 << a.page_shift) >= TK)
-    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, TK, true>), grid, dim3(256), 0, st, a);
+  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs * attn_prompt_parts(D, a.page_shift)));
+  if (a.page_shift >= 6 && D < 256)
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, D < 256 ? 64 : 32, true>), grid, dim3(256), 0, st, a);
+  else if (a.page_shift >= 5)
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, 32, true>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, TK, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, D < 256 ? DV : 64, 32, false>), grid, dim3(256), 0, st, a);
 }
 
 template <class T>
 hipError_t launch_prompt_of(const AttnArgs& a, int dim, hipStream_t st) {
   if (dim == 64)
-    launch_prompt<T, 64, 64, 64>(a, st);
+    launch_prompt<T, 64, 64>(a, st);
   else if (dim == 128)
-    launch_prompt<T, 128, 128, 64>(a, st);
+    launch_prompt<T, 128, 128>(a, st);
   else
-    launch_prompt<T, 256, 128, 32>(a, st);
+    launch_prompt<T, 256, 128>(a, st);
   return hipGetLastError();
 }
 
 }  // namespace
+
+// Workgroups that share the output dimensions of a row tile (a quarter each where pages of 16 tokens take more registers).
+int attn_prompt_parts(int dim, int page_shift) { return dim < 256 ? 1 : page_shift >= 5 ? 2 : 4; }
 
 hipError_t launch_attn_prompt(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {
   return fp16 ? launch_prompt_of<Fp16>(a, dim, st) : launch_prompt_of<Bf16>(a, dim, st);

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
     id = gp(a.table)[(int64_t)s * a.width + (first >> a.page_shift)];
     if ((uint32_t)id >= (uint64_t)a.n_pages) {
       id = -1;
-      if (tid == 0) ss_raise(a.err, SS_ERR_PAGE);
+      if (tid == 0) raise_bit(a.err, SS_ERR_PAGE);
     }
   }
   const int off = first & (page - 1);

@@ -250,8 +250,9 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
   if (a.window < (1 << 30)) seen = std::min<int64_t>(cap, (int64_t)a.window + max_rows + a.sinks);
   int64_t chunk = cap, slots = 1;
   const int64_t units = (int64_t)p->seqs * p->kv_heads;
+  const int parts_of_dim = ss::attn_prompt_parts(p->dim, shift);
   if (*prompt) {
-    const int64_t want = 512 / std::max<int64_t>(units * a.tiles * (p->dim == 256 ? 2 : 1), 1);
+    const int64_t want = 512 / std::max<int64_t>(units * a.tiles * parts_of_dim, 1);
     if (want > 1 && seen > 512) chunk = std::max<int64_t>((seen + want - 1) / want, 512);
     chunk = (chunk + 127) / 128 * 128;
   } else {
@@ -265,10 +266,10 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
                                 (a.window + std::max(max_rows, kFewRows) + chunk - 2) / chunk + 1);
   if (*prompt && chunk >= seen) slots = 1;
   // Two workgroups fit a CU: of at most 512, the second 256 go to the CUs of the first, the lightest to the heaviest.
-  const int64_t per_tile = units * slots * (p->dim == 256 ? 2 : 1), all = per_tile * a.tiles;
+  const int64_t per_tile = units * slots * parts_of_dim, all = per_tile * a.tiles;
   a.rising = *prompt && all > 256 && all <= 512 ? (int)((all - 256) / per_tile) : 0;
   a.slots = (int)slots;
-  if (2 * slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
+  if (parts_of_dim * slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
     return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
   const int64_t parts = slots > 1 ? slots * p->rows * p->heads : 0;
   *ws = (parts * p->dim * 4 + 255) / 256 * 256 + parts * 8;

@@ -120,10 +120,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int p = p0 + 32 * w + c, i = p / a.group;
   const bool in = p < np;
   const int qpos = in ? sr.pos0 + i : -1;
-  // positions of the wave's first and last row; a wave past the rows has none and skips the products
-  const int wp0 = p0 + 32 * w;
-  const bool work = wp0 < np;
-  const int pos_lo = sr.pos0 + wp0 / a.group, pos_hi = sr.pos0 + (min(wp0 + 32, np) - 1) / a.group;
   ss_u32x4 qf[KS];
   {
     const uint16_t* qp = a.q + (int64_t)(sr.r0 + (in ? i : 0)) * a.q_row +
@@ -136,16 +132,19 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float m = kNegInf, l = 0.f;
 
-  // Pages of a tile's 16-token groups (one where the tile lies in one page), -1 where there is none. The kernel does not write
-  // the table, so these are scalar loads, which do not stand behind the stages' loads in the vector memory queue.
+  // Pages of a tile's 16-token groups (one where the tile lies in one page), -1 where there is none: the table's entries 64 at
+  // a time in one register, an entry a lane. (Scalar loads of single entries cost some 500 cycles of every tile.)
   constexpr int NP = ONE ? 1 : TK / 16;
-  const __attribute__((address_space(4))) int32_t* tab =
-      (const __attribute__((address_space(4))) int32_t*)(a.table + (int64_t)s * a.width);
-  const uint32_t n_pages = (uint32_t)a.n_pages;
+  const int32_t* tab = a.table + (int64_t)s * a.width;
+  int first_entry = -64, entries = -1;
   auto page_id = [&](int t, int j) {
     const int at = (t + 16 * j) >> a.page_shift;
-    const int id = tab[min(at, a.width - 1)];
-    return at < a.width && (uint32_t)id < n_pages ? id : -1;
+    if ((uint32_t)(at - first_entry) >= 64u) {
+      first_entry = at;
+      entries = at + lane < a.width ? gp(tab)[at + lane] : -1;
+      entries = (uint32_t)entries < (uint32_t)a.n_pages ? entries : -1;
+    }
+    return __builtin_amdgcn_readlane(entries, at - first_entry);
   };
   const int64_t page_bytes = (int64_t)a.kv_heads * page * D * 2;
   const char* kbase = reinterpret_cast<const char*>(a.k) + (int64_t)kh * page * D * 2;
@@ -182,18 +181,16 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       int id = r.ids[0];
 #pragma unroll
       for (int q = 1; q < NP; ++q) id = j == q ? r.ids[q] : id;
-      dma16(kbase + id * page_bytes + ((r.t + 16 * j) & (page - 1)) * KROW + n * RK * KROW +
-                (koff0 ^ (16 * kswizzle<D>(n * RK))),
-            kl + (w * KI + n) * 1024);
+      const char* at = kbase + id * page_bytes + (((r.t + 16 * j) & (page - 1)) + n * RK) * KROW;
+      dma16(at + (koff0 ^ (16 * kswizzle<D>(n * RK))), kl + (w * KI + n) * 1024);
     }
   };
   auto load_v = [&](const Tile& r, uint8_t* vl) {
 #pragma unroll
     for (int n = 0; n < VI; ++n) {
       if constexpr (ONE) {
-        dma16(vbase + r.ids[0] * page_bytes + (r.t & (page - 1)) * 2 + n * RV * page * 2 +
-                  (voff0 ^ (16 * vswizzle<TK>(n * RV))),
-              vl + (w * VI + n) * 1024);
+        const char* at = vbase + r.ids[0] * page_bytes + ((r.t & (page - 1)) + n * RV * page) * 2;
+        dma16(at + (voff0 ^ (16 * vswizzle<TK>(n * RV))), vl + (w * VI + n) * 1024);
       } else {
         const int j = (vpiece0 ^ vswizzle<TK>(n * RV)) / 2;
         int id = r.ids[0];
@@ -212,19 +209,16 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int kswz = kswizzle<D>(krow), vswz = vswizzle<TK>(c);
 
   auto sees = [&](int tok, bool held) { return held && tok <= qpos && (tok > qpos - a.window || tok < a.sinks); };
-  // Whether rows at positions [lo, hi] all see the whole tile, and every page of it is there.
-  auto whole_tile = [&](int t, int lo, int hi, uint32_t held) {
-    return t + TK - 1 <= lo && (t > hi - a.window || t + TK <= a.sinks) && held == kAll;
-  };
+  // A plain tile: every row of the workgroup sees all of it. The tiles that hold first tokens only are taken as not plain.
   const int blk_lo = sr.pos0 + p0 / a.group, blk_hi = sr.pos0 + (min(p0 + 128, np) - 1) / a.group;
+  const int plain_a = blk_hi - a.window + 1, plain_b = blk_lo - TK + 1;
+  auto plain = [&](const Tile& r) { return r.t >= plain_a && r.t <= plain_b && r.held == kAll; };
   auto kread = [&](const uint8_t* kl, int f) {
     return *reinterpret_cast<const ss_u32x4*>(kl + (krow + 32 * (f / KS)) * KROW + 16 * ((2 * (f % KS) + h) ^ kswz));
   };
   auto vread = [&](const uint8_t* vl, int d, int nk) {
     return *reinterpret_cast<const ss_u32x4*>(vl + (c + 32 * d) * VROW + 16 * ((2 * nk + h) ^ vswz));
   };
-  // Whether the wave has a row that sees some of the tile.
-  auto active = [&](int t) { return work && t <= pos_hi && (t < a.sinks || t + TK - 1 > pos_lo - a.window); };
   auto scores = [&](const uint8_t* kl, f32x16 (&y)[ST]) {
 #pragma unroll
     for (int n = 0; n < ST; ++n) y[n] = f32x16{};
@@ -234,7 +228,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   auto mask = [&](const Tile& r, f32x16 (&x)[ST]) {
     const int t = r.t;
     const uint32_t held = r.held;
-    if (whole_tile(t, pos_lo, pos_hi, held)) return;
     // This lane's token e of score tile n is seen where lo < 32 n + 16 (e / 8) + e % 8 <= hi. The comparisons are kept in
     // small groups: all at once they would take more scalar registers than there are.
     const int hi = qpos - t - 8 * h, lo = hi - a.window;
@@ -269,14 +262,30 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       if (miss) raise_bit(a.err, SS_ERR_PAGE);
     }
   };
+  // In a tile that is not plain non-finite values are taken out of the stage before any
+  // wave uses it; `odd` says that there were any, and they are dealt with after the last tile.
+  auto clean = [&](uint8_t* vl) {
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      ss_u32x4* at = reinterpret_cast<ss_u32x4*>(vl + (n * 256 + tid) * 16);
+      const ss_u32x4 x = *at;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bad |= nonfinite2<T>(x[j]);
+      if (bad) {
+        *at = parts_of<T>(x, -1);
+        odd = 1;
+      }
+    }
+    local_barrier();
+  };
   // The softmax and value product of tile r, whose scores are x, with the scores of the next tile (in kl) worked out
   // between into y: the matrix unit has them while the exponentials take the vector unit.
-  auto step = [&](const Tile& r, const uint8_t* kl, const uint8_t* vl, f32x16 (&x)[ST], f32x16 (&y)[ST]) {
-    if (!active(r.t)) {
-      scores(kl, y);
-      return;
+  auto step = [&](const Tile& r, const uint8_t* kl, uint8_t* vl, f32x16 (&x)[ST], f32x16 (&y)[ST]) {
+    if (!plain(r)) {
+      clean(vl);
+      mask(r, x);
     }
-    mask(r, x);
     float mx = x[0][0];
 #pragma unroll
     for (int n = 0; n < ST; ++n)
@@ -306,7 +315,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       else if (f < NK + NV)
         fr[f % RING] = vread(vl, (f - NK) / (2 * ST), (f - NK) % (2 * ST));
     };
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): no scalar load is in flight, so the reads below are waited for by count
 #pragma unroll
     for (int f = 0; f < AHEAD; ++f) fetch(f);
 #pragma unroll
@@ -338,24 +346,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       if (f % 2) __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // In a tile that some row of the workgroup does not see whole, non-finite values are taken out of the stage before any
-  // wave uses it; `odd` says that there were any, and they are dealt with after the last tile.
-  auto clean = [&](int t, uint32_t held, uint8_t* vl) {
-    if (whole_tile(t, blk_lo, blk_hi, held)) return;
-#pragma unroll
-    for (int n = 0; n < VI; ++n) {
-      ss_u32x4* at = reinterpret_cast<ss_u32x4*>(vl + (n * 256 + tid) * 16);
-      const ss_u32x4 x = *at;
-      bool bad = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) bad |= nonfinite2<T>(x[j]);
-      if (bad) {
-        *at = parts_of<T>(x, -1);
-        odd = 1;
-      }
-    }
-    local_barrier();
-  };
   auto sync = [&]() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of the stage have landed
@@ -379,20 +369,18 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     Tile r2 = tile_at(next_tile(r1.t + TK));
     if (r2.t < t_end) load_k(r2, k0);
     if (r1.t < t_end) load_v(r1, v1);
-    clean(r0.t, r0.held, v0);
     step(r0, k1, v0, x, y);
     if (r1.t >= t_end) break;
     sync();
     r0 = tile_at(next_tile(r2.t + TK));
     if (r0.t < t_end) load_k(r0, k1);
     if (r2.t < t_end) load_v(r2, v0);
-    clean(r1.t, r1.held, v1);
     step(r1, k0, v1, y, x);
     r1 = r0;
     r0 = r2;
   }
   __syncthreads();
-  const bool fix = work && odd;
+  const bool fix = odd;
   l += other_half(l, h);
   const int64_t at = (int64_t)(sr.r0 + i) * a.heads + kh * a.group + (p - i * a.group);
   const int64_t pa = (int64_t)slot * a.rows * a.heads + at;
@@ -428,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   // for the tokens seen; each lane adds to what it wrote itself.
 #pragma unroll 1
   for (int t = next_tile(t_begin); t < t_end; t = next_tile(t + TK)) {
-    if (whole_tile(t, blk_lo, blk_hi, tile_at(t).held)) continue;
+    if (plain(tile_at(t))) continue;
 #pragma unroll 1
     for (int nk = 0; nk < 2 * ST; ++nk) {
       const int first = t + 16 * nk + 8 * h, id = page_id(t, nk);

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
-  float m = kNegInf, l = 0.f;
+  float m = kNegInf, l = 0.f, top = kNegInf;
 
   // Pages of a tile's 16-token groups (one where the tile lies in one page), -1 where there is none: the table's entries 64 at
   // a time in one register, an entry a lane. (Scalar loads of single entries cost some 500 cycles of every tile.)
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   int first_entry = -64, entries = -1;
   auto page_id = [&](int t, int j) {
     const int at = (t + 16 * j) >> a.page_shift;
-    if ((uint32_t)(at - first_entry) >= 64u) {
+    if (__builtin_expect((uint32_t)(at - first_entry) >= 64u, 0)) {
       first_entry = at;
       entries = at + lane < a.width ? gp(tab)[at + lane] : -1;
       entries = (uint32_t)entries < (uint32_t)a.n_pages ? entries : -1;
@@ -174,9 +174,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     }
     return r;
   };
-  auto load_k = [&](const Tile& r, uint8_t* kl) {
-#pragma unroll
-    for (int n = 0; n < KI; ++n) {
+  auto load_k = [&](const Tile& r, uint8_t* kl, int n) {
+    {
       const int j = ONE ? 0 : (w * KI + n) * (64 / KC) / 16;  // the load's 16-token group
       int id = r.ids[0];
 #pragma unroll
@@ -185,9 +184,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       dma16(at + (koff0 ^ (16 * kswizzle<D>(n * RK))), kl + (w * KI + n) * 1024);
     }
   };
-  auto load_v = [&](const Tile& r, uint8_t* vl) {
-#pragma unroll
-    for (int n = 0; n < VI; ++n) {
+  auto load_v = [&](const Tile& r, uint8_t* vl, int n) {
+    {
       if constexpr (ONE) {
         const char* at = vbase + r.ids[0] * page_bytes + ((r.t & (page - 1)) + n * RV * page) * 2;
         dma16(at + (voff0 ^ (16 * vswizzle<TK>(n * RV))), vl + (w * VI + n) * 1024);
@@ -279,20 +277,27 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     }
     local_barrier();
   };
-  // The softmax and value product of tile r, whose scores are x, with the scores of the next tile (in kl) worked out
-  // between into y: the matrix unit has them while the exponentials take the vector unit.
-  auto step = [&](const Tile& r, const uint8_t* kl, uint8_t* vl, f32x16 (&x)[ST], f32x16 (&y)[ST]) {
-    if (!plain(r)) {
-      clean(vl);
-      mask(r, x);
-    }
-    float mx = x[0][0];
+  auto max_of = [&](const f32x16 (&y)[ST]) {
+    float v = y[0][0];
 #pragma unroll
     for (int n = 0; n < ST; ++n)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[n][e]);
-    mx = fmaxf(mx, other_half(mx, h)) * a.scale - T::kShift;
-    if (__any(mx > m + kLazy || (m == kNegInf && mx > kNegInf))) {
+      for (int e = 0; e < 16; ++e) v = fmaxf(v, y[n][e]);
+    return v;
+  };
+  // The softmax and value product of tile r, whose scores are x with the lane's largest one in `top`; between, the scores of
+  // the next tile (in kl) are worked out into y: the matrix unit has them while the exponentials take the vector unit.
+  // The loads of the keys of rk (to kn) and the values of rv (to vn) go out one at a time beside the products: all at once
+  // they hold up the wave for as long as the memory path takes them in.
+  auto step = [&](const Tile& r, const uint8_t* kl, uint8_t* vl, f32x16 (&x)[ST], f32x16 (&y)[ST], const Tile& rk,
+                  uint8_t* kn, const Tile& rv, uint8_t* vn) {
+    if (__builtin_expect(!plain(r), 0)) {
+      clean(vl);
+      mask(r, x);
+      top = max_of(x);
+    }
+    const float mx = fmaxf(top, other_half(top, h)) * a.scale - T::kShift;
+    if (__builtin_expect(__any(mx > m + kLazy || (m == kNegInf && mx > kNegInf)), 0)) {
       const float mn = fmaxf(m, mx);
       const float f = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);  // nothing summed yet (or NaN) where m is -inf
       l *= f;
@@ -335,14 +340,19 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
           pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
         }
       }
+      if (f % (NK / KI) == 1) load_k(rk, kn, f / (NK / KI));
       if (f % 2) __builtin_amdgcn_sched_barrier(0);
     }
     l += part[0] + part[1];
+    top = y[0][0];
 #pragma unroll
     for (int f = NK; f < NK + NV; ++f) {
       const int d = (f - NK) / (2 * ST), nk = (f - NK) % (2 * ST);
       fetch(f + AHEAD);
       acc[d] = mfma32<T>(fr[f % RING], pf[nk / 2][nk % 2], acc[d]);
+#pragma unroll
+      for (int q = (f - NK) * 16 * ST / NV; q < (f - NK + 1) * 16 * ST / NV; ++q) top = fmaxf(top, y[q / 16][q % 16]);
+      if ((f - NK) % (NV / VI) == 1) load_v(rv, vn, (f - NK) / (NV / VI));
       if (f % 2) __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -354,31 +364,33 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   };
 
   if (tid == 0) odd = 0;  // before the first tile's barrier
-  // Tile i: keys in stage i % 2 from two steps before its softmax, values from one.
+  // Tile i: keys in stage i % 2 from two steps before its softmax, values from one. Loads for tiles past the last one are
+  // issued too (of page 0 where there is none): what they bring is not read.
   f32x16 x[ST], y[ST];
   Tile r0 = tile_at(next_tile(t_begin)), r1 = tile_at(next_tile(r0.t + TK));
   if (r0.t < t_end) {
-    load_k(r0, k0);
-    if (r1.t < t_end) load_k(r1, k1);
-    load_v(r0, v0);
+#pragma unroll
+    for (int n = 0; n < KI; ++n) load_k(r0, k0, n);
+#pragma unroll
+    for (int n = 0; n < KI; ++n) load_k(r1, k1, n);
+#pragma unroll
+    for (int n = 0; n < VI; ++n) load_v(r0, v0, n);
     sync();
     scores(k0, x);
+    top = max_of(x);
   }
   while (r0.t < t_end) {
     sync();  // keys of r1 and values of r0 are there, the other stages free: every wave has finished with them
-    Tile r2 = tile_at(next_tile(r1.t + TK));
-    if (r2.t < t_end) load_k(r2, k0);
-    if (r1.t < t_end) load_v(r1, v1);
-    step(r0, k1, v0, x, y);
+    const Tile r2 = tile_at(next_tile(r1.t + TK));
+    step(r0, k1, v0, x, y, r2, k0, r1, v1);
     if (r1.t >= t_end) break;
     sync();
-    r0 = tile_at(next_tile(r2.t + TK));
-    if (r0.t < t_end) load_k(r0, k1);
-    if (r2.t < t_end) load_v(r2, v0);
-    step(r1, k0, v1, y, x);
-    r1 = r0;
+    const Tile r3 = tile_at(next_tile(r2.t + TK));
+    step(r1, k0, v1, y, x, r3, k1, r2, v0);
     r0 = r2;
+    r1 = r3;
   }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // no load into LDS outlives the wave
   __syncthreads();
   const bool fix = odd;
   l += other_half(l, h);

@@ -340,7 +340,13 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
           pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
         }
       }
-      if (f % (NK / KI) == 1) load_k(rk, kn, f / (NK / KI));
+      constexpr int EVERY = NK / (KI + VI) < 1 ? 1 : NK / (KI + VI);
+      if (f % EVERY == EVERY - 1) {
+        if (f / EVERY < KI)
+          load_k(rk, kn, f / EVERY);
+        else if (f / EVERY < KI + VI)
+          load_v(rv, vn, f / EVERY - KI);
+      }
       if (f % 2) __builtin_amdgcn_sched_barrier(0);
     }
     l += part[0] + part[1];
@@ -352,7 +358,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       acc[d] = mfma32<T>(fr[f % RING], pf[nk / 2][nk % 2], acc[d]);
 #pragma unroll
       for (int q = (f - NK) * 16 * ST / NV; q < (f - NK + 1) * 16 * ST / NV; ++q) top = fmaxf(top, y[q / 16][q % 16]);
-      if ((f - NK) % (NV / VI) == 1) load_v(rv, vn, (f - NK) / (NV / VI));
       if (f % 2) __builtin_amdgcn_sched_barrier(0);
     }
   };

@@ -39,14 +39,15 @@ SS_DEV float max_over_quads(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^
   return fmaxf(ss_uf(lo), ss_uf(hi));
 }
 
-template <class T, int D, int NT>
-__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
+template <class T, int D, int NT, int W>
+__global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16;
-  constexpr bool kQLds = NT * KS > 8;  // more than 32 registers of queries stay in LDS, one copy for the four waves
+  constexpr bool kQLds = NT * KS > 8;  // more than 32 registers of queries stay in LDS, one copy for the waves
+  constexpr int VH = NT * D > 256 ? 2 : 1;  // parts that a tile's values are loaded in: the second where the keys were
   __shared__ ss_u32x4 q_lds[kQLds ? NT * KS : 1][64];
   __shared__ int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
-  __shared__ __attribute__((aligned(16))) float join_o[4][16][D + 4];
-  __shared__ float join_m[4][NT][16], join_l[4][NT][16];
+  __shared__ __attribute__((aligned(16))) float join_o[W][16][D + 4];
+  __shared__ float join_m[W][NT][16], join_l[W][NT][16];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   int b = blockIdx.x;
@@ -56,25 +57,31 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   b /= a.tiles;
   const int h = b % a.kv_heads, s = b / a.kv_heads;
   const int page = 1 << a.page_shift;
+  // Without a window the chunk is the slot, and its pages are asked for before the sequence's length is known.
+  const bool all = a.window >= (1 << 30);
+  const int32_t* tab = a.table + (int64_t)s * a.width;
+  auto entry = [&](int t) { return gp(tab)[min(t >> a.page_shift, a.width - 1)]; };
+  int early = -1;
+  if (all && 8 * tid < a.chunk) early = entry(slot * a.chunk + 8 * tid);
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width * page, a.err);
   const int p0 = tile * NT * 16, np = sr.n * a.group;  // packed rows [p0, min(p0 + 16 NT, np))
   if (p0 >= np) return;                                // whole workgroup, before any barrier
   const int i0 = p0 / a.group, i1 = (min(p0 + NT * 16, np) - 1) / a.group;
-  const Seen sn = seen_tokens(sr.pos0 + i0, sr.pos0 + i1, sr.end, a.window, a.sinks);
+  const int pos_lo = sr.pos0 + i0, pos_hi = sr.pos0 + i1;
+  const Seen sn = seen_tokens(pos_lo, pos_hi, sr.end, a.window, a.sinks);
   // Slots cover the chunks that hold first tokens, then those from the window's on.
   const int sc = (sn.s_end + a.chunk - 1) / a.chunk;
   const int wc = max(sn.w_begin / a.chunk, sc);
   const int ch = slot < sc ? slot : wc + slot - sc;
   const int t_begin = ch * a.chunk, t_end = min(t_begin + a.chunk, sn.end);
-  const bool empty = t_begin >= t_end;
-  if (empty && a.slots > 1) return;  // the join reads no further than the last token's chunk
+  if (t_begin >= t_end && a.slots > 1) return;  // the join reads no further than the last token's chunk
 
-  for (int j = tid; j < a.chunk / 8; j += 256) {
-    const int t = t_begin + 8 * j, at = t >> a.page_shift;
+  for (int j = tid; j < a.chunk / 8; j += 64 * W) {
+    const int t = t_begin + 8 * j;
     int id = -1;
     if (t < t_end) {
-      id = gp(a.table)[(int64_t)s * a.width + at];
-      if ((uint32_t)id >= (uint64_t)a.n_pages) {
+      id = all && j == tid ? early : entry(t);
+      if ((uint32_t)id >= (uint32_t)a.n_pages) {
         id = -1;
         if (t < sn.s_end || t + 8 > sn.w_begin) raise_bit(a.err, SS_ERR_PAGE);
       }
@@ -93,7 +100,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if constexpr (kQLds) {
-        if (((n * KS + ks) & 3) == w) q_lds[n * KS + ks][lane] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
+        if ((n * KS + ks) % W == w) q_lds[n * KS + ks][lane] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
       } else {
         qf[n][ks] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
       }
@@ -108,29 +115,42 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[n][d] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int pos_lo = sr.pos0 + i0, pos_hi = sr.pos0 + i1;
   __syncthreads();
 
   const int nt = (t_end - t_begin + 31) / 32;
+  auto unseen = [&](int t0) { return t0 >= sn.s_end && t0 + 32 <= sn.w_begin; };
+  // Whether every row of the workgroup sees all 32 tokens.
+  auto whole = [&](int t0, int idv) {
+    return t0 + 31 <= pos_lo && (t0 > pos_hi - a.window || t0 + 32 <= a.sinks) && __all(idv >= 0);
+  };
+  auto sees = [&](int tok, int pos, int idv) {
+    return idv >= 0 && tok <= pos && (tok > pos - a.window || tok < a.sinks);
+  };
+  auto values = [&](int t0, int idv) {
+    return a.v + ((int64_t)max(idv, 0) * a.kv_heads + h) * page * D + (int64_t)c * page + ((t0 + 8 * g) & (page - 1));
+  };
+  bool any_odd = false;
 #pragma unroll 1
-  for (int tt = w; tt < nt; tt += 4) {
+  for (int tt = w; tt < nt; tt += W) {
     const int t0 = t_begin + 32 * tt;
-    if (t0 >= sn.s_end && t0 + 32 <= sn.w_begin) continue;  // no row sees any of it
+    if (unseen(t0)) continue;
     const int idk = page_of[4 * tt + (c >> 2)], idv = page_of[4 * tt + g];
-    const int tk = (t0 + 8 * (c >> 2)) & (page - 1), tv = (t0 + 8 * g) & (page - 1);
+    const int tk = (t0 + 8 * (c >> 2)) & (page - 1);
     const uint16_t* kp = a.k + (((int64_t)max(idk, 0) * a.kv_heads + h) * page + tk + (c & 3)) * D + 8 * g;
-    const uint16_t* vp = a.v + ((int64_t)max(idv, 0) * a.kv_heads + h) * page * D + (int64_t)c * page + tv;
-    ss_u32x4 kf[2][KS], vf[DT];
+    const uint16_t* vp = values(t0, idv);
+    ss_u32x4 kf[2][KS], vf[DT / VH];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *(const SS_G ss_u32x4*)(kp + 4 * t * D + 32 * ks);
+    auto load_v = [&](int part) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vf[d] = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * d * page);
-    // Whether every row of the workgroup sees all 32 tokens.
-    const bool whole = t0 + 31 <= pos_lo && (t0 > pos_hi - a.window || t0 + 32 <= a.sinks) && __all(idv >= 0);
+      for (int d = 0; d < DT / VH; ++d) vf[d] = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (part * (DT / VH) + d) * page);
+    };
+    load_v(0);
+    __builtin_amdgcn_sched_barrier(0);
+    const bool part_seen = !whole(t0, idv);
     ss_u32x4 pf[NT];
-    uint32_t vis[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[8];
@@ -138,20 +158,14 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       for (int t = 0; t < 2; ++t) {
         ss_f32x4 sv = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) sv = T::mfma16(kf[t][ks], kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv);
+        for (int ks = 0; ks < KS; ++ks)
+          sv = T::mfma16(kf[t][ks], kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[4 * t + i] = sv[i];
       }
-      vis[n] = 0xFFu;
-      if (!whole) {
-        vis[n] = 0;
+      if (part_seen) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int tok = t0 + 8 * g + e;
-          const bool see = idv >= 0 && tok <= qpos[n] && (tok > qpos[n] - a.window || tok < a.sinks);
-          vis[n] |= see ? 1u << e : 0u;
-          x[e] = see ? x[e] : kNegInf;
-        }
+        for (int e = 0; e < 8; ++e) x[e] = sees(t0 + 8 * g + e, qpos[n], idv) ? x[e] : kNegInf;
       }
       float mx = x[0];
 #pragma unroll
@@ -177,43 +191,30 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[n][i] = T::pack(p[2 * i], p[2 * i + 1]);
     }
-    bool odd = false;
-    if (!whole) {
-      bool mine = false;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+    for (int part = 0; part < VH; ++part) {
+      if (part_seen) {
+        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine |= nonfinite2<T>(vf[d][i]);
-      odd = __any(mine);
-    }
-    if (odd) {
+        for (int d = 0; d < DT / VH; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll 1
-        for (int kind = 0; kind < 3; ++kind) {
-          const ss_u32x4 at = parts_of<T>(vf[d], kind);
-          const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+          for (int i = 0; i < 4; ++i) odd |= nonfinite2<T>(vf[d][i]);
+        if (__any(odd)) {
+          any_odd = true;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            ss_u32x4 ones;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              ones[i] = ((vis[n] >> (2 * i)) & 1u) * T::kOne | (((vis[n] >> (2 * i + 1)) & 1u) * T::kOne) << 16;
-            const ss_f32x4 hits = T::mfma16(at, ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][d][i] += hits[i] > 0.f ? add : 0.f;
-          }
+          for (int d = 0; d < DT / VH; ++d) vf[d] = parts_of<T>(vf[d], -1);
         }
-        vf[d] = parts_of<T>(vf[d], -1);
       }
+#pragma unroll
+      for (int d = 0; d < DT / VH; ++d)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          acc[n][part * (DT / VH) + d] = T::mfma16(vf[d], pf[n], acc[n][part * (DT / VH) + d]);
+      if (part + 1 < VH) load_v(part + 1);
     }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n][d] = T::mfma16(vf[d], pf[n], acc[n][d]);
   }
 
-  // The four waves' sums, weighted by how far each wave's maximum is below the largest.
+  // The waves' sums, weighted by how far each wave's maximum is below the largest.
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     l[n] = ss_rows_sum(l[n]);
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   for (int n = 0; n < NT; ++n) {
     float top = kNegInf;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) top = fmaxf(top, join_m[k][n][c]);
+    for (int k = 0; k < W; ++k) top = fmaxf(top, join_m[k][n][c]);
     const float f = m[n] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -236,23 +237,50 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       for (int i = 0; i < 4; ++i) o[i] = m[n] == kNegInf ? o[i] : o[i] * f;
       *reinterpret_cast<ss_f32x4*>(&join_o[w][c][16 * d + 4 * g]) = o;
     }
+    if (any_odd) {
+      // Infinities and NaN that were taken out of the wave's tiles, to the columns that see them.
+#pragma unroll 1
+      for (int tt = w; tt < nt; tt += W) {
+        const int t0 = t_begin + 32 * tt, idv = page_of[4 * tt + g];
+        if (unseen(t0) || whole(t0, idv)) continue;
+        const uint16_t* vp = values(t0, idv);
+        ss_u32x4 ones;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = t0 + 8 * g + 2 * i;
+          ones[i] = (sees(tok, qpos[n], idv) ? T::kOne : 0u) | (sees(tok + 1, qpos[n], idv) ? T::kOne << 16 : 0u);
+        }
+#pragma unroll 1
+        for (int d = 0; d < DT; ++d) {
+          const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * d * page);
+#pragma unroll 1
+          for (int kind = 0; kind < 3; ++kind) {
+            const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+            const ss_f32x4 hits = T::mfma16(parts_of<T>(v, kind), ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (hits[i] > 0.f) join_o[w][c][16 * d + 4 * g + i] += add;
+          }
+        }
+      }
+    }
     __syncthreads();
 #pragma unroll 1
-    for (int j = tid; j < 16 * (D / 4); j += 256) {
+    for (int j = tid; j < 16 * (D / 4); j += 64 * W) {
       const int col = j / (D / 4), d4 = 4 * (j % (D / 4));
       const int p = p0 + 16 * n + col;
       if (p < np) {
         float big = kNegInf, sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) big = fmaxf(big, join_m[k][n][col]);
+        for (int k = 0; k < W; ++k) big = fmaxf(big, join_m[k][n][col]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < W; ++k) {
           const float mk = join_m[k][n][col];
           sum += mk == kNegInf ? join_l[k][n][col] : join_l[k][n][col] * __builtin_amdgcn_exp2f(mk - big);
         }
         ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[0][col][d4]);
 #pragma unroll
-        for (int k = 1; k < 4; ++k) {
+        for (int k = 1; k < W; ++k) {
           const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[k][col][d4]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] += x[i];
@@ -354,7 +382,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 template <class T, int D, int NT>
 hipError_t launch_few(const AttnArgs& a, hipStream_t st) {
   const unsigned grid = (unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs);
-  hipLaunchKernelGGL((attn_few_kernel<T, D, NT>), dim3(grid), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((attn_few_kernel<T, D, NT, 4>), dim3(grid), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -363,8 +391,8 @@ hipError_t launch_few_of(const AttnArgs& a, int dim, hipStream_t st) {
   const int nt = a.packed / 16;
   if (dim == 64) return nt == 1 ? launch_few<T, 64, 1>(a, st) : nt == 2 ? launch_few<T, 64, 2>(a, st) : launch_few<T, 64, 4>(a, st);
   if (dim == 128)
-    return nt == 1 ? launch_few<T, 128, 1>(a, st) : launch_few<T, 128, 2>(a, st);
-  return launch_few<T, 256, 1>(a, st);
+    return nt == 1 ? launch_few<T, 128, 1>(a, st) : nt == 2 ? launch_few<T, 128, 2>(a, st) : launch_few<T, 128, 4>(a, st);
+  return nt == 1 ? launch_few<T, 256, 1>(a, st) : launch_few<T, 256, 2>(a, st);
 }
 
 template <class T, int D>
@@ -385,11 +413,11 @@ hipError_t launch_join_of(const AttnArgs& a, int dim, hipStream_t st) {
 
 }  // namespace
 
-// Packed rows of a workgroup: as few tiles of 16 as hold them all, as far as two waves of a SIMD have the registers: up
-// to 4 tiles of 64 dimensions, 2 of 128, 1 of 256.
+// Packed rows of a workgroup: as few tiles of 16 as hold them all, up to 4 (2 of 256 dimensions, whose sums of four tiles
+// would take every register).
 int attn_few_packed(int dim, int packed) {
-  if (packed <= 16 || dim == 256) return 16;
-  return packed <= 32 || dim == 128 ? 32 : 64;
+  if (packed <= 16) return 16;
+  return packed <= 32 || dim == 256 ? 32 : 64;
 }
 
 hipError_t launch_attn_few(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {

@@ -149,6 +149,31 @@ def stream_of(t) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The current torch stream on GPU `index`, as a hipStream_t handle."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on_device(index: int):
+    """A context in which GPU `index` is the current one (launches on another device's stream are refused by HIP)."""
+    import torch
+
+    return _here if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+
+
 def device_error(clear: bool = True) -> int:
     """Status bits raised by kernels on the current device since the last clear (synchronises)."""
     flags = ctypes.c_int(0)

@@ -214,9 +214,12 @@ int check_paged(int rows, int seqs, int max_rows, int heads, int kv_heads, int d
 
 // How a call of ssmoe_paged_attention is laid out (its checks included). `prompt`: the kernel for many rows of a sequence.
 //
-// Few rows (up to kFewRows): chunk is the tokens of one workgroup, so that a batch of full tables makes about 2048
-// workgroups, but none of fewer than 128 tokens (a tile for each wave) or more than 4096. It goes by seqs, kv_heads and the
-// table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call.
+// Few rows (up to kFewRows): chunk is the tokens of one workgroup, so that a batch of full tables makes a workgroup a CU, but
+// none of fewer than 128 tokens (a tile for each wave), and none of more than 512 to 4096 (by how far the sequences and key
+// heads alone fill the CUs: a short sequence on a wide table has to find its CUs too). It goes by seqs, kv_heads and the
+// table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call. With 256 /
+// 512 / 1024 / 2048 workgroups, kernel and join in us: one sequence of 131,072 tokens 47 / 48 / 55 / 54; eight of 6,145
+// with three rows at 256 dimensions 29 / 39 / 45 / 45; 32 with four rows under a window of 1,024 21 / 25 / 20 / 20.
 // Many rows: the tokens are split only where the row tiles alone would leave CUs without work.
 constexpr int kFewRows = 8;
 int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
@@ -256,8 +259,9 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
     if (want > 1 && seen > 512) chunk = std::max<int64_t>((seen + want - 1) / want, 512);
     chunk = (chunk + 127) / 128 * 128;
   } else {
-    chunk = (seen * units + 2047) / 2048;
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), 4096);
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(16 * units, 512), 4096);
+    chunk = (seen * units + 255) / 256;
+    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), most);
   }
   a.chunk = (int)chunk;
   slots = (cap + chunk - 1) / chunk;
@@ -1402,7 +1406,9 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
   a.adjacent = p->adjacent != 0;
   a.factor = p->factor;
   a.tiles = (int)(((int64_t)a.max_rows + 14) / 8);
-  a.head_groups = 1;
+  // A workgroup's four waves take its heads in turn; where there are few groups of positions the heads are shared out too.
+  const int64_t groups = std::max<int64_t>((int64_t)a.tiles * p->seqs, 1);
+  a.head_groups = (int)std::min<int64_t>((1024 + groups - 1) / groups, (p->heads + p->kv_heads + 3) / 4);
   if ((int64_t)a.tiles * a.head_groups * p->seqs > INT32_MAX)
     return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
   return hip_check(ss::launch_rope_append(a, p->type == SSMOE_FP16, static_cast<hipStream_t>(stream)), "rope launch");

@@ -32,7 +32,7 @@ def move_pages(k: torch.Tensor, v: torch.Tensor, src: torch.Tensor, dst: torch.T
     if page_bytes < 2048 or page_bytes % 2048:
         raise ValueError(f"a page must have a positive multiple of 2048 bytes, got {page_bytes}")
     dev = check_device(k, v, src, dst, table)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.check(_lib.lib().ssmoe_move_pages(k.data_ptr(), v.data_ptr(), layers, n_pages, page_bytes, src.data_ptr(),
                                                dst.data_ptr(), src.numel(), _lib.ptr(table),
-                                               0 if table is None else table.numel(), _lib.stream_of(k)))
+                                               0 if table is None else table.numel(), _lib.raw_stream(dev)))

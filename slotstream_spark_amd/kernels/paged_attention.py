@@ -13,8 +13,8 @@ the plain causal form a layer or the draft head (engine/mtp.py:209-227) can be g
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
@@ -24,16 +24,30 @@ TYPES = {torch.bfloat16: 0, torch.float16: 1}
 PAGES = (16, 32, 64, 128, 256)
 DIMS = (64, 128, 256)
 
-_P, _I, _I64, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+# ssmoe_paged_attention_args: 3 + 8 pointers and strides, 2 int64, 11 int, a float (padded to 8 bytes)
+_ARGS = struct.Struct("@Pqq8Pqq11if0q")
 
 
-class _Args(ctypes.Structure):
-    _fields_ = ([("q", _P), ("q_row", _I64), ("q_head", _I64)]
-                + [(n, _P) for n in ("k_pages", "v_pages", "cu_rows", "kv_len", "table", "out", "lse", "ws")]
-                + [("ws_bytes", _I64), ("n_pages", _I64)]
-                + [(n, _I) for n in ("rows", "seqs", "max_rows", "heads", "kv_heads", "dim", "page", "width", "window",
-                                     "sinks", "type")]
-                + [("scale", _F)])
+def pack_args(q=0, q_row=0, q_head=0, k_pages=0, v_pages=0, cu_rows=0, kv_len=0, table=0, out=0, lse=0, ws=0, ws_bytes=0,
+              n_pages=0, rows=0, seqs=0, max_rows=0, heads=0, kv_heads=0, dim=0, page=0, width=0, window=0, sinks=0, type=0,
+              scale=0.0) -> bytes:
+    """The C struct of a call, which the library reads during the call only."""
+    return _ARGS.pack(q, q_row, q_head, k_pages, v_pages, cu_rows, kv_len, table, out, lse, ws, ws_bytes, n_pages, rows,
+                      seqs, max_rows, heads, kv_heads, dim, page, width, window, sinks, type, scale)
+
+
+class Plans(dict):
+    """What the checks of a call's shapes, types and strides found, by those: nothing of the tensors themselves is kept.
+    Emptied when it holds many (a serving loop meets a few)."""
+
+    def keep(self, key, plan):
+        if len(self) >= 4096:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+_plans = Plans()
 
 
 def check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int]:
@@ -76,9 +90,8 @@ def check_rows(name: str, t: torch.Tensor, heads: int | None, dim: int, dtype) -
         raise ValueError(f"{name} must be [rows, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype} like the cache, got {t.dtype}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[0] > 1 and t.stride(0) % 8) or (t.shape[1] > 1 and t.stride(1) % 8)
-                      or t.data_ptr() % 16):
-        raise ValueError(f"{name} needs contiguous dimensions, strides that are multiples of 8 elements and 16-byte alignment")
+    if t.numel() and (t.stride(2) != 1 or (t.shape[0] > 1 and t.stride(0) % 8) or (t.shape[1] > 1 and t.stride(1) % 8)):
+        raise ValueError(f"{name} needs contiguous dimensions and strides that are multiples of 8 elements")
 
 
 def strides(t: torch.Tensor) -> tuple[int, int]:
@@ -86,10 +99,11 @@ def strides(t: torch.Tensor) -> tuple[int, int]:
     return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
 
 
-def check_device(*tensors) -> torch.device:
-    dev = tensors[0].device
+def check_device(*tensors) -> int:
+    """The index of the GPU that all of them (None apart) are on."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != dev):
+        if t is not None and (t.get_device() != dev or dev < 0):
             raise ValueError("all tensors must be on the same GPU")
     return dev
 
@@ -103,31 +117,46 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     `lse` fp32 [rows, heads] receives ln sum_j exp(scale q_i . k_j). A row that sees nothing is 0, its lse -inf; rows past
     cu_rows[-1] are left as they were in `out` and `lse`. Capturable; workspaces come from torch's allocator at each
     call, so calls and captured graphs never share one."""
+    max_rows, window, sinks = int(max_rows), int(window), int(sinks)
+    key = (q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.dtype, k_pages.is_contiguous(), v_pages.shape, v_pages.dtype,
+           v_pages.is_contiguous(), cu_rows.shape, cu_rows.dtype, kv_len.shape, kv_len.dtype, table.shape, table.dtype,
+           table.is_contiguous(), max_rows, window, sinks, scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plans.keep(key, _plan(q, k_pages, v_pages, cu_rows, kv_len, table, max_rows, window, sinks, scale))
+    head, sizes, tail, nb, shape = plan
+    dev = check_device(q, k_pages, v_pages, cu_rows, kv_len, table, out, lse)
+    q_at = q.data_ptr()
+    if q_at % 16:
+        raise ValueError("q needs 16-byte alignment")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {q.dtype} {tuple(shape)}")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous fp32 {tuple(shape[:2])}")
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    args = _ARGS.pack(q_at, *head, k_pages.data_ptr(), v_pages.data_ptr(), cu_rows.data_ptr(), kv_len.data_ptr(),
+                      table.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr(),
+                      nb, *sizes, *tail)
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().ssmoe_paged_attention(args, _lib.raw_stream(dev)))
+    return out
+
+
+def _plan(q, k_pages, v_pages, cu_rows, kv_len, table, max_rows, window, sinks, scale):
+    """Checks a call's shapes, types and strides: (strides of q, sizes, mask and scale, workspace bytes, shape of out)."""
     n_pages, kv_heads, page, dim = check_cache(k_pages, v_pages)
     seqs, width = check_batch(cu_rows, kv_len, table, max_rows)
     check_rows("q", q, None, dim, k_pages.dtype)
     rows, heads = q.shape[0], q.shape[1]
     if heads < 1 or heads % kv_heads:
         raise ValueError(f"q has {heads} heads, not a positive multiple of the cache's {kv_heads}")
-    dev = check_device(q, k_pages, v_pages, cu_rows, kv_len, table, out, lse)
-    if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or tuple(out.shape) != (rows, heads, dim) or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {q.dtype} {(rows, heads, dim)}")
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (rows, heads) or not lse.is_contiguous()):
-        raise ValueError(f"lse must be contiguous fp32 {(rows, heads)}")
-    q_row, q_head = strides(q)
-    a = _Args(q.data_ptr(), q_row, q_head, k_pages.data_ptr(), v_pages.data_ptr(), cu_rows.data_ptr(), kv_len.data_ptr(),
-              table.data_ptr(), out.data_ptr(), _lib.ptr(lse), None, 0, n_pages, rows, seqs, int(max_rows), heads, kv_heads,
-              dim, page, width, int(window), int(sinks), TYPES[q.dtype],
-              1.0 / math.sqrt(dim) if scale is None else float(scale))
+    head = strides(q)
+    sizes = (n_pages, rows, seqs, max_rows, heads, kv_heads, dim, page, width)
+    tail = (window, sinks, TYPES[q.dtype], 1.0 / math.sqrt(dim) if scale is None else float(scale))
     L = _lib.lib()
-    nb = L.ssmoe_paged_attention_workspace_bytes(ctypes.byref(a))
+    nb = L.ssmoe_paged_attention_workspace_bytes(_ARGS.pack(0, *head, *(0,) * 8, 0, *sizes, *tail))
     if nb < 0:
         raise ValueError(L.ssmoe_last_error().decode(errors="replace"))
-    with torch.cuda.device(dev):
-        if nb:
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-            a.ws, a.ws_bytes = ws.data_ptr(), nb
-        _lib.check(L.ssmoe_paged_attention(ctypes.byref(a), _lib.stream_of(q)))
-    return out
+    return head, sizes, tail, nb, q.shape

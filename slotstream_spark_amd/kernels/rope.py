@@ -2,25 +2,27 @@
 between the fused query/key/value projection of a layer and its attention (kernels/paged_attention.py)."""
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from .. import _lib
-from .paged_attention import TYPES, check_batch, check_cache, check_device, check_rows, strides
+from .paged_attention import Plans, TYPES, check_batch, check_cache, check_device, check_rows, strides
 
-_P, _I, _I64, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+# ssmoe_rope_append_args
+_ARGS = struct.Struct("@3P6qPPq7Pq12if0q")
 
 
-class _Args(ctypes.Structure):
-    _fields_ = ([(n, _P) for n in ("q", "k", "v")]
-                + [(n, _I64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
-                + [("q_out", _P), ("positions", _P), ("pos_stride", _I64)]
-                + [(n, _P) for n in ("inv_freq", "axis", "k_pages", "v_pages", "cu_rows", "kv_len", "table")]
-                + [("n_pages", _I64)]
-                + [(n, _I) for n in ("rows", "seqs", "max_rows", "heads", "kv_heads", "dim", "page", "width", "rot", "axes",
-                                     "adjacent", "type")]
-                + [("factor", _F)])
+def pack_args(q=0, k=0, v=0, q_row=0, q_head=0, k_row=0, k_head=0, v_row=0, v_head=0, q_out=0, positions=0, pos_stride=0,
+              inv_freq=0, axis=0, k_pages=0, v_pages=0, cu_rows=0, kv_len=0, table=0, n_pages=0, rows=0, seqs=0, max_rows=0,
+              heads=0, kv_heads=0, dim=0, page=0, width=0, rot=0, axes=0, adjacent=0, type=0, factor=1.0) -> bytes:
+    """The C struct of a call, which the library reads during the call only."""
+    return _ARGS.pack(q, k, v, q_row, q_head, k_row, k_head, v_row, v_head, q_out, positions, pos_stride, inv_freq, axis,
+                      k_pages, v_pages, cu_rows, kv_len, table, n_pages, rows, seqs, max_rows, heads, kv_heads, dim, page,
+                      width, rot, axes, adjacent, type, factor)
+
+
+_plans = Plans()
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -35,6 +37,34 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     `adjacent`; elements from rot on are copied. cos and sin are multiplied by `factor`. q, k and v may be views into
     one projection (strides multiples of 8 elements); `out` may be q itself where q is contiguous. Rows past
     cu_rows[-1] are left as they were."""
+    max_rows = int(max_rows)
+    key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape,
+           positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, inv_freq.is_contiguous(), k_pages.shape,
+           k_pages.dtype, k_pages.is_contiguous(), v_pages.shape, v_pages.dtype, v_pages.is_contiguous(), cu_rows.shape,
+           cu_rows.dtype, kv_len.shape, kv_len.dtype, table.shape, table.dtype, table.is_contiguous(), max_rows,
+           None if axis is None else (axis.shape, axis.dtype))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plans.keep(key, _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis))
+    row_strides, sizes, rot, axes, kind, shape = plan
+    dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out)
+    q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (q_at | k_at | v_at) % 16:
+        raise ValueError("q, k and v need 16-byte alignment")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {q.dtype} {tuple(shape)}")
+    args = _ARGS.pack(q_at, k_at, v_at, *row_strides, out.data_ptr(), positions.data_ptr(), shape[0], inv_freq.data_ptr(),
+                      0 if axis is None else axis.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), cu_rows.data_ptr(),
+                      kv_len.data_ptr(), table.data_ptr(), *sizes, rot, axes, 1 if adjacent else 0, kind, float(factor))
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().ssmoe_rope_append(args, _lib.raw_stream(dev)))
+    return out
+
+
+def _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis):
+    """Checks a call's shapes, types and strides: (strides, sizes, rot, axes, type, shape of out)."""
     n_pages, kv_heads, page, dim = check_cache(k_pages, v_pages)
     seqs, width = check_batch(cu_rows, kv_len, table, max_rows)
     dtype = k_pages.dtype
@@ -59,15 +89,5 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         raise ValueError("positions must have at least one axis")
     if axis is not None and (axis.dtype != torch.int32 or tuple(axis.shape) != (rot // 2,) or not axis.is_contiguous()):
         raise ValueError(f"axis must be contiguous int32 [{rot // 2}]")
-    dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out)
-    if out is None:
-        out = torch.empty((rows, heads, dim), dtype=dtype, device=dev)
-    elif out.dtype != dtype or tuple(out.shape) != (rows, heads, dim) or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {dtype} {(rows, heads, dim)}")
-    a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides(q), *strides(k), *strides(v), out.data_ptr(),
-              positions.data_ptr(), rows, inv_freq.data_ptr(), _lib.ptr(axis), k_pages.data_ptr(), v_pages.data_ptr(),
-              cu_rows.data_ptr(), kv_len.data_ptr(), table.data_ptr(), n_pages, rows, seqs, int(max_rows), heads, kv_heads,
-              dim, page, width, rot, axes, int(bool(adjacent)), TYPES[dtype], float(factor))
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().ssmoe_rope_append(ctypes.byref(a), _lib.stream_of(q)))
-    return out
+    return ((*strides(q), *strides(k), *strides(v)),
+            (n_pages, rows, seqs, max_rows, heads, kv_heads, dim, page, width), rot, axes, TYPES[dtype], q.shape)

@@ -1,6 +1,5 @@
 """The paged cache's entry points without a GPU: argument refusals of the C ABI before a device is touched, workspace
 sizes, the Python mirrors' ValueErrors, and the definition the GPU tests compare with against torch's own softmax."""
-import ctypes
 import math
 
 import pytest
@@ -26,7 +25,7 @@ def attn(**kw):
              ws_bytes=1 << 40, n_pages=10, rows=4, seqs=2, max_rows=2, heads=8, kv_heads=2, dim=64, page=16, width=8, window=0,
              sinks=0, type=0, scale=0.125)
     a.update(kw)
-    return pa._Args(**a)
+    return pa.pack_args(**{k: 0 if v is None else v for k, v in a.items()})
 
 
 @pytest.mark.parametrize("kw,msg", [
@@ -43,18 +42,18 @@ def attn(**kw):
     (dict(width=4096, ws=P + 16), b"workspace holds"),
 ])
 def test_attention_refuses(L, kw, msg):
-    assert L.ssmoe_paged_attention(ctypes.byref(attn(**kw)), None) == EINVAL
+    assert L.ssmoe_paged_attention(attn(**kw), None) == EINVAL
     assert msg in L.ssmoe_last_error(), L.ssmoe_last_error()
 
 
 def test_attention_workspace(L):
-    size = lambda **kw: L.ssmoe_paged_attention_workspace_bytes(ctypes.byref(attn(**kw)))
+    size = lambda **kw: L.ssmoe_paged_attention_workspace_bytes(attn(**kw))
     assert size(width=8) == 0                      # a table of one chunk: nothing to join
     assert size(width=4096) > 0 and size(dim=100) == -1 and L.ssmoe_paged_attention_workspace_bytes(None) == -1
     assert size(width=4096, window=64) < size(width=4096)
     assert L.ssmoe_paged_attention(None, None) == EINVAL
-    assert L.ssmoe_paged_attention(ctypes.byref(attn(rows=0, q=None)), None) == 0      # nothing to do, no launch
-    assert L.ssmoe_paged_attention(ctypes.byref(attn(seqs=0, q=None)), None) == 0
+    assert L.ssmoe_paged_attention(attn(rows=0, q=None), None) == 0      # nothing to do, no launch
+    assert L.ssmoe_paged_attention(attn(seqs=0, q=None), None) == 0
 
 
 def rope_args(**kw):
@@ -62,7 +61,7 @@ def rope_args(**kw):
              pos_stride=4, inv_freq=P, axis=None, k_pages=P, v_pages=P, cu_rows=P, kv_len=P, table=P, n_pages=10, rows=4,
              seqs=2, max_rows=2, heads=8, kv_heads=2, dim=64, page=16, width=8, rot=64, axes=1, adjacent=0, type=0, factor=1.0)
     a.update(kw)
-    return rope._Args(**a)
+    return rope.pack_args(**{k: 0 if v is None else v for k, v in a.items()})
 
 
 @pytest.mark.parametrize("kw,msg", [
@@ -72,13 +71,13 @@ def rope_args(**kw):
     (dict(k=P + 8), b"16-byte"), (dict(v_row=129), b"strides"), (dict(inv_freq=P + 4), b"8-byte"), (dict(heads=3), b"multiple"),
 ])
 def test_rope_refuses(L, kw, msg):
-    assert L.ssmoe_rope_append(ctypes.byref(rope_args(**kw)), None) == EINVAL
+    assert L.ssmoe_rope_append(rope_args(**kw), None) == EINVAL
     assert msg in L.ssmoe_last_error(), L.ssmoe_last_error()
 
 
 def test_rope_nothing_to_do(L):
     assert L.ssmoe_rope_append(None, None) == EINVAL
-    assert L.ssmoe_rope_append(ctypes.byref(rope_args(rows=0, q=None)), None) == 0
+    assert L.ssmoe_rope_append(rope_args(rows=0, q=None), None) == 0
 
 
 def test_move_refuses(L):
@@ -105,7 +104,7 @@ def test_python_refusals():
                     (dict(k_pages=b.k[:, :1], v_pages=b.v[:, :1]), "contiguous"), (dict(cu_rows=b.cu.long()), "int32"),
                     (dict(cu_rows=b.cu[:2]), "cu_rows must be"), (dict(kv_len=b.kv_len[:1]), "kv_len"),
                     (dict(table=b.table[0]), "table must be"), (dict(max_rows=0), "max_rows"),
-                    (dict(q=torch.zeros(3, 4, 65, dtype=b.dtype)[:, :, 1:]), "16-byte"),
+                    (dict(q=torch.zeros(3, 4, 65, dtype=b.dtype)[:, :, 1:]), "multiples of 8"),
                     (dict(q=torch.zeros(3, 4, 100, dtype=b.dtype)[:, :, :64]), "multiples of 8")):
         with pytest.raises(ValueError, match=msg):
             pa.paged_attention(**{**good, **kw})

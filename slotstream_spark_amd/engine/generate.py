@@ -4,7 +4,9 @@ generate.py:152-238, at temperature 0).
 MoEStack is the main model of the loop as far as this path reaches: token rows -> embedding rows -> the chained MoE
 layers of a verify round (MTPStepGraph, one HIP graph) -> final norm -> lm_head with the greedy round fused behind it.
 Without attention each row depends on its own token only, so the greedy sequence is fixed by the first token, and a
-speculative decode must emit exactly the sequence plain one-row steps emit, whatever the drafts are.
+speculative decode must emit exactly the sequence plain one-row steps emit, whatever the drafts are. With attention layers
+(`attn`) a row depends on the tokens before it through the paged cache; the few-row attention gives a row the same bits in
+a round as alone, so the same holds.
 
 A round, as in the reference: the MTP head drafts DEPTH tokens after the pending one (on a fork of its state), the
 stack verifies pending + drafts in one pass, the host walks the rows with the plain loop's stopping rules, keeps the
@@ -23,21 +25,35 @@ from ..kernels.head_ops import gather_rows
 from . import mtp as mtp_mod
 from . import rollback as rb
 from .accept import AcceptResult
-from .step import MoEWeights, MTPStepGraph
+from .attention import SeqCache
+from .prefill import MoEPrefillLayer
+from .step import MoEWeights, MTPStepGraph, residual_rmsnorm
 
 
 class MoEStack:
     """`len(layers)` MoE layers on one residual stream behind an embedding table and in front of the lm_head, run
-    `depth` + 1 rows at a time. `st` (rollback.SeqState) and `record` (rollback.StepRecord, empty) hold the sequence."""
+    `depth` + 1 rows at a time. `st` (rollback.SeqState) and `record` (rollback.StepRecord, empty) hold the sequence.
+    `attn` (an AttentionLayer per layer, norms `attn_norms` before them) over `pages` (a KVPages, one sequence of which becomes the
+    stack's) adds attention; max_ctx is then at most what its table covers less a round's rows. `prompt_chunk` > 0: prompts go through the prompt forms of the layers (MoEPrefillLayer, and
+    the many-row attention) in chunks of so many tokens instead of `rows` at a time."""
 
     def __init__(self, pool, layers: list[MoEWeights], lm_head: AffineWeight, embed: torch.Tensor,
                  depth: int = mtp_mod.DEPTH, norm_weights=None, eps: float = 1e-6, top_k: int = 10,
-                 max_ctx: int = 1 << 20, device="cuda"):
+                 max_ctx: int = 1 << 20, device="cuda", attn=None, attn_norms=None, pages=None, prompt_chunk: int = 0):
         if embed.dim() != 2 or embed.shape[1] != pool.hidden or embed.dtype != torch.bfloat16:
             raise ValueError(f"embed must be bf16 [V, {pool.hidden}]")
+        if (attn is None) != (pages is None):
+            raise ValueError("attn and pages come together")
+        self.cache = SeqCache(pages) if pages is not None else None
         self.graph = MTPStepGraph(pool, layers, lm_head, depth, norm_weights=norm_weights, eps=eps, top_k=top_k,
-                                  device=device)
+                                  device=device, attn=attn, attn_norms=attn_norms, cache=self.cache)
+        self.chunk = int(prompt_chunk)
+        self.prompt_layers = [MoEPrefillLayer(pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=top_k,
+                                              router_bias=w.router_bias, max_tokens=self.chunk)
+                              for l, w in enumerate(layers)] if self.chunk > 0 else None
         self.depth, self.rows, self.nl = depth, depth + 1, len(layers)
+        if pages is not None:   # a pass writes `rows` tokens, also where fewer are kept
+            max_ctx = min(max_ctx, pages.width * pages.page - self.rows)
         self.embed, self.max_ctx, self.device = embed, max_ctx, torch.device(device)
         self.argmax = LMHeadArgmax(lm_head, max_rows=self.rows, round_bf16=True, device=device)
         # the plain steps' logits, kept for the finiteness check of _mtp_decode's plain loop (generate.py:186-189)
@@ -45,12 +61,17 @@ class MoEStack:
         self.last_finite: list[bool] = []
         self.tok_rows = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
         self.row_ids = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
-        self.st = rb.SeqState()
+        self.st = self._state()
         self.record = rb.StepRecord(self.st, self.rows)
+
+    def _state(self) -> rb.SeqState:
+        return rb.SeqState(attn={"cache": self.cache} if self.cache is not None else {})
 
     def reset(self) -> None:
         """A new sequence (the captured graph and the buffers stay)."""
-        self.st = rb.SeqState()
+        if self.cache is not None:
+            self.cache.reset()
+        self.st = self._state()
         self.record = rb.StepRecord(self.st, self.rows)
 
     @property
@@ -62,6 +83,8 @@ class MoEStack:
         t = list(tokens) + [0] * (self.rows - len(tokens))
         self.tok_rows.copy_(torch.tensor(t, dtype=torch.int32))
         g = self.graph
+        if self.cache is not None:
+            self.cache.place(self.st.pos, self.rows)   # rows past the given tokens are written over by the next pass
         gather_rows(self.embed, self.tok_rows, out=g.x_in)
         g.drafts.copy_(self.tok_rows[1:])
         return g.step()
@@ -95,6 +118,38 @@ class MoEStack:
         return nxt, torch.cat(multi, 0)
 
 
+    def prompt(self, tokens: list[int]) -> tuple[list[int], torch.Tensor]:
+        """The prompt of a sequence: (the greedy next token after the last one, the final stream rows [len, H]). Through
+        forward(), or with a prompt_chunk through the layers' prompt forms."""
+        if self.prompt_layers is None:
+            return self.forward(tokens)
+        g, w, eps, multi = self.graph, self.graph.norm_weights, self.graph.eps, []
+        for c0 in range(0, len(tokens), self.chunk):
+            chunk = [int(t) for t in tokens[c0:c0 + self.chunk]]
+            n = len(chunk)
+            x = gather_rows(self.embed, torch.tensor(chunk, dtype=torch.int32).to(self.device))
+            mixed = torch.empty_like(x)
+            if self.cache is not None:
+                self.cache.place(self.st.pos, n)
+                cu, kv_len, table, positions = self.cache.rows(n)
+            for l, layer in enumerate(self.prompt_layers):
+                if self.cache is not None:
+                    residual_rmsnorm(x, None, mixed, weight=g.attn_norms[l], eps=eps)
+                    a = g.attn[l](mixed, positions, self.cache.pages.k[l], self.cache.pages.v[l], cu, kv_len, table, n)
+                    residual_rmsnorm(x, a, mixed, stream_out=x, weight=w[l], eps=eps)
+                else:
+                    residual_rmsnorm(x, None, mixed, weight=w[l], eps=eps)
+                y = layer(mixed)[0]
+                residual_rmsnorm(x, y, mixed, stream_out=x, weight=w[l + 1], eps=eps)
+            multi.append(x)
+            self.st.pos += n
+            self.st.tokens += chunk
+        last = mixed[-1:].expand(self.rows, -1).contiguous()
+        self.argmax(last, ids=self.row_ids, logits=self.plain_logits)
+        self.last_finite = [bool(torch.isfinite(self.plain_logits[0]).all())]
+        return [int(self.row_ids[0])], torch.cat(multi, 0)
+
+
 def mtp_decode(stack: MoEStack, head: mtp_mod.MTPHead, prompt: list[int], max_tokens: int, eos=(), on_token=None,
                draft_fn=None):
     """Greedy self-speculative decode after `prompt` -> (tokens, nan, round_seconds, stats), as _mtp_decode.
@@ -105,7 +160,7 @@ def mtp_decode(stack: MoEStack, head: mtp_mod.MTPHead, prompt: list[int], max_to
     out, step_s, nan = [], [], False
     st = {"rounds": 0, "plain_steps": 0, "drafted": 0, "accepted": 0, "attempts_by_depth": [0] * D,
           "accepted_by_depth": [0] * D, "emitted_by_round": [], "verify_rows": 0}
-    nxt, multi = stack.forward(prompt)
+    nxt, multi = stack.prompt(prompt)
     head.consume(prompt, multi)
     if not stack.last_finite[-1]:
         return out, True, step_s, st

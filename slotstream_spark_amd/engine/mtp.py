@@ -1,6 +1,7 @@
-"""MTP draft head of the MoE path, without its attention (drop-in for slotstream_spark/engine/mtp.py:78-277).
+"""MTP draft head of the MoE path (drop-in for slotstream_spark/engine/mtp.py:78-277).
 
-One head step over S rows, as MTPHead.step (engine/mtp.py:209-227) with the attention output taken as zero:
+One head step over S rows, as MTPHead.step (engine/mtp.py:209-227) with the attention output taken as zero unless the head
+is given an attention (HeadAttention):
 
     h     = fuse(embedded, multi)                              engine/mtp.py:184-192
             e = lin(rmsnorm(embedded)), per branch c: lin(rmsnorm_fullwidth(multi))[c] + e
@@ -16,9 +17,10 @@ branch mean behind the up GEMV), with the bits of the separate ops. `draft(token
 each step's embedding row is read by the first launch at the token the previous step's lm_head argmax wrote, so the
 k drafts reach the host once, at the end, and the chain can be captured in a HIP graph (DraftGraph).
 
-Out of this path: the attention segment (hc_mix of attn_hyper_connection, QSA over the head's own KV/indexer cache,
-its residual). MTPState keeps the position bookkeeping of the reference's state (pos, aligned, fork, reset) with no
-cache behind it.
+The attention segment is optional: HeadAttention puts hc_mix of attn_hyper_connection, plain causal attention over the
+head's own paged cache (engine/attention.py, in the place of the reference's QSA) and its residual between fuse and the MoE.
+MTPState keeps the position bookkeeping of the reference's state (pos, aligned, fork, reset): entry i of the cache is the
+head's i-th row. Drafts are rows past the state's position; the next consume writes over them.
 """
 from __future__ import annotations
 
@@ -29,6 +31,8 @@ import torch
 from ..kernels.gemv_affine import AffineWeight, LMHeadArgmax, gemv
 from ..kernels.head_ops import (EPI_ADD, EPI_INJECT, EPI_SIGMOID, EPI_SILU_DIV, gather_rows, hc_inject, hc_mean,
                                 head_gemv, lin_epi, rmsnorm)
+from ..memory.kv_pages import KVPages
+from .attention import AttentionLayer, SeqCache
 from .verify import MoEVerifyLayer
 
 MAP_ROW = 48   # the head's layer index in the 49-row expert map (engine/mtp.py:38)
@@ -86,6 +90,15 @@ class MTPState:
         self.pos = 0
 
 
+@dataclass
+class HeadAttention:
+    """The head's attention segment: attn_hyper_connection (with inject), the layer, and the pages whose layer 0 holds the head's
+    keys and values (one sequence of them becomes the head's)."""
+    hc: HyperConnection
+    layer: AttentionLayer
+    pages: KVPages
+
+
 class _Rows:
     """Intermediates of head steps over S rows each, one slice per step (kept so a caller can read them back)."""
 
@@ -118,7 +131,7 @@ class MTPHead:
     the head's map row (MAP_ROW in the full model) with at least `max_rows` tokens per call."""
 
     def __init__(self, weights: HeadWeights, moe: MoEVerifyLayer, lm_head: AffineWeight, hc: int, eps: float = 1e-6,
-                 max_ctx: int = 1 << 20, max_rows: int = 4):
+                 max_ctx: int = 1 << 20, max_rows: int = 4, attn: HeadAttention | None = None):
         self.w, self.moe, self.lm_head = weights, moe, lm_head
         self.H, self.hc, self.eps = moe.hidden, int(hc), float(eps)
         self.topk = moe.top_k
@@ -129,7 +142,13 @@ class MTPHead:
             raise ValueError(f"embed must be [V, {H}]")
         checks = [("pre_fc_norm_embedding", w.pre_fc_norm_embedding, (H,)), ("fc_embedding", w.fc_embedding, (H, H)),
                   ("pre_fc_norm_hidden", w.pre_fc_norm_hidden, (n,)), ("fc_hidden", w.fc_hidden, (H, H))]
-        for name, hcw, inject in (("mlp_hc", w.mlp_hc, True), ("mixer_hc", w.mixer_hc, False)):
+        hcs = [("mlp_hc", w.mlp_hc, True), ("mixer_hc", w.mixer_hc, False)]
+        self.attn, self.cache = attn, None
+        if attn is not None:
+            hcs.append(("attn.hc", attn.hc, True))
+            if attn.layer.hidden != H:
+                raise ValueError(f"the attention layer takes H = {attn.layer.hidden}, the head H = {H}")
+        for name, hcw, inject in hcs:
             L = hcw.down.shape[0]
             checks += [(name + ".hc_norm", hcw.hc_norm, (n,)), (name + ".down", hcw.down, (L, n)),
                        (name + ".up", hcw.up, (n, L))]
@@ -146,6 +165,9 @@ class MTPHead:
         if w.embed.shape[0] < self.vocab:
             raise ValueError("the embedding table must cover the lm_head's vocabulary")
         self.argmax = LMHeadArgmax(lm_head, max_rows=self.max_rows, round_bf16=True, device=w.embed.device)
+        if attn is not None:
+            self.cache = SeqCache(attn.pages)
+            max_ctx = min(max_ctx, attn.pages.width * attn.pages.page)
         self.state = MTPState(max_ctx)
         self.prev_multi: torch.Tensor | None = None
         self.consumed = 0
@@ -183,8 +205,30 @@ class MTPHead:
         lin_epi(hn, hcw.inject, EPI_INJECT, hc=self.hc, out=inj)
         return mixed, inj
 
-    def _step_rows(self, embedded, multi, r: _Rows, i: int, idx: torch.Tensor | None = None):
+    def _attend(self, h: torch.Tensor, pos: int, base: torch.Tensor | None = None, append_only: bool = False):
+        """The attention segment over the fused rows h [S, hc H] at the positions pos .. (or those behind the device int32
+        `base`, whose pages the caller has reserved): h with the injected output; with append_only the rows' keys and values are
+        written and nothing is returned (engine/mtp.py:209-227)."""
+        a, S, n = self.attn, h.shape[0], self.hc * self.H
+        new = lambda cols: torch.empty((S, cols), dtype=torch.bfloat16, device=h.device)  # noqa: E731
+        mixed, inj = self.hc_mix(a.hc, h, new(n), new(a.hc.down.shape[0]), new(n), new(self.H), new(self.hc))
+        if base is None:
+            self.cache.place(pos, S)
+            cu, kv_len, table, positions = self.cache.rows(S)
+        else:
+            cu, _, table, _ = self.cache.rows(S)
+            kv_len, positions = base + (pos + S), base + torch.arange(pos, pos + S, dtype=torch.int32, device=h.device)
+        args = (mixed, positions, a.pages.k[0], a.pages.v[0], cu, kv_len, table, S)
+        if append_only:
+            a.layer.append(*args)
+            return None
+        return hc_inject(h, a.layer(*args), inj)
+
+    def _step_rows(self, embedded, multi, r: _Rows, i: int, idx: torch.Tensor | None = None, pos: int = 0,
+                   base: torch.Tensor | None = None):
         h = self.fuse(embedded, multi, r, i, idx)
+        if self.attn is not None:
+            h = self._attend(h, pos, base)
         if self.hc != 4:
             # the separate launches (the fused branch mean takes four branches)
             self.hc_mix(self.w.mlp_hc, h, r.hn[i], r.low[i], r.mix_w[i], r.mixed[i], r.inj[i])
@@ -221,10 +265,12 @@ class MTPHead:
         r = self._rows(1, S)
         if state_only:
             h = self.fuse(embedded, multi, r, 0)
+            if self.attn is not None:
+                self._attend(h, state.pos, append_only=True)
             state.pos += S
             return None, h
         state.pos += S
-        return self._step_rows(embedded, multi, r, 0)
+        return self._step_rows(embedded, multi, r, 0, pos=state.pos - S)
 
     def logits(self, out: torch.Tensor) -> torch.Tensor:
         """lm_head over the head's output rows -> fp32 [S, V]: lin's bf16 result as fp32 (engine/mtp.py:232-236)."""
@@ -233,6 +279,8 @@ class MTPHead:
     # ------------------------------------------------------------------ the engine-facing calls
     def reset(self) -> None:
         self.state.reset()
+        if self.cache is not None:
+            self.cache.reset()
         self.prev_multi = None
         self.consumed = 0
 
@@ -266,10 +314,12 @@ class MTPHead:
         return self._draft_rows[k]
 
     def draft_async(self, token: torch.Tensor, multi: torch.Tensor, k: int, out: torch.Tensor,
-                    state: MTPState | None = None) -> torch.Tensor:
+                    state: MTPState | None = None, base: torch.Tensor | None = None) -> torch.Tensor:
         """k greedy drafts after the device token `token` (int32 [1]) chained from `multi` (bf16 [1, hc H]) into
         `out` (int32 [k]) with no host synchronisation: step i embeds out[i - 1] (token for i = 0) by a device-side
-        gather, runs the head, and writes the argmax of its lm_head row to out[i]. Same launches on every call."""
+        gather, runs the head, and writes the argmax of its lm_head row to out[i]. Same launches on every call. With an
+        attention, the drafts are the cache's rows behind the state's position, or behind state.pos + `base` where that is given
+        (a device int32 [1], whose pages the caller has reserved: the captured form)."""
         if token.dtype != torch.int32 or token.numel() != 1 or out.dtype != torch.int32 or out.numel() != k:
             raise ValueError(f"token must be int32 [1] and out int32 [{k}]")
         if tuple(multi.shape) != (1, self.hc * self.H):
@@ -281,7 +331,7 @@ class MTPHead:
         prev_h = multi
         for i in range(k):
             src = token if i == 0 else out[i - 1:i]
-            o, prev_h = self._step_rows(None, prev_h, r, i, idx=src)
+            o, prev_h = self._step_rows(None, prev_h, r, i, idx=src, pos=st.pos + i, base=base)
             self.argmax(o, ids=out[i:i + 1])
         st.pos += k
         return out
@@ -300,7 +350,8 @@ class MTPHead:
 
 class DraftGraph:
     """The k-step draft chain captured once as a HIP graph: set `token` (int32 [1]) and `multi` (bf16 [1, hc H]) in
-    place, replay, read `out` (int32 [k]). The head's state is not advanced (drafting runs on a fork)."""
+    place, replay, read `out` (int32 [k]). The head's state is not advanced (drafting runs on a fork). With an attention, a
+    replay drafts behind the position the head's state has then."""
 
     def __init__(self, head: MTPHead, k: int):
         dev = head.w.embed.device
@@ -308,12 +359,23 @@ class DraftGraph:
         self.token = torch.zeros(1, dtype=torch.int32, device=dev)
         self.multi = torch.zeros(1, head.hc * head.H, dtype=torch.bfloat16, device=dev)
         self.out = torch.zeros(k, dtype=torch.int32, device=dev)
+        self.base = torch.zeros(1, dtype=torch.int32, device=dev)
         self.graph = None
 
     def _body(self) -> None:
-        self.head.draft_async(self.token, self.multi, self.k, self.out, state=MTPState(self.k))
+        self.head.draft_async(self.token, self.multi, self.k, self.out, state=MTPState(self.k),
+                              base=self.base if self.head.attn is not None else None)
+
+    def _place(self) -> None:
+        h = self.head
+        if h.attn is not None:
+            if h.state.pos + self.k > h.state.max_ctx:
+                raise ValueError(f"head context {h.state.pos + self.k} exceeds {h.state.max_ctx}")
+            h.cache.pages.reserve(h.cache.seq, h.state.pos + self.k)
+            self.base.fill_(h.state.pos)
 
     def capture(self) -> None:
+        self._place()
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -328,5 +390,6 @@ class DraftGraph:
     def replay(self) -> torch.Tensor:
         if self.graph is None:
             self.capture()
+        self._place()
         self.graph.replay()
         return self.out

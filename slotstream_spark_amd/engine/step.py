@@ -80,12 +80,17 @@ class MTPStepGraph:
     draft head's logits of the round (`draft_logits` [depth, V]), the round's uniforms and drafts drawn from
     q = softmax(draft_logits / temperature): the rule divides by q(x), so it preserves the target distribution only
     for drafts drawn from q. `draw_drafts(uniforms)` draws them into `drafts` on the device (ssmoe_sample_rows);
-    argmax drafts (the greedy proposal) belong to the greedy round."""
+    argmax drafts (the greedy proposal) belong to the greedy round.
+
+    `attn` (one AttentionLayer per layer, with `attn_norms`, the norms before them, and `cache`, the SeqCache of the sequence)
+    puts an attention layer and its residual before each MoE: the rows are the tokens that cache.place() named last. The
+    layers then run one launch each (the chained launch has no place between them)."""
 
     def __init__(self, pool, layers: list[MoEWeights], lm_head: AffineWeight, depth: int,
                  head: MoEWeights | None = None, norm_weights: list[torch.Tensor | None] | None = None,
                  eps: float = 1e-6, top_k: int = 10, keep_logits: bool = False, fused: bool = True,
-                 single_launch: bool = True, accept: str = "greedy", temperature: float = 1.0, device="cuda"):
+                 single_launch: bool = True, accept: str = "greedy", temperature: float = 1.0, device="cuda",
+                 attn=None, attn_norms: list[torch.Tensor | None] | None = None, cache=None):
         if not 1 <= depth <= 3:
             raise ValueError("depth must be 1..3 (the verify kernel takes up to 4 rows)")
         self.depth, self.rows = depth, depth + 1
@@ -99,7 +104,14 @@ class MTPStepGraph:
             raise ValueError(f"lm_head takes K = {lm_head.k}, the layers H = {H}")
         self.device = torch.device(device)
         self.eps = float(eps)
-        self.fused = bool(fused)
+        self.attn, self.cache = list(attn) if attn is not None else None, cache
+        if (self.attn is None) != (cache is None) or (self.attn is not None and (
+                len(self.attn) != self.nl or cache.pages.layers < self.nl or any(a.hidden != H for a in self.attn))):
+            raise ValueError(f"attn takes one AttentionLayer of hidden size {H} per layer and a cache of as many layers")
+        self.attn_norms = list(attn_norms) if attn_norms is not None else [None] * self.nl
+        if len(self.attn_norms) != self.nl:
+            raise ValueError(f"need {self.nl} attention norms")
+        self.fused = bool(fused) and self.attn is None
         self.norm_weights = list(norm_weights) if norm_weights is not None else [None] * (self.nl + 1)
         if len(self.norm_weights) != self.nl + 1:
             raise ValueError(f"need {self.nl + 1} norm weights (one per layer and the final norm)")
@@ -116,6 +128,8 @@ class MTPStepGraph:
         self.drafts = torch.zeros(depth, dtype=torch.int32, device=dev)
         self.streams = [self.x_in] + [torch.zeros((R, H), **bf) for _ in range(self.nl)]
         self.mixed = [torch.zeros((R, H), **bf) for _ in range(self.nl + 1)]
+        self.attn_in, self.attn_mid = ((torch.zeros((R, H), **bf), torch.zeros((R, H), **bf)) if self.attn is not None
+                                       else (None, None))
         self.ys = [torch.zeros((R, H), **bf) for _ in range(self.nl)]
         self.ids = torch.zeros((self.nl, R, top_k), dtype=torch.int32, device=dev)
         self.weights = torch.zeros((self.nl, R, top_k), dtype=torch.float32, device=dev)
@@ -155,7 +169,18 @@ class MTPStepGraph:
     def _body(self) -> None:
         """Every launch of the round on the current stream, reading only the static buffers."""
         w = self.norm_weights
-        if self.fused:
+        if self.attn is not None:
+            cu, kv_len, table, positions = self.cache.rows(self.rows)
+            pages, an = self.cache.pages, self.attn_norms
+            residual_rmsnorm(self.x_in, None, self.attn_in, weight=an[0], eps=self.eps)
+            for l, layer in enumerate(self.layers):
+                a = self.attn[l](self.attn_in, positions, pages.k[l], pages.v[l], cu, kv_len, table, self.rows)
+                residual_rmsnorm(self.streams[l], a, self.mixed[l], stream_out=self.attn_mid, weight=w[l], eps=self.eps)
+                layer(self.mixed[l], y=self.ys[l], ids=self.ids[l], weights=self.weights[l])
+                last = l + 1 == self.nl
+                residual_rmsnorm(self.attn_mid, self.ys[l], self.mixed[self.nl] if last else self.attn_in,
+                                 stream_out=self.streams[l + 1], weight=w[l + 1] if last else an[l + 1], eps=self.eps)
+        elif self.fused:
             if self.chain is not None:
                 self.chain.run(self.streams[0])
             else:

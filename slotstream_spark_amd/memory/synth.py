@@ -97,3 +97,18 @@ def head_weights(hidden: int, hc: int, lowrank: int, vocab: int, seed: int, devi
                        pre_fc_norm_embedding=norm_w(hidden), fc_embedding=proj(hidden, hidden),
                        pre_fc_norm_hidden=norm_w(n), fc_hidden=proj(hidden, hidden), mlp_hc=hcw(True),
                        mixer_hc=hcw(False))
+
+
+def attention_layer(hidden: int, heads: int, kv_heads: int, dim: int, seed: int, rot: int | None = None, base: float = 1e6,
+                    norms: bool = False, device="cuda", **kw):
+    """A random-init engine.attention.AttentionLayer: projections N(0, 1 / fan_in), frequencies base^(-2 i / rot), and with
+    `norms` q and k norms 1 + N(0, 0.1)."""
+    from ..engine.attention import AttentionLayer
+
+    half = (dim if rot is None else rot) // 2
+    f = base ** (-torch.arange(half, dtype=torch.float64) / half)
+    n = [(normal_bf16((dim,), 0.1, seed * 4 + 2 + i, device).float() + 1).to(torch.bfloat16) if norms else None
+         for i in range(2)]
+    return AttentionLayer(normal_bf16(((heads + 2 * kv_heads) * dim, hidden), hidden ** -0.5, seed * 4, device),
+                          normal_bf16((hidden, heads * dim), (heads * dim) ** -0.5, seed * 4 + 1, device), heads, kv_heads, dim,
+                          f.to(device), q_norm=n[0], k_norm=n[1], **kw)

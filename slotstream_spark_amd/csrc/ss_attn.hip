@@ -43,10 +43,14 @@ template <class T, int D, int NT, int W>
 __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16;
   constexpr bool kQLds = NT * KS > 8;  // more than 32 registers of queries stay in LDS, one copy for the waves
-  constexpr int VH = NT * D > 256 ? 2 : 1;  // parts that a tile's values are loaded in: the second where the keys were
+  // Parts that a tile's values are loaded in, each where operands that have been used were; LATE: the first one too waits
+  // for the keys' registers.
+  constexpr int VH = NT * D > 256 ? 2 : 1;
+  constexpr bool LATE = D == 256 && NT == 2;
+  constexpr int JH = D == 256 ? 2 : 1, JD = D / JH;  // parts of the dimensions that the waves' sums are joined in
   __shared__ ss_u32x4 q_lds[kQLds ? NT * KS : 1][64];
   __shared__ int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
-  __shared__ __attribute__((aligned(16))) float join_o[W][16][D + 4];
+  __shared__ __attribute__((aligned(16))) float join_o[W][16][JD + 4];
   __shared__ float join_m[W][NT][16], join_l[W][NT][16];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -147,22 +151,30 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
 #pragma unroll
       for (int d = 0; d < DT / VH; ++d) vf[d] = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (part * (DT / VH) + d) * page);
     };
-    load_v(0);
+    if (!LATE) load_v(0);
     __builtin_amdgcn_sched_barrier(0);
     const bool part_seen = !whole(t0, idv);
+    ss_f32x4 sv[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sv[n][t] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          sv[n][t] = T::mfma16(kf[t][ks], kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv[n][t]);
+      }
+    if (LATE) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     ss_u32x4 pf[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[8];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        ss_f32x4 sv = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          sv = T::mfma16(kf[t][ks], kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * t + i] = sv[i];
-      }
+      for (int e = 0; e < 8; ++e) x[e] = sv[n][e / 4][e % 4];
       if (part_seen) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = sees(t0 + 8 * g + e, qpos[n], idv) ? x[e] : kNegInf;
@@ -231,11 +243,13 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
     for (int k = 0; k < W; ++k) top = fmaxf(top, join_m[k][n][c]);
     const float f = m[n] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      ss_f32x4 o = acc[n][d];
+    for (int jh = 0; jh < JH; ++jh) {
+#pragma unroll
+    for (int dd = 0; dd < DT / JH; ++dd) {
+      ss_f32x4 o = acc[n][jh * (DT / JH) + dd];
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = m[n] == kNegInf ? o[i] : o[i] * f;
-      *reinterpret_cast<ss_f32x4*>(&join_o[w][c][16 * d + 4 * g]) = o;
+      *reinterpret_cast<ss_f32x4*>(&join_o[w][c][16 * dd + 4 * g]) = o;
     }
     if (any_odd) {
       // Infinities and NaN that were taken out of the wave's tiles, to the columns that see them.
@@ -251,8 +265,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
           ones[i] = (sees(tok, qpos[n], idv) ? T::kOne : 0u) | (sees(tok + 1, qpos[n], idv) ? T::kOne << 16 : 0u);
         }
 #pragma unroll 1
-        for (int d = 0; d < DT; ++d) {
-          const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * d * page);
+        for (int d = 0; d < DT / JH; ++d) {
+          const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (jh * (DT / JH) + d) * page);
 #pragma unroll 1
           for (int kind = 0; kind < 3; ++kind) {
             const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
@@ -266,8 +280,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
     }
     __syncthreads();
 #pragma unroll 1
-    for (int j = tid; j < 16 * (D / 4); j += 64 * W) {
-      const int col = j / (D / 4), d4 = 4 * (j % (D / 4));
+    for (int j = tid; j < 16 * (JD / 4); j += 64 * W) {
+      const int col = j / (JD / 4), dl = 4 * (j % (JD / 4)), d4 = jh * JD + dl;
       const int p = p0 + 16 * n + col;
       if (p < np) {
         float big = kNegInf, sum = 0.f;
@@ -278,10 +292,10 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
           const float mk = join_m[k][n][col];
           sum += mk == kNegInf ? join_l[k][n][col] : join_l[k][n][col] * __builtin_amdgcn_exp2f(mk - big);
         }
-        ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[0][col][d4]);
+        ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[0][col][dl]);
 #pragma unroll
         for (int k = 1; k < W; ++k) {
-          const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[k][col][d4]);
+          const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[k][col][dl]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] += x[i];
         }
@@ -305,6 +319,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
       }
     }
     __syncthreads();
+    }
   }
 }
 

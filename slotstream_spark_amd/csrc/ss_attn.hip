@@ -6,11 +6,17 @@
 //
 // The rows of a sequence times the heads of a key head are one "packed" axis: NT tiles of 16, the columns of
 // v_mfma_f32_16x16x32. A workgroup takes one chunk of the tokens of one (sequence, key head, NT tiles); its four waves
-// take the chunk's 32-token tiles in turn, each straight from memory into MFMA operands, no LDS:
+// take the chunk's 32-token tiles in turn:
 //   S^T = K Q^T: A row m of S tile t (0, 1) is token 8 (m / 4) + 4 t + m % 4, so lane (c, g) = (lane % 16, lane / 16) ends
 //     with the scores of column c at tokens 8 g + 0..7: its probabilities are, as they are, the B operand of
 //   O^T = V^T P^T, whose A operand is 8 consecutive tokens 8 g.. of dimension 16 d + c.
 // The running maximum is one value per column, equal in its four lanes; the sum of the weights stays per lane to the end.
+//
+// Each wave has a slot of LDS for a tile's keys and one for its values, filled by direct loads: the next tile's keys go out
+// when this one's scores are done, its values after the products, and nothing waits for another wave. (Operands straight from
+// memory into registers touch 16 rows with every load, 16 bytes of a row by lanes 16 apart, which the memory path takes as 64
+// accesses where rows of adjacent lanes are 16.) In LDS the 16-byte piece p of a row lies at p ^ swizzle(row), so that
+// the 16 rows of one operand read fall on different banks.
 //
 // A chunk begins at a multiple of its size from the sequence's first token and its tiles go to waves by their place in
 // it, and masked tokens add exact zeros: the bits of a row do not depend on the other rows of the call. The
@@ -18,7 +24,7 @@
 //
 // Values at places that a row does not see must not reach it, whatever they hold: a probability of 0 times an infinity is
 // not 0. Only tiles that some row does not see whole can hold such places. There the operand is searched for non-finite
-// values; where any are, they are taken out of the product and added back, by three more products with ones in their
+// values; where any are, they are taken out of the product and added at the join, by three more products with ones in their
 // places and ones for the tokens seen, to the rows that see them.
 #include <hip/hip_runtime.h>
 
@@ -39,19 +45,40 @@ SS_DEV float max_over_quads(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^
   return fmaxf(ss_uf(lo), ss_uf(hi));
 }
 
-template <class T, int D, int NT, int W>
-__global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnArgs a) {
-  constexpr int KS = D / 32, DT = D / 16;
+typedef __attribute__((address_space(3))) void lds_void;
+SS_DEV void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, 0, 0); }
+
+// s_waitcnt for all but the last `n` vector-memory operations (vmcnt in bits 3:0 and 15:14, the other counts at their maxima).
+template <int N>
+SS_DEV void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+
+// Where the 16-byte piece p of a key row lies: at p ^ key_swizzle(row). The 16 rows of an operand read differ in bits 0, 1, 3
+// and 4; a row of 64 dimensions is half of the 256 bytes that the banks cover (bit 0 says which), the others cover them.
+template <int D>
+SS_DEV constexpr int key_swizzle(int row) {
+  return D == 64 ? ((row >> 1) & 1) | ((row >> 3) & 3) << 1 : (row & 3) | ((row >> 3) & 3) << 2;
+}
+
+template <class T, int D, int NT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArgs a) {
+  constexpr int W = 4, KS = D / 32, DT = D / 16;
   constexpr bool kQLds = NT * KS > 8;  // more than 32 registers of queries stay in LDS, one copy for the waves
-  // Parts that a tile's values are loaded in, each where operands that have been used were; LATE: the first one too waits
-  // for the keys' registers.
-  constexpr int VH = NT * D > 256 ? 2 : 1;
-  constexpr bool LATE = D == 256 && NT == 2;
-  constexpr int JH = D == 256 ? 2 : 1, JD = D / JH;  // parts of the dimensions that the waves' sums are joined in
+  constexpr int KROW = D * 2, KC = D / 8, SLOT = 32 * KROW;  // bytes of a key row, its pieces; bytes of a slot
+  constexpr int LI = SLOT / 1024;                            // load instructions of a slot
+  constexpr int RK = 64 / KC;                                // key rows of one (of values 16: a row is 64 bytes)
+  constexpr int JH = 2, JD = D / JH;  // parts of the dimensions that the waves' sums are joined in
+  __shared__ __attribute__((aligned(1024))) uint8_t k_slot[W][SLOT];
+  __shared__ __attribute__((aligned(1024))) uint8_t v_slot[W][SLOT];
   __shared__ ss_u32x4 q_lds[kQLds ? NT * KS : 1][64];
-  __shared__ int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
-  __shared__ __attribute__((aligned(16))) float join_o[W][16][JD + 4];
+  __shared__ __attribute__((aligned(16))) int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
   __shared__ float join_m[W][NT][16], join_l[W][NT][16];
+  typedef float JoinRow[16][JD + 4];
+  JoinRow* join_o = reinterpret_cast<JoinRow*>(&k_slot[0][0]);  // after the last tile
+  static_assert(W * sizeof(JoinRow) <= W * SLOT, "the waves' sums fit the key slots");
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   int b = blockIdx.x;
@@ -122,7 +149,12 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
   __syncthreads();
 
   const int nt = (t_end - t_begin + 31) / 32;
-  auto unseen = [&](int t0) { return t0 >= sn.s_end && t0 + 32 <= sn.w_begin; };
+  // The wave's tiles: w, w + W, ... but those that no row sees, from the first tokens' end to the window's begin.
+  const int gap_a = (sn.s_end - t_begin + 31) >> 5, gap_b = (sn.w_begin - t_begin) >> 5;
+  auto next_tile = [&](int tt) {
+    if (tt >= gap_a && tt < gap_b) tt = gap_b + ((tt - gap_b) & (W - 1));
+    return tt;
+  };
   // Whether every row of the workgroup sees all 32 tokens.
   auto whole = [&](int t0, int idv) {
     return t0 + 31 <= pos_lo && (t0 > pos_hi - a.window || t0 + 32 <= a.sinks) && __all(idv >= 0);
@@ -130,45 +162,66 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
   auto sees = [&](int tok, int pos, int idv) {
     return idv >= 0 && tok <= pos && (tok > pos - a.window || tok < a.sinks);
   };
-  auto values = [&](int t0, int idv) {
-    return a.v + ((int64_t)max(idv, 0) * a.kv_heads + h) * page * D + (int64_t)c * page + ((t0 + 8 * g) & (page - 1));
+  const int64_t page_bytes = (int64_t)a.kv_heads * page * D * 2;
+  const char* kbase = reinterpret_cast<const char*>(a.k) + (int64_t)h * page * D * 2;
+  const char* vbase = reinterpret_cast<const char*>(a.v) + (int64_t)h * page * D * 2;
+  uint8_t* kl = k_slot[w];
+  uint8_t* vl = v_slot[w];
+  // What this lane fetches: in its n-th load of keys row n RK + lane / KC, of values row (dimension) 16 n + lane / 4.
+  const uint32_t koff = (lane / KC) * KROW + 16 * ((lane % KC) ^ key_swizzle<D>(lane / KC));
+  const int vpiece = (lane & 3) ^ ((lane >> 4) & 3);
+  auto load_k = [&](int tt) {
+    const int4 ids = *reinterpret_cast<const int4*>(&page_of[4 * tt]);
+    const int id[4] = {ids.x, ids.y, ids.z, ids.w};
+#pragma unroll
+    for (int n = 0; n < LI; ++n) {
+      const int row = n * RK, j = row / 8;  // a load's rows are of one 8-token group
+      const int64_t at = __builtin_amdgcn_readfirstlane(max(id[j], 0));
+      const int tok = (t_begin + 32 * tt + row) & (page - 1);
+      dma16(kbase + at * page_bytes + tok * KROW + (koff ^ (16 * key_swizzle<D>(row))), kl + 1024 * n);
+    }
+  };
+  auto load_v = [&](int tt) {
+    const int id = page_of[4 * tt + vpiece], tok = (t_begin + 32 * tt + 8 * vpiece) & (page - 1);
+    const char* at = vbase + max(id, 0) * page_bytes + ((int64_t)(lane >> 2) * page + tok) * 2;
+#pragma unroll
+    for (int n = 0; n < LI; ++n) dma16(at + (int64_t)n * 32 * page, vl + 1024 * n);
+  };
+  auto kread = [&](int t, int ks) {
+    const int row = 8 * (c >> 2) + 4 * t + (c & 3);
+    return *reinterpret_cast<const ss_u32x4*>(kl + row * KROW + 16 * ((4 * ks + g) ^ key_swizzle<D>(row)));
+  };
+  auto vread = [&](int d) {
+    return *reinterpret_cast<const ss_u32x4*>(vl + (16 * d + c) * 64 + 16 * (g ^ ((c >> 2) & 3)));
   };
   bool any_odd = false;
+  int tt = next_tile(w);
+  if (tt < nt) {
+    load_k(tt);
+    load_v(tt);
+  }
 #pragma unroll 1
-  for (int tt = w; tt < nt; tt += W) {
-    const int t0 = t_begin + 32 * tt;
-    if (unseen(t0)) continue;
-    const int idk = page_of[4 * tt + (c >> 2)], idv = page_of[4 * tt + g];
-    const int tk = (t0 + 8 * (c >> 2)) & (page - 1);
-    const uint16_t* kp = a.k + (((int64_t)max(idk, 0) * a.kv_heads + h) * page + tk + (c & 3)) * D + 8 * g;
-    const uint16_t* vp = values(t0, idv);
-    ss_u32x4 kf[2][KS], vf[DT / VH];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *(const SS_G ss_u32x4*)(kp + 4 * t * D + 32 * ks);
-    auto load_v = [&](int part) {
-#pragma unroll
-      for (int d = 0; d < DT / VH; ++d) vf[d] = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (part * (DT / VH) + d) * page);
-    };
-    if (!LATE) load_v(0);
-    __builtin_amdgcn_sched_barrier(0);
+  while (tt < nt) {
+    const int t0 = t_begin + 32 * tt, idv = page_of[4 * tt + g];
+    const int tn = next_tile(tt + W), tl = min(tn, nt - 1);  // past the last tile one more is loaded and not used
     const bool part_seen = !whole(t0, idv);
+    wait_loads<LI>();  // this tile's keys are there, its values may be on their way
     ss_f32x4 sv[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sv[n][t] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t) sv[n][t] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          sv[n][t] = T::mfma16(kf[t][ks], kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv[n][t]);
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const ss_u32x4 kf = kread(t, ks);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          sv[n][t] = T::mfma16(kf, kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv[n][t]);
       }
-    if (LATE) {
-      __builtin_amdgcn_sched_barrier(0);
-      load_v(0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    __builtin_amdgcn_sched_barrier(0);  // the reads above have been used, so the slot may be filled again
+    load_k(tl);
     ss_u32x4 pf[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -203,28 +256,36 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[n][i] = T::pack(p[2 * i], p[2 * i + 1]);
     }
+    wait_loads<LI>();  // this tile's values are there, the next one's keys may be on their way
+    bool odd = false;
+    if (part_seen) {
 #pragma unroll
-    for (int part = 0; part < VH; ++part) {
-      if (part_seen) {
-        bool odd = false;
+      for (int d = 0; d < DT; ++d) {
+        const ss_u32x4 vf = vread(d);
 #pragma unroll
-        for (int d = 0; d < DT / VH; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) odd |= nonfinite2<T>(vf[d][i]);
-        if (__any(odd)) {
-          any_odd = true;
-#pragma unroll
-          for (int d = 0; d < DT / VH; ++d) vf[d] = parts_of<T>(vf[d], -1);
-        }
+        for (int i = 0; i < 4; ++i) odd |= nonfinite2<T>(vf[i]);
       }
-#pragma unroll
-      for (int d = 0; d < DT / VH; ++d)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          acc[n][part * (DT / VH) + d] = T::mfma16(vf[d], pf[n], acc[n][part * (DT / VH) + d]);
-      if (part + 1 < VH) load_v(part + 1);
+      odd = __any(odd);
+      any_odd |= odd;
     }
+    if (odd) {  // the wave's own slot: cleaned in place
+#pragma unroll 1
+      for (int d = 0; d < DT; ++d) {
+        const ss_u32x4 vf = vread(d);
+        *reinterpret_cast<ss_u32x4*>(vl + (16 * d + c) * 64 + 16 * (g ^ ((c >> 2) & 3))) = parts_of<T>(vf, -1);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const ss_u32x4 vf = vread(d);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[n][d] = T::mfma16(vf, pf[n], acc[n][d]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(tl);
+    tt = tn;
   }
+  wait_loads<0>();  // no load into LDS outlives the tiles
 
   // The waves' sums, weighted by how far each wave's maximum is below the largest.
 #pragma unroll
@@ -254,10 +315,11 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void attn_few_kernel(AttnAr
     if (any_odd) {
       // Infinities and NaN that were taken out of the wave's tiles, to the columns that see them.
 #pragma unroll 1
-      for (int tt = w; tt < nt; tt += W) {
+      for (int tt = next_tile(w); tt < nt; tt = next_tile(tt + W)) {
         const int t0 = t_begin + 32 * tt, idv = page_of[4 * tt + g];
-        if (unseen(t0) || whole(t0, idv)) continue;
-        const uint16_t* vp = values(t0, idv);
+        if (whole(t0, idv)) continue;
+        const uint16_t* vp = reinterpret_cast<const uint16_t*>(vbase + max(idv, 0) * page_bytes) + (int64_t)c * page +
+                             ((t0 + 8 * g) & (page - 1));
         ss_u32x4 ones;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -397,7 +459,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 template <class T, int D, int NT>
 hipError_t launch_few(const AttnArgs& a, hipStream_t st) {
   const unsigned grid = (unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs);
-  hipLaunchKernelGGL((attn_few_kernel<T, D, NT, 4>), dim3(grid), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((attn_few_kernel<T, D, NT>), dim3(grid), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

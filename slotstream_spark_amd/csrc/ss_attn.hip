@@ -48,6 +48,13 @@ SS_DEV float max_over_quads(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^
 typedef __attribute__((address_space(3))) void lds_void;
 SS_DEV void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, 0, 0); }
 
+// A barrier over LDS alone: it waits for no load or store in flight.
+SS_DEV void local_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // s_waitcnt for all but the last `n` vector-memory operations (vmcnt in bits 3:0 and 15:14, the other counts at their maxima).
 template <int N>
 SS_DEV void wait_loads() {
@@ -64,21 +71,25 @@ SS_DEV constexpr int key_swizzle(int row) {
 }
 
 template <class T, int D, int NT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   constexpr int W = 4, KS = D / 32, DT = D / 16;
   constexpr bool kQLds = NT * KS > 8;  // more than 32 registers of queries stay in LDS, one copy for the waves
   constexpr int KROW = D * 2, KC = D / 8, SLOT = 32 * KROW;  // bytes of a key row, its pieces; bytes of a slot
   constexpr int LI = SLOT / 1024;                            // load instructions of a slot
   constexpr int RK = 64 / KC;                                // key rows of one (of values 16: a row is 64 bytes)
-  constexpr int JH = 2, JD = D / JH;  // parts of the dimensions that the waves' sums are joined in
-  __shared__ __attribute__((aligned(1024))) uint8_t k_slot[W][SLOT];
+  constexpr int JH = 2, JD = D / JH;  // the waves' sums are joined in two halves of the dimensions, one where the keys were
+  // Keys and queries in dynamic LDS: where all of it is static and leaves room for one workgroup a CU, the compiler takes 512
+  // registers a wave and moves sums between their halves for every product (8 sequences of up to 8,192 tokens, 3 rows, 256
+  // dimensions: 22.4 us; so 21.2).
+  extern __shared__ __attribute__((aligned(1024))) uint8_t dyn_lds[];
   __shared__ __attribute__((aligned(1024))) uint8_t v_slot[W][SLOT];
-  __shared__ ss_u32x4 q_lds[kQLds ? NT * KS : 1][64];
+  uint8_t* const k_slot = dyn_lds;
+  ss_u32x4(*const q_lds)[64] = reinterpret_cast<ss_u32x4(*)[64]>(dyn_lds + W * SLOT);
   __shared__ __attribute__((aligned(16))) int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
   __shared__ float join_m[W][NT][16], join_l[W][NT][16];
   typedef float JoinRow[16][JD + 4];
-  JoinRow* join_o = reinterpret_cast<JoinRow*>(&k_slot[0][0]);  // after the last tile
-  static_assert(W * sizeof(JoinRow) <= W * SLOT, "the waves' sums fit the key slots");
+  JoinRow* const join_o[JH] = {reinterpret_cast<JoinRow*>(k_slot), reinterpret_cast<JoinRow*>(&v_slot[0][0])};
+  static_assert(sizeof(JoinRow) <= SLOT, "the waves' sums fit the slots");
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   int b = blockIdx.x;
@@ -119,7 +130,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
     }
     page_of[j] = id;
   }
-  ss_u32x4 qf[kQLds ? 1 : NT][KS];
+  // Queries: the four waves share the loads where they stay in LDS. They are not waited for before the tiles' first loads.
+  constexpr int QS = (NT * KS + W - 1) / W;
+  ss_u32x4 qf[kQLds ? 1 : NT][KS], qs[kQLds ? QS : 1];
   int qpos[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -131,7 +144,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if constexpr (kQLds) {
-        if ((n * KS + ks) % W == w) q_lds[n * KS + ks][lane] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
+        if ((n * KS + ks) % W == w) qs[(n * KS + ks) / W] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
       } else {
         qf[n][ks] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
       }
@@ -146,7 +159,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[n][d] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  __syncthreads();
+  local_barrier();
 
   const int nt = (t_end - t_begin + 31) / 32;
   // The wave's tiles: w, w + W, ... but those that no row sees, from the first tokens' end to the window's begin.
@@ -165,7 +178,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
   const int64_t page_bytes = (int64_t)a.kv_heads * page * D * 2;
   const char* kbase = reinterpret_cast<const char*>(a.k) + (int64_t)h * page * D * 2;
   const char* vbase = reinterpret_cast<const char*>(a.v) + (int64_t)h * page * D * 2;
-  uint8_t* kl = k_slot[w];
+  uint8_t* kl = k_slot + w * SLOT;
   uint8_t* vl = v_slot[w];
   // What this lane fetches: in its n-th load of keys row n RK + lane / KC, of values row (dimension) 16 n + lane / 4.
   const uint32_t koff = (lane / KC) * KROW + 16 * ((lane % KC) ^ key_swizzle<D>(lane / KC));
@@ -199,6 +212,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
   if (tt < nt) {
     load_k(tt);
     load_v(tt);
+  }
+  if constexpr (kQLds) {
+#pragma unroll
+    for (int q = 0; q < QS; ++q)
+      if (q * W + w < NT * KS) q_lds[q * W + w][lane] = qs[q];
+    local_barrier();
   }
 #pragma unroll 1
   while (tt < nt) {
@@ -296,7 +315,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
       join_l[w][n][c] = l[n];
     }
   }
-  __syncthreads();
+  local_barrier();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float top = kNegInf;
@@ -304,13 +323,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
     for (int k = 0; k < W; ++k) top = fmaxf(top, join_m[k][n][c]);
     const float f = m[n] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
 #pragma unroll
-    for (int jh = 0; jh < JH; ++jh) {
-#pragma unroll
-    for (int dd = 0; dd < DT / JH; ++dd) {
-      ss_f32x4 o = acc[n][jh * (DT / JH) + dd];
+    for (int d = 0; d < DT; ++d) {
+      ss_f32x4 o = acc[n][d];
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = m[n] == kNegInf ? o[i] : o[i] * f;
-      *reinterpret_cast<ss_f32x4*>(&join_o[w][c][16 * dd + 4 * g]) = o;
+      *reinterpret_cast<ss_f32x4*>(&join_o[d / (DT / JH)][w][c][16 * (d % (DT / JH)) + 4 * g]) = o;
     }
     if (any_odd) {
       // Infinities and NaN that were taken out of the wave's tiles, to the columns that see them.
@@ -326,26 +343,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
           const int tok = t0 + 8 * g + 2 * i;
           ones[i] = (sees(tok, qpos[n], idv) ? T::kOne : 0u) | (sees(tok + 1, qpos[n], idv) ? T::kOne << 16 : 0u);
         }
-#pragma unroll 1
-        for (int d = 0; d < DT / JH; ++d) {
-          const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (jh * (DT / JH) + d) * page);
-#pragma unroll 1
-          for (int kind = 0; kind < 3; ++kind) {
-            const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
-            const ss_f32x4 hits = T::mfma16(parts_of<T>(v, kind), ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (hits[i] > 0.f) join_o[w][c][16 * d + 4 * g + i] += add;
+        for (int jh = 0; jh < JH; ++jh)
+#pragma unroll 1
+          for (int d = 0; d < DT / JH; ++d) {
+            const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (jh * (DT / JH) + d) * page);
+#pragma unroll 1
+            for (int kind = 0; kind < 3; ++kind) {
+              const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+              const ss_f32x4 hits = T::mfma16(parts_of<T>(v, kind), ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (hits[i] > 0.f) join_o[jh][w][c][16 * d + 4 * g + i] += add;
+            }
           }
-        }
       }
     }
-    __syncthreads();
+    local_barrier();
+#pragma unroll
+    for (int jh = 0; jh < JH; ++jh)
 #pragma unroll 1
-    for (int j = tid; j < 16 * (JD / 4); j += 64 * W) {
-      const int col = j / (JD / 4), dl = 4 * (j % (JD / 4)), d4 = jh * JD + dl;
-      const int p = p0 + 16 * n + col;
-      if (p < np) {
+      for (int j = tid; j < 16 * (JD / 4); j += 256) {
+        const int col = j / (JD / 4), dl = 4 * (j % (JD / 4)), d4 = jh * JD + dl;
+        const int p = p0 + 16 * n + col;
+        if (p >= np) continue;
         float big = kNegInf, sum = 0.f;
 #pragma unroll
         for (int k = 0; k < W; ++k) big = fmaxf(big, join_m[k][n][col]);
@@ -354,10 +375,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
           const float mk = join_m[k][n][col];
           sum += mk == kNegInf ? join_l[k][n][col] : join_l[k][n][col] * __builtin_amdgcn_exp2f(mk - big);
         }
-        ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[0][col][dl]);
+        ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[jh][0][col][dl]);
 #pragma unroll
         for (int k = 1; k < W; ++k) {
-          const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[k][col][dl]);
+          const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[jh][k][col][dl]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] += x[i];
         }
@@ -379,9 +400,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnArg
           if (a.lse && d4 == 0) a.lse[at] = sum == 0.f ? kNegInf : (big + __log2f(sum)) * 0.693147180559945309f;
         }
       }
-    }
-    __syncthreads();
-    }
+    if (n + 1 < NT) local_barrier();
   }
 }
 
@@ -458,8 +477,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 template <class T, int D, int NT>
 hipError_t launch_few(const AttnArgs& a, hipStream_t st) {
+  constexpr size_t kDyn = 4 * 32 * D * 2 + (NT * D / 32 > 8 ? NT * (D / 32) * 1024 : 0);  // key slots, queries
+  const auto kern = attn_few_kernel<T, D, NT>;
+  KernelCfg cfg;
+  const hipError_t e = kernel_cfg(reinterpret_cast<const void*>(kern), 256, kDyn, &cfg);  // raises the kernel's LDS limit
+  if (e != hipSuccess) return e;
   const unsigned grid = (unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs);
-  hipLaunchKernelGGL((attn_few_kernel<T, D, NT>), dim3(grid), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), kDyn, st, a);
   return hipGetLastError();
 }
 

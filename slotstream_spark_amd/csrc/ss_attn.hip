@@ -46,7 +46,8 @@ SS_DEV float max_over_quads(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
-SS_DEV void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, 0, 0); }
+template <int OFF>  // bytes added to both addresses
+SS_DEV void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, OFF, 0); }
 
 // A barrier over LDS alone: it waits for no load or store in flight.
 SS_DEV void local_barrier() {
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   constexpr int RK = 64 / KC;                                // key rows of one (of values 16: a row is 64 bytes)
   constexpr int JH = 2, JD = D / JH;  // the waves' sums are joined in two halves of the dimensions, one where the keys were
   // Keys and queries in dynamic LDS: where all of it is static and leaves room for one workgroup a CU, the compiler takes 512
-  // registers a wave and moves sums between their halves for every product (8 sequences of up to 8,192 tokens, 3 rows, 256
+  // registers a wave and moves sums between their halves for every product (8 sequences of up to 6,145 tokens, 3 rows, 256
   // dimensions: 22.4 us; so 21.2).
   extern __shared__ __attribute__((aligned(1024))) uint8_t dyn_lds[];
   __shared__ __attribute__((aligned(1024))) uint8_t v_slot[W][SLOT];
@@ -87,17 +88,20 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   ss_u32x4(*const q_lds)[64] = reinterpret_cast<ss_u32x4(*)[64]>(dyn_lds + W * SLOT);
   __shared__ __attribute__((aligned(16))) int32_t page_of[512];  // page of each 8-token group of the chunk, -1: none
   __shared__ float join_m[W][NT][16], join_l[W][NT][16];
+  __shared__ ss_f32x4 join_f[NT * 16];
+  __shared__ int64_t join_at[NT * 16];
+  __shared__ int32_t qpos[NT * 16];  // positions of the columns' rows, -1: none
   typedef float JoinRow[16][JD + 4];
   JoinRow* const join_o[JH] = {reinterpret_cast<JoinRow*>(k_slot), reinterpret_cast<JoinRow*>(&v_slot[0][0])};
   static_assert(sizeof(JoinRow) <= SLOT, "the waves' sums fit the slots");
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
-  int b = blockIdx.x;
-  const int slot = b % a.slots;
-  b /= a.slots;
-  const int tile = b % a.tiles;
-  b /= a.tiles;
-  const int h = b % a.kv_heads, s = b / a.kv_heads;
+  uint32_t b = blockIdx.x;
+  const int slot = b % (uint32_t)a.slots;
+  b /= (uint32_t)a.slots;
+  const int tile = b % (uint32_t)a.tiles;
+  b /= (uint32_t)a.tiles;
+  const int h = b % (uint32_t)a.kv_heads, s = b / (uint32_t)a.kv_heads;
   const int page = 1 << a.page_shift;
   // Without a window the chunk is the slot, and its pages are asked for before the sequence's length is known.
   const bool all = a.window >= (1 << 30);
@@ -108,7 +112,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width * page, a.err);
   const int p0 = tile * NT * 16, np = sr.n * a.group;  // packed rows [p0, min(p0 + 16 NT, np))
   if (p0 >= np) return;                                // whole workgroup, before any barrier
-  const int i0 = p0 / a.group, i1 = (min(p0 + NT * 16, np) - 1) / a.group;
+  const uint32_t group = a.group;
+  const int i0 = p0 / group, i1 = (min(p0 + NT * 16, np) - 1) / group;
   const int pos_lo = sr.pos0 + i0, pos_hi = sr.pos0 + i1;
   const Seen sn = seen_tokens(pos_lo, pos_hi, sr.end, a.window, a.sinks);
   // Slots cover the chunks that hold first tokens, then those from the window's on.
@@ -131,20 +136,18 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     page_of[j] = id;
   }
   // Queries: the four waves share the loads where they stay in LDS. They are not waited for before the tiles' first loads.
-  constexpr int QS = (NT * KS + W - 1) / W;
-  ss_u32x4 qf[kQLds ? 1 : NT][KS], qs[kQLds ? QS : 1];
-  int qpos[NT];
+  ss_u32x4 qf[kQLds ? 1 : NT][KS];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int p = p0 + 16 * n + c, i = p / a.group;
+    const int p = p0 + 16 * n + c, i = p / group;
     const bool in = p < np;
-    qpos[n] = in ? sr.pos0 + i : -1;
+    if (w == 0) qpos[16 * n + c] = in ? sr.pos0 + i : -1;
     const uint16_t* qp = a.q + (int64_t)(sr.r0 + (in ? i : 0)) * a.q_row +
                          (int64_t)(h * a.group + (in ? p - i * a.group : 0)) * a.q_head + 8 * g;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if constexpr (kQLds) {
-        if ((n * KS + ks) % W == w) qs[(n * KS + ks) / W] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
+        if ((n * KS + ks) % W == w) dma16<0>(qp + 32 * ks, &q_lds[n * KS + ks][0]);
       } else {
         qf[n][ks] = *(const SS_G ss_u32x4*)(qp + 32 * ks);
       }
@@ -175,30 +178,44 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   auto sees = [&](int tok, int pos, int idv) {
     return idv >= 0 && tok <= pos && (tok > pos - a.window || tok < a.sinks);
   };
-  const int64_t page_bytes = (int64_t)a.kv_heads * page * D * 2;
+  const uint32_t page_bytes = (uint32_t)a.kv_heads * page * D * 2;
   const char* kbase = reinterpret_cast<const char*>(a.k) + (int64_t)h * page * D * 2;
   const char* vbase = reinterpret_cast<const char*>(a.v) + (int64_t)h * page * D * 2;
   uint8_t* kl = k_slot + w * SLOT;
   uint8_t* vl = v_slot[w];
-  // What this lane fetches: in its n-th load of keys row n RK + lane / KC, of values row (dimension) 16 n + lane / 4.
+  // What this lane fetches: in its n-th load of keys row n RK + lane / KC, of values row (dimension) 16 n + lane / 4. The rows
+  // of 8 keys lie as close in a page as in the slot, so one address serves them with a constant added to both.
   const uint32_t koff = (lane / KC) * KROW + 16 * ((lane % KC) ^ key_swizzle<D>(lane / KC));
   const int vpiece = (lane & 3) ^ ((lane >> 4) & 3);
   auto load_k = [&](int tt) {
     const int4 ids = *reinterpret_cast<const int4*>(&page_of[4 * tt]);
     const int id[4] = {ids.x, ids.y, ids.z, ids.w};
 #pragma unroll
-    for (int n = 0; n < LI; ++n) {
-      const int row = n * RK, j = row / 8;  // a load's rows are of one 8-token group
-      const int64_t at = __builtin_amdgcn_readfirstlane(max(id[j], 0));
-      const int tok = (t_begin + 32 * tt + row) & (page - 1);
-      dma16(kbase + at * page_bytes + tok * KROW + (koff ^ (16 * key_swizzle<D>(row))), kl + 1024 * n);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = __builtin_amdgcn_readfirstlane(max(id[j], 0));
+      const uint32_t tok = (t_begin + 32 * tt + 8 * j) & (page - 1);
+      const char* from = kbase + ((uint64_t)at * page_bytes + tok * KROW);
+      uint8_t* to = kl + 8 * KROW * j;
+      dma16<0>(from + (koff ^ (16 * key_swizzle<D>(8 * j))), to);
+      if constexpr (LI >= 8) dma16<1024>(from + (koff ^ (16 * key_swizzle<D>(8 * j + RK))), to);
+      if constexpr (LI >= 16) {
+        dma16<2048>(from + (koff ^ (16 * key_swizzle<D>(8 * j + 2 * RK))), to);
+        dma16<3 * 1024>(from + (koff ^ (16 * key_swizzle<D>(8 * j + 3 * RK))), to);
+      }
     }
   };
   auto load_v = [&](int tt) {
     const int id = page_of[4 * tt + vpiece], tok = (t_begin + 32 * tt + 8 * vpiece) & (page - 1);
-    const char* at = vbase + max(id, 0) * page_bytes + ((int64_t)(lane >> 2) * page + tok) * 2;
+    const char* at = vbase + ((uint64_t)(uint32_t)max(id, 0) * page_bytes + ((lane >> 2) * page + tok) * 2);
+    const int64_t step = 32 * page;
 #pragma unroll
-    for (int n = 0; n < LI; ++n) dma16(at + (int64_t)n * 32 * page, vl + 1024 * n);
+    for (int n = 0; n < LI; n += 4) {
+      dma16<0>(at, vl + 1024 * n);
+      dma16<1024>(at += step - 1024, vl + 1024 * n);
+      dma16<2048>(at += step - 1024, vl + 1024 * n);
+      dma16<3 * 1024>(at += step - 1024, vl + 1024 * n);
+      at += step + 3 * 1024;
+    }
   };
   auto kread = [&](int t, int ks) {
     const int row = 8 * (c >> 2) + 4 * t + (c & 3);
@@ -208,103 +225,112 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     return *reinterpret_cast<const ss_u32x4*>(vl + (16 * d + c) * 64 + 16 * (g ^ ((c >> 2) & 3)));
   };
   bool any_odd = false;
-  int tt = next_tile(w);
-  if (tt < nt) {
-    load_k(tt);
-    load_v(tt);
-  }
-  if constexpr (kQLds) {
-#pragma unroll
-    for (int q = 0; q < QS; ++q)
-      if (q * W + w < NT * KS) q_lds[q * W + w][lane] = qs[q];
-    local_barrier();
-  }
+  // The loop's first turn has no tile yet and only loads. A wave issues an instruction in some 5 cycles, so short calls go by
+  // how many they execute: with the first loads in the loop, one address for 8 keys, the columns' factors worked out
+  // once and the maximum raised lazily, a sequence of 32 tokens takes 8.4 us at 256 dimensions and two column tiles (12.5
+  // without), 4.2 at 128 and one (4.5).
+  int tt = nt > 0 ? -1 : 0, tn = next_tile(w);
 #pragma unroll 1
   while (tt < nt) {
-    const int t0 = t_begin + 32 * tt, idv = page_of[4 * tt + g];
-    const int tn = next_tile(tt + W), tl = min(tn, nt - 1);  // past the last tile one more is loaded and not used
+    const int t0 = t_begin + 32 * tt, idv = page_of[4 * max(tt, 0) + g];
+    const bool more = tn < nt;
     const bool part_seen = !whole(t0, idv);
-    wait_loads<LI>();  // this tile's keys are there, its values may be on their way
     ss_f32x4 sv[NT][2];
+    if (tt >= 0) {
+      wait_loads<LI>();  // this tile's keys are there, its values may be on their way
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) sv[n][t] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 2; ++t) sv[n][t] = ss_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const ss_u32x4 kf = kread(t, ks);
+        for (int t = 0; t < 2; ++t) {
+          const ss_u32x4 kf = kread(t, ks);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          sv[n][t] = T::mfma16(kf, kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv[n][t]);
-      }
+          for (int n = 0; n < NT; ++n)
+            sv[n][t] = T::mfma16(kf, kQLds ? q_lds[n * KS + ks][lane] : qf[kQLds ? 0 : n][ks], sv[n][t]);
+        }
+    }
     __builtin_amdgcn_sched_barrier(0);  // the reads above have been used, so the slot may be filled again
-    load_k(tl);
-    ss_u32x4 pf[NT];
+    if (more) load_k(tn);
+    if (tt >= 0) {
+      ss_u32x4 pf[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float x[8];
+      for (int n = 0; n < NT; ++n) {
+        float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = sv[n][e / 4][e % 4];
-      if (part_seen) {
+        for (int e = 0; e < 8; ++e) x[e] = sv[n][e / 4][e % 4];
+        if (part_seen) {
+          const int pos = qpos[16 * n + c];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = sees(t0 + 8 * g + e, qpos[n], idv) ? x[e] : kNegInf;
+          for (int e = 0; e < 8; ++e) x[e] = sees(t0 + 8 * g + e, pos, idv) ? x[e] : kNegInf;
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+        mx = max_over_quads(mx) * a.scale - T::kShift;
+        // The maximum is raised where it is passed by more than kLazy: the weights are at most 2^kLazy until then.
+        const float mn = mx > m[n] + T::kLazy ? mx : m[n];
+        const float mu = mn == kNegInf ? 0.f : mn;
+        if (__any(mn > m[n] && m[n] != kNegInf)) {
+          const float f = __builtin_amdgcn_exp2f(m[n] - mu);
+          l[n] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][d][i] *= f;
+        }
+        m[n] = mn;
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -mu));
+          l[n] += p[e];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pf[n][i] = T::pack(p[2 * i], p[2 * i + 1]);
       }
-      float mx = x[0];
+      // This tile's values are there, the next one's keys may be on their way.
+      if (more)
+        wait_loads<LI>();
+      else
+        wait_loads<0>();
+      bool odd = false;
+      if (part_seen) {  // zero times the values is zero where all are finite
+        ss_f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-      mx = max_over_quads(mx) * a.scale - T::kShift;
-      const float mn = fmaxf(m[n], mx);
-      const float mu = mn == kNegInf ? 0.f : mn;
-      if (__any(mn > m[n])) {
-        const float f = __builtin_amdgcn_exp2f(m[n] - mu);
-        l[n] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][d][i] *= f;
+        for (int d = 0; d < DT; ++d) z = T::mfma16(vread(d), ss_u32x4{0u, 0u, 0u, 0u}, z);
+        odd = __any(z[0] != 0.f || z[1] != 0.f || z[2] != 0.f || z[3] != 0.f);
+        any_odd |= odd;
       }
-      m[n] = mn;
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -mu));
-        l[n] += p[e];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pf[n][i] = T::pack(p[2 * i], p[2 * i + 1]);
-    }
-    wait_loads<LI>();  // this tile's values are there, the next one's keys may be on their way
-    bool odd = false;
-    if (part_seen) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const ss_u32x4 vf = vread(d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) odd |= nonfinite2<T>(vf[i]);
-      }
-      odd = __any(odd);
-      any_odd |= odd;
-    }
-    if (odd) {  // the wave's own slot: cleaned in place
+      if (odd) {  // the wave's own slot: cleaned in place
 #pragma unroll 1
+        for (int d = 0; d < DT; ++d) {
+          const ss_u32x4 vf = vread(d);
+          *reinterpret_cast<ss_u32x4*>(vl + (16 * d + c) * 64 + 16 * (g ^ ((c >> 2) & 3))) = parts_of<T>(vf, -1);
+        }
+      }
+#pragma unroll
       for (int d = 0; d < DT; ++d) {
         const ss_u32x4 vf = vread(d);
-        *reinterpret_cast<ss_u32x4*>(vl + (16 * d + c) * 64 + 16 * (g ^ ((c >> 2) & 3))) = parts_of<T>(vf, -1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][d] = T::mfma16(vf, pf[n], acc[n][d]);
       }
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const ss_u32x4 vf = vread(d);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n][d] = T::mfma16(vf, pf[n], acc[n][d]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_v(tl);
+    if (more) load_v(tn);
+    if constexpr (kQLds)
+      if (tt < 0) {
+        if (more)
+          wait_loads<2 * LI>();  // the queries are older than the tile
+        else
+          wait_loads<0>();
+        local_barrier();
+      }
     tt = tn;
+    tn = next_tile(tt + W);
   }
-  wait_loads<0>();  // no load into LDS outlives the tiles
 
   // The waves' sums, weighted by how far each wave's maximum is below the largest.
 #pragma unroll
@@ -315,22 +341,50 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       join_l[w][n][c] = l[n];
     }
   }
-  local_barrier();
+  local_barrier();  // all waves are done with their tiles as well
+  const float* const jm = &join_m[0][0][0];
+  const float* const jl = &join_l[0][0][0];
+  if (tid < 16 * NT && p0 + tid < np) {
+    // A column: the waves' factors, and where its row and head lie.
+    constexpr int WS = 16 * NT;
+    float big = kNegInf, sum = 0.f;
+    ss_f32x4 f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float top = kNegInf;
+    for (int k = 0; k < W; ++k) big = fmaxf(big, jm[WS * k + tid]);
 #pragma unroll
-    for (int k = 0; k < W; ++k) top = fmaxf(top, join_m[k][n][c]);
-    const float f = m[n] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      ss_f32x4 o = acc[n][d];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = m[n] == kNegInf ? o[i] : o[i] * f;
-      *reinterpret_cast<ss_f32x4*>(&join_o[d / (DT / JH)][w][c][16 * (d % (DT / JH)) + 4 * g]) = o;
+    for (int k = 0; k < W; ++k) {
+      const float mk = jm[WS * k + tid];
+      f[k] = mk == kNegInf ? 1.f : __builtin_amdgcn_exp2f(mk - big);
+      sum += jl[WS * k + tid] * f[k];
     }
+    const int p = p0 + tid, i = p / group;
+    int64_t at = (int64_t)(sr.r0 + i) * a.heads + h * a.group + (p - i * a.group);
+    if (a.slots > 1) {
+      at += (int64_t)slot * a.rows * a.heads;
+      gp(a.pml)[2 * at] = big;
+      gp(a.pml)[2 * at + 1] = sum;
+    } else {
+      const float r = sum == 0.f ? 0.f : 1.f / sum;
+      if (a.lse) a.lse[at] = sum == 0.f ? kNegInf : (big + __log2f(sum)) * 0.693147180559945309f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) f[k] *= r;
+    }
+    join_f[tid] = f;
+    join_at[tid] = at * D;
+  }
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {
+    if (n) local_barrier();  // the last columns are read
+#pragma unroll
+    for (int k = 0; k < NT; ++k)
+      if (k == n) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          *reinterpret_cast<ss_f32x4*>(&join_o[d / (DT / JH)][w][c][16 * (d % (DT / JH)) + 4 * g]) = acc[k][d];
+      }
     if (any_odd) {
       // Infinities and NaN that were taken out of the wave's tiles, to the columns that see them.
+      const int pos = qpos[16 * n + c];
 #pragma unroll 1
       for (int tt = next_tile(w); tt < nt; tt = next_tile(tt + W)) {
         const int t0 = t_begin + 32 * tt, idv = page_of[4 * tt + g];
@@ -341,66 +395,46 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tok = t0 + 8 * g + 2 * i;
-          ones[i] = (sees(tok, qpos[n], idv) ? T::kOne : 0u) | (sees(tok + 1, qpos[n], idv) ? T::kOne << 16 : 0u);
+          ones[i] = (sees(tok, pos, idv) ? T::kOne : 0u) | (sees(tok + 1, pos, idv) ? T::kOne << 16 : 0u);
         }
-#pragma unroll
-        for (int jh = 0; jh < JH; ++jh)
 #pragma unroll 1
-          for (int d = 0; d < DT / JH; ++d) {
-            const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * (jh * (DT / JH) + d) * page);
+        for (int d = 0; d < DT; ++d) {
+          const ss_u32x4 v = *(const SS_G ss_u32x4*)(vp + (int64_t)16 * d * page);
+          float* o = &(d < DT / JH ? join_o[0] : join_o[1])[w][c][16 * (d % (DT / JH)) + 4 * g];
 #pragma unroll 1
-            for (int kind = 0; kind < 3; ++kind) {
-              const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
-              const ss_f32x4 hits = T::mfma16(parts_of<T>(v, kind), ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
+          for (int kind = 0; kind < 3; ++kind) {
+            const float add = kind == 0 ? -kNegInf : kind == 1 ? kNegInf : __builtin_nanf("");
+            const ss_f32x4 hits = T::mfma16(parts_of<T>(v, kind), ones, ss_f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (hits[i] > 0.f) join_o[jh][w][c][16 * d + 4 * g + i] += add;
-            }
+            for (int i = 0; i < 4; ++i)
+              if (hits[i] > 0.f) o[i] += add;
           }
+        }
       }
     }
     local_barrier();
-#pragma unroll
-    for (int jh = 0; jh < JH; ++jh)
+    const int d4 = 4 * (tid % (D / 4));
+    const JoinRow* jo = d4 < JD ? join_o[0] : join_o[1];
 #pragma unroll 1
-      for (int j = tid; j < 16 * (JD / 4); j += 256) {
-        const int col = j / (JD / 4), dl = 4 * (j % (JD / 4)), d4 = jh * JD + dl;
-        const int p = p0 + 16 * n + col;
-        if (p >= np) continue;
-        float big = kNegInf, sum = 0.f;
+    for (int col = tid / (D / 4); col < min(16, np - p0 - 16 * n); col += 1024 / D) {
+      const ss_f32x4 f = join_f[16 * n + col];
+      ss_f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < W; ++k) big = fmaxf(big, join_m[k][n][col]);
+      for (int k = 0; k < W; ++k) {
+        const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&jo[k][col][d4 % JD]);
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const float mk = join_m[k][n][col];
-          sum += mk == kNegInf ? join_l[k][n][col] : join_l[k][n][col] * __builtin_amdgcn_exp2f(mk - big);
-        }
-        ss_f32x4 o = *reinterpret_cast<const ss_f32x4*>(&join_o[jh][0][col][dl]);
-#pragma unroll
-        for (int k = 1; k < W; ++k) {
-          const ss_f32x4 x = *reinterpret_cast<const ss_f32x4*>(&join_o[jh][k][col][dl]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] += x[i];
-        }
-        const int i = p / a.group;
-        const int64_t at = (int64_t)(sr.r0 + i) * a.heads + h * a.group + (p - i * a.group);
-        if (a.slots > 1) {
-          const int64_t pa = (int64_t)slot * a.rows * a.heads + at;
-          *reinterpret_cast<SS_G ss_f32x4*>(gp(a.po) + pa * D + d4) = o;
-          if (d4 == 0) {
-            gp(a.pml)[2 * pa] = big;
-            gp(a.pml)[2 * pa + 1] = sum;
-          }
-        } else {
-          const float r = sum == 0.f ? 0.f : 1.f / sum;
-          uint2 word;
-          word.x = T::pack(o[0] * r, o[1] * r);
-          word.y = T::pack(o[2] * r, o[3] * r);
-          *reinterpret_cast<uint2*>(a.out + at * D + d4) = word;
-          if (a.lse && d4 == 0) a.lse[at] = sum == 0.f ? kNegInf : (big + __log2f(sum)) * 0.693147180559945309f;
-        }
+        for (int i = 0; i < 4; ++i) o[i] += x[i] * f[k];
       }
-    if (n + 1 < NT) local_barrier();
+      const int64_t at = join_at[16 * n + col] + d4;
+      if (a.slots > 1) {
+        *reinterpret_cast<SS_G ss_f32x4*>(gp(a.po) + at) = o;
+      } else {
+        uint2 word;
+        word.x = T::pack(o[0], o[1]);
+        word.y = T::pack(o[2], o[3]);
+        *reinterpret_cast<uint2*>(a.out + at) = word;
+      }
+    }
   }
 }
 
@@ -414,12 +448,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) float part[WIDE ? GROUPS : 1][D];
   __shared__ float part_l[GROUPS], part_m[GROUPS];
   const int tid = threadIdx.x, d4 = 4 * (tid % TD), k = tid / TD;
-  const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
-  int64_t b = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * GROUPS + k;
+  const uint32_t all = (uint32_t)a.seqs * a.max_rows * a.heads;  // below 2^31
+  uint32_t b = WIDE ? blockIdx.x : blockIdx.x * GROUPS + k;
   if (b >= all) return;
-  const int head = (int)(b % a.heads);
-  b /= a.heads;
-  const int i = (int)(b % a.max_rows), s = (int)(b / a.max_rows);
+  const int head = (int)(b % (uint32_t)a.heads);
+  b /= (uint32_t)a.heads;
+  const int i = (int)(b % (uint32_t)a.max_rows), s = (int)(b / (uint32_t)a.max_rows);
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width << a.page_shift, nullptr);
   if (i >= sr.n) return;
   // The slots of the workgroup that had this row, as it counted them.

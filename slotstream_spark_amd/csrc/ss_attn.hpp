@@ -44,8 +44,10 @@ typedef _Float16 ss_f16x8 __attribute__((ext_vector_type(8)));
 // The element types. kShift: probabilities are kept 2^kShift times as large, the running maximum that much lower. fp16
 // has no exponents below 2^-14 with full precision, so a probability of 2^-14 of the row's largest would lose bits;
 // with the factor they are whole to 2^-24, and at most 2^10 leaves room for fp32 sums. bf16 has fp32's exponents.
+// kLazy: a running maximum is raised only when a score passes it by 2^kLazy; until then weights are up to 2^(kShift + kLazy),
+// at most 2^14 in fp16.
 struct Bf16 {
-  static constexpr float kShift = 0.f;
+  static constexpr float kShift = 0.f, kLazy = 8.f;
   static constexpr uint32_t kExp = 0x7F80u, kOne = 0x3F80u;
   SS_DEV static ss_f32x4 mfma16(const ss_u32x4& a, const ss_u32x4& b, const ss_f32x4& c) { return ss_mfma(a, b, c); }
   // One v_cvt_pk_bf16_f32 (of two conversions and an or, the compiler makes four instructions).
@@ -57,7 +59,7 @@ struct Bf16 {
   SS_DEV static float widen(uint32_t u) { return ss_bf16_to_f32(u); }
 };
 struct Fp16 {
-  static constexpr float kShift = 10.f;
+  static constexpr float kShift = 10.f, kLazy = 4.f;
   static constexpr uint32_t kExp = 0x7C00u, kOne = 0x3C00u;
   SS_DEV static ss_f32x4 mfma16(const ss_u32x4& a, const ss_u32x4& b, const ss_f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ss_f16x8, a), __builtin_bit_cast(ss_f16x8, b), c, 0,

@@ -19,8 +19,6 @@
 // whole, where values at unseen places are also kept out of the products (as in ss_attn.hip).
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "ss_attn.hpp"
 #include "ss_launch.hpp"
 
@@ -76,7 +74,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int KROW = D * 2, VROW = TK * 2;                   // bytes of a row in LDS
   constexpr int KC = D / 8, VC = TK / 8;                       // 16-byte pieces of a row
   constexpr int KI = TK * KROW / 4096, VI = DV * VROW / 4096;   // 1 KB load instructions a wave
-  constexpr float kLazy = std::is_same<T, Bf16>::value ? 8.f : 4.f;
   __shared__ __attribute__((aligned(1024))) uint8_t k0[TK * KROW];
   __shared__ __attribute__((aligned(1024))) uint8_t k1[TK * KROW];
   __shared__ __attribute__((aligned(1024))) uint8_t v0[DV * VROW];
@@ -297,7 +294,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       top = max_of(x);
     }
     const float mx = fmaxf(top, other_half(top, h)) * a.scale - T::kShift;
-    if (__builtin_expect(__any(mx > m + kLazy || (m == kNegInf && mx > kNegInf)), 0)) {
+    if (__builtin_expect(__any(mx > m + T::kLazy || (m == kNegInf && mx > kNegInf)), 0)) {
       const float mn = fmaxf(m, mx);
       const float f = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);  // nothing summed yet (or NaN) where m is -inf
       l *= f;

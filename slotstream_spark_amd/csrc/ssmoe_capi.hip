@@ -207,6 +207,8 @@ int check_paged(int rows, int seqs, int max_rows, int heads, int kv_heads, int d
   if (!*shift) return fail(SSMOE_EINVAL, "page must be 16, 32, 64, 128 or 256 tokens, got %d", page);
   if (width < 1 || (int64_t)width * page > (1 << 30))
     return fail(SSMOE_EINVAL, "a table row must cover 1 .. 2^30 tokens, got %d pages of %d", width, page);
+  if ((int64_t)kv_heads * page * dim * 2 > INT32_MAX)
+    return fail(SSMOE_EINVAL, "a page of %d tokens, %d heads and %d dimensions must be below 2 GiB", page, kv_heads, dim);
   if (n_pages < 1 || n_pages > INT32_MAX) return fail(SSMOE_EINVAL, "need 1 <= n_pages < 2^31");
   if (type != SSMOE_BF16 && type != SSMOE_FP16) return fail(SSMOE_EINVAL, "type must be SSMOE_BF16 or SSMOE_FP16, got %d", type);
   return ok();
@@ -1469,7 +1471,7 @@ int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page
   if (n == 0) return ok();
   if (!k || !v || !src || !dst) return fail(SSMOE_EINVAL, "k, v, src and dst must be non-null");
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(SSMOE_EINVAL, "k and v must be 16-byte aligned");
-  if (2 * (page_bytes / 2048) * n > ((int64_t)1 << 34) / layers) return fail(SSMOE_EINVAL, "too many bytes for one call");
+  if (page_bytes / 2048 > ((int64_t)1 << 30) / n / layers) return fail(SSMOE_EINVAL, "too many bytes for one call");
   ss::MoveArgs a{};
   a.k = static_cast<uint8_t*>(k);
   a.v = static_cast<uint8_t*>(v);

@@ -34,6 +34,7 @@ def attn(**kw):
     (dict(max_rows=0), b"max_rows >= 1"), (dict(rows=-1), b"rows >= 0"), (dict(seqs=-1), b"seqs >= 0"),
     (dict(width=0), b"table row"), (dict(width=1 << 27), b"table row"), (dict(n_pages=0), b"n_pages"),
     (dict(n_pages=1 << 31), b"n_pages"), (dict(type=2), b"type must be"), (dict(window=-1), b"window and sinks"),
+    (dict(heads=65536, kv_heads=32768, dim=256, page=128, width=1), b"below 2 GiB"),
     (dict(sinks=-1), b"window and sinks"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"),
     (dict(scale=math.nan), b"scale"), (dict(scale=math.inf), b"scale"), (dict(q=None), b"non-null"),
     (dict(k_pages=None), b"non-null"), (dict(out=None), b"non-null"), (dict(table=None), b"non-null"),

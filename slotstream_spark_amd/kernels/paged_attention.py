@@ -79,8 +79,8 @@ def check_batch(cu_rows: torch.Tensor, kv_len: torch.Tensor, table: torch.Tensor
     if tuple(cu_rows.shape) != (seqs + 1,) or tuple(kv_len.shape) != (seqs,):
         raise ValueError(f"cu_rows must be [{seqs + 1}] and kv_len [{seqs}], got {tuple(cu_rows.shape)} and "
                          f"{tuple(kv_len.shape)}")
-    if max_rows < 1:
-        raise ValueError("max_rows must be >= 1")
+    if not 1 <= max_rows < 1 << 31:
+        raise ValueError("max_rows must be >= 1 and below 2^31")
     return seqs, table.shape[1]
 
 
@@ -119,8 +119,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     call, so calls and captured graphs never share one."""
     max_rows, window, sinks = int(max_rows), int(window), int(sinks)
     key = (q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.dtype, k_pages.is_contiguous(), v_pages.shape, v_pages.dtype,
-           v_pages.is_contiguous(), cu_rows.shape, cu_rows.dtype, kv_len.shape, kv_len.dtype, table.shape, table.dtype,
-           table.is_contiguous(), max_rows, window, sinks, scale)
+           v_pages.is_contiguous(), cu_rows.shape, cu_rows.stride(), cu_rows.dtype, kv_len.shape, kv_len.stride(), kv_len.dtype,
+           table.shape, table.dtype, table.is_contiguous(), max_rows, window, sinks, scale)
     plan = _plans.get(key)
     if plan is None:
         plan = _plans.keep(key, _plan(q, k_pages, v_pages, cu_rows, kv_len, table, max_rows, window, sinks, scale))
@@ -155,6 +155,8 @@ def _plan(q, k_pages, v_pages, cu_rows, kv_len, table, max_rows, window, sinks, 
     head = strides(q)
     sizes = (n_pages, rows, seqs, max_rows, heads, kv_heads, dim, page, width)
     tail = (window, sinks, TYPES[q.dtype], 1.0 / math.sqrt(dim) if scale is None else float(scale))
+    if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31 or not 0 < tail[3] < 1e30:
+        raise ValueError("need 0 <= window, sinks < 2^31 and 0 < scale < 1e30")
     L = _lib.lib()
     nb = L.ssmoe_paged_attention_workspace_bytes(_ARGS.pack(0, *head, *(0,) * 8, 0, *sizes, *tail))
     if nb < 0:

@@ -41,10 +41,12 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape,
            positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, inv_freq.is_contiguous(), k_pages.shape,
            k_pages.dtype, k_pages.is_contiguous(), v_pages.shape, v_pages.dtype, v_pages.is_contiguous(), cu_rows.shape,
-           cu_rows.dtype, kv_len.shape, kv_len.dtype, table.shape, table.dtype, table.is_contiguous(), max_rows,
-           None if axis is None else (axis.shape, axis.dtype))
+           cu_rows.stride(), cu_rows.dtype, kv_len.shape, kv_len.stride(), kv_len.dtype, table.shape, table.dtype,
+           table.is_contiguous(), max_rows, None if axis is None else (axis.shape, axis.stride(), axis.dtype), factor)
     plan = _plans.get(key)
     if plan is None:
+        if not abs(factor) < 1e30:
+            raise ValueError("factor must be finite and below 1e30")
         plan = _plans.keep(key, _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis))
     row_strides, sizes, rot, axes, kind, shape = plan
     dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out)

@@ -131,6 +131,43 @@ def test_python_refusals():
             kv_pages.move_pages(*a)
 
 
+def test_a_checked_shape_does_not_let_other_strides_pass():
+    """What the checks found is kept by shapes, types and strides: a strided tensor of a known shape is still refused."""
+    k, v = torch.zeros(8, 2, 16, 64, dtype=torch.bfloat16), torch.zeros(8, 2, 64, 16, dtype=torch.bfloat16)
+    q, x = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    good = dict(cu_rows=i32(4), kv_len=i32(3), table=i32(3, 2))
+    f, pos, axis = torch.ones(16, dtype=torch.float64), i32(3), i32(16)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="same GPU"):
+            pa.paged_attention(q, k, v, **good, max_rows=1)
+        with pytest.raises(ValueError, match="same GPU"):
+            rope.rope_append(q, x, x, pos, f, k, v, **good, max_rows=1, axis=axis)
+    for name, bad in (("cu_rows", i32(8)[::2]), ("kv_len", i32(6)[::2]), ("table", i32(3, 4)[:, ::2])):
+        with pytest.raises(ValueError, match=f"{name} must be a contiguous"):
+            pa.paged_attention(q, k, v, **{**good, name: bad}, max_rows=1)
+        with pytest.raises(ValueError, match=f"{name} must be a contiguous"):
+            rope.rope_append(q, x, x, pos, f, k, v, **{**good, name: bad}, max_rows=1, axis=axis)
+    with pytest.raises(ValueError, match="axis must be"):
+        rope.rope_append(q, x, x, pos, f, k, v, **good, max_rows=1, axis=i32(32)[::2])
+    with pytest.raises(ValueError, match="positions must be"):
+        rope.rope_append(q, x, x, i32(6)[::2], f, k, v, **good, max_rows=1, axis=axis)
+    with pytest.raises(ValueError, match="inv_freq must be"):
+        rope.rope_append(q, x, x, pos, torch.ones(32, dtype=torch.float64)[::2], k, v, **good, max_rows=1, axis=axis)
+
+
+@pytest.mark.parametrize("kw", [dict(max_rows=1 << 31), dict(window=1 << 31), dict(sinks=1 << 40), dict(window=-1),
+                                dict(scale=1e39), dict(scale=0.0), dict(scale=math.nan)])
+def test_numbers_that_do_not_fit_are_refused(kw):
+    k, v = torch.zeros(8, 2, 16, 64, dtype=torch.bfloat16), torch.zeros(8, 2, 64, 16, dtype=torch.bfloat16)
+    q, i32 = torch.zeros(3, 4, 64, dtype=torch.bfloat16), lambda *s: torch.zeros(*s, dtype=torch.int32)
+    with pytest.raises(ValueError, match="max_rows|window|scale"):
+        pa.paged_attention(q, k, v, i32(4), i32(3), i32(3, 2), **{"max_rows": 1, **kw})
+    with pytest.raises(ValueError, match="factor"):
+        rope.rope_append(q, q[:, :2], q[:, :2], i32(3), torch.ones(16, dtype=torch.float64), k, v, i32(4), i32(3), i32(3, 2), 1,
+                         factor=1e39)
+
+
 def test_definition_against_torch():
     """attention64 on whole causal sequences is torch's softmax attention, rope64 a rotation of complex numbers."""
     b = Batch([20, 7], [20, 7], 4, 2, 64, 16)

@@ -231,7 +231,7 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
                            p->type, &shift))
     return rc;
   if (p->window < 0 || p->sinks < 0) return fail(SSMOE_EINVAL, "window and sinks must be >= 0");
-  if (!(p->scale > 0) || !std::isfinite(p->scale)) return fail(SSMOE_EINVAL, "scale must be positive and finite");
+  if (!(p->scale >= 1e-30f && p->scale <= 1e30f)) return fail(SSMOE_EINVAL, "scale must be positive, in [1e-30, 1e30]");
   ss::AttnArgs a{};
   const int max_rows = p->max_rows < p->rows ? p->max_rows : (p->rows > 0 ? p->rows : 1);
   const int64_t cap = (int64_t)p->width * p->page;
@@ -252,7 +252,8 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
   a.tiles = (max_rows * a.group + a.packed - 1) / a.packed;
   // tokens of a sequence that the call may read
   int64_t seen = cap;
-  if (a.window < (1 << 30)) seen = std::min<int64_t>(cap, (int64_t)a.window + max_rows + a.sinks);
+  if (a.window < (1 << 30))
+    seen = std::min<int64_t>(cap, (int64_t)a.window + std::max(max_rows, kFewRows) + a.sinks);
   int64_t chunk = cap, slots = 1;
   const int64_t units = (int64_t)p->seqs * p->kv_heads;
   const int parts_of_dim = ss::attn_prompt_parts(p->dim, shift);

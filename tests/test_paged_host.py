@@ -47,6 +47,17 @@ def test_attention_refuses(L, kw, msg):
     assert msg in L.ssmoe_last_error(), L.ssmoe_last_error()
 
 
+def test_chunks_do_not_go_by_the_rows_of_a_call(L):
+    """The workspace is slots x rows x heads: with `rows` fixed its size says how a sequence is cut into chunks, which must be the
+    same for every max_rows that decoding and verification use (a row's bits go by it)."""
+    for window in range(0, 4096, 37):
+        for kv_heads, seqs in ((1, 3), (2, 32), (4, 11)):
+            sizes = {L.ssmoe_paged_attention_workspace_bytes(attn(
+                rows=64, max_rows=m, kv_heads=kv_heads, seqs=seqs, page=64, width=700, window=window, sinks=5))
+                for m in range(1, 9)}
+            assert len(sizes) == 1, (window, kv_heads, seqs, sizes)
+
+
 def test_attention_workspace(L):
     size = lambda **kw: L.ssmoe_paged_attention_workspace_bytes(attn(**kw))
     assert size(width=8) == 0                      # a table of one chunk: nothing to join

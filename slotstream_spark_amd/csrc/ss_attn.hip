@@ -331,6 +331,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     tt = tn;
     tn = next_tile(tt + W);
   }
+  wait_loads<0>();  // no load into LDS outlives the tiles (without tiles the queries are on their way)
 
   // The waves' sums, weighted by how far each wave's maximum is below the largest.
 #pragma unroll

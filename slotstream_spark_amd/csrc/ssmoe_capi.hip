@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <exception>
 #include <mutex>
 #include <string>
 
@@ -212,6 +213,16 @@ int check_paged(int rows, int seqs, int max_rows, int heads, int kv_heads, int d
   if (n_pages < 1 || n_pages > INT32_MAX) return fail(SSMOE_EINVAL, "need 1 <= n_pages < 2^31");
   if (type != SSMOE_BF16 && type != SSMOE_FP16) return fail(SSMOE_EINVAL, "type must be SSMOE_BF16 or SSMOE_FP16, got %d", type);
   return ok();
+}
+
+// Whether [rows][heads][dim] 16-bit elements of two tensors (strides in elements) share bytes.
+bool overlap(const void* a, int64_t a_row, int64_t a_head, int a_heads, const void* b, int64_t b_row, int64_t b_head,
+             int b_heads, int rows, int dim) {
+  auto end = [&](const void* p, int64_t row, int64_t head, int heads) {
+    return reinterpret_cast<uintptr_t>(p) + 2 * (uintptr_t)((rows - 1) * row + (heads - 1) * head + dim);
+  };
+  return reinterpret_cast<uintptr_t>(a) < end(b, b_row, b_head, b_heads) &&
+         reinterpret_cast<uintptr_t>(b) < end(a, a_row, a_head, a_heads);
 }
 
 // How a call of ssmoe_paged_attention is laid out (its checks included). `prompt`: the kernel for many rows of a sequence.
@@ -1376,6 +1387,13 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
   for (const void* t : {p->q, p->k, p->v, (const void*)p->q_out, (const void*)p->k_pages, (const void*)p->v_pages})
     if (!aligned(t, 16)) return fail(SSMOE_EINVAL, "q, k, v, q_out and the pages must be 16-byte aligned");
   if (!aligned(p->inv_freq, 8)) return fail(SSMOE_EINVAL, "inv_freq must be 8-byte aligned");
+  // Every element of q is read and written by one thread, so q_out may be q itself, laid out alike.
+  const int64_t o_row = (int64_t)p->heads * p->dim;
+  const bool same = p->q_out == p->q && (p->q_row == o_row || p->rows == 1) && (p->q_head == p->dim || p->heads == 1);
+  if ((!same && overlap(p->q, p->q_row, p->q_head, p->heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim)) ||
+      overlap(p->k, p->k_row, p->k_head, p->kv_heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim) ||
+      overlap(p->v, p->v_row, p->v_head, p->kv_heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim))
+    return fail(SSMOE_EINVAL, "q_out must be q itself (contiguous) or overlap none of q, k and v");
   a.q = static_cast<const uint16_t*>(p->q);
   a.k = static_cast<const uint16_t*>(p->k);
   a.v = static_cast<const uint16_t*>(p->v);
@@ -1439,6 +1457,8 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
   if (ws > 0 && (!p->ws || p->ws_bytes < ws || !aligned(p->ws, 256)))
     return fail(SSMOE_EINVAL, "workspace holds %lld bytes, the call needs %lld (256-byte aligned)",
                 (long long)(p->ws ? p->ws_bytes : 0), (long long)ws);
+  if (overlap(p->q, p->q_row, p->q_head, p->heads, p->out, (int64_t)p->heads * p->dim, p->dim, p->heads, p->rows, p->dim))
+    return fail(SSMOE_EINVAL, "out must not overlap q");
   a.q = static_cast<const uint16_t*>(p->q);
   a.q_row = p->q_row;
   a.q_head = p->q_head;
@@ -1458,9 +1478,12 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
   }
   const bool fp16 = p->type == SSMOE_FP16;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (int rc = hip_check(prompt ? ss::launch_attn_prompt(a, p->dim, fp16, st) : ss::launch_attn_few(a, p->dim, fp16, st),
-                         "attention launch"))
-    return rc;
+  hipError_t e = hipErrorOutOfMemory;
+  try {  // the few-row launch keeps its kernels' limits in a map
+    e = prompt ? ss::launch_attn_prompt(a, p->dim, fp16, st) : ss::launch_attn_few(a, p->dim, fp16, st);
+  } catch (const std::exception&) {
+  }
+  if (int rc = hip_check(e, "attention launch")) return rc;
   return a.slots > 1 ? hip_check(ss::launch_attn_join(a, p->dim, fp16, st), "attention join launch") : ok();
 }
 

@@ -288,3 +288,28 @@ def test_prompt_strides_padding_rows_and_graph():
         graph.replay()
         want = paged_attention(fused[:90, 2:10], k, v, cu, kv_len, table, n)
         assert torch.equal(out[:90].view(torch.int16), want.view(torch.int16)), step
+
+
+def test_output_behind_its_queries():
+    b = Batch([2, 12], [300, 400], 8, 2, 64, 16, seed=5)
+    q, *rest = b.args()
+    want = paged_attention(q, *rest)
+    both = torch.empty((2, *q.shape), dtype=q.dtype, device="cuda")
+    both[0] = q
+    assert paged_attention(both[0], *rest, out=both[1]).data_ptr() == both[1].data_ptr()
+    assert torch.equal(both[1], want) and torch.equal(both[0], q)
+    with pytest.raises(_lib.SsmoeError, match="overlap"):
+        paged_attention(both[0], *rest, out=both[0])
+
+
+@pytest.mark.parametrize("window", [16370, 16376, 16379, 16380])
+def test_rows_under_a_window_have_the_bits_they_have_alone(window):
+    """The rows of a call and each row alone, where a chunk's size is about to change: 2 x (window + rows + first tokens) tokens over
+    256 workgroups pass 128."""
+    b = Batch([4], [20000], 4, 2, 64, 64, seed=window)
+    q, k, v, cu, kv_len, table, n = b.args()
+    got = paged_attention(q, k, v, cu, kv_len, table, n, window=window, sinks=4)
+    one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for i in range(4):
+        alone = paged_attention(q[i:i + 1], k, v, one, kv_len - 3 + i, table, 1, window=window, sinks=4)
+        assert torch.equal(got[i], alone[0]), i

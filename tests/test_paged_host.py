@@ -87,6 +87,18 @@ def test_rope_refuses(L, kw, msg):
     assert msg in L.ssmoe_last_error(), L.ssmoe_last_error()
 
 
+def test_outputs_over_inputs_are_refused(L):
+    """4 rows of 8 heads of 64, packed rows of 512 elements from P on (what is accepted is run on the GPU)."""
+    q, far = dict(q=P, q_row=512, q_head=64, rows=4), 1 << 24
+    for out in (P, P + 16, P + 4 * 1024 - 16, P - 4 * 1024 + 16):
+        assert L.ssmoe_paged_attention(attn(**q, out=out), None) == EINVAL
+        assert b"out must not overlap q" in L.ssmoe_last_error(), out
+    for kw in (dict(q_out=P + 16), dict(q_out=P, q_row=1024), dict(q_out=far), dict(q_out=2 * far + 16),
+               dict(q_out=far - 4 * 1024 + 16), dict(q_out=P, k=P + 1024)):
+        assert L.ssmoe_rope_append(rope_args(**{**q, "k": far, "v": 2 * far, **kw}), None) == EINVAL
+        assert b"q_out must be q itself" in L.ssmoe_last_error(), kw
+
+
 def test_rope_nothing_to_do(L):
     assert L.ssmoe_rope_append(None, None) == EINVAL
     assert L.ssmoe_rope_append(rope_args(rows=0, q=None), None) == 0

@@ -98,9 +98,16 @@ class SeqCache:
             self._rows[n] = (torch.arange(n, dtype=torch.int32).to(dev), torch.arange(n, dtype=torch.int32).to(dev))
         return self._cu[n], self.kv_len, self.table, self._rows[n][0]
 
+    def room(self, pos: int, n: int) -> None:
+        """Pages that the tokens pos .. pos + n - 1 may be written to: what the sequence held from `pos` on (rows taken back, drafts) is
+        given up, and a page that a fork holds too is copied first."""
+        if pos < self.pages.length[self.seq]:
+            self.pages.truncate(self.seq, pos)
+        self.pages.reserve(self.seq, pos + n)
+
     def place(self, pos: int, n: int) -> None:
         """The next call's rows are the tokens pos .. pos + n - 1: their pages are there, the tensors of rows(n) say so."""
-        self.pages.reserve(self.seq, pos + n)
+        self.room(pos, n)
         self.rows(n)
         positions, steps = self._rows[n]
         self.kv_len.fill_(pos + n)

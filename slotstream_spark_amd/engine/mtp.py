@@ -371,7 +371,7 @@ class DraftGraph:
         if h.attn is not None:
             if h.state.pos + self.k > h.state.max_ctx:
                 raise ValueError(f"head context {h.state.pos + self.k} exceeds {h.state.max_ctx}")
-            h.cache.pages.reserve(h.cache.seq, h.state.pos + self.k)
+            h.cache.room(h.state.pos, self.k)
             self.base.fill_(h.state.pos)
 
     def capture(self) -> None:

@@ -141,6 +141,22 @@ def test_evict_keeps_the_window_and_the_first_tokens():
         kv.extend(b, 1)
 
 
+@pytest.mark.parametrize("pos", [0, 5, 16, 20, 31, 32, 33, 39])
+def test_rows_written_again_leave_a_fork_alone(pos):
+    """A sequence of 40 tokens is forked, then goes back to `pos` (a rejected draft) and writes from there: the fork keeps every token."""
+    from slotstream_spark_amd.engine.attention import SeqCache
+    kv = pages()
+    cache = SeqCache(kv)
+    cache.place(0, 40)
+    write(kv, cache.seq, 0, range(1, 41))
+    child = kv.fork(cache.seq)
+    cache.place(pos, 4)
+    assert cache.rows(4)[1].tolist() == [pos + 4] and cache.rows(4)[3].tolist() == list(range(pos, pos + 4))
+    write(kv, cache.seq, pos, range(101, 105))
+    assert read(kv, child) == list(range(1, 41))
+    assert read(kv, cache.seq) == list(range(1, pos + 1)) + list(range(101, 105))
+
+
 def test_refusals():
     kv = pages(n=3)
     s = kv.new()

@@ -386,10 +386,11 @@ class DraftGraph:
         with torch.cuda.graph(g):
             self._body()
         self.graph = g
+        self._resizes = self.head.cache.pages.resizes if self.head.attn is not None else 0
 
     def replay(self) -> torch.Tensor:
-        if self.graph is None:
-            self.capture()
+        if self.graph is None or (self.head.attn is not None and self.head.cache.pages.resizes != self._resizes):
+            self.capture()   # a resized cache is other tensors
         self._place()
         self.graph.replay()
         return self.out

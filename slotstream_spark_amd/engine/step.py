@@ -216,6 +216,7 @@ class MTPStepGraph:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=self.stream):
             self._body()
+        self._resizes = self.cache.pages.resizes if self.cache is not None else 0
 
     def step(self, x: torch.Tensor | None = None, drafts: torch.Tensor | None = None) -> torch.Tensor:
         """Replay the round (capturing it on first use) after copying `x` / `drafts` into the static inputs; returns
@@ -225,8 +226,8 @@ class MTPStepGraph:
             self.x_in.copy_(x)
         if drafts is not None:
             self.drafts.copy_(drafts)
-        if self.graph is None:
-            self.capture()
+        if self.graph is None or (self.cache is not None and self.cache.pages.resizes != self._resizes):
+            self.capture()   # a resized cache is other tensors
         self.stream.wait_stream(cur)
         self.graph.replay()
         cur.wait_stream(self.stream)

@@ -24,7 +24,9 @@ from ..kernels.paged_attention import DIMS, PAGES, TYPES
 class KVPages:
     """`n_pages` pages for `layers` layers: k [layers, n_pages, kv_heads, page, dim], v [layers, n_pages, kv_heads, dim,
     page], zero at first. Up to `max_seqs` sequences of up to `max_tokens` tokens; table int32 [max_seqs, width] on the device, -1
-    where a sequence holds no page. `length[s]` is the number of tokens that a sequence has room for and counts as its own."""
+    where a sequence holds no page. `length[s]` is the number of tokens that a sequence has room for and counts as its own.
+    `resizes` counts the times that k and v became other tensors (a captured graph holds the ones it was captured with). A page given
+    back may be handed out at once: where sequences are worked on in several streams, their owners wait for each other first."""
 
     def __init__(self, layers: int, n_pages: int, kv_heads: int, dim: int, page: int = 64, max_seqs: int = 1,
                  max_tokens: int = 131072, dtype=torch.bfloat16, device="cuda"):
@@ -41,6 +43,7 @@ class KVPages:
         self._refs = np.zeros(n_pages, np.int64)
         self._free = list(range(n_pages))   # a heap: the lowest id goes first
         self.length = [0] * max_seqs
+        self.resizes = 0
         self._live = [False] * max_seqs
 
     # ------------------------------------------------------------------ what is held
@@ -213,6 +216,7 @@ class KVPages:
             return out
 
         self.k, self.v = sized(self.k), sized(self.v)
+        self.resizes += 1
         refs = np.zeros(n_pages, np.int64)
         refs[:keep] = self._refs[:keep]
         self._refs, self.n_pages = refs, n_pages

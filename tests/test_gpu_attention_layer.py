@@ -296,6 +296,35 @@ def test_prompt_forms_agree(parts):
         MoEStack(a.graph.layers[0].pool, [], None, a.embed, attn=[])
 
 
+def test_a_resized_cache_is_captured_anew(parts):
+    """The captured round and the captured drafts follow k and v to their new places (the old ones are poisoned here)."""
+    stack, head = make_stack(parts), make_head(parts, 1)
+    prompt, rounds = [5, 17, 300, 8, 1234], [[77], [9], [2], [64], [1000]]
+
+    def run(resize):
+        stack.reset()
+        head.reset()
+        graph, out = DraftGraph(head, 2), []
+        _, multi = stack.forward(prompt)
+        head.consume(prompt, multi)
+        for i, tokens in enumerate(rounds):
+            if resize and i in (2, 4):
+                for pages in (stack.cache.pages, head.cache.pages):
+                    old = pages.k, pages.v
+                    pages.resize(pages.n_pages + 3)
+                    for t in old:
+                        t.fill_(float("nan"))
+            nxt, multi = stack.forward(tokens)
+            head.consume(tokens, multi)
+            graph.token.fill_(nxt[0])
+            graph.multi.copy_(head.prev_multi)
+            out += nxt + graph.replay().cpu().tolist()
+        return out
+
+    want = run(False)
+    assert run(True) == want and stack.cache.pages.resizes == 2 and _lib.device_error() == 0
+
+
 def test_two_streams_at_once():
     """Two sequences of one cache decoded on two streams at the same time."""
     layer = attention_layer(512, 8, 2, 128, 31)

@@ -537,12 +537,13 @@ int ssmoe_gather_rows(const void* src, int64_t n_src, int64_t row_bytes, const i
 
 /* Turns query and key rows by their positions and writes the key and value rows into the cache at their sequence's
  * places. q [rows][heads][dim], k and v [rows][kv_heads][dim] with the given strides (elements, multiples of 8), e.g. the
- * parts of one fused projection; q_out [rows][heads][dim] contiguous (may be q where that is contiguous). For
+ * parts of one fused projection; q_out [rows][heads][dim] contiguous. For
  * frequency i of rot / 2 the angle is positions[axis[i] * pos_stride + row] * inv_freq[i] (fp64, reduced to a
  * fraction of a turn in fp64); axis NULL means axis 0 (text), 3 axes with an axis per frequency are the (time,
  * height, width) positions of images and video. The pair turned is (i, i + rot / 2), or (2 i, 2 i + 1) with adjacent;
  * elements from rot on are copied. cos and sin are multiplied by factor. One rounding to 16 bits at the end. Rows with
- * a position below 0 are turned but not written. Two rows that share a place (a page in two sequences' tables) race. */
+ * a position below 0 are turned but not written. q_out is q itself (contiguous) or overlaps none of q, k and v. Two rows that
+ * share a place (a page in two sequences' tables) race. */
 typedef struct {
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
@@ -562,7 +563,7 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* a, void* stream);
 /* out row i = sum_j softmax_j(scale * q_i . k_j) v_j over the tokens j <= p of its sequence (p its position), under
  * window > 0 only those with p - j < window or j < sinks (the first tokens that stay visible); lse (fp32 [rows][heads], or
  * NULL) = ln sum_j exp(scale * q_i . k_j). Head h reads key head h / (heads / kv_heads). A row that sees nothing is 0 with
- * lse -inf. q [rows][heads][dim] with the given strides (elements, multiples of 8), out contiguous. Scores, maxima, sums and
+ * lse -inf. q [rows][heads][dim] with the given strides (elements, multiples of 8), out contiguous and apart from q. Scores, maxima, sums and
  * partial results are fp32; a probability is rounded to the element type before its product with the values. What the
  * cache holds at tokens that a row does not see does not reach it, infinities and NaN included.
  * Calls with max_rows <= 8 (decoding, verification): the bits of a row depend on its sequence's tokens, seqs, kv_heads and

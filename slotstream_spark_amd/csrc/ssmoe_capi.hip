@@ -231,9 +231,16 @@ bool overlap(const void* a, int64_t a_row, int64_t a_head, int a_heads, const vo
 // none of fewer than 128 tokens (a tile for each wave), and none of more than 512 to 4096 (by how far the sequences and key
 // heads alone fill the CUs: a short sequence on a wide table has to find its CUs too). It goes by seqs, kv_heads and the
 // table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call. With 256 /
-// 512 / 1024 / 2048 workgroups, kernel and join in us: one sequence of 131,072 tokens 47 / 48 / 55 / 54; eight of 6,145
-// with three rows at 256 dimensions 29 / 39 / 45 / 45; 32 with four rows under a window of 1,024 21 / 25 / 20 / 20.
-// Many rows: the tokens are split only where the row tiles alone would leave CUs without work.
+// 512 / 1024 / 2048 workgroups, kernel and join in us: one sequence of 131,072 tokens 50 / 49 / 49 / 52; eight of 6,145
+// with three rows at 256 dimensions 25 / 30 / 37 / 37; 32 with four rows under a window of 1,024 21 / 25 / 20 / 21.
+// Many rows: the tokens are split only where the row tiles alone would leave CUs without work (two workgroups fit a CU): three
+// sequences of 333 rows over up to 5,000 tokens 76 us and a join of 10, unsplit 89; 2,048 rows of one sequence 54
+// unsplit, 75 and 21 in two.
+//
+// Up to 8 rows a sequence are few (a verify round has at most 4). A call of 4 / 8 / 12 / 16 rows over 8,000 tokens in us, few
+// against many: 8 sequences of 32 heads on 4, 128 dimensions 32 / 43 / 68 / 70 against 33 / 35 / 37 / 43; 32 of 32 on 8 186 /
+// 191 / 200 / 204 against 195 / 195 / 204 / 201; 8 of 16 on 2, 256 dimensions 33 / 43 / 56 / 69 against 42 / 45 / 48 / 52; 16
+// of 24 on 8, 64 dimensions 44 / 46 / 50 / 51 against 58 / 58 / 57 / 56.
 constexpr int kFewRows = 8;
 int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
   if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
@@ -1427,7 +1434,8 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
   a.adjacent = p->adjacent != 0;
   a.factor = p->factor;
   a.tiles = (int)(((int64_t)a.max_rows + 14) / 8);
-  // A workgroup's four waves take its heads in turn; where there are few groups of positions the heads are shared out too.
+  // A workgroup's four waves take its heads in turn; where there are few groups of positions the heads are shared out too (64
+  // single tokens of 36 heads 6 us, 15 with one workgroup each).
   const int64_t groups = std::max<int64_t>((int64_t)a.tiles * p->seqs, 1);
   a.head_groups = (int)std::min<int64_t>((1024 + groups - 1) / groups, (p->heads + p->kv_heads + 3) / 4);
   if ((int64_t)a.tiles * a.head_groups * p->seqs > INT32_MAX)

@@ -130,7 +130,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q_at % 16:
         raise ValueError("q needs 16-byte alignment")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(shape)}")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):

@@ -54,7 +54,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     if (q_at | k_at | v_at) % 16:
         raise ValueError("q, k and v need 16-byte alignment")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {q.dtype} {tuple(shape)}")
     args = _ARGS.pack(q_at, k_at, v_at, *row_strides, out.data_ptr(), positions.data_ptr(), shape[0], inv_freq.data_ptr(),

@@ -229,8 +229,11 @@ bool overlap(const void* a, int64_t a_row, int64_t a_head, int a_heads, const vo
 //
 // Few rows (up to kFewRows): chunk is the tokens of one workgroup, so that a batch of full tables makes a workgroup a CU, but
 // none of fewer than 128 tokens (a tile for each wave), and none of more than 512 to 4096 (by how far the sequences and key
-// heads alone fill the CUs: a short sequence on a wide table has to find its CUs too). It goes by seqs, kv_heads and the
-// table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call. With 256 /
+// heads alone fill the CUs: a short sequence on a wide table has to find its CUs too). Where a split would take less than 512
+// tokens off a workgroup (256 of 256 dimensions) it is not worth the join: a call on a table of 256 / 512 / 768 tokens, whole
+// against split, takes 6.0 / 7.7 / 9.5 against 7.8 / 7.9 / 8.7 us (one row of 32 heads on 4, 128 dimensions, in a graph; the
+// host saves 3 us besides), 7.6 / 10.2 / 12.8 against 8.8 / 9.0 / 9.7 (16 on 2, 256 dimensions), 16 sequences of 768 / 1,024
+// tokens 11.7 / 14.1 against 14.5 / 17.2. It goes by seqs, kv_heads, dim and the table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call. With 256 /
 // 512 / 1024 / 2048 workgroups, kernel and join in us: one sequence of 131,072 tokens 50 / 49 / 49 / 52; eight of 6,145
 // with three rows at 256 dimensions 25 / 30 / 37 / 37; 32 with four rows under a window of 1,024 21 / 25 / 20 / 21.
 // Many rows: the tokens are split only where the row tiles alone would leave CUs without work (two workgroups fit a CU): three
@@ -283,6 +286,7 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
     const int64_t most = std::min<int64_t>(std::max<int64_t>(16 * units, 512), 4096);
     chunk = (seen * units + 255) / 256;
     chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), most);
+    if (cap <= 4096 && (cap - chunk) * std::max(p->dim, 128) <= 512 * 128) chunk = (cap + 127) / 128 * 128;
   }
   a.chunk = (int)chunk;
   slots = (cap + chunk - 1) / chunk;

@@ -313,3 +313,23 @@ def test_rows_under_a_window_have_the_bits_they_have_alone(window):
     for i in range(4):
         alone = paged_attention(q[i:i + 1], k, v, one, kv_len - 3 + i, table, 1, window=window, sinks=4)
         assert torch.equal(got[i], alone[0]), i
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 4), (1, 24), (3, 24), (8, 16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_short_sequences_on_a_wide_table(dim, rows, heads):
+    """A table of 8,192 tokens is split into chunks: sequences that end at, before and behind a chunk's and a tile's end."""
+    lens = [rows, 31, 32, 33, 127, 128, 129, 255, 257, 511, 512, 513, 1025, 2049]
+    for page, window, sinks in ((64, 0, 0), (16, 100, 7)):
+        check(Batch([rows] * len(lens), [max(n, rows) for n in lens], heads, 2, dim, page, seed=dim + rows, width=8192 // page),
+              window, sinks)
+
+
+def test_a_row_is_the_same_on_tables_of_one_chunk_and_of_several():
+    """A table of 512 tokens of 128 dimensions is one chunk, one of 4,096 is several: both against the definition, and one against the other within twice
+    its bound."""
+    outs = []
+    for width in (32, 256):
+        b = Batch([2, 1], [500, 77], 8, 2, 128, 16, seed=3, width=width)
+        outs.append(check(b).double().cpu())
+    assert ((outs[0] - outs[1]).abs() <= 2 * attention_bound(b)).all()

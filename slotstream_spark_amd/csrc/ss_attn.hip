@@ -394,7 +394,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       for (int tt = next_tile(w); tt < nt; tt = next_tile(tt + W)) {
         const int t0 = t_begin + 32 * tt, idv = page_of[4 * tt + g];
         if (whole(t0, idv)) continue;
-        const uint16_t* vp = reinterpret_cast<const uint16_t*>(vbase + max(idv, 0) * page_bytes) + (int64_t)c * page +
+        const uint16_t* vp = reinterpret_cast<const uint16_t*>(vbase + (uint64_t)max(idv, 0) * page_bytes) + (int64_t)c * page +
                              ((t0 + 8 * g) & (page - 1));
         ss_u32x4 ones;
 #pragma unroll

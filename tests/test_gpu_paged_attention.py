@@ -333,3 +333,22 @@ def test_a_row_is_the_same_on_tables_of_one_chunk_and_of_several():
         b = Batch([2, 1], [500, 77], 8, 2, 128, 16, seed=3, width=width)
         outs.append(check(b).double().cpu())
     assert ((outs[0] - outs[1]).abs() <= 2 * attention_bound(b)).all()
+
+
+@pytest.mark.parametrize("rows", [2, 9])
+def test_infinite_value_past_32_bits(rows):
+    """An infinity that the last row alone sees, in a page whose byte offset passes 2^32."""
+    kv_heads, page, dim, n = 8, 256, 256, 4200
+    v = torch.zeros(n, kv_heads, dim, page, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(n, kv_heads, page, dim, dtype=torch.bfloat16, device="cuda")
+    b = Batch([rows], [300], 8, 8, dim, page, seed=12, spare=0)
+    b.v[int(b.table[0, 1]), :, 7, 299 - 256] = math.inf
+    far = torch.tensor([n - 1, n - 3], dtype=torch.int32)
+    for j in range(2):
+        k[int(far[j])] = b.k[int(b.table[0, j])].cuda()
+        v[int(far[j])] = b.v[int(b.table[0, j])].cuda()
+    want = paged_attention(*b.args())
+    assert (want[-1, :, 7] == math.inf).all() and torch.isfinite(want[:-1]).all()
+    q, _, _, cu, kv_len, _, m = b.args()
+    got = paged_attention(q, k, v, cu, kv_len, far.cuda()[None].contiguous(), m)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))

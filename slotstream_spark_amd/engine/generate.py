@@ -46,8 +46,13 @@ class MoEStack:
         if (attn is None) != (pages is None):
             raise ValueError("attn and pages come together")
         self.cache = SeqCache(pages) if pages is not None else None
-        self.graph = MTPStepGraph(pool, layers, lm_head, depth, norm_weights=norm_weights, eps=eps, top_k=top_k,
-                                  device=device, attn=attn, attn_norms=attn_norms, cache=self.cache)
+        try:
+            self.graph = MTPStepGraph(pool, layers, lm_head, depth, norm_weights=norm_weights, eps=eps, top_k=top_k,
+                                      device=device, attn=attn, attn_norms=attn_norms, cache=self.cache)
+        except Exception:
+            if self.cache is not None:   # a refused stack keeps no sequence
+                pages.free(self.cache.seq)
+            raise
         self.chunk = int(prompt_chunk)
         self.prompt_layers = [MoEPrefillLayer(pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=top_k,
                                               router_bias=w.router_bias, max_tokens=self.chunk)
@@ -122,6 +127,8 @@ class MoEStack:
     def prompt(self, tokens: list[int]) -> tuple[list[int], torch.Tensor]:
         """The prompt of a sequence: (the greedy next token after the last one, the final stream rows [len, H]). Through
         forward(), or with a prompt_chunk through the layers' prompt forms."""
+        if not tokens:
+            raise ValueError("a prompt needs at least one token")
         if self.prompt_layers is None:
             return self.forward(tokens)
         g, w, eps, multi = self.graph, self.graph.norm_weights, self.graph.eps, []

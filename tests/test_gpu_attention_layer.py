@@ -296,6 +296,19 @@ def test_prompt_forms_agree(parts):
         MoEStack(a.graph.layers[0].pool, [], None, a.embed, attn=[])
 
 
+def test_refused_stacks_and_prompts(parts):
+    pool, lws, lm = parts
+    pages = KVPages(NL, 4, 4, 64, 16)
+    mw = [MoEWeights(w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g) for w in lws[:NL]]
+    embed = head_weights(H, 1, 32, V, seed=921).embed
+    for _ in range(2):                       # one sequence only: the first refusal has given it back
+        with pytest.raises(ValueError, match="one AttentionLayer"):
+            MoEStack(pool, mw, lm, embed, depth=D, top_k=K, attn=[attention_layer(H, 16, 4, 64, 960)], pages=pages)
+    for chunk in (0, 16):
+        with pytest.raises(ValueError, match="at least one token"):
+            make_stack(parts, chunk).prompt([])
+
+
 def test_a_resized_cache_is_captured_anew(parts):
     """The captured round and the captured drafts follow k and v to their new places (the old ones are poisoned here)."""
     stack, head = make_stack(parts), make_head(parts, 1)

@@ -9,9 +9,9 @@
 // rows by 8 dimensions and transposed in registers into the cache's token-contiguous order, 16 bytes per dimension where
 // all 8 tokens are the call's, single values at the ends.
 //
-// Bound by memory on prompts: 8,190 rows of 16 + 2 + 2 heads of 256 dimensions, a quarter of them turned by three axes, 167 MB
-// in 36 us (38 with every wave working out its own angles); 64 single tokens of 32 + 4 + 4 heads of 128 take 6.6 us (8.8),
-// most of it the chain of a row's place, its page, its angles and its rows.
+// Bound by memory on prompts: 8,190 rows of 16 + 2 + 2 heads of 256 dimensions, a quarter of them turned by three axes, 168 MB
+// in 39 us from memory (4.3 TB/s; a copy reaches 4.9); 64 single tokens of 32 + 4 + 4 heads of 128 take 6 to 7 us, most of it
+// the chain of a row's place, its page, its angles and its rows. With every wave working out its own angles 8.8.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"
@@ -26,7 +26,11 @@ template <class T>
 __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   __shared__ __attribute__((aligned(16))) float cs_of[8 * 128], sn_of[8 * 128];  // [8 positions][rot / 2]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint32_t b = blockIdx.x;
+  // Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of neighbours, whose 16-byte parts of a line of values then
+  // meet in one L2 (8,190 rows of 40 heads of 128: 53 us in launch order, 49 so; 64 sequences of 4 rows 10.2 and 9.3; 8,190 rows
+  // of 18 heads of 256 38 and 38).
+  const uint32_t xcd = blockIdx.x % 8, even = gridDim.x / 8, more = gridDim.x % 8;
+  uint32_t b = xcd * even + min(xcd, more) + blockIdx.x / 8;
   const int hg = b % (uint32_t)a.head_groups;
   b /= (uint32_t)a.head_groups;
   const int tile = b % (uint32_t)a.tiles, s = b / (uint32_t)a.tiles;
@@ -65,6 +69,15 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   }
   __syncthreads();
 
+  // Query heads, then key heads; a thread's loads for some of its heads go out together.
+  const int hs = a.heads + a.kv_heads;
+  auto from = [&](int64_t r, int h) {
+    return h < a.heads ? a.q + r * a.q_row + h * a.q_head : a.k + r * a.k_row + (h - a.heads) * a.k_head;
+  };
+  auto to = [&](int64_t r, int h, int rr) {
+    return h < a.heads ? a.out + (r * a.heads + h) * D
+                       : a.k_pages + (((int64_t)id * a.kv_heads + (h - a.heads)) * page + off + rr) * D;
+  };
   // Turned elements: items of (row, 8 frequencies).
   for (int it = lane; it < 8 * chunks; it += 64) {
     const int rr = (uint32_t)it / (uint32_t)chunks, j = it - rr * chunks, row = first + rr - sr.pos0;
@@ -83,52 +96,60 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
       sn[e] = sv[e / 4][e % 4];
     }
     const int o0 = a.adjacent ? 16 * j : 8 * j, o1 = a.adjacent ? 16 * j + 8 : half + 8 * j;
-    for (int h = h0; h < a.heads + a.kv_heads; h += stride) {
-      const bool isq = h < a.heads;
-      const uint16_t* src = isq ? a.q + r * a.q_row + h * a.q_head : a.k + r * a.k_row + (h - a.heads) * a.k_head;
-      const ss_u32x4 x0 = *(const SS_G ss_u32x4*)(src + o0), x1 = *(const SS_G ss_u32x4*)(src + o1);
-      ss_u32x4 y0, y1;
-      if (a.adjacent) {
+    for (int ha = h0; ha < hs; ha += 2 * stride) {
+      ss_u32x4 x0[2], x1[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = T::widen(x0[e] & 0xFFFFu), p1 = T::widen(x0[e] >> 16);
-          const float q0 = T::widen(x1[e] & 0xFFFFu), q1 = T::widen(x1[e] >> 16);
-          y0[e] = T::pack(p0 * cs[e] - p1 * sn[e], p1 * cs[e] + p0 * sn[e]);
-          y1[e] = T::pack(q0 * cs[4 + e] - q1 * sn[4 + e], q1 * cs[4 + e] + q0 * sn[4 + e]);
+      for (int u = 0; u < 2; ++u)
+        if (ha + u * stride < hs) {
+          const uint16_t* src = from(r, ha + u * stride);
+          x0[u] = *(const SS_G ss_u32x4*)(src + o0);
+          x1[u] = *(const SS_G ss_u32x4*)(src + o1);
         }
-      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = T::widen(x0[e] & 0xFFFFu), p1 = T::widen(x0[e] >> 16);
-          const float q0 = T::widen(x1[e] & 0xFFFFu), q1 = T::widen(x1[e] >> 16);
-          y0[e] = T::pack(p0 * cs[2 * e] - q0 * sn[2 * e], p1 * cs[2 * e + 1] - q1 * sn[2 * e + 1]);
-          y1[e] = T::pack(q0 * cs[2 * e] + p0 * sn[2 * e], q1 * cs[2 * e + 1] + p1 * sn[2 * e + 1]);
+      for (int u = 0; u < 2; ++u) {
+        const int h = ha + u * stride;
+        if (h >= hs || (h >= a.heads && id < 0)) break;
+        ss_u32x4 y0, y1;
+        if (a.adjacent) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = T::widen(x0[u][e] & 0xFFFFu), p1 = T::widen(x0[u][e] >> 16);
+            const float q0 = T::widen(x1[u][e] & 0xFFFFu), q1 = T::widen(x1[u][e] >> 16);
+            y0[e] = T::pack(p0 * cs[e] - p1 * sn[e], p1 * cs[e] + p0 * sn[e]);
+            y1[e] = T::pack(q0 * cs[4 + e] - q1 * sn[4 + e], q1 * cs[4 + e] + q0 * sn[4 + e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = T::widen(x0[u][e] & 0xFFFFu), p1 = T::widen(x0[u][e] >> 16);
+            const float q0 = T::widen(x1[u][e] & 0xFFFFu), q1 = T::widen(x1[u][e] >> 16);
+            y0[e] = T::pack(p0 * cs[2 * e] - q0 * sn[2 * e], p1 * cs[2 * e + 1] - q1 * sn[2 * e + 1]);
+            y1[e] = T::pack(q0 * cs[2 * e] + p0 * sn[2 * e], q1 * cs[2 * e + 1] + p1 * sn[2 * e + 1]);
+          }
         }
+        uint16_t* dst = to(r, h, rr);
+        *(SS_G ss_u32x4*)(dst + o0) = y0;
+        *(SS_G ss_u32x4*)(dst + o1) = y1;
       }
-      uint16_t* dst;
-      if (isq) {
-        dst = a.out + (r * a.heads + h) * D;
-      } else {
-        if (id < 0) continue;
-        dst = a.k_pages + (((int64_t)id * a.kv_heads + (h - a.heads)) * page + off + rr) * D;
-      }
-      *(SS_G ss_u32x4*)(dst + o0) = y0;
-      *(SS_G ss_u32x4*)(dst + o1) = y1;
     }
   }
   // Elements past rot, as they are.
   const int rest = (D - a.rot) / 8;
   for (int it = lane; it < 8 * rest; it += 64) {
-    const int rr = it / rest, o = a.rot + 8 * (it - rr * rest), row = first + rr - sr.pos0;
+    const int rr = (uint32_t)it / (uint32_t)rest, o = a.rot + 8 * (it - rr * rest), row = first + rr - sr.pos0;
     if (row < 0 || row >= sr.n) continue;
     const int64_t r = sr.r0 + row;
-    for (int h = h0; h < a.heads + a.kv_heads; h += stride) {
-      const bool isq = h < a.heads;
-      if (!isq && id < 0) continue;
-      const uint16_t* src = isq ? a.q + r * a.q_row + h * a.q_head : a.k + r * a.k_row + (h - a.heads) * a.k_head;
-      uint16_t* dst = isq ? a.out + (r * a.heads + h) * D
-                          : a.k_pages + (((int64_t)id * a.kv_heads + (h - a.heads)) * page + off + rr) * D;
-      *(SS_G ss_u32x4*)(dst + o) = *(const SS_G ss_u32x4*)(src + o);
+    for (int ha = h0; ha < hs; ha += 4 * stride) {
+      ss_u32x4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (ha + u * stride < hs) x[u] = *(const SS_G ss_u32x4*)(from(r, ha + u * stride) + o);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int h = ha + u * stride;
+        if (h >= hs || (h >= a.heads && id < 0)) break;
+        *(SS_G ss_u32x4*)(to(r, h, rr) + o) = x[u];
+      }
     }
   }
   // Value rows.

@@ -1438,10 +1438,12 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
   a.adjacent = p->adjacent != 0;
   a.factor = p->factor;
   a.tiles = (int)(((int64_t)a.max_rows + 14) / 8);
-  // A workgroup's four waves take its heads in turn; where there are few groups of positions the heads are shared out too (64
-  // single tokens of 36 heads 6 us, 15 with one workgroup each).
+  // A workgroup's four waves take its heads in turn; where there are few groups of positions the heads are shared out too, to
+  // some three workgroups a CU. Shared by 1 / 2 / 3 / 4 / 5 / 9, in us: 8,190 rows (1,026 groups) of 40 heads of 128 45 / 53 /
+  // 47 / 68 / 45 / 52, of 18 of 256 37 / 45 / 39 / 55 / 42 / 43; 4,090 (514) of 16 of 128 13.8 / 14.0 / 14.4 / 17.2 / 17.2 / 17.3;
+  // 2,040 (258) of 40 of 128 17.5 / 15.6 / 15.5 / 17.1 / 15.3 / 17.1; 510 (66) of 36 of 128 14.8 / 13.2 / 12.0 / 12.0 / 11.5 / 11.2.
   const int64_t groups = std::max<int64_t>((int64_t)a.tiles * p->seqs, 1);
-  a.head_groups = (int)std::min<int64_t>((1024 + groups - 1) / groups, (p->heads + p->kv_heads + 3) / 4);
+  a.head_groups = (int)std::min<int64_t>((768 + groups - 1) / groups, (p->heads + p->kv_heads + 3) / 4);
   if ((int64_t)a.tiles * a.head_groups * p->seqs > INT32_MAX)
     return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
   return hip_check(ss::launch_rope_append(a, p->type == SSMOE_FP16, static_cast<hipStream_t>(stream)), "rope launch");

@@ -20,7 +20,9 @@ k drafts reach the host once, at the end, and the chain can be captured in a HIP
 The attention segment is optional: HeadAttention puts hc_mix of attn_hyper_connection, plain causal attention over the
 head's own paged cache (engine/attention.py, in the place of the reference's QSA) and its residual between fuse and the MoE.
 MTPState keeps the position bookkeeping of the reference's state (pos, aligned, fork, reset): entry i of the cache is the
-head's i-th row. Drafts are rows past the state's position; the next consume writes over them.
+head's i-th row. Drafts are rows past the state's position; the next consume writes over them. The forks of a state share the head's
+one cache: one of them at a time has rows behind the head's own, and a step of a state whose rows are gone, or that would write over
+the head's own, is refused.
 """
 from __future__ import annotations
 
@@ -69,10 +71,11 @@ class HeadWeights:
 
 
 class MTPState:
-    """Position of the head's cache (engine/mtp.py:84-115): one entry per consumed token except the first."""
+    """Position of the head's cache (engine/mtp.py:84-115): one entry per consumed token except the first. `past` is the mark
+    of the state's last rows in the cache of an attention (CacheRows)."""
 
     def __init__(self, max_ctx: int):
-        self.max_ctx, self.pos = max_ctx, 0
+        self.max_ctx, self.pos, self.past = max_ctx, 0, None
 
     @property
     def offset(self) -> int:
@@ -83,11 +86,39 @@ class MTPState:
 
     def fork(self) -> "MTPState":
         s = MTPState(self.max_ctx)
-        s.pos = self.pos
+        s.pos, s.past = self.pos, self.past
         return s
 
     def reset(self) -> None:
-        self.pos = 0
+        self.pos, self.past = 0, None
+
+
+class CacheRows:
+    """Whose rows the one cache of a head holds: those of the head's own state, behind them those of the fork that was stepped
+    last. A state's rows get a mark when they are written, `marks` are those that the cache still holds, each with the end of
+    its rows: a state whose mark is not there has lost rows to another one."""
+
+    def __init__(self):
+        self.marks: list[tuple[object, int]] = []
+
+    def find(self, state: MTPState, own: MTPState) -> int:
+        """How many of the marks are of the rows before the position of `state`. ValueError where the cache does not hold them, or
+        where rows behind them are the head's (`own`)."""
+        if state.pos < own.pos and state is not own:
+            raise ValueError(f"a state at {state.pos} cannot write over the head's own rows up to {own.pos}")
+        if state.pos == 0:
+            return 0
+        for i, (mark, end) in enumerate(self.marks):
+            if mark is state.past and state.pos <= end:
+                return i + 1
+        raise ValueError(f"the head's cache no longer holds the {state.pos} rows of this state: another state has written since")
+
+    def write(self, state: MTPState, own: MTPState, n: int) -> None:
+        """`n` rows behind the position of `state` become its own; all others from there on are gone."""
+        at, held = state.pos, self.find(state, own)
+        keep = [] if state is own else [(mark, min(end, at)) for mark, end in self.marks[:held]]
+        state.past = object()
+        self.marks = keep + [(state.past, at + n)]
 
 
 @dataclass
@@ -168,7 +199,7 @@ class MTPHead:
         if attn is not None:
             self.cache = SeqCache(attn.pages)
             max_ctx = min(max_ctx, attn.pages.width * attn.pages.page)
-        self.state = MTPState(max_ctx)
+        self.state, self.held = MTPState(max_ctx), CacheRows()
         self.prev_multi: torch.Tensor | None = None
         self.consumed = 0
         self._draft_rows: dict[int, _Rows] = {}
@@ -204,6 +235,13 @@ class MTPHead:
             return mixed, None
         lin_epi(hn, hcw.inject, EPI_INJECT, hc=self.hc, out=inj)
         return mixed, inj
+
+    def _room(self, state: MTPState, n: int) -> None:
+        """Pages for `n` rows of `state` at its position (CacheRows says whether it may have them)."""
+        if self.attn is not None:
+            self.held.find(state, self.state)
+            self.cache.room(state.pos, n)
+            self.held.write(state, self.state, n)
 
     def _attend(self, h: torch.Tensor, pos: int, base: torch.Tensor | None = None, append_only: bool = False):
         """The attention segment over the fused rows h [S, hc H] at the positions pos .. (or those behind the device int32
@@ -262,6 +300,7 @@ class MTPHead:
             raise ValueError(f"embedded must be [S, {self.H}] and multi [S, {self.hc * self.H}]")
         if S < 1 or (not state_only and S > self.max_rows):
             raise ValueError(f"a head step takes 1..{self.max_rows} rows, got {S}")
+        self._room(state, S)
         r = self._rows(1, S)
         if state_only:
             h = self.fuse(embedded, multi, r, 0)
@@ -281,6 +320,7 @@ class MTPHead:
         self.state.reset()
         if self.cache is not None:
             self.cache.reset()
+            self.held = CacheRows()
         self.prev_multi = None
         self.consumed = 0
 
@@ -327,6 +367,10 @@ class MTPHead:
         st = state if state is not None else self.state.fork()
         if st.pos + k > st.max_ctx:
             raise ValueError(f"head context {st.pos + k} exceeds {st.max_ctx}")
+        if base is None:
+            self._room(st, k)
+        elif self.attn is not None:   # rows of no state
+            self.held.write(self.state.fork(), self.state, k)
         r = self.draft_rows(k)
         prev_h = multi
         for i in range(k):
@@ -371,7 +415,7 @@ class DraftGraph:
         if h.attn is not None:
             if h.state.pos + self.k > h.state.max_ctx:
                 raise ValueError(f"head context {h.state.pos + self.k} exceeds {h.state.max_ctx}")
-            h.cache.room(h.state.pos, self.k)
+            h._room(h.state.fork(), self.k)
             self.base.fill_(h.state.pos)
 
     def capture(self) -> None:

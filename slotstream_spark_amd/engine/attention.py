@@ -100,10 +100,9 @@ class SeqCache:
 
     def room(self, pos: int, n: int) -> None:
         """Pages that the tokens pos .. pos + n - 1 may be written to: what the sequence held from `pos` on (rows taken back, drafts) is
-        given up, and a page that a fork holds too is copied first."""
-        if pos < self.pages.length[self.seq]:
-            self.pages.truncate(self.seq, pos)
-        self.pages.reserve(self.seq, pos + n)
+        given up, and a page that a fork holds too is copied first. Nothing changes where it is refused."""
+        at = min(pos, self.pages.length[self.seq])
+        self.pages.rewrite(self.seq, at, pos + n - at)
 
     def place(self, pos: int, n: int) -> None:
         """The next call's rows are the tokens pos .. pos + n - 1: their pages are there, the tensors of rows(n) say so."""

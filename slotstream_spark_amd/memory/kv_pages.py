@@ -96,26 +96,35 @@ class KVPages:
         self._check(seq)
         if tokens < 0:
             raise ValueError(f"cannot extend by {tokens} tokens; truncate() takes tokens away")
-        have, want = self.length[seq], self.length[seq] + tokens
+        self.rewrite(seq, self.length[seq], tokens)
+
+    def rewrite(self, seq: int, at: int, tokens: int) -> None:
+        """truncate() to `at` and extend() by `tokens` in one: pages that both have stay, those given up serve the same call, and
+        where it is refused the sequence keeps what it had."""
+        self._check(seq)
+        if not 0 <= at <= self.length[seq] or tokens < 0:
+            raise ValueError(f"cannot write {tokens} tokens from {at} on over {self.length[seq]}")
+        want = at + tokens
         if want > self.width * self.page:
             raise ValueError(f"{want} tokens exceed the table's {self.width * self.page}")
-        if tokens == 0:
-            return
-        row = self._table[seq]
-        first, last = have // self.page, (want - 1) // self.page + 1
-        new = [w for w in range(first, last) if row[w] < 0]
-        shared = [w for w in range(first, last) if row[w] >= 0 and self._refs[row[w]] > 1]
-        if have % self.page and first in new:
-            raise ValueError(f"the page of token {have - 1} of sequence {seq} was evicted")
-        ids = self._take(len(new) + len(shared))
-        if shared:
-            old = [int(row[w]) for w in shared]
-            self._move(old, ids[len(new):])
-            self._drop(old)
-        for w, p in zip(new + shared, ids):
-            row[w] = p
+        row, last = self._table[seq], -(-want // self.page)
+        first = at // self.page if tokens else last
+        new = [w for w in range(first, last) if row[w] < 0 or self._refs[row[w]] > 1]
+        kept = int(row[first]) if at % self.page and first in new else None   # holds tokens before `at`
+        if kept == -1:
+            raise ValueError(f"the page of token {at - 1} of sequence {seq} was evicted")
+        gone = row[last:][row[last:] >= 0].tolist()
+        if len(new) > self.free_pages + sum(self._refs[p] == 1 for p in gone):
+            self._take(len(new))   # raises: nothing has changed yet
+        self._drop(gone)
+        row[last:] = -1
+        ids = self._take(len(new))
+        if kept is not None:
+            self._move([kept], ids[:1])
+        self._drop(row[new].tolist())
+        row[new] = ids
         self.length[seq] = want
-        if ids:
+        if ids or gone:
             self._publish(seq)
 
     def reserve(self, seq: int, tokens: int) -> None:
@@ -129,13 +138,7 @@ class KVPages:
         self._check(seq)
         if not 0 <= length <= self.length[seq]:
             raise ValueError(f"cannot keep {length} of {self.length[seq]} tokens")
-        row, first = self._table[seq], -(-length // self.page)
-        gone = row[first:][row[first:] >= 0]
-        self.length[seq] = length
-        if len(gone):
-            self._drop(gone.tolist())
-            row[first:] = -1
-            self._publish(seq)
+        self.rewrite(seq, length, 0)
 
     def free(self, seq: int) -> None:
         """Gives back every page of a sequence and the sequence itself."""

@@ -308,8 +308,9 @@ class MTPHead:
                 self._attend(h, state.pos, append_only=True)
             state.pos += S
             return None, h
+        got = self._step_rows(embedded, multi, r, 0, pos=state.pos)
         state.pos += S
-        return self._step_rows(embedded, multi, r, 0, pos=state.pos - S)
+        return got
 
     def logits(self, out: torch.Tensor) -> torch.Tensor:
         """lm_head over the head's output rows -> fp32 [S, V]: lin's bf16 result as fp32 (engine/mtp.py:232-236)."""

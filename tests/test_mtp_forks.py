@@ -6,6 +6,7 @@ import random
 import pytest
 import torch
 
+from slotstream_spark_amd import _lib
 from slotstream_spark_amd.engine import mtp
 from slotstream_spark_amd.engine.attention import SeqCache
 from tests.test_kv_pages import pages
@@ -180,3 +181,28 @@ def test_any_order_of_calls(seed, head):
         for t in states:
             assert t.pos == len(model[id(t)])
     assert refused
+
+
+def test_a_step_that_fails_does_not_advance(head):
+    """Too few pages, or an attention that refuses its arguments: the state stays where it was, and goes on afterwards."""
+    head, own = Head(pages(n=6, seqs=2, tokens=200)), list(range(14))
+    head.feed(own, head.state, state_only=True)
+    other = head.cache.pages.new()
+    head.cache.pages.extend(other, head.cache.pages.free_pages * 16)
+    for state_only in (False, True):
+        with pytest.raises(_lib.Exhausted):
+            head.feed([1] * 3, head.state, state_only)
+        assert head.state.pos == 14
+    head.cache.pages.free(other)
+
+    def refuse(*args):
+        raise ValueError("refused")
+
+    layer, head.attn.layer = head.attn.layer, Layer()
+    head.attn.layer.append = refuse
+    for state_only in (False, True):
+        with pytest.raises(ValueError, match="refused"):
+            head.feed([1, 2], head.state, state_only)
+        assert head.state.pos == 14
+    head.attn.layer = layer
+    assert head.feed([1, 2], head.state) == own + [1, 2]

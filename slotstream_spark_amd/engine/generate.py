@@ -49,26 +49,26 @@ class MoEStack:
         try:
             self.graph = MTPStepGraph(pool, layers, lm_head, depth, norm_weights=norm_weights, eps=eps, top_k=top_k,
                                       device=device, attn=attn, attn_norms=attn_norms, cache=self.cache)
+            self.chunk = int(prompt_chunk)
+            self.prompt_layers = [MoEPrefillLayer(pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=top_k,
+                                                  router_bias=w.router_bias, max_tokens=self.chunk)
+                                  for l, w in enumerate(layers)] if self.chunk > 0 else None
+            self.depth, self.rows, self.nl = depth, depth + 1, len(layers)
+            if pages is not None:   # a pass writes `rows` tokens, also where fewer are kept
+                max_ctx = min(max_ctx, pages.width * pages.page - self.rows)
+            self.embed, self.max_ctx, self.device = embed, max_ctx, torch.device(device)
+            self.argmax = LMHeadArgmax(lm_head, max_rows=self.rows, round_bf16=True, device=device)
+            # the plain steps' logits, kept for the finiteness check of _mtp_decode's plain loop (generate.py:186-189)
+            self.plain_logits = torch.empty((self.rows, lm_head.n), dtype=torch.float32, device=self.device)
+            self.last_finite: list[bool] = []
+            self.tok_rows = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
+            self.row_ids = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
+            self.st = self._state()
+            self.record = rb.StepRecord(self.st, self.rows)
         except Exception:
             if self.cache is not None:   # a refused stack keeps no sequence
                 pages.free(self.cache.seq)
             raise
-        self.chunk = int(prompt_chunk)
-        self.prompt_layers = [MoEPrefillLayer(pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=top_k,
-                                              router_bias=w.router_bias, max_tokens=self.chunk)
-                              for l, w in enumerate(layers)] if self.chunk > 0 else None
-        self.depth, self.rows, self.nl = depth, depth + 1, len(layers)
-        if pages is not None:   # a pass writes `rows` tokens, also where fewer are kept
-            max_ctx = min(max_ctx, pages.width * pages.page - self.rows)
-        self.embed, self.max_ctx, self.device = embed, max_ctx, torch.device(device)
-        self.argmax = LMHeadArgmax(lm_head, max_rows=self.rows, round_bf16=True, device=device)
-        # the plain steps' logits, kept for the finiteness check of _mtp_decode's plain loop (generate.py:186-189)
-        self.plain_logits = torch.empty((self.rows, lm_head.n), dtype=torch.float32, device=self.device)
-        self.last_finite: list[bool] = []
-        self.tok_rows = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
-        self.row_ids = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
-        self.st = self._state()
-        self.record = rb.StepRecord(self.st, self.rows)
 
     def _state(self) -> rb.SeqState:
         return rb.SeqState(attn={"cache": self.cache} if self.cache is not None else {})

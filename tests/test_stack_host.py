@@ -1,0 +1,83 @@
+"""MoEStack without a GPU: what it holds after a refusal and how its positions move, with the step graph, the prompt layers and the
+lm_head replaced by stand-ins."""
+import pytest
+import torch
+
+from slotstream_spark_amd import _lib
+from slotstream_spark_amd.engine import generate, rollback as rb
+from slotstream_spark_amd.engine.step import MoEWeights
+from tests.test_kv_pages import pages
+
+H, V = 64, 32
+
+
+class Graph:
+    """Stands for MTPStepGraph: rows pass through."""
+
+    def __init__(self, pool, layers, lm_head, depth, norm_weights=None, eps=1e-6, top_k=10, device="cpu", attn=None,
+                 attn_norms=None, cache=None):
+        self.nl, self.rows, self.eps = len(layers), depth + 1, eps
+        self.norm_weights, self.attn, self.attn_norms = [None] * (self.nl + 1), attn, [None] * self.nl
+        self.x_in = torch.zeros(self.rows, H, dtype=torch.bfloat16)
+        self.streams, self.mixed = [self.x_in] * (self.nl + 1), [self.x_in] * (self.nl + 1)
+        self.drafts = torch.zeros(depth, dtype=torch.int32)
+
+    def step(self):
+        return None
+
+    def result(self):
+        return None
+
+
+class Argmax:
+    def __init__(self, lm_head, max_rows, round_bf16, device):
+        pass
+
+    def __call__(self, x, ids, logits):
+        ids.fill_(3)
+        logits.zero_()
+
+
+class Prompt:
+    def __init__(self, *args, **kw):
+        pass
+
+    def __call__(self, x):
+        return (x,)
+
+
+class Pool:
+    hidden = H
+
+
+class Head:
+    n = V
+
+
+@pytest.fixture
+def build(monkeypatch):
+    monkeypatch.setattr(generate, "MTPStepGraph", Graph)
+    monkeypatch.setattr(generate, "LMHeadArgmax", Argmax)
+    monkeypatch.setattr(generate, "MoEPrefillLayer", Prompt)
+    monkeypatch.setattr(generate, "gather_rows", lambda src, idx, out=None: src[idx.long()] if out is None else out.copy_(src[idx.long()]))
+
+    def make(kv, **kw):
+        w = MoEWeights(*[torch.zeros(4, H, dtype=torch.bfloat16)] * 5)
+        return generate.MoEStack(Pool, [w, w], Head, torch.zeros(V, H, dtype=torch.bfloat16), depth=2, device="cpu",
+                                 attn=None if kv is None else [None, None], pages=kv, **kw)
+    return make
+
+
+@pytest.mark.parametrize("part", ["MTPStepGraph", "MoEPrefillLayer", "LMHeadArgmax"])
+def test_a_refused_stack_keeps_no_sequence(build, monkeypatch, part):
+    """Whatever part refuses, the only sequence of the pages is free again."""
+    def refuse(*a, **kw):
+        raise ValueError("refused")
+
+    kv = pages(seqs=1)
+    with monkeypatch.context() as m:
+        m.setattr(generate, part, refuse)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="refused"):
+                build(kv, prompt_chunk=16)
+    assert build(kv).cache.seq == 0

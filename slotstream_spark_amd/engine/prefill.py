@@ -24,6 +24,9 @@ from ..memory.slot_pool import SlotPool
 class MoEPrefillLayer:
     def __init__(self, pool: SlotPool, layer: int, router_w, sh_gate, sh_up, sh_down, sh_g, top_k: int = 10,
                  router_bias: torch.Tensor | None = None, max_tokens: int = 2048):
+        for t in (router_w, sh_gate, sh_up, sh_down, sh_g):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_contiguous():
+                raise ValueError("router and shared-expert weights must be contiguous bf16 tensors")
         self.pool, self.layer, self.top_k = pool, layer, top_k
         self.router_w, self.sh_gate, self.sh_up, self.sh_down, self.sh_g = router_w, sh_gate, sh_up, sh_down, sh_g
         self.router_bias = router_bias
@@ -31,9 +34,6 @@ class MoEPrefillLayer:
         self.experts = router_w.shape[0]
         if self.experts != pool.experts:
             raise ValueError(f"router has {self.experts} experts, the pool {pool.experts}")
-        for t in (router_w, sh_gate, sh_up, sh_down, sh_g):
-            if t.dtype != torch.bfloat16 or not t.is_contiguous():
-                raise ValueError("router and shared-expert weights must be contiguous bf16")
         self.max_tokens = max_tokens
         self.shared_inter = sh_gate.shape[0]
         # shared gate, up and shared_expert_gate rows in one weight [2 Is + 1 (padded to 8), H]

@@ -81,3 +81,16 @@ def test_a_refused_stack_keeps_no_sequence(build, monkeypatch, part):
             with pytest.raises(ValueError, match="refused"):
                 build(kv, prompt_chunk=16)
     assert build(kv).cache.seq == 0
+
+
+def test_prompt_layers_refuse_affine_shared_weights():
+    """The verify layer takes 4-bit shared weights (AffineWeight), the prompt layer does not: a ValueError says so."""
+    from slotstream_spark_amd.engine.prefill import MoEPrefillLayer
+    from slotstream_spark_amd.kernels.gemv_affine import AffineWeight
+
+    pool = type("P", (), {"hidden": H, "inter": H, "experts": 4, "device": "cpu"})
+    bf = torch.zeros(4, H, dtype=torch.bfloat16)
+    q4 = AffineWeight(torch.zeros(4, H // 8, dtype=torch.int32), bf[:, :1], bf[:, :1], 4, 64, 4, H)
+    for name in ("router_w", "sh_gate", "sh_up", "sh_down", "sh_g"):
+        with pytest.raises(ValueError, match="contiguous bf16"):
+            MoEPrefillLayer(pool, 0, **{**dict(router_w=bf, sh_gate=bf, sh_up=bf, sh_down=bf, sh_g=bf), name: q4})

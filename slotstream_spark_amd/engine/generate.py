@@ -99,8 +99,8 @@ class MoEStack:
         """The verify pass of a round over pending + drafts (exactly `rows` tokens) with the record begun."""
         if len(tokens) != self.rows:
             raise ValueError(f"a round verifies {self.rows} tokens, got {len(tokens)}")
-        self.record.begin()
         self._pass(tokens)
+        self.record.begin()   # a pass that raised is no round
         self.st.pos += self.rows
         self.st.tokens += [int(t) for t in tokens]
         return self.graph.result()

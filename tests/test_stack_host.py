@@ -94,3 +94,24 @@ def test_prompt_layers_refuse_affine_shared_weights():
     for name in ("router_w", "sh_gate", "sh_up", "sh_down", "sh_g"):
         with pytest.raises(ValueError, match="contiguous bf16"):
             MoEPrefillLayer(pool, 0, **{**dict(router_w=bf, sh_gate=bf, sh_up=bf, sh_down=bf, sh_g=bf), name: q4})
+
+
+@pytest.mark.parametrize("with_cache", [False, True])
+def test_a_refused_round_leaves_no_record_behind(build, with_cache):
+    """A verify round whose pass raises is no outstanding round; the next one is."""
+    stack = build(pages(n=3, seqs=2) if with_cache else None)
+    if with_cache:
+        other = stack.cache.pages.new()
+        stack.cache.pages.extend(other, 48)
+        with pytest.raises(_lib.Exhausted):
+            stack.step([1, 2, 3])
+        stack.cache.pages.free(other)
+    else:
+        with pytest.raises(IndexError):
+            stack.step([1, 2, V])
+    assert stack.record.outstanding == 0 and stack.record.rounds == 0 and stack.st.pos == 0 and stack.st.tokens == []
+    ck = rb.checkpoint(stack)
+    stack.step([1, 2, 3])
+    assert stack.record.outstanding == 1 and stack.record.rounds == 1
+    rb.rollback(stack, stack.record, ck, 2, 3)
+    assert stack.record.outstanding == 0 and stack.st.tokens == [1, 2]

@@ -8,7 +8,8 @@ reference runs QSA (seg_attn, model/layers.py; the head's, engine/mtp.py:209-227
 window with first tokens that stay visible, and one or several position axes.
 
 SeqCache is one sequence of a KVPages as an engine loop holds it: `pos` and `last` are what rollback() sets on the caches of a
-SeqState (engine/rollback.py:26-41), and the batch tensors stay in place, so that a captured step follows them.
+SeqState (engine/rollback.py:26-41), and the batch tensors stay in place, so that a captured step follows them. A MoEStack keeps
+`pos` at its own position; the draft head, whose forks have positions of their own, keeps them in MTPState.
 """
 from __future__ import annotations
 

@@ -95,14 +95,19 @@ class MoEStack:
         g.drafts.copy_(self.tok_rows[1:])
         return g.step()
 
+    def _advance(self, tokens: list[int]) -> None:
+        self.st.pos += len(tokens)
+        self.st.tokens += tokens
+        for c in self.st.attn.values():
+            c.pos = self.st.pos
+
     def step(self, tokens: list[int]) -> AcceptResult:
         """The verify pass of a round over pending + drafts (exactly `rows` tokens) with the record begun."""
         if len(tokens) != self.rows:
             raise ValueError(f"a round verifies {self.rows} tokens, got {len(tokens)}")
         self._pass(tokens)
         self.record.begin()   # a pass that raised is no round
-        self.st.pos += self.rows
-        self.st.tokens += [int(t) for t in tokens]
+        self._advance([int(t) for t in tokens])
         return self.graph.result()
 
     def forward(self, tokens: list[int]) -> tuple[list[int], torch.Tensor]:
@@ -118,8 +123,7 @@ class MoEStack:
             nxt += self.row_ids.cpu().tolist()[:len(chunk)]
             fin += torch.isfinite(self.plain_logits[:len(chunk)]).all(dim=1).cpu().tolist()
             multi.append(self.multi[:len(chunk)].clone())
-            self.st.pos += len(chunk)
-            self.st.tokens += chunk
+            self._advance(chunk)
         self.last_finite = [bool(f) for f in fin]
         return nxt, torch.cat(multi, 0)
 
@@ -150,8 +154,7 @@ class MoEStack:
                 y = layer(mixed)[0]
                 residual_rmsnorm(x, y, mixed, stream_out=x, weight=w[l + 1], eps=eps)
             multi.append(x)
-            self.st.pos += n
-            self.st.tokens += chunk
+            self._advance(chunk)
         last = mixed[-1:].expand(self.rows, -1).contiguous()
         self.argmax(last, ids=self.row_ids, logits=self.plain_logits)
         self.last_finite = [bool(torch.isfinite(self.plain_logits[0]).all())]

@@ -115,3 +115,26 @@ def test_a_refused_round_leaves_no_record_behind(build, with_cache):
     assert stack.record.outstanding == 1 and stack.record.rounds == 1
     rb.rollback(stack, stack.record, ck, 2, 3)
     assert stack.record.outstanding == 0 and stack.st.tokens == [1, 2]
+
+
+@pytest.mark.parametrize("prompt_chunk", [0, 16])
+def test_the_caches_position_follows_the_stacks(build, monkeypatch, prompt_chunk):
+    """SeqCache.pos is the sequence's position after prompts, plain steps, rounds kept whole or in part, and a reset."""
+    monkeypatch.setattr(generate, "residual_rmsnorm", lambda *a, **kw: None)
+    stack = build(pages(n=12), prompt_chunk=prompt_chunk)
+    stack.graph.attn = [lambda x, *args: x] * 2
+    same = lambda n: stack.st.pos == stack.cache.pos == stack.st.attn["cache"].pos == len(stack.st.tokens) == n  # noqa: E731
+    stack.prompt(list(range(1, 20)))
+    assert same(19)
+    stack.forward([5])
+    assert same(20)
+    stack.forward([5, 6, 7, 8])
+    assert same(24)
+    for keep in (1, 3, 2):
+        at, ck = stack.st.pos, rb.checkpoint(stack)
+        stack.step([1, 2, 3])
+        assert same(at + 3)
+        rb.rollback(stack, stack.record, ck, keep, 3)
+        assert same(at + keep) and stack.cache.last is None
+    stack.reset()
+    assert same(0)

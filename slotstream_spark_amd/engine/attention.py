@@ -80,24 +80,25 @@ class AttentionLayer:
 
 
 class SeqCache:
-    """One sequence of `pages`, with text positions (a row's position is its token's place)."""
+    """One sequence of `pages`, with text positions (a row's position is its token's place). Beside the pages it holds 12 bytes for each
+    token that the table covers."""
 
     def __init__(self, pages: KVPages):
-        self.pages, self.seq = pages, pages.new()
-        self.pos, self.last = 0, None
-        dev = pages.k.device
-        self.table = pages.table[self.seq:self.seq + 1]
+        self.pages, self.pos, self.last = pages, 0, None
+        dev, most = pages.k.device, pages.width * pages.page
         self.kv_len = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._cu: dict[int, torch.Tensor] = {}
-        self._rows: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
+        self._cu = torch.zeros((most + 1, 2), dtype=torch.int32, device=dev)   # cu_rows of n rows: [0, n]
+        self._cu[:, 1] = torch.arange(most + 1, dtype=torch.int32, device=dev)
+        self._positions = torch.zeros(most, dtype=torch.int32, device=dev)
+        self.seq = pages.new()
+        self.table = pages.table[self.seq:self.seq + 1]
 
     def rows(self, n: int):
-        """(cu_rows, kv_len, table, positions) of `n` rows: tensors that stay in place; place() sets their contents."""
-        if n not in self._rows:
-            dev = self.pages.k.device
-            self._cu[n] = torch.tensor([0, n], dtype=torch.int32).to(dev)
-            self._rows[n] = (torch.arange(n, dtype=torch.int32).to(dev), torch.arange(n, dtype=torch.int32).to(dev))
-        return self._cu[n], self.kv_len, self.table, self._rows[n][0]
+        """(cu_rows, kv_len, table, positions) of `n` rows: tensors that stay in place; place() sets the contents of kv_len and
+        positions, which are those of the call that it named last."""
+        if not 0 <= n < self._cu.shape[0]:
+            raise ValueError(f"{n} rows exceed the table's {self._cu.shape[0] - 1}")
+        return self._cu[n], self.kv_len, self.table, self._positions[:n]
 
     def room(self, pos: int, n: int) -> None:
         """Pages that the tokens pos .. pos + n - 1 may be written to: what the sequence held from `pos` on (rows taken back, drafts) is
@@ -108,10 +109,8 @@ class SeqCache:
     def place(self, pos: int, n: int) -> None:
         """The next call's rows are the tokens pos .. pos + n - 1: their pages are there, the tensors of rows(n) say so."""
         self.room(pos, n)
-        self.rows(n)
-        positions, steps = self._rows[n]
         self.kv_len.fill_(pos + n)
-        torch.add(steps, pos, out=positions)
+        torch.add(self._cu[:n, 1], pos, out=self._positions[:n])
 
     def reset(self) -> None:
         self.pos, self.last = 0, None

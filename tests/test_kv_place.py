@@ -54,3 +54,26 @@ def test_rounds_over_a_page_border_keep_their_pages():
         check(kv)
         assert kv.length[cache.seq] == pos + 3
     assert len(published) == -(-102 // 16)
+
+
+def test_the_batch_tensors_of_all_row_counts_share_one_memory():
+    """A long-lived sequence meets every prompt length: what it holds on the device does not grow, the tensors of one row count stay
+    in place, and each says its own count."""
+    from slotstream_spark_amd.engine.attention import SeqCache
+    kv = pages(n=13, page=16, tokens=200)
+    cache, places, held = SeqCache(kv), {}, set()
+    for _ in range(2):
+        for n in range(1, 201):
+            cache.place(0, n)
+            cu, kv_len, table, positions = cache.rows(n)
+            assert cu.tolist() == [0, n] and kv_len.tolist() == [n] and positions.tolist() == list(range(n))
+            at = [t.data_ptr() for t in (cu, kv_len, table, positions)]
+            assert places.setdefault(n, at) == at and all(t.is_contiguous() for t in (cu, positions))
+            held |= {t.untyped_storage().data_ptr() for t in (cu, positions)}
+            cache.reset()
+    assert len(held) <= 2
+    cache.place(0, 7)
+    cache.place(7, 3)
+    assert cache.rows(3)[3].tolist() == [7, 8, 9] and cache.rows(5)[0].tolist() == [0, 5] and cache.rows(0)[0].tolist() == [0, 0]
+    with pytest.raises(ValueError, match="exceed"):
+        cache.rows(kv.width * kv.page + 1)

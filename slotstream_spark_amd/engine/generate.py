@@ -144,15 +144,15 @@ class MoEStack:
             if self.cache is not None:
                 self.cache.place(self.st.pos, n)
                 cu, kv_len, table, positions = self.cache.rows(n)
+            attn = self.cache is not None
+            residual_rmsnorm(x, None, mixed, weight=(g.attn_norms if attn else w)[0], eps=eps)
             for l, layer in enumerate(self.prompt_layers):
-                if self.cache is not None:
-                    residual_rmsnorm(x, None, mixed, weight=g.attn_norms[l], eps=eps)
+                if attn:
                     a = g.attn[l](mixed, positions, self.cache.pages.k[l], self.cache.pages.v[l], cu, kv_len, table, n)
                     residual_rmsnorm(x, a, mixed, stream_out=x, weight=w[l], eps=eps)
-                else:
-                    residual_rmsnorm(x, None, mixed, weight=w[l], eps=eps)
                 y = layer(mixed)[0]
-                residual_rmsnorm(x, y, mixed, stream_out=x, weight=w[l + 1], eps=eps)
+                nxt = g.attn_norms[l + 1] if attn and l + 1 < self.nl else w[l + 1]
+                residual_rmsnorm(x, y, mixed, stream_out=x, weight=nxt, eps=eps)
             multi.append(x)
             self._advance(chunk)
         last = mixed[-1:].expand(self.rows, -1).contiguous()

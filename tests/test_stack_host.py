@@ -138,3 +138,18 @@ def test_the_caches_position_follows_the_stacks(build, monkeypatch, prompt_chunk
         assert same(at + keep) and stack.cache.last is None
     stack.reset()
     assert same(0)
+
+
+@pytest.mark.parametrize("attn", [False, True])
+def test_a_prompt_norms_each_row_once(build, monkeypatch, attn):
+    """Launches of the norm over a chunk: the first, and behind every residual the norm that the next segment takes."""
+    calls = []
+    monkeypatch.setattr(generate, "residual_rmsnorm", lambda x, y, mixed, stream_out=None, weight=None, eps=0: calls.append(
+        (y is not None, stream_out is x, weight)))
+    stack = build(pages(n=12) if attn else None, prompt_chunk=16)
+    g = stack.graph
+    g.norm_weights, g.attn_norms = ["mlp0", "mlp1", "final"], ["attn0", "attn1"]
+    g.attn = [lambda x, *args: x] * 2
+    stack.prompt(list(range(20)))
+    want = [(False, False, "attn0"), (True, True, "mlp0"), (True, True, "attn1"), (True, True, "mlp1"), (True, True, "final")]
+    assert calls == 2 * (want if attn else [(False, False, "mlp0"), (True, True, "mlp1"), (True, True, "final")])

@@ -50,9 +50,11 @@ class MoEStack:
             self.graph = MTPStepGraph(pool, layers, lm_head, depth, norm_weights=norm_weights, eps=eps, top_k=top_k,
                                       device=device, attn=attn, attn_norms=attn_norms, cache=self.cache)
             self.chunk = int(prompt_chunk)
-            self.prompt_layers = [MoEPrefillLayer(pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=top_k,
-                                                  router_bias=w.router_bias, max_tokens=self.chunk)
-                                  for l, w in enumerate(layers)] if self.chunk > 0 else None
+            self.prompt_layers = [] if self.chunk > 0 else None
+            for l, w in enumerate(layers if self.chunk > 0 else []):   # one after the other: one set of buffers
+                self.prompt_layers.append(MoEPrefillLayer(
+                    pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=top_k, router_bias=w.router_bias,
+                    max_tokens=self.chunk, buffers=self.prompt_layers[0] if l else None))
             self.depth, self.rows, self.nl = depth, depth + 1, len(layers)
             if pages is not None:   # a pass writes `rows` tokens, also where fewer are kept
                 max_ctx = min(max_ctx, pages.width * pages.page - self.rows)

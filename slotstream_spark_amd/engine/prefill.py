@@ -22,8 +22,11 @@ from ..memory.slot_pool import SlotPool
 
 
 class MoEPrefillLayer:
+    """`buffers`: another layer of the same sizes whose buffers (the workspace, and those of ids, weights and routed, which a call
+    returns parts of) this one uses too; the two then run one after the other on one stream."""
+
     def __init__(self, pool: SlotPool, layer: int, router_w, sh_gate, sh_up, sh_down, sh_g, top_k: int = 10,
-                 router_bias: torch.Tensor | None = None, max_tokens: int = 2048):
+                 router_bias: torch.Tensor | None = None, max_tokens: int = 2048, buffers: MoEPrefillLayer | None = None):
         for t in (router_w, sh_gate, sh_up, sh_down, sh_g):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_contiguous():
                 raise ValueError("router and shared-expert weights must be contiguous bf16 tensors")
@@ -41,6 +44,13 @@ class MoEPrefillLayer:
         pad = (-n_sh) % 8
         self.sh_cat = torch.cat([sh_gate, sh_up, sh_g] + ([sh_g.new_zeros((pad, self.hidden))] if pad else [])).contiguous()
         dev, R = pool.device, max_tokens * top_k
+        if buffers is not None:
+            sizes = lambda l: (l.max_tokens, l.top_k, l.experts, l.hidden, l.inter, torch.device(l.pool.device))  # noqa: E731
+            if sizes(buffers) != sizes(self):
+                raise ValueError(f"buffers of a layer of {sizes(buffers)} do not fit one of {sizes(self)}")
+            self.workspace, self.h_buf, self.out_rows = buffers.workspace, buffers.h_buf, buffers.out_rows
+            self.ids, self.weights, self.routed = buffers.ids, buffers.weights, buffers.routed
+            return
         L = _lib.lib()
         nb = L.ssmoe_moe_prefill_workspace_bytes(max_tokens, top_k, self.experts)
         self.workspace = torch.empty(int(nb), dtype=torch.uint8, device=dev)

@@ -4,9 +4,11 @@ import pytest
 import torch
 
 from slotstream_spark_amd import _lib
+from slotstream_spark_amd.engine.generate import mtp_decode
 from slotstream_spark_amd.engine.mtp import MTPState
+from slotstream_spark_amd.engine.prefill import MoEPrefillLayer
 from slotstream_spark_amd.memory.synth import normal_bf16
-from tests.test_gpu_attention_layer import H, bits, make_head, parts  # noqa: F401  (parts is a fixture)
+from tests.test_gpu_attention_layer import H, K, NL, V, bits, make_head, make_stack, parts  # noqa: F401  (parts is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -34,4 +36,31 @@ def test_forks_of_the_heads_state(parts, hc):  # noqa: F811
     with pytest.raises(ValueError, match="head's own rows"):
         a.step(a.embed([7]), a.prev_multi, MTPState(64), state_only=True)
     assert a.draft(9, 3) == b.draft(9, 3) and torch.equal(bits(a.draft_rows(3).out), bits(b.draft_rows(3).out))
+    assert _lib.device_error() == 0
+
+
+def test_prompt_layers_with_shared_buffers(parts):  # noqa: F811
+    """A prompt through layers that share their buffers has the bits of one through layers with buffers of their own."""
+    pool, lws, lm = parts
+    a, b = make_stack(parts, 16), make_stack(parts, 16)
+    b.prompt_layers = [MoEPrefillLayer(pool, l, w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g, top_k=K, max_tokens=16)
+                       for l, w in enumerate(lws[:NL])]
+    tokens = [(37 * i + 5) % V for i in range(40)]
+    (na, ma), (nb, mb) = a.prompt(tokens), b.prompt(tokens)
+    assert na == nb and torch.equal(bits(ma), bits(mb)) and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("prompt_chunk", [0, 16])
+def test_positions_of_a_loop(parts, prompt_chunk):  # noqa: F811
+    """With the head's own drafts and without: stack, cache and head stand at the end of what was emitted."""
+    stack, head, prompt = make_stack(parts, prompt_chunk), make_head(parts, 1), [5, 17, 300, 8, 1234, 77, 9, 9, 2, 64, 1000, 41, 3, 50, 11]
+    for draft_fn in (None, lambda pending, depth, n_out: [1] * depth):
+        stack.reset()
+        head.reset()
+        out, nan, _, st = mtp_decode(stack, head, prompt, 20, draft_fn=draft_fn)
+        assert len(out) == 20 and not nan and st["rounds"] > 0
+        # the last token is emitted and not run; a round that ends the loop may keep drafts behind the last emitted token's row
+        assert stack.st.pos == stack.cache.pos == head.consumed == len(stack.st.tokens) and head.state.aligned(head.consumed)
+        assert stack.st.tokens[:len(prompt) + 19] == prompt + out[:19]
+        assert len(prompt) + 19 <= stack.st.pos <= len(prompt) + 19 + stack.depth
     assert _lib.device_error() == 0

@@ -153,3 +153,23 @@ def test_a_prompt_norms_each_row_once(build, monkeypatch, attn):
     stack.prompt(list(range(20)))
     want = [(False, False, "attn0"), (True, True, "mlp0"), (True, True, "attn1"), (True, True, "mlp1"), (True, True, "final")]
     assert calls == 2 * (want if attn else [(False, False, "mlp0"), (True, True, "mlp1"), (True, True, "final")])
+
+
+def test_the_prompt_layers_of_a_stack_share_their_buffers(build, monkeypatch):
+    """48 layers for chunks of 2,048 tokens would hold 10 GB of buffers that only one of them uses at a time."""
+    from slotstream_spark_amd.engine.prefill import MoEPrefillLayer
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libssmoe.so not built (python -m slotstream_spark_amd.build)")
+    monkeypatch.setattr(generate, "MoEPrefillLayer", MoEPrefillLayer)
+    for name, value in (("inter", 128), ("experts", 4), ("device", "cpu")):
+        monkeypatch.setattr(Pool, name, value, raising=False)
+    layers = build(pages(seqs=2), prompt_chunk=16, top_k=2).prompt_layers
+    buffers = [[t.data_ptr() for t in (l.workspace, l.h_buf, l.out_rows, l.ids, l.weights, l.routed)] for l in layers]
+    assert len(buffers) == 2 and buffers[0] == buffers[1] and layers[0].sh_cat is not layers[1].sh_cat
+    bf = torch.zeros(4, H, dtype=torch.bfloat16)
+    alone = MoEPrefillLayer(Pool, 0, bf, bf, bf, bf, bf, top_k=2, max_tokens=16)
+    assert alone.h_buf.data_ptr() not in buffers[0]
+    for kw in (dict(max_tokens=17), dict(top_k=3)):
+        with pytest.raises(ValueError, match="do not fit"):
+            MoEPrefillLayer(Pool, 0, bf, bf, bf, bf, bf, **{"top_k": 2, "max_tokens": 16, **kw}, buffers=alone)

@@ -33,7 +33,8 @@ extern "C" {
 #define SSMOE_ERR_PAGE 32     /* a page id outside [0, n_pages) where a cache token is read, written or moved: read as not
                                * there, not written */
 #define SSMOE_ERR_BATCH 64    /* cu_rows or kv_len contradict the call (rows outside [0, rows), more than max_rows of a
-                               * sequence, a length below 0 or beyond the table): cut to what the call's shapes allow */
+                               * sequence, a length below 0 or beyond the table): cut to what the call's shapes allow; or an
+                               * axis outside [0, axes): its frequency is turned by position 0 */
 
 /* Text of the last error on this host thread ("" if none). */
 const char* ssmoe_last_error(void);

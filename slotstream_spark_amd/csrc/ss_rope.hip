@@ -60,7 +60,11 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
     const int rr = (uint32_t)it / (uint32_t)half, f = it - rr * half, row = first + rr - sr.pos0;
     if (row < 0 || row >= sr.n) continue;
     const int ax = a.axis ? gp(a.axis)[f] : 0;
-    const int p = (uint32_t)ax < (uint32_t)a.axes ? gp(a.positions)[ax * a.pos_stride + sr.r0 + row] : 0;
+    int p = 0;
+    if ((uint32_t)ax < (uint32_t)a.axes)
+      p = gp(a.positions)[ax * a.pos_stride + sr.r0 + row];
+    else
+      raise_bit(a.err, SS_ERR_BATCH);
     const double turns = (double)p * (gp(a.inv_freq)[f] * 0.15915494309189533577);
     float sn, cs;
     sincospif(2.f * (float)(turns - __builtin_rint(turns)), &sn, &cs);

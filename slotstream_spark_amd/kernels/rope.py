@@ -33,7 +33,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     dim] into the cache at their sequence's places (row i of n at token kv_len - n + i) and returns the turned q.
 
     positions int32 [rows] or [axes, rows]; inv_freq fp64 [rot / 2]; the angle of frequency i is positions[axis[i], row] *
-    inv_freq[i], axis int32 [rot / 2] (None: axis 0). The pair turned by it is (i, i + rot / 2), or (2 i, 2 i + 1) with
+    inv_freq[i], axis int32 [rot / 2] (None: axis 0; an entry outside [0, axes) raises SSMOE_ERR_BATCH in the device status). The pair turned by it is (i, i + rot / 2), or (2 i, 2 i + 1) with
     `adjacent`; elements from rot on are copied. cos and sin are multiplied by `factor`. q, k and v may be views into
     one projection (strides multiples of 8 elements); `out` may be q itself where q is contiguous, and overlaps none of them
     else. Rows past cu_rows[-1] are left as they were."""

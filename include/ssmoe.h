@@ -543,8 +543,8 @@ int ssmoe_gather_rows(const void* src, int64_t n_src, int64_t row_bytes, const i
  * fraction of a turn in fp64); axis NULL means axis 0 (text), 3 axes with an axis per frequency are the (time,
  * height, width) positions of images and video. The pair turned is (i, i + rot / 2), or (2 i, 2 i + 1) with adjacent;
  * elements from rot on are copied. cos and sin are multiplied by factor. One rounding to 16 bits at the end. Rows with
- * a position below 0 are turned but not written. q_out is q itself (contiguous) or overlaps none of q, k and v. Two rows that
- * share a place (a page in two sequences' tables) race. */
+ * a position below 0 are turned but not written. q_out is q itself (contiguous) or apart from q, k and v; q_out and the pages are apart
+ * from all else that the call reads or writes. Two rows that share a place (a page in two sequences' tables) race. */
 typedef struct {
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
@@ -564,7 +564,8 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* a, void* stream);
 /* out row i = sum_j softmax_j(scale * q_i . k_j) v_j over the tokens j <= p of its sequence (p its position), under
  * window > 0 only those with p - j < window or j < sinks (the first tokens that stay visible); lse (fp32 [rows][heads], or
  * NULL) = ln sum_j exp(scale * q_i . k_j). Head h reads key head h / (heads / kv_heads). A row that sees nothing is 0 with
- * lse -inf. q [rows][heads][dim] with the given strides (elements, multiples of 8), out contiguous and apart from q. Scores, maxima, sums and
+ * lse -inf. q [rows][heads][dim] with the given strides (elements, multiples of 8), out contiguous. out, lse and ws are
+ * apart from each other and from all that the call reads. Scores, maxima, sums and
  * partial results are fp32; a probability is rounded to the element type before its product with the values. What the
  * cache holds at tokens that a row does not see does not reach it, infinities and NaN included.
  * Calls with max_rows <= 8 (decoding, verification): the bits of a row depend on its sequence's tokens, seqs, kv_heads and
@@ -589,7 +590,8 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* a, void* stream);
 /* Page dst[i] := page src[i] for i < n, keys and values of every layer ([layers][n_pages][page_bytes] each), and table
  * entries (int32 [entries], or NULL) equal to src[i] become dst[i] (the lowest such i): the copies of a fork, the moves of a
  * compaction. src and dst int32 [n] on the device; no page may be in dst twice, or in src and dst (the result of such a
- * page is undefined, nothing else is touched). page_bytes a multiple of 2048. */
+ * page is undefined, nothing else is touched). page_bytes a multiple of 2048. k, v and the table are apart from each other and from src
+ * and dst. */
 int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page_bytes, const int32_t* src,
                      const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream);
 

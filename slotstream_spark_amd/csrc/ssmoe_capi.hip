@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <exception>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -223,6 +224,28 @@ bool overlap(const void* a, int64_t a_row, int64_t a_head, int a_heads, const vo
   };
   return reinterpret_cast<uintptr_t>(a) < end(b, b_row, b_head, b_heads) &&
          reinterpret_cast<uintptr_t>(b) < end(a, a_row, a_head, a_heads);
+}
+
+// The bytes that an argument names; none where it is null.
+struct Span {
+  const char* name;
+  uintptr_t a, b;
+  Span(const char* n, const void* p, int64_t bytes)
+      : name(n), a(reinterpret_cast<uintptr_t>(p)), b(p && bytes > 0 ? a + (uintptr_t)bytes : a) {}
+  // [rows][heads][dim] 16-bit elements, strides in elements
+  Span(const char* n, const void* p, int rows, int64_t row, int heads, int64_t head, int dim)
+      : Span(n, p, 2 * ((rows - 1) * row + (heads - 1) * head + dim)) {}
+};
+// What a call writes must lie apart from all else that it writes or reads.
+int check_apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  auto meet = [](const Span& x, const Span& y) { return x.a < y.b && y.a < x.b; };
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    for (auto o = w + 1; o != written.end(); ++o)
+      if (meet(*w, *o)) return fail(SSMOE_EINVAL, "%s must not overlap %s", w->name, o->name);
+    for (const Span& r : read)
+      if (meet(*w, r)) return fail(SSMOE_EINVAL, "%s must not overlap %s", w->name, r.name);
+  }
+  return ok();
 }
 
 // How a call of ssmoe_paged_attention is laid out (its checks included). `prompt`: the kernel for many rows of a sequence.
@@ -1405,6 +1428,19 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
       overlap(p->k, p->k_row, p->k_head, p->kv_heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim) ||
       overlap(p->v, p->v_row, p->v_head, p->kv_heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim))
     return fail(SSMOE_EINVAL, "q_out must be q itself (contiguous) or overlap none of q, k and v");
+  const int64_t cache = 2 * p->n_pages * p->kv_heads * p->page * p->dim, pos = p->axes > 1 ? (p->axes - 1) * p->pos_stride : 0;
+  const Span q("q", p->q, p->rows, p->q_row, p->heads, p->q_head, p->dim);
+  if (int rc = check_apart({{"q_out", p->q_out, 2 * p->rows * o_row}, {"k_pages", p->k_pages, cache}, {"v_pages", p->v_pages, cache}},
+                           {same ? Span("q", nullptr, 0) : q,
+                            {"k", p->k, p->rows, p->k_row, p->kv_heads, p->k_head, p->dim},
+                            {"v", p->v, p->rows, p->v_row, p->kv_heads, p->v_head, p->dim},
+                            {"positions", p->positions, 4 * (pos + p->rows)},
+                            {"inv_freq", p->inv_freq, 4 * (int64_t)p->rot},
+                            {"axis", p->axis, 2 * (int64_t)p->rot},
+                            {"cu_rows", p->cu_rows, 4 * ((int64_t)p->seqs + 1)},
+                            {"kv_len", p->kv_len, 4 * (int64_t)p->seqs},
+                            {"table", p->table, 4 * (int64_t)p->seqs * p->width}}))
+    return rc;
   a.q = static_cast<const uint16_t*>(p->q);
   a.k = static_cast<const uint16_t*>(p->k);
   a.v = static_cast<const uint16_t*>(p->v);
@@ -1473,6 +1509,15 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
                 (long long)(p->ws ? p->ws_bytes : 0), (long long)ws);
   if (overlap(p->q, p->q_row, p->q_head, p->heads, p->out, (int64_t)p->heads * p->dim, p->dim, p->heads, p->rows, p->dim))
     return fail(SSMOE_EINVAL, "out must not overlap q");
+  const int64_t cache = 2 * p->n_pages * p->kv_heads * p->page * p->dim, heads = (int64_t)p->rows * p->heads;
+  if (int rc = check_apart({{"out", p->out, 2 * heads * p->dim}, {"lse", p->lse, 4 * heads}, {"ws", p->ws, ws}},
+                           {{"q", p->q, p->rows, p->q_row, p->heads, p->q_head, p->dim},
+                            {"k_pages", p->k_pages, cache},
+                            {"v_pages", p->v_pages, cache},
+                            {"cu_rows", p->cu_rows, 4 * ((int64_t)p->seqs + 1)},
+                            {"kv_len", p->kv_len, 4 * (int64_t)p->seqs},
+                            {"table", p->table, 4 * (int64_t)p->seqs * p->width}}))
+    return rc;
   a.q = static_cast<const uint16_t*>(p->q);
   a.q_row = p->q_row;
   a.q_head = p->q_head;
@@ -1509,7 +1554,12 @@ int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page
   if (n == 0) return ok();
   if (!k || !v || !src || !dst) return fail(SSMOE_EINVAL, "k, v, src and dst must be non-null");
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(SSMOE_EINVAL, "k and v must be 16-byte aligned");
-  if (page_bytes / 2048 > ((int64_t)1 << 30) / n / layers) return fail(SSMOE_EINVAL, "too many bytes for one call");
+  if (page_bytes / 2048 > ((int64_t)1 << 30) / n / layers || page_bytes > INT64_MAX / n_pages / layers)
+    return fail(SSMOE_EINVAL, "too many bytes for one call");
+  const int64_t cache = layers * n_pages * page_bytes;
+  if (int rc = check_apart({{"k", k, cache}, {"v", v, cache}, {"table", table, 4 * entries}},
+                           {{"src", src, 4 * (int64_t)n}, {"dst", dst, 4 * (int64_t)n}}))
+    return rc;
   ss::MoveArgs a{};
   a.k = static_cast<uint8_t*>(k);
   a.v = static_cast<uint8_t*>(v);

@@ -12,7 +12,7 @@ def move_pages(k: torch.Tensor, v: torch.Tensor, src: torch.Tensor, dst: torch.T
                table: torch.Tensor | None = None) -> None:
     """Page dst[i] := page src[i] of every layer; k and v are [layers, n_pages, ...] of the same bytes a page. src and dst
     int32 [n] on the GPU. Entries of `table` (int32, any shape) that name src[i] name dst[i] afterwards. No page may be twice
-    in dst, nor in both src and dst (its contents would be undefined); ids outside the cache are skipped and raise
+    in dst, nor in both src and dst (its contents would be undefined); k, v and the table overlap each other, src and dst nowhere; ids outside the cache are skipped and raise
     SSMOE_ERR_PAGE in the device status."""
     if k.dim() < 3 or k.shape[:2] != v.shape[:2] or k.dtype != v.dtype or k.numel() != v.numel():
         raise ValueError("k and v must be [layers, n_pages, ...] of one type and size")

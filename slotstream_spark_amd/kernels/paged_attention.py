@@ -115,8 +115,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """q [rows, heads, dim] -> [rows, heads, dim] of q's type. `max_rows` bounds the rows of one sequence. window 0: every
     token up to the row's own; else the last `window` of them and the first `sinks`. scale: 1 / sqrt(dim) unless given.
     `lse` fp32 [rows, heads] receives ln sum_j exp(scale q_i . k_j). A row that sees nothing is 0, its lse -inf; rows past
-    cu_rows[-1] are left as they were in `out` and `lse`. `out` must not overlap q. Capturable; workspaces come from torch's allocator at each
-    call, so calls and captured graphs never share one."""
+    cu_rows[-1] are left as they were in `out` and `lse`, which must not overlap each other nor anything that the call reads.
+    Capturable; workspaces come from torch's allocator at each call, so calls and captured graphs never share one."""
     max_rows, window, sinks = int(max_rows), int(window), int(sinks)
     key = (q.shape, q.stride(), q.dtype, k_pages.shape, k_pages.dtype, k_pages.is_contiguous(), v_pages.shape, v_pages.dtype,
            v_pages.is_contiguous(), cu_rows.shape, cu_rows.stride(), cu_rows.dtype, kv_len.shape, kv_len.stride(), kv_len.dtype,

@@ -35,8 +35,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     positions int32 [rows] or [axes, rows]; inv_freq fp64 [rot / 2]; the angle of frequency i is positions[axis[i], row] *
     inv_freq[i], axis int32 [rot / 2] (None: axis 0; an entry outside [0, axes) raises SSMOE_ERR_BATCH in the device status). The pair turned by it is (i, i + rot / 2), or (2 i, 2 i + 1) with
     `adjacent`; elements from rot on are copied. cos and sin are multiplied by `factor`. q, k and v may be views into
-    one projection (strides multiples of 8 elements); `out` may be q itself where q is contiguous, and overlaps none of them
-    else. Rows past cu_rows[-1] are left as they were."""
+    one projection (strides multiples of 8 elements); `out` may be q itself where q is contiguous; else it and the pages overlap
+    each other and the inputs nowhere. Rows past cu_rows[-1] are left as they were."""
     max_rows = int(max_rows)
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape,
            positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, inv_freq.is_contiguous(), k_pages.shape,

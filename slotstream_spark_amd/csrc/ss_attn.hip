@@ -100,9 +100,13 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   static_assert(sizeof(JoinRow) <= SLOT, "the waves' sums fit the slots");
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
-  uint32_t b = blockIdx.x;
-  const int slot = b % (uint32_t)a.slots;
-  b /= (uint32_t)a.slots;
+  // Slot by slot, so that those which have work are neighbours: of a table wider than its sequences they are the first ones. (Workgroups
+  // are dealt to the 8 XCDs and their CUs in turn: with a sequence's slots side by side every 32nd had work on a table of 32 slots,
+  // all on one XCD. 64 sequences of up to 2,000 tokens and 8 key heads on tables of 2,112 / 8,192 / 32,768 / 131,072 tokens: 63 / 67 /
+  // 68 / 85 us, so 63 / 98 / 283 / 902; of up to 16,384 on 16,448 and 131,072 483 and 486, so 539 and 2,950.)
+  const uint32_t units = (uint32_t)(a.tiles * a.kv_heads) * (uint32_t)a.seqs;
+  const int slot = blockIdx.x / units;
+  uint32_t b = blockIdx.x - slot * units;
   const int tile = b % (uint32_t)a.tiles;
   b /= (uint32_t)a.tiles;
   const int h = b % (uint32_t)a.kv_heads, s = b / (uint32_t)a.kv_heads;

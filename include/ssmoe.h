@@ -569,7 +569,9 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* a, void* stream);
  * partial results are fp32; a probability is rounded to the element type before its product with the values. What the
  * cache holds at tokens that a row does not see does not reach it, infinities and NaN included.
  * Calls with max_rows <= 8 (decoding, verification): the bits of a row depend on its sequence's tokens, seqs, kv_heads and
- * the width of the table, not on the other rows of the call.
+ * the width of the table, not on the other rows of the call. With more, all of the call's sequences take the many-row form, single
+ * tokens among them: split over their length only as far as the row tiles of all sequences at max_rows leave CUs without work.
+ * Two calls over one q and out, each with its part of cu_rows, kv_len and table, serve prompts and single tokens apart.
  * ws: at least ssmoe_paged_attention_workspace_bytes(a) bytes, 256-byte aligned (may be NULL when that is 0); nothing
  * is kept in it between calls, and calls that may run at the same time need one each. */
 typedef struct {

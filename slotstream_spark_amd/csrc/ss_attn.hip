@@ -27,9 +27,9 @@
 // values; where any are, they are taken out of the product and added at the join, by three more products with ones in their
 // places and ones for the tokens seen, to the rows that see them.
 //
-// Measured, kernel alone: 64 sequences of up to 16,384 tokens (32 heads on 8, 128 dimensions, 2.7 GB) 540 us, 5.0 TB/s, where a
-// streaming read reaches 5.3; one of 131,072 tokens (268 MB) 41 us; one of 777 5.5 us, the chain of a sequence's place, its
-// pages, its keys and the columns' sums. Operands straight from memory into registers took 582 us for the first.
+// Measured, kernel alone: 64 sequences of up to 16,384 tokens (32 heads on 8, 128 dimensions, 2.7 GB) 478 us, 5.7 TB/s, where a
+// streaming read reaches 5.3; one of 131,072 tokens (268 MB) 42 us; one of 777 5.2 us, the chain of a sequence's place, its
+// pages, its keys and the columns' sums. Operands straight from memory into registers took 8 % longer for the first.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"
@@ -296,6 +296,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
           p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -mu));
           l[n] += p[e];
         }
+        // A weight is rounded to the element type here, once, as the matrix unit takes it (a half step of it, as much as the result's
+        // own rounding); the row's sum has the weights before that.
 #pragma unroll
         for (int i = 0; i < 4; ++i) pf[n][i] = T::pack(p[2 * i], p[2 * i + 1]);
       }

@@ -27,7 +27,7 @@ struct AttnArgs {
   int window;  // keys a row sees counted back from its own; INT_MAX / 2 for all
   int sinks;   // first tokens that stay visible under a window
   int slots;   // chunks of one sequence that the grid covers
-  int chunk;   // tokens of a chunk, a multiple of 128, at most 4096
+  int chunk;   // tokens of a chunk, a multiple of 128; at most 4096 with few rows, up to the whole table with many
   int packed;  // packed rows (rows times heads of a key head) of a workgroup
   int tiles;   // workgroups over the packed rows of one sequence and key head
   int rising;  // many rows: the tiles at the end of the launch that go up

@@ -20,7 +20,7 @@
 //
 // Bound by the matrix units and what runs beside them: a tile of 64 tokens and 128 dimensions is 32 products (1,024 cycles of a
 // SIMD) beside some 290 other instructions, 32 exponentials among them. 8,191 rows of 32 heads under a window of 4,096 (551
-// GFLOP) take 580-620 us, 0.92 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
+// GFLOP) take 570-620 us, 0.89 to 0.97 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
           const float q0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], a.scale, -mu));
           const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e + 1], a.scale, -mu));
           part[q / 2 % 2] += q0;
-          part[q / 2 % 2] += q1;
+          part[q / 2 % 2] += q1;  // the sum has the weights as they are, the product rounded once to the element type
           pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
         }
       }

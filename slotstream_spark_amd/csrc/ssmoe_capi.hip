@@ -252,7 +252,8 @@ int check_apart(std::initializer_list<Span> written, std::initializer_list<Span>
 //
 // Few rows (up to kFewRows): chunk is the tokens of one workgroup, so that a batch of full tables makes a workgroup a CU, but
 // none of fewer than 128 tokens (a tile for each wave), and none of more than 512 to 4096 (by how far the sequences and key
-// heads alone fill the CUs: a short sequence on a wide table has to find its CUs too). Where a split would take less than 512
+// heads alone fill the CUs: a short sequence on a wide table has to find its CUs too; one of 131,072 tokens and 4 key heads is
+// 1,028 workgroups of 512). Where a split would take less than 512
 // tokens off a workgroup (256 of 256 dimensions) it is not worth the join: a call on a table of 256 / 512 / 768 tokens, whole
 // against split, takes 6.0 / 7.7 / 9.5 against 7.8 / 7.9 / 8.7 us (one row of 32 heads on 4, 128 dimensions, in a graph; the
 // host saves 3 us besides), 7.6 / 10.2 / 12.8 against 8.8 / 9.0 / 9.7 (16 on 2, 256 dimensions), 16 sequences of 768 / 1,024

@@ -34,7 +34,8 @@ class MoEStack:
     """`len(layers)` MoE layers on one residual stream behind an embedding table and in front of the lm_head, run
     `depth` + 1 rows at a time. `st` (rollback.SeqState) and `record` (rollback.StepRecord, empty) hold the sequence.
     `attn` (an AttentionLayer per layer, norms `attn_norms` before them) over `pages` (a KVPages, one sequence of which becomes
-    the stack's) adds attention; max_ctx is then at most what its table covers less a round's rows. `prompt_chunk` > 0: prompts
+    the stack's) adds attention; max_ctx is then at most what its table covers less a round's rows. Under windows the stack keeps
+    its pages all the same: pages.evict(stack.cache.seq, window, sinks, back=stack.rows) between rounds gives those behind them back. `prompt_chunk` > 0: prompts
     go through the prompt forms of the layers (MoEPrefillLayer, and the many-row attention) in chunks of so many tokens
     instead of `rows` at a time."""
 

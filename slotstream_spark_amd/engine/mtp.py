@@ -357,10 +357,12 @@ class MTPHead:
     def draft_async(self, token: torch.Tensor, multi: torch.Tensor, k: int, out: torch.Tensor,
                     state: MTPState | None = None, base: torch.Tensor | None = None) -> torch.Tensor:
         """k greedy drafts after the device token `token` (int32 [1]) chained from `multi` (bf16 [1, hc H]) into
-        `out` (int32 [k]) with no host synchronisation: step i embeds out[i - 1] (token for i = 0) by a device-side
-        gather, runs the head, and writes the argmax of its lm_head row to out[i]. Same launches on every call. With an
+        `out` (int32 [k]): step i embeds out[i - 1] (token for i = 0) by a device-side
+        gather, runs the head, and writes the argmax of its lm_head row to out[i]. Same launches on every call, and no host
+        synchronisation (but for the table's copy where an attention without `base` takes or gives back pages). With an
         attention, the drafts are the cache's rows behind the state's position, or behind state.pos + `base` where that is given
-        (a device int32 [1], whose pages the caller has reserved: the captured form)."""
+        (a device int32 [1], whose pages the caller has reserved: the captured form; those rows are no state's, so a fork that
+        had rows in the cache has lost them)."""
         if token.dtype != torch.int32 or token.numel() != 1 or out.dtype != torch.int32 or out.numel() != k:
             raise ValueError(f"token must be int32 [1] and out int32 [{k}]")
         if tuple(multi.shape) != (1, self.hc * self.H):

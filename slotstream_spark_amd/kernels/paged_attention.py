@@ -113,7 +113,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     scale: float | None = None, out: torch.Tensor | None = None,
                     lse: torch.Tensor | None = None) -> torch.Tensor:
     """q [rows, heads, dim] -> [rows, heads, dim] of q's type. `max_rows` bounds the rows of one sequence. window 0: every
-    token up to the row's own; else the last `window` of them and the first `sinks`. scale: 1 / sqrt(dim) unless given.
+    token up to the row's own; else the last `window` of them and the first `sinks`. scale: 1 / sqrt(dim) unless given. One kernel
+    for the call, chosen by max_rows (up to 8 or more): single tokens in a batch with a prompt go through the prompt's, without
+    the split over their length and the bits of a call of few rows. Two calls over one q and `out`, with cu_rows[:m + 1] and
+    cu_rows[m:], serve them apart (rows outside a call's cu_rows are left alone).
     `lse` fp32 [rows, heads] receives ln sum_j exp(scale q_i . k_j). A row that sees nothing is 0, its lse -inf; rows past
     cu_rows[-1] are left as they were in `out` and `lse`, which must not overlap each other nor anything that the call reads.
     Capturable; workspaces come from torch's allocator at each call, so calls and captured graphs never share one."""

@@ -109,6 +109,10 @@ class SeqCache:
     def place(self, pos: int, n: int) -> None:
         """The next call's rows are the tokens pos .. pos + n - 1: their pages are there, the tensors of rows(n) say so."""
         self.room(pos, n)
+        self.point(pos, n)
+
+    def point(self, pos: int, n: int) -> None:
+        """place() where room() has been called for these tokens, others behind them among them."""
         self.kv_len.fill_(pos + n)
         torch.add(self._cu[:n, 1], pos, out=self._positions[:n])
 

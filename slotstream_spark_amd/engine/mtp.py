@@ -251,7 +251,7 @@ class MTPHead:
         new = lambda cols: torch.empty((S, cols), dtype=torch.bfloat16, device=h.device)  # noqa: E731
         mixed, inj = self.hc_mix(a.hc, h, new(n), new(a.hc.down.shape[0]), new(n), new(self.H), new(self.hc))
         if base is None:
-            self.cache.place(pos, S)
+            self.cache.point(pos, S)   # the caller has made room for all its rows
             cu, kv_len, table, positions = self.cache.rows(S)
         else:
             cu, _, table, _ = self.cache.rows(S)

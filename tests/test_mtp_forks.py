@@ -206,3 +206,15 @@ def test_a_step_that_fails_does_not_advance(head):
         assert head.state.pos == 14
     head.attn.layer = layer
     assert head.feed([1, 2], head.state) == own + [1, 2]
+
+
+def test_drafts_over_a_page_border_publish_the_table_once(head):
+    """15 rows and three drafts, pages of 16 tokens: one page is taken, once, and stays for the next drafts."""
+    head.feed(list(range(15)), head.state, state_only=True)
+    kv, published = head.cache.pages, []
+    publish = kv._publish
+    kv._publish = lambda seq: (published.append(seq), publish(seq))
+    for _ in range(3):
+        head.drafts(50, 3)
+    assert len(published) == 1
+    assert head.feed([60, 61], head.state) == list(range(15)) + [60, 61] and len(published) == 1

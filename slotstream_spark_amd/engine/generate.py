@@ -34,10 +34,10 @@ class MoEStack:
     """`len(layers)` MoE layers on one residual stream behind an embedding table and in front of the lm_head, run
     `depth` + 1 rows at a time. `st` (rollback.SeqState) and `record` (rollback.StepRecord, empty) hold the sequence.
     `attn` (an AttentionLayer per layer, norms `attn_norms` before them) over `pages` (a KVPages, one sequence of which becomes
-    the stack's) adds attention; max_ctx is then at most what its table covers less a round's rows. Under windows the stack keeps
-    its pages all the same: pages.evict(stack.cache.seq, window, sinks, back=stack.rows) between rounds gives those behind them back. `prompt_chunk` > 0: prompts
-    go through the prompt forms of the layers (MoEPrefillLayer, and the many-row attention) in chunks of so many tokens
-    instead of `rows` at a time."""
+    the stack's) adds attention; max_ctx is then at most what its table covers less a round's rows. Where every layer
+    has a window the stack keeps all its pages the same: pages.evict(stack.cache.seq, the widest window, the most first tokens,
+    back=stack.rows) between rounds gives back those that no row sees any more. `prompt_chunk` > 0: prompts go through the prompt
+    forms of the layers (MoEPrefillLayer, and the many-row attention) in chunks of so many tokens instead of `rows` at a time."""
 
     def __init__(self, pool, layers: list[MoEWeights], lm_head: AffineWeight, embed: torch.Tensor,
                  depth: int = mtp_mod.DEPTH, norm_weights=None, eps: float = 1e-6, top_k: int = 10,

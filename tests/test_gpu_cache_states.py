@@ -62,3 +62,21 @@ def test_positions_of_a_loop(parts, prompt_chunk):  # noqa: F811
         assert stack.st.pos == stack.cache.pos == head.consumed == len(prompt) + 19 and head.state.aligned(head.consumed)
         assert stack.st.tokens == prompt + out[:19]                # the last token is emitted and not run
     assert _lib.device_error() == 0
+
+
+def test_pages_behind_the_window_given_back_between_rounds(parts):  # noqa: F811
+    """A loop under windows that evicts before each round emits the same tokens and holds fewer pages."""
+    prompt, outs, free = [5, 17, 300, 8, 1234, 77, 9, 9, 2, 64, 1000, 41, 3, 50, 11, 600, 23, 90, 4], [], []
+    for evict in (False, True):
+        stack, head = make_stack(parts, 16, max_tokens=96, window=20), make_head(parts, 1)
+
+        def drafts(pending, depth, n_out):
+            if evict:
+                stack.cache.pages.evict(stack.cache.seq, 20, 2, back=stack.rows)
+            return [pending, 1] if n_out % 3 else [1, pending]
+
+        out, nan, _, st = mtp_decode(stack, head, prompt, 40, draft_fn=drafts)
+        assert not nan and st["rounds"] > 10
+        outs.append(out)
+        free.append(stack.cache.pages.free_pages)
+    assert outs[0] == outs[1] and free[1] > free[0] and _lib.device_error() == 0

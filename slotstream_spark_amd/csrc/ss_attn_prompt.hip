@@ -20,7 +20,7 @@
 //
 // Bound by the matrix units and what runs beside them: a tile of 64 tokens and 128 dimensions is 32 products (1,024 cycles of a
 // SIMD) beside some 290 other instructions, 32 exponentials among them. 8,191 rows of 32 heads under a window of 4,096 (551
-// GFLOP) take 570-620 us, 0.89 to 0.97 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
+// GFLOP) take 560-620 us, 0.89 to 0.98 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"

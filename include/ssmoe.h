@@ -597,6 +597,54 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* a, void* stream);
 int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page_bytes, const int32_t* src,
                      const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream);
 
+/* ---------------------------------------------------------------- a paged cache in 8 bits, and trees of drafts */
+
+/* Pages of e4m3 numbers (OCP, no infinities): keys [n_pages][kv_heads][page][dim] and values [n_pages][kv_heads][dim][page] of a byte
+ * each, and scales uint8 [n_pages][kv_heads][2][page]: token t's keys are its numbers times 2^(scales[..][0][t] - 127), its
+ * values times 2^(scales[..][1][t] - 127). Written by ssmoe_rope_append_e4m3, which takes the least exponent from -126 on with which
+ * no number is over 448 and rounds once from fp32; a power of two costs e4m3 no precision. Elements that are infinite or NaN are left out of
+ * that choice and kept as NaN (both signs of it read as NaN). A byte of 255 is not written, and what it reads as is not
+ * defined. Queries and rows are SSMOE_BF16 (fp16 has no exponents for a probability times such a scale). Batches, windows
+ * and what unseen places may hold as above. scales 16-byte aligned, apart from what a call writes beside it. */
+int ssmoe_rope_append_e4m3(const ssmoe_rope_append_args* a, uint8_t* scales, void* stream);
+
+/* ssmoe_paged_attention over e4m3 pages (scales non-null) and for rows of trees (tree non-null).
+ * tree uint64 [rows]: row i sees the tokens before its sequence's rows and of those rows the ones whose bits are set in its word (bit
+ * j: the sequence's row j; its own bit as any other); bits of rows that the sequence has not are not looked at. max_rows at most 64.
+ * Under a window the row's position is that of as many rows behind the cache as it sees; the window must be at least max_rows.
+ * Scores, sums and partial results are fp32; a probability is rounded once, with its token's power of two, before its product. */
+int64_t ssmoe_paged_attention_ext_workspace_bytes(const ssmoe_paged_attention_args* a, int e4m3, int tree); /* -1: refused */
+int ssmoe_paged_attention_ext(const ssmoe_paged_attention_args* a, const uint8_t* scales, const uint64_t* tree, void* stream);
+
+/* ssmoe_move_pages with the pages' scales ([layers][n_pages][scale_bytes], a multiple of 32); page_bytes a multiple of 1024. */
+int ssmoe_move_pages_e4m3(void* k, void* v, uint8_t* scales, int layers, int64_t n_pages, int64_t page_bytes, int64_t scale_bytes,
+                          const int32_t* src, const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream);
+
+/* A tree of drafts: the rows cu_rows[s] .. cu_rows[s + 1] of a sequence, row 0 its pending token, parents[i] of every other row the
+ * row (of the sequence, before i) that it was drafted behind. At most 64 rows.
+ * masks uint64 [rows]: a row and its ancestors, as ssmoe_paged_attention_ext takes them; positions int32 [rows] (or NULL): kv_len -
+ * rows + the row's depth, as ssmoe_rope_append takes them. A parent that is no row before its own is taken as none, and raises
+ * SSMOE_ERR_BATCH. */
+int ssmoe_tree_masks(const int32_t* parents, const int32_t* cu_rows, const int32_t* kv_len, uint64_t* masks, int32_t* positions,
+                     int rows, int seqs, int max_rows, void* stream);
+
+/* The greedy round of a tree. From row 0 on: the row's choice is the first maximum of its logits (target fp32 [rows][vocab]); the
+ * next row is the first one behind it whose token is that choice; a row with a logit that is not finite ends the branch before its
+ * choice (flag 1). out int32 [seqs][4 + 2 max_rows]: n_accept (drafts followed), n_emit (choices), 0, flags, the choices [max_rows],
+ * the branch's rows [max_rows] (n_accept + 1 of them, 0 first), -1 where there is none. A sequence without rows has
+ * n_accept = n_emit = 0 and no row. ws: ssmoe_accept_tree_workspace_bytes, 8-byte aligned, not kept between calls. */
+int64_t ssmoe_accept_tree_workspace_bytes(int rows, int seqs, int max_rows, int vocab); /* -1: arguments refused */
+int ssmoe_accept_tree(const float* target, const int32_t* tokens, const int32_t* parents, const int32_t* cu_rows, int rows, int seqs,
+                      int max_rows, int vocab, void* ws, int64_t ws_bytes, int32_t* out, void* stream);
+
+/* The accepted branch moves up: in every layer of k [layers][n_pages][kv_heads][page][dim] and v [layers][n_pages][kv_heads][dim][page]
+ * (`bytes` of an element: 2, or 1 with scales [layers][n_pages][kv_heads][2][page]) the token kv_len - rows + d of a sequence becomes
+ * its token kv_len - rows + path[d], path the branch's rows in `accepted` (ssmoe_accept_tree's out), d up to n_accept. Tokens past them hold
+ * what they held or a moved row's copy. A path that does not rise or names no row of the sequence is followed up to there (SSMOE_ERR_BATCH). */
+int ssmoe_keep_rows(void* k, void* v, uint8_t* scales, int layers, int64_t n_pages, int kv_heads, int page, int dim, int bytes,
+                    const int32_t* cu_rows, const int32_t* kv_len, const int32_t* table, int width, const int32_t* accepted, int rows,
+                    int seqs, int max_rows, void* stream);
+
 /* ---------------------------------------------------------------- expert slot pool */
 
 /* An expert slot pool in HBM fed from experts.bin (layout slotstream-pool-layer-expert-piece-v1: the record of

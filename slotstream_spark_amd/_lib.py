@@ -70,6 +70,14 @@ SIGNATURES = {
     "ssmoe_paged_attention_workspace_bytes": (_I64, [_P]),
     "ssmoe_paged_attention": (_I, [_P, _P]),
     "ssmoe_move_pages": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _I, _P, _I64, _P]),
+    "ssmoe_rope_append_e4m3": (_I, [_P, _P, _P]),
+    "ssmoe_paged_attention_ext_workspace_bytes": (_I64, [_P, _I, _I]),
+    "ssmoe_paged_attention_ext": (_I, [_P, _P, _P, _P]),
+    "ssmoe_move_pages_e4m3": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _P, _P, _I, _P, _I64, _P]),
+    "ssmoe_tree_masks": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "ssmoe_accept_tree_workspace_bytes": (_I64, [_I, _I, _I, _I]),
+    "ssmoe_accept_tree": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _I64, _P, _P]),
+    "ssmoe_keep_rows": (_I, [_P, _P, _P, _I, _I64, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "ssmoe_pool_open": (_I, [ctypes.c_char_p, _I, _I, _I64, _I, _I64, _P, _P, ctypes.POINTER(_P)]),
     "ssmoe_pool_close": (_I, [_P]),
     "ssmoe_pool_set_reader": (_I, [_P, _I, _I]),

@@ -32,6 +32,8 @@ struct AttnArgs {
   int tiles;   // workgroups over the packed rows of one sequence and key head
   int rising;  // many rows: the tiles at the end of the launch that go up
   float scale; // of the scores, times log2(e)
+  const uint8_t* scales;  // [n_pages][kv_heads][2][page] exponents of e4m3 keys and values (k, v then hold bytes), or null
+  const uint64_t* tree;   // [rows] which of its sequence's rows a row sees, or null (causal)
 };
 
 // ss_raise through a global pointer (a flat atomic would make every later wait of the wave one for all its LDS reads).
@@ -130,10 +132,51 @@ SS_DEV Seen seen_tokens(int pos_a, int pos_b, int end, int window, int sinks) {
   return r;
 }
 
+// ---------------------------------------------------------------- pages of e4m3 numbers
+// A token's keys (its values) are its e4m3 numbers times 2^(s - 127), s a byte of 1 to 254: a power of two, so that a key
+// times its scale is a bfloat16 as it is (3 bits of mantissa), and the conversion instruction applies it on the way. 255 is read
+// as 254: what an unseen place holds stays finite.
+SS_DEV float scale_of(uint32_t s) { return ss_uf(min(s, 254u) << 23); }
+// 8 e4m3 numbers, two words, times `scale` (a power of two) as bfloat16.
+SS_DEV ss_u32x4 widen8(uint32_t lo, uint32_t hi, float scale) {
+  ss_u32x4 r;
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+  return r;
+}
+// A word of four e4m3 numbers without its NaN (all but the sign set).
+SS_DEV uint32_t without_nan8(uint32_t w) {
+  uint32_t r = w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (((w >> (8 * i)) & 0x7Fu) == 0x7Fu) r &= ~(0xFFu << (8 * i));
+  return r;
+}
+
+// ---------------------------------------------------------------- rows of a tree
+// Which of the 8 tokens from `first` on a row of a tree sees, a bit each: tokens before `base` (the place of the sequence's first
+// row) that its window `pos - window` or the first tokens let it, and from base on those of its mask.
+SS_DEV uint32_t tree_sees(int first, int base, int end, uint64_t mask, int pos, int window, int sinks) {
+  const int off = base - first;  // tokens of the 8 before base
+  uint32_t r = off >= 8 ? 0xFFu : off <= 0 ? 0u : (1u << off) - 1;
+  const int w = pos - window + 1 - first, k = sinks - first;  // below w only those below k
+  const uint32_t far = w >= 8 ? 0xFFu : w <= 0 ? 0u : (1u << w) - 1, kept = k >= 8 ? 0xFFu : k <= 0 ? 0u : (1u << k) - 1;
+  r &= ~far | kept;
+  if (off < 8 && off > -64) r |= (uint32_t)(off >= 0 ? mask << off : mask >> -off) & 0xFFu;
+  const int left = end - first;
+  return r & (left >= 8 ? 0xFFu : left <= 0 ? 0u : (1u << left) - 1);
+}
+
 int attn_prompt_parts(int dim, int page_shift);
 hipError_t launch_attn_prompt(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
+hipError_t launch_attn_prompt_tree(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
+hipError_t launch_attn_prompt_e4m3(const AttnArgs& a, int dim, hipStream_t st);
 hipError_t launch_attn_few(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
-int attn_few_packed(int dim, int packed);
+hipError_t launch_attn_few_tree(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
+hipError_t launch_attn_few_e4m3(const AttnArgs& a, int dim, hipStream_t st);
+int attn_few_packed(int dim, int packed, bool e4m3);
 hipError_t launch_attn_join(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 
 }  // namespace ss

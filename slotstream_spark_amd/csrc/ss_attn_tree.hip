@@ -1,0 +1,10 @@
+// Attention of few rows, the rows of trees of drafts, over 16-bit pages (the kernel is in ss_attn_few.hpp).
+#include "ss_attn_few.hpp"
+
+namespace ss {
+
+hipError_t launch_attn_few_tree(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {
+  return fp16 ? launch_few_of<Fp16, false, true>(a, dim, st) : launch_few_of<Bf16, false, true>(a, dim, st);
+}
+
+}  // namespace ss

@@ -22,7 +22,146 @@ namespace ss {
 
 namespace {
 
+// ---------------------------------------------------------------- rows as e4m3 numbers
+// A vector x of a token and head is kept as e4m3 numbers of x 2^-e, rounded once from fp32, and the byte e + 127: e the least exponent
+// with max |x| <= 448 2^e, from -126 on. What is not finite is left out of the maximum and kept as NaN.
+SS_DEV float finite_abs(float x) {
+  const float y = fabsf(x);
+  return y < __builtin_inff() ? y : 0.f;
+}
+// The byte of a vector whose largest magnitude is `top`: 448 is 1.75 2^8, so the mantissa says which exponent is enough.
+SS_DEV uint32_t exponent8(float top) {
+  const uint32_t u = ss_fu(top);
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(e, 1);
+}
+// x 2^-e for the byte of e, NaN where x is not finite.
+SS_DEV float scaled8(float x, float by) { return fabsf(x) < __builtin_inff() ? x * by : __builtin_nanf(""); }
+SS_DEV float inverse8(uint32_t byte) { return ss_uf((254u - byte) << 23); }
+SS_DEV uint32_t pack8(float a, float b, float c, float d) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+}
+// The maximum over the lanes l ^ 1, ..., l ^ (n - 1), n = 4, 8, 16 or 32.
+SS_DEV float max_over(float v, int n) {
+  v = fmaxf(v, ss_uf(ss_xor_lane<1>(ss_fu(v))));
+  v = fmaxf(v, ss_uf(ss_xor_lane<2>(ss_fu(v))));
+  if (n > 4) v = fmaxf(v, ss_uf(ss_xor_lane<4>(ss_fu(v))));
+  if (n > 8) v = fmaxf(v, ss_uf(ss_xor_lane<8>(ss_fu(v))));
+  if (n > 16) {
+    uint32_t lo, hi;
+    ss_pair<16>(ss_fu(v), lo, hi);
+    v = fmaxf(ss_uf(lo), ss_uf(hi));
+  }
+  return v;
+}
+
+// Key and value rows of the 8 positions from `first` on, into page `id` at `off`.
 template <class T>
+SS_DEV void append_e4m3(const RopeArgs& a, const SeqRows& sr, int first, int id, int off, int h0, int stride, const float* cs_of,
+                        const float* sn_of) {
+  if (id < 0) return;
+  const int lane = threadIdx.x & 63, D = a.dim, page = 1 << a.page_shift, half = a.rot / 2, chunks = a.rot / 16;
+  const int lo = max(sr.pos0 - first, 0), hi = min(sr.pos0 + sr.n - first, 8), rows = hi - lo;  // the call's tokens of the 8
+  uint8_t* const kp = reinterpret_cast<uint8_t*>(a.k_pages) + (int64_t)id * a.kv_heads * page * D;
+  uint8_t* const vp = reinterpret_cast<uint8_t*>(a.v_pages) + (int64_t)id * a.kv_heads * page * D;
+  uint8_t* const ep = a.scales + (int64_t)id * a.kv_heads * 2 * page + off;
+  // Keys: L lanes a row and head, lane j with the frequencies 8 j .. 8 j + 7 or 16 elements past rot.
+  const int L = D / 16, keys = rows * a.kv_heads * L, kunits = (keys + 63) / 64;
+  int unit = h0 + (a.heads > h0 ? (a.heads - h0 + stride - 1) / stride * stride : 0) - a.heads;  // this wave's first one past the queries
+  for (; unit < kunits; unit += stride) {
+    const int it = min(64 * unit + lane, keys - 1), j = it % L, rh = (uint32_t)it / (uint32_t)L;  // lanes past the last repeat it
+    const int h = rh % a.kv_heads, rr = lo + rh / a.kv_heads;
+    const uint16_t* src = a.k + (int64_t)(sr.r0 + first + rr - sr.pos0) * a.k_row + (int64_t)h * a.k_head;
+    const bool turn = j < chunks;
+    const int o0 = !turn || a.adjacent ? 16 * j : 8 * j, o1 = !turn || a.adjacent ? 16 * j + 8 : half + 8 * j;
+    const ss_u32x4 x0 = *(const SS_G ss_u32x4*)(src + o0), x1 = *(const SS_G ss_u32x4*)(src + o1);
+    float y[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = T::widen(e % 2 ? x0[e / 2] >> 16 : x0[e / 2] & 0xFFFFu);
+      y[8 + e] = T::widen(e % 2 ? x1[e / 2] >> 16 : x1[e / 2] & 0xFFFFu);
+    }
+    if (turn) {
+      const float *cs = cs_of + rr * half + 8 * j, *sn = sn_of + rr * half + 8 * j;
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        // frequency f turns elements (f, 8 + f), or (2 f, 2 f + 1) with adjacent
+        const float p = a.adjacent ? y[2 * f] : y[f], q = a.adjacent ? y[2 * f + 1] : y[8 + f];
+        const float u = p * cs[f] - q * sn[f], v = q * cs[f] + p * sn[f];
+        if (a.adjacent) {
+          y[2 * f] = u;
+          y[2 * f + 1] = v;
+        } else {
+          y[f] = u;
+          y[8 + f] = v;
+        }
+      }
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, finite_abs(y[e]));
+    const uint32_t byte = exponent8(max_over(top, L));
+    const float by = inverse8(byte);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = scaled8(y[e], by);
+    if (64 * unit + lane >= keys) continue;
+    uint8_t* dst = kp + ((int64_t)h * page + off + rr) * D;
+    uint2 c0, c1;
+    c0.x = pack8(y[0], y[1], y[2], y[3]);
+    c0.y = pack8(y[4], y[5], y[6], y[7]);
+    c1.x = pack8(y[8], y[9], y[10], y[11]);
+    c1.y = pack8(y[12], y[13], y[14], y[15]);
+    *reinterpret_cast<uint2*>(dst + o0) = c0;
+    *reinterpret_cast<uint2*>(dst + o1) = c1;
+    if (j == 0) gp(ep)[h * 2 * page + rr] = (uint8_t)byte;
+  }
+  // Values: 8 rows by 8 dimensions a lane, transposed on the way.
+  const int per = D / 8, vals = per * a.kv_heads, vunits = (vals + 63) / 64;
+  for (unit -= kunits; unit < vunits; unit += stride) {
+    const int it = min(64 * unit + lane, vals - 1), h = (uint32_t)it / (uint32_t)per, d = 8 * (it - h * per);
+    const bool mine = 64 * unit + lane < vals;
+    ss_u32x4 x[8];
+#pragma unroll
+    for (int rr = 0; rr < 8; ++rr) {
+      x[rr] = ss_u32x4{0u, 0u, 0u, 0u};
+      if (rr >= lo && rr < hi)
+        x[rr] = *(const SS_G ss_u32x4*)(a.v + (int64_t)(sr.r0 + first + rr - sr.pos0) * a.v_row + (int64_t)h * a.v_head + d);
+    }
+    float by[8];
+#pragma unroll
+    for (int rr = 0; rr < 8; ++rr) {
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(finite_abs(T::widen(x[rr][e] & 0xFFFFu)), finite_abs(T::widen(x[rr][e] >> 16))));
+      const uint32_t byte = exponent8(max_over(top, per));
+      by[rr] = inverse8(byte);
+      if (mine && d == 0 && rr >= lo && rr < hi) gp(ep)[(h * 2 + 1) * page + rr] = (uint8_t)byte;
+    }
+    if (!mine) continue;
+    uint8_t* dst = vp + ((int64_t)h * D + d) * page + off;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float y[8];
+#pragma unroll
+      for (int rr = 0; rr < 8; ++rr) y[rr] = scaled8(T::widen(e % 2 ? x[rr][e / 2] >> 16 : x[rr][e / 2] & 0xFFFFu), by[rr]);
+      uint2 c;
+      c.x = pack8(y[0], y[1], y[2], y[3]);
+      c.y = pack8(y[4], y[5], y[6], y[7]);
+      if (lo == 0 && hi == 8) {
+        *reinterpret_cast<uint2*>(dst + (int64_t)e * page) = c;
+      } else {
+#pragma unroll
+        for (int rr = 0; rr < 8; ++rr)
+          if (rr >= lo && rr < hi) gp(dst)[(int64_t)e * page + rr] = (uint8_t)((rr < 4 ? c.x : c.y) >> (8 * (rr % 4)));
+      }
+    }
+  }
+}
+
+// E8: the cache's pages are e4m3 numbers with exponents; keys and values then go in two parts of their own, in units of a wave
+// behind the query heads: of keys 16 elements of a row a lane, of values 8 rows by 8 dimensions.
+template <class T, bool E8>
 __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   __shared__ __attribute__((aligned(16))) float cs_of[8 * 128], sn_of[8 * 128];  // [8 positions][rot / 2]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -74,7 +213,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   __syncthreads();
 
   // Query heads, then key heads; a thread's loads for some of its heads go out together.
-  const int hs = a.heads + a.kv_heads;
+  const int hs = E8 ? a.heads : a.heads + a.kv_heads;
   auto from = [&](int64_t r, int h) {
     return h < a.heads ? a.q + r * a.q_row + h * a.q_head : a.k + r * a.k_row + (h - a.heads) * a.k_head;
   };
@@ -156,6 +295,10 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
       }
     }
   }
+  if constexpr (E8) {
+    append_e4m3<T>(a, sr, first, id, off, h0, stride, cs_of, sn_of);
+    return;
+  }
   // Value rows.
   if (id < 0) return;
   const int lo = max(sr.pos0 - first, 0), hi = min(sr.pos0 + sr.n - first, 8);  // the call's tokens of the 8
@@ -193,10 +336,12 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
 
 hipError_t launch_rope_append(const RopeArgs& a, bool fp16, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.seqs * a.tiles * a.head_groups));
-  if (fp16)
-    hipLaunchKernelGGL((rope_append_kernel<Fp16>), grid, dim3(256), 0, st, a);
+  if (a.scales)
+    hipLaunchKernelGGL((rope_append_kernel<Bf16, true>), grid, dim3(256), 0, st, a);
+  else if (fp16)
+    hipLaunchKernelGGL((rope_append_kernel<Fp16, false>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((rope_append_kernel<Bf16>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((rope_append_kernel<Bf16, false>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -26,6 +26,7 @@ struct RopeArgs {
   float factor;
   int tiles;        // groups of 8 positions of one sequence
   int head_groups;  // workgroups that share the heads of a tile
+  uint8_t* scales;  // [n_pages][kv_heads][2][page] exponents: the pages then hold e4m3 numbers; or null
 };
 hipError_t launch_rope_append(const RopeArgs& a, bool fp16, hipStream_t st);
 
@@ -39,6 +40,9 @@ struct MoveArgs {
   int64_t n_pages, page_bytes, entries;
   int layers, n;
   unsigned copy_blocks, table_blocks;
+  uint8_t* scales;  // [layers][n_pages][scale_bytes] that move with the pages; or null
+  int64_t scale_bytes;
+  unsigned scale_blocks;
 };
 hipError_t launch_move_pages(MoveArgs a, hipStream_t st);
 

@@ -16,6 +16,7 @@
 #include "ss_common.hpp"
 #include "ss_launch.hpp"
 #include "ss_rope.hpp"
+#include "ss_tree.hpp"
 
 // Per-device status word raised by kernels on bad input.
 __device__ int ss_status_storage;
@@ -269,7 +270,7 @@ int check_apart(std::initializer_list<Span> written, std::initializer_list<Span>
 // 191 / 200 / 204 against 195 / 195 / 204 / 201; 8 of 16 on 2, 256 dimensions 33 / 43 / 56 / 69 against 42 / 45 / 48 / 52; 16
 // of 24 on 8, 64 dimensions 44 / 46 / 50 / 51 against 58 / 58 / 57 / 56.
 constexpr int kFewRows = 8;
-int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
+int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
   if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
   int shift = 0;
   if (int rc = check_paged(p->rows, p->seqs, p->max_rows, p->heads, p->kv_heads, p->dim, p->page, p->width, p->n_pages,
@@ -277,6 +278,11 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
     return rc;
   if (p->window < 0 || p->sinks < 0) return fail(SSMOE_EINVAL, "window and sinks must be >= 0");
   if (!(p->scale >= 1e-30f && p->scale <= 1e30f)) return fail(SSMOE_EINVAL, "scale must be positive, in [1e-30, 1e30]");
+  if (e4m3 && p->type != SSMOE_BF16) return fail(SSMOE_EINVAL, "e4m3 pages take queries of type SSMOE_BF16");
+  if (tree && p->max_rows > ss::kTreeRows)
+    return fail(SSMOE_EINVAL, "a tree has at most %d rows of a sequence, max_rows is %d", ss::kTreeRows, p->max_rows);
+  if (tree && p->window > 0 && p->window < p->max_rows)
+    return fail(SSMOE_EINVAL, "with a tree the window must hold max_rows rows: %d of %d", p->window, p->max_rows);
   ss::AttnArgs a{};
   const int max_rows = p->max_rows < p->rows ? p->max_rows : (p->rows > 0 ? p->rows : 1);
   const int64_t cap = (int64_t)p->width * p->page;
@@ -293,7 +299,7 @@ int plan_attention(const ssmoe_paged_attention_args* p, ss::AttnArgs* out, int64
   a.scale = p->scale * 1.44269504088896340736f;
   if ((int64_t)max_rows * a.group > (1 << 30)) return fail(SSMOE_EINVAL, "max_rows * heads / kv_heads must be at most 2^30");
   *prompt = p->max_rows > kFewRows;
-  a.packed = *prompt ? 128 : ss::attn_few_packed(p->dim, max_rows * a.group);
+  a.packed = *prompt ? 128 : ss::attn_few_packed(p->dim, max_rows * a.group, e4m3);
   a.tiles = (max_rows * a.group + a.packed - 1) / a.packed;
   // tokens of a sequence that the call may read
   int64_t seen = cap;
@@ -1403,7 +1409,11 @@ int ssmoe_gather_rows(const void* src, int64_t n_src, int64_t row_bytes, const i
                    "gather launch");
 }
 
-int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
+}  // extern "C"
+
+namespace {
+
+int rope_append(const ssmoe_rope_append_args* p, uint8_t* scales, bool e4m3, void* stream) {
   if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
   ss::RopeArgs a{};
   if (int rc = check_paged(p->rows, p->seqs, p->max_rows, p->heads, p->kv_heads, p->dim, p->page, p->width, p->n_pages,
@@ -1413,7 +1423,9 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
     return fail(SSMOE_EINVAL, "rot must be a multiple of 16 in [16, dim], got %d of %d", p->rot, p->dim);
   if (p->axes < 1) return fail(SSMOE_EINVAL, "need axes >= 1");
   if (!std::isfinite(p->factor)) return fail(SSMOE_EINVAL, "factor must be finite");
+  if (e4m3 && p->type != SSMOE_BF16) return fail(SSMOE_EINVAL, "e4m3 pages take rows of type SSMOE_BF16");
   if (p->rows == 0 || p->seqs == 0) return ok();
+  if (e4m3 && !scales) return fail(SSMOE_EINVAL, "scales must be non-null");
   if (!p->q || !p->k || !p->v || !p->q_out || !p->positions || !p->inv_freq || !p->k_pages || !p->v_pages || !p->cu_rows ||
       !p->kv_len || !p->table)
     return fail(SSMOE_EINVAL, "q, k, v, q_out, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len and table must be non-null");
@@ -1429,9 +1441,10 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
       overlap(p->k, p->k_row, p->k_head, p->kv_heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim) ||
       overlap(p->v, p->v_row, p->v_head, p->kv_heads, p->q_out, o_row, p->dim, p->heads, p->rows, p->dim))
     return fail(SSMOE_EINVAL, "q_out must be q itself (contiguous) or overlap none of q, k and v");
-  const int64_t cache = 2 * p->n_pages * p->kv_heads * p->page * p->dim, pos = p->axes > 1 ? (p->axes - 1) * p->pos_stride : 0;
+  const int64_t cache = (e4m3 ? 1 : 2) * p->n_pages * p->kv_heads * p->page * p->dim, pos = p->axes > 1 ? (p->axes - 1) * p->pos_stride : 0;
   const Span q("q", p->q, p->rows, p->q_row, p->heads, p->q_head, p->dim);
-  if (int rc = check_apart({{"q_out", p->q_out, 2 * p->rows * o_row}, {"k_pages", p->k_pages, cache}, {"v_pages", p->v_pages, cache}},
+  if (int rc = check_apart({{"q_out", p->q_out, 2 * p->rows * o_row}, {"k_pages", p->k_pages, cache}, {"v_pages", p->v_pages, cache},
+                            {"scales", scales, 2 * p->n_pages * p->kv_heads * p->page}},
                            {same ? Span("q", nullptr, 0) : q,
                             {"k", p->k, p->rows, p->k_row, p->kv_heads, p->k_head, p->dim},
                             {"v", p->v, p->rows, p->v_row, p->kv_heads, p->v_head, p->dim},
@@ -1474,6 +1487,7 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
   a.width = p->width;
   a.adjacent = p->adjacent != 0;
   a.factor = p->factor;
+  a.scales = scales;
   a.tiles = (int)(((int64_t)a.max_rows + 14) / 8);
   // A workgroup's four waves take its heads in turn; where there are few groups of positions the heads are shared out too, to
   // some three workgroups a CU. Shared by 1 / 2 / 3 / 4 / 5 / 9, in us: 8,190 rows (1,026 groups) of 40 heads of 128 45 / 53 /
@@ -1486,19 +1500,15 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) {
   return hip_check(ss::launch_rope_append(a, p->type == SSMOE_FP16, static_cast<hipStream_t>(stream)), "rope launch");
 }
 
-int64_t ssmoe_paged_attention_workspace_bytes(const ssmoe_paged_attention_args* p) {
+// The attention over 16-bit pages, with scales over e4m3 ones, with a tree by its masks.
+int paged_attention(const ssmoe_paged_attention_args* p, const uint8_t* scales, const uint64_t* tree, void* stream) {
   ss::AttnArgs a{};
   int64_t ws = 0;
   bool prompt = false;
-  return plan_attention(p, &a, &ws, &prompt) ? -1 : ws;
-}
-
-int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
-  ss::AttnArgs a{};
-  int64_t ws = 0;
-  bool prompt = false;
-  if (int rc = plan_attention(p, &a, &ws, &prompt)) return rc;
+  if (int rc = plan_attention(p, scales != nullptr, tree != nullptr, &a, &ws, &prompt)) return rc;
   if (p->rows == 0 || p->seqs == 0) return ok();
+  if (tree && !aligned(tree, 8)) return fail(SSMOE_EINVAL, "tree must be 8-byte aligned");
+  if (scales && !aligned(scales, 16)) return fail(SSMOE_EINVAL, "scales must be 16-byte aligned");
   if (!p->q || !p->k_pages || !p->v_pages || !p->cu_rows || !p->kv_len || !p->table || !p->out)
     return fail(SSMOE_EINVAL, "q, k_pages, v_pages, cu_rows, kv_len, table and out must be non-null");
   if (p->q_row < 0 || p->q_head < 0 || p->q_row % 8 || p->q_head % 8)
@@ -1510,11 +1520,13 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
                 (long long)(p->ws ? p->ws_bytes : 0), (long long)ws);
   if (overlap(p->q, p->q_row, p->q_head, p->heads, p->out, (int64_t)p->heads * p->dim, p->dim, p->heads, p->rows, p->dim))
     return fail(SSMOE_EINVAL, "out must not overlap q");
-  const int64_t cache = 2 * p->n_pages * p->kv_heads * p->page * p->dim, heads = (int64_t)p->rows * p->heads;
+  const int64_t cache = (scales ? 1 : 2) * p->n_pages * p->kv_heads * p->page * p->dim, heads = (int64_t)p->rows * p->heads;
   if (int rc = check_apart({{"out", p->out, 2 * heads * p->dim}, {"lse", p->lse, 4 * heads}, {"ws", p->ws, ws}},
                            {{"q", p->q, p->rows, p->q_row, p->heads, p->q_head, p->dim},
                             {"k_pages", p->k_pages, cache},
                             {"v_pages", p->v_pages, cache},
+                            {"scales", scales, 2 * p->n_pages * p->kv_heads * p->page},
+                            {"tree", tree, 8 * (int64_t)p->rows},
                             {"cu_rows", p->cu_rows, 4 * ((int64_t)p->seqs + 1)},
                             {"kv_len", p->kv_len, 4 * (int64_t)p->seqs},
                             {"table", p->table, 4 * (int64_t)p->seqs * p->width}}))
@@ -1530,6 +1542,8 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
   a.out = static_cast<uint16_t*>(p->out);
   a.lse = p->lse;
   a.n_pages = p->n_pages;
+  a.scales = scales;
+  a.tree = tree;
   if (int rc = status_ptr(&a.err)) return rc;
   if (ws > 0) {
     const int64_t parts = (int64_t)a.slots * p->rows * p->heads;
@@ -1540,25 +1554,34 @@ int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e = hipErrorOutOfMemory;
   try {  // the few-row launch keeps its kernels' limits in a map
-    e = prompt ? ss::launch_attn_prompt(a, p->dim, fp16, st) : ss::launch_attn_few(a, p->dim, fp16, st);
+    if (scales)
+      e = prompt ? ss::launch_attn_prompt_e4m3(a, p->dim, st) : ss::launch_attn_few_e4m3(a, p->dim, st);
+    else if (tree)
+      e = prompt ? ss::launch_attn_prompt_tree(a, p->dim, fp16, st) : ss::launch_attn_few_tree(a, p->dim, fp16, st);
+    else
+      e = prompt ? ss::launch_attn_prompt(a, p->dim, fp16, st) : ss::launch_attn_few(a, p->dim, fp16, st);
   } catch (const std::exception&) {
   }
   if (int rc = hip_check(e, "attention launch")) return rc;
   return a.slots > 1 ? hip_check(ss::launch_attn_join(a, p->dim, fp16, st), "attention join launch") : ok();
 }
 
-int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page_bytes, const int32_t* src,
-                     const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream) {
-  if (layers < 1 || n_pages < 1 || n_pages > INT32_MAX || page_bytes < 2048 || page_bytes % 2048)
-    return fail(SSMOE_EINVAL, "need layers >= 1, 1 <= n_pages < 2^31 and page_bytes a positive multiple of 2048");
+int move_pages(void* k, void* v, uint8_t* scales, bool e4m3, int layers, int64_t n_pages, int64_t page_bytes, int64_t scale_bytes,
+               const int32_t* src, const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream) {
+  const int64_t unit = e4m3 ? 1024 : 2048;
+  if (layers < 1 || n_pages < 1 || n_pages > INT32_MAX || page_bytes < unit || page_bytes % unit)
+    return fail(SSMOE_EINVAL, "need layers >= 1, 1 <= n_pages < 2^31 and page_bytes a positive multiple of %lld", (long long)unit);
+  if (e4m3 && (scale_bytes < 32 || scale_bytes % 32 || scale_bytes > page_bytes))
+    return fail(SSMOE_EINVAL, "scale_bytes must be a positive multiple of 32, at most page_bytes");
   if (n < 0 || entries < 0 || entries > INT32_MAX) return fail(SSMOE_EINVAL, "need n >= 0 and 0 <= entries < 2^31");
   if (n == 0) return ok();
   if (!k || !v || !src || !dst) return fail(SSMOE_EINVAL, "k, v, src and dst must be non-null");
-  if (!aligned(k, 16) || !aligned(v, 16)) return fail(SSMOE_EINVAL, "k and v must be 16-byte aligned");
-  if (page_bytes / 2048 > ((int64_t)1 << 30) / n / layers || page_bytes > INT64_MAX / n_pages / layers)
+  if (e4m3 && !scales) return fail(SSMOE_EINVAL, "scales must be non-null");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(scales, 16)) return fail(SSMOE_EINVAL, "k, v and scales must be 16-byte aligned");
+  if (page_bytes / unit > ((int64_t)1 << 30) / n / layers || page_bytes > INT64_MAX / n_pages / layers)
     return fail(SSMOE_EINVAL, "too many bytes for one call");
   const int64_t cache = layers * n_pages * page_bytes;
-  if (int rc = check_apart({{"k", k, cache}, {"v", v, cache}, {"table", table, 4 * entries}},
+  if (int rc = check_apart({{"k", k, cache}, {"v", v, cache}, {"table", table, 4 * entries}, {"scales", scales, layers * n_pages * scale_bytes}},
                            {{"src", src, 4 * (int64_t)n}, {"dst", dst, 4 * (int64_t)n}}))
     return rc;
   ss::MoveArgs a{};
@@ -1567,6 +1590,8 @@ int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page
   a.src = src;
   a.dst = dst;
   a.table = entries > 0 ? table : nullptr;
+  a.scales = scales;
+  a.scale_bytes = scale_bytes;
   if (int rc = status_ptr(&a.err)) return rc;
   a.n_pages = n_pages;
   a.page_bytes = page_bytes;
@@ -1574,6 +1599,151 @@ int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page
   a.layers = layers;
   a.n = n;
   return hip_check(ss::launch_move_pages(a, static_cast<hipStream_t>(stream)), "page move launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int ssmoe_rope_append(const ssmoe_rope_append_args* p, void* stream) { return rope_append(p, nullptr, false, stream); }
+
+int ssmoe_rope_append_e4m3(const ssmoe_rope_append_args* p, uint8_t* scales, void* stream) {
+  return rope_append(p, scales, true, stream);
+}
+
+int64_t ssmoe_paged_attention_workspace_bytes(const ssmoe_paged_attention_args* p) {
+  return ssmoe_paged_attention_ext_workspace_bytes(p, 0, 0);
+}
+
+int64_t ssmoe_paged_attention_ext_workspace_bytes(const ssmoe_paged_attention_args* p, int e4m3, int tree) {
+  ss::AttnArgs a{};
+  int64_t ws = 0;
+  bool prompt = false;
+  return plan_attention(p, e4m3 != 0, tree != 0, &a, &ws, &prompt) ? -1 : ws;
+}
+
+int ssmoe_paged_attention(const ssmoe_paged_attention_args* p, void* stream) {
+  return paged_attention(p, nullptr, nullptr, stream);
+}
+
+int ssmoe_paged_attention_ext(const ssmoe_paged_attention_args* p, const uint8_t* scales, const uint64_t* tree, void* stream) {
+  return paged_attention(p, scales, tree, stream);
+}
+
+int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page_bytes, const int32_t* src,
+                     const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream) {
+  return move_pages(k, v, nullptr, false, layers, n_pages, page_bytes, 0, src, dst, n, table, entries, stream);
+}
+
+int ssmoe_move_pages_e4m3(void* k, void* v, uint8_t* scales, int layers, int64_t n_pages, int64_t page_bytes, int64_t scale_bytes,
+                          const int32_t* src, const int32_t* dst, int n, int32_t* table, int64_t entries, void* stream) {
+  return move_pages(k, v, scales, true, layers, n_pages, page_bytes, scale_bytes, src, dst, n, table, entries, stream);
+}
+
+int ssmoe_tree_masks(const int32_t* parents, const int32_t* cu_rows, const int32_t* kv_len, uint64_t* masks, int32_t* positions,
+                     int rows, int seqs, int max_rows, void* stream) {
+  if (rows < 0 || seqs < 0 || max_rows < 1 || max_rows > ss::kTreeRows)
+    return fail(SSMOE_EINVAL, "need rows >= 0, seqs >= 0 and max_rows in 1 .. %d, got %d, %d and %d", ss::kTreeRows, rows, seqs, max_rows);
+  if (rows == 0 || seqs == 0) return ok();
+  if (!parents || !cu_rows || !masks || (positions && !kv_len))
+    return fail(SSMOE_EINVAL, "parents, cu_rows, masks and with positions kv_len must be non-null");
+  if (!aligned(masks, 8)) return fail(SSMOE_EINVAL, "masks must be 8-byte aligned");
+  if (int rc = check_apart({{"masks", masks, 8 * (int64_t)rows}, {"positions", positions, 4 * (int64_t)rows}},
+                           {{"parents", parents, 4 * (int64_t)rows},
+                            {"cu_rows", cu_rows, 4 * ((int64_t)seqs + 1)},
+                            {"kv_len", kv_len, 4 * (int64_t)seqs}}))
+    return rc;
+  ss::TreeMaskArgs a{parents, cu_rows, kv_len, masks, positions, nullptr, rows, seqs, max_rows};
+  if (int rc = status_ptr(&a.err)) return rc;
+  return hip_check(ss::launch_tree_masks(a, static_cast<hipStream_t>(stream)), "tree mask launch");
+}
+
+// Spans of a row: of 8,192 values, less where the rows alone make too few workgroups for the card.
+static void accept_tree_spans(int rows, int vocab, int* splits, int* span) {
+  int64_t n = std::max<int64_t>((vocab + 8191) / 8192, (1024 + rows - 1) / std::max(rows, 1));
+  n = std::max<int64_t>(std::min<int64_t>(n, (vocab + 1023) / 1024), 1);
+  *span = (int)(((vocab + n - 1) / n + 3) / 4 * 4);
+  *splits = (vocab + *span - 1) / *span;
+}
+
+static int check_accept_tree(int rows, int seqs, int max_rows, int vocab) {
+  if (rows < 0 || seqs < 0 || max_rows < 1 || max_rows > ss::kTreeRows)
+    return fail(SSMOE_EINVAL, "need rows >= 0, seqs >= 0 and max_rows in 1 .. %d, got %d, %d and %d", ss::kTreeRows, rows, seqs, max_rows);
+  if (vocab < 1 || vocab > (1 << 24)) return fail(SSMOE_EINVAL, "vocab must be in 1 .. 2^24, got %d", vocab);
+  if ((int64_t)rows * ((vocab + 1023) / 1024) > INT32_MAX / 2) return fail(SSMOE_EINVAL, "too many rows for one call: split it over sequences");
+  return ok();
+}
+
+int64_t ssmoe_accept_tree_workspace_bytes(int rows, int seqs, int max_rows, int vocab) {
+  if (check_accept_tree(rows, seqs, max_rows, vocab)) return -1;
+  int splits = 0, span = 0;
+  accept_tree_spans(rows, vocab, &splits, &span);
+  return (int64_t)rows * splits * 8;
+}
+
+int ssmoe_accept_tree(const float* target, const int32_t* tokens, const int32_t* parents, const int32_t* cu_rows, int rows, int seqs,
+                      int max_rows, int vocab, void* ws, int64_t ws_bytes, int32_t* out, void* stream) {
+  if (int rc = check_accept_tree(rows, seqs, max_rows, vocab)) return rc;
+  if (seqs == 0) return ok();
+  if (!cu_rows || !out || (rows > 0 && (!target || !tokens || !parents)))
+    return fail(SSMOE_EINVAL, "target, tokens, parents, cu_rows and out must be non-null");
+  ss::TreeAcceptArgs a{target, tokens, parents, cu_rows, out, static_cast<uint64_t*>(ws), nullptr, rows, seqs, max_rows, vocab, 0, 0};
+  accept_tree_spans(rows, vocab, &a.splits, &a.span);
+  const int64_t need = (int64_t)rows * a.splits * 8;
+  if (need > 0 && (!ws || ws_bytes < need || !aligned(ws, 8)))
+    return fail(SSMOE_EINVAL, "workspace holds %lld bytes, the call needs %lld (8-byte aligned)", (long long)(ws ? ws_bytes : 0),
+                (long long)need);
+  if (!aligned(target, 4)) return fail(SSMOE_EINVAL, "target must be 4-byte aligned");
+  if (int rc = check_apart({{"out", out, 4 * (int64_t)seqs * (4 + 2 * max_rows)}, {"ws", ws, need}},
+                           {{"target", target, 4 * (int64_t)rows * vocab},
+                            {"tokens", tokens, 4 * (int64_t)rows},
+                            {"parents", parents, 4 * (int64_t)rows},
+                            {"cu_rows", cu_rows, 4 * ((int64_t)seqs + 1)}}))
+    return rc;
+  if (int rc = status_ptr(&a.err)) return rc;
+  return hip_check(ss::launch_tree_accept(a, static_cast<hipStream_t>(stream)), "tree acceptance launch");
+}
+
+int ssmoe_keep_rows(void* k, void* v, uint8_t* scales, int layers, int64_t n_pages, int kv_heads, int page, int dim, int bytes,
+                    const int32_t* cu_rows, const int32_t* kv_len, const int32_t* table, int width, const int32_t* accepted, int rows,
+                    int seqs, int max_rows, void* stream) {
+  ss::KeepArgs a{};
+  if (int rc = check_paged(rows, seqs, max_rows, kv_heads, kv_heads, dim, page, width, n_pages, SSMOE_BF16, &a.page_shift)) return rc;
+  if (layers < 1) return fail(SSMOE_EINVAL, "need layers >= 1");
+  if (bytes != 1 && bytes != 2) return fail(SSMOE_EINVAL, "bytes of an element must be 1 (e4m3) or 2, got %d", bytes);
+  if (max_rows > ss::kTreeRows) return fail(SSMOE_EINVAL, "a tree has at most %d rows of a sequence, max_rows is %d", ss::kTreeRows, max_rows);
+  const int64_t one = (int64_t)kv_heads * page * dim;
+  if (n_pages > INT64_MAX / 4 / one / layers || (int64_t)layers * kv_heads > INT32_MAX / std::max(seqs, 1))
+    return fail(SSMOE_EINVAL, "too many layers and sequences for one call");
+  if (rows == 0 || seqs == 0) return ok();
+  if (!k || !v || !cu_rows || !kv_len || !table || !accepted || (bytes == 1 && !scales))
+    return fail(SSMOE_EINVAL, "k, v, cu_rows, kv_len, table, accepted and of e4m3 scales must be non-null");
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(SSMOE_EINVAL, "k and v must be 16-byte aligned");
+  const int64_t cache = layers * n_pages * one * bytes;
+  if (int rc = check_apart({{"k", k, cache}, {"v", v, cache}, {"scales", bytes == 1 ? scales : nullptr, layers * n_pages * kv_heads * 2 * page}},
+                           {{"cu_rows", cu_rows, 4 * ((int64_t)seqs + 1)},
+                            {"kv_len", kv_len, 4 * (int64_t)seqs},
+                            {"table", table, 4 * (int64_t)seqs * width},
+                            {"accepted", accepted, 4 * (int64_t)seqs * (4 + 2 * max_rows)}}))
+    return rc;
+  a.k = static_cast<uint8_t*>(k);
+  a.v = static_cast<uint8_t*>(v);
+  a.scales = bytes == 1 ? scales : nullptr;
+  a.cu = cu_rows;
+  a.kv_len = kv_len;
+  a.table = table;
+  a.took = accepted;
+  if (int rc = status_ptr(&a.err)) return rc;
+  a.n_pages = n_pages;
+  a.layers = layers;
+  a.seqs = seqs;
+  a.rows = rows;
+  a.max_rows = max_rows;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.width = width;
+  a.size = bytes;
+  return hip_check(ss::launch_keep_rows(a, static_cast<hipStream_t>(stream)), "row move launch");
 }
 
 int ssmoe_pool_open(const char* experts_path, int layers, int experts, int64_t record_bytes, int max_slots,

@@ -28,7 +28,7 @@ _plans = Plans()
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                 k_pages: torch.Tensor, v_pages: torch.Tensor, cu_rows: torch.Tensor, kv_len: torch.Tensor,
                 table: torch.Tensor, max_rows: int, axis: torch.Tensor | None = None, adjacent: bool = False,
-                factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+                factor: float = 1.0, out: torch.Tensor | None = None, scales: torch.Tensor | None = None) -> torch.Tensor:
     """Turns q [rows, heads, dim] and k [rows, kv_heads, dim] by their rows' positions, writes k and v [rows, kv_heads,
     dim] into the cache at their sequence's places (row i of n at token kv_len - n + i) and returns the turned q.
 
@@ -36,20 +36,26 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     inv_freq[i], axis int32 [rot / 2] (None: axis 0; an entry outside [0, axes) raises SSMOE_ERR_BATCH in the device status). The pair turned by it is (i, i + rot / 2), or (2 i, 2 i + 1) with
     `adjacent`; elements from rot on are copied. cos and sin are multiplied by `factor`. q, k and v may be views into
     one projection (strides multiples of 8 elements); `out` may be q itself where q is contiguous; else it and the pages overlap
-    each other and the inputs nowhere. Rows past cu_rows[-1] are left as they were."""
+    each other and the inputs nowhere. Rows past cu_rows[-1] are left as they were.
+
+    `scales` uint8 [n_pages, kv_heads, 2, page]: the pages are of e4m3 numbers, q, k and v bf16. A token's and head's keys (values) are
+    kept as x 2^-e rounded once, e the least exponent from -126 on with which none is over 448, and scales[.., 0 (1), t] = e + 127. An
+    infinity or NaN is left out of that choice and kept as NaN. scales is written as the pages are, and overlaps nothing either."""
     max_rows = int(max_rows)
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape,
            positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, inv_freq.is_contiguous(), k_pages.shape,
            k_pages.dtype, k_pages.is_contiguous(), v_pages.shape, v_pages.dtype, v_pages.is_contiguous(), cu_rows.shape,
            cu_rows.stride(), cu_rows.dtype, kv_len.shape, kv_len.stride(), kv_len.dtype, table.shape, table.dtype,
            table.is_contiguous(), max_rows, None if axis is None else (axis.shape, axis.stride(), axis.dtype), factor)
+    if scales is not None:
+        key += (scales.shape, scales.dtype, scales.is_contiguous())
     plan = _plans.get(key)
     if plan is None:
         if not abs(factor) < 1e30:
             raise ValueError("factor must be finite and below 1e30")
-        plan = _plans.keep(key, _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis))
+        plan = _plans.keep(key, _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis, scales))
     row_strides, sizes, rot, axes, kind, shape = plan
-    dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out)
+    dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out, scales)
     q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if (q_at | k_at | v_at) % 16:
         raise ValueError("q, k and v need 16-byte alignment")
@@ -61,15 +67,18 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
                       0 if axis is None else axis.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), cu_rows.data_ptr(),
                       kv_len.data_ptr(), table.data_ptr(), *sizes, rot, axes, 1 if adjacent else 0, kind, float(factor))
     with _lib.on_device(dev):
-        _lib.check(_lib.lib().ssmoe_rope_append(args, _lib.raw_stream(dev)))
+        if scales is None:
+            _lib.check(_lib.lib().ssmoe_rope_append(args, _lib.raw_stream(dev)))
+        else:
+            _lib.check(_lib.lib().ssmoe_rope_append_e4m3(args, scales.data_ptr(), _lib.raw_stream(dev)))
     return out
 
 
-def _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis):
+def _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis, scales=None):
     """Checks a call's shapes, types and strides: (strides, sizes, rot, axes, type, shape of out)."""
-    n_pages, kv_heads, page, dim = check_cache(k_pages, v_pages)
+    n_pages, kv_heads, page, dim = check_cache(k_pages, v_pages, scales)
     seqs, width = check_batch(cu_rows, kv_len, table, max_rows)
-    dtype = k_pages.dtype
+    dtype = k_pages.dtype if scales is None else torch.bfloat16
     check_rows("q", q, None, dim, dtype)
     check_rows("k", k, kv_heads, dim, dtype)
     check_rows("v", v, kv_heads, dim, dtype)

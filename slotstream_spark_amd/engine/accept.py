@@ -68,6 +68,23 @@ class AcceptResult:
         return AcceptResult(o[0], o[1], o[2], o[3], o[4: 4 + o[1]])
 
 
+@dataclass
+class TreeResult:
+    """The greedy round of a tree (kernels/tree.accept_tree) of one sequence: `tokens` the target's choices along the branch, `path` its
+    rows, row 0 (the pending token) first: n_accept drafts were followed, so n_accept + 1 rows are kept."""
+    n_accept: int
+    n_emit: int
+    flags: int
+    tokens: list = field(default_factory=list)
+    path: list = field(default_factory=list)
+
+    @staticmethod
+    def from_out(out) -> "TreeResult":
+        o = [int(v) for v in out]
+        most = (len(o) - 4) // 2
+        return TreeResult(o[0], o[1], o[3], o[4: 4 + o[1]], [r for r in o[4 + most:] if r >= 0])
+
+
 class Acceptor:
     """Device acceptance for depth D over a V-token vocabulary (workspace and output owned here)."""
 

@@ -56,7 +56,8 @@ class AttentionLayer:
     def _lin(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         return lin_epi(x, w, out=out) if x.shape[0] <= FEW_ROWS else gemm_bf16(x, w, out=out)
 
-    def append(self, x: torch.Tensor, positions, k_pages, v_pages, cu_rows, kv_len, table, max_rows: int) -> torch.Tensor:
+    def append(self, x: torch.Tensor, positions, k_pages, v_pages, cu_rows, kv_len, table, max_rows: int,
+               scales: torch.Tensor | None = None) -> torch.Tensor:
         """Projects x bf16 [R, H], writes its key and value rows into the cache, returns the turned queries [R, heads, dim]."""
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.hidden or not x.is_contiguous():
             raise ValueError(f"x must be a contiguous bf16 [R, {self.hidden}] tensor")
@@ -68,14 +69,16 @@ class AttentionLayer:
             qk = rmsnorm(self._lin(x, self.wqkv[:self.n_qk]), self.qk_norm, self.eps, group=d).view(R, h + kv, d)
             q, k, v = qk[:, :h], qk[:, h:], self._lin(x, self.wqkv[self.n_qk:]).view(R, kv, d)
         return rope_append(q, k, v, positions, self.inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows,
-                           axis=self.axis, adjacent=self.adjacent, factor=self.factor)
+                           axis=self.axis, adjacent=self.adjacent, factor=self.factor, scales=scales)
 
     def __call__(self, x: torch.Tensor, positions, k_pages, v_pages, cu_rows, kv_len, table, max_rows: int,
-                 out: torch.Tensor | None = None) -> torch.Tensor:
-        """x bf16 [R, H] (normalised rows of the batch) -> bf16 [R, H]; the batch as rope_append and paged_attention take it."""
-        q = self.append(x, positions, k_pages, v_pages, cu_rows, kv_len, table, max_rows)
+                 out: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                 tree: torch.Tensor | None = None) -> torch.Tensor:
+        """x bf16 [R, H] (normalised rows of the batch) -> bf16 [R, H]; the batch, the scales of e4m3 pages and the words of a tree's
+        rows as rope_append and paged_attention take them."""
+        q = self.append(x, positions, k_pages, v_pages, cu_rows, kv_len, table, max_rows, scales)
         o = paged_attention(q, k_pages, v_pages, cu_rows, kv_len, table, max_rows, window=self.window, sinks=self.sinks,
-                            scale=self.scale)
+                            scale=self.scale, scales=scales, tree=tree)
         return self._lin(o.view(x.shape[0], self.heads * self.dim), self.wo, out)
 
 

@@ -22,9 +22,11 @@ import torch
 
 from ..kernels.gemv_affine import AffineWeight, LMHeadArgmax
 from ..kernels.head_ops import gather_rows
+from ..kernels.paged_attention import TREE_ROWS
+from ..kernels.tree import accept_tree, keep_rows, tree_masks
 from . import mtp as mtp_mod
 from . import rollback as rb
-from .accept import AcceptResult
+from .accept import AcceptResult, TreeResult
 from .attention import SeqCache
 from .prefill import MoEPrefillLayer
 from .step import MoEWeights, MTPStepGraph, residual_rmsnorm
@@ -37,7 +39,8 @@ class MoEStack:
     the stack's) adds attention; max_ctx is then at most what its table covers less a round's rows. Where every layer
     has a window the stack keeps all its pages the same: pages.evict(stack.cache.seq, the widest window, the most first tokens,
     back=stack.rows) between rounds gives back those that no row sees any more. `prompt_chunk` > 0: prompts go through the prompt
-    forms of the layers (MoEPrefillLayer, and the many-row attention) in chunks of so many tokens instead of `rows` at a time."""
+    forms of the layers (MoEPrefillLayer, and the many-row attention) in chunks of so many tokens instead of `rows` at a time.
+    Pages in 8 bits (KVPages of torch.float8_e4m3fn) are written and read as such. tree_step() verifies a tree of drafts."""
 
     def __init__(self, pool, layers: list[MoEWeights], lm_head: AffineWeight, embed: torch.Tensor,
                  depth: int = mtp_mod.DEPTH, norm_weights=None, eps: float = 1e-6, top_k: int = 10,
@@ -60,6 +63,7 @@ class MoEStack:
             if pages is not None:   # a pass writes `rows` tokens, also where fewer are kept
                 max_ctx = min(max_ctx, pages.width * pages.page - self.rows)
             self.embed, self.max_ctx, self.device = embed, max_ctx, torch.device(device)
+            self.lm_head, self._tree_head = lm_head, None
             self.argmax = LMHeadArgmax(lm_head, max_rows=self.rows, round_bf16=True, device=device)
             # the plain steps' logits, kept for the finiteness check of _mtp_decode's plain loop (generate.py:186-189)
             self.plain_logits = torch.empty((self.rows, lm_head.n), dtype=torch.float32, device=self.device)
@@ -138,30 +142,130 @@ class MoEStack:
             raise ValueError("a prompt needs at least one token")
         if self.prompt_layers is None:
             return self.forward(tokens)
-        g, w, eps, multi = self.graph, self.graph.norm_weights, self.graph.eps, []
+        multi = []
         for c0 in range(0, len(tokens), self.chunk):
             chunk = [int(t) for t in tokens[c0:c0 + self.chunk]]
             n = len(chunk)
             x = gather_rows(self.embed, torch.tensor(chunk, dtype=torch.int32).to(self.device))
-            mixed = torch.empty_like(x)
+            batch = None
             if self.cache is not None:
                 self.cache.place(self.st.pos, n)
                 cu, kv_len, table, positions = self.cache.rows(n)
-            attn = self.cache is not None
-            residual_rmsnorm(x, None, mixed, weight=(g.attn_norms if attn else w)[0], eps=eps)
-            for l, layer in enumerate(self.prompt_layers):
-                if attn:
-                    a = g.attn[l](mixed, positions, self.cache.pages.k[l], self.cache.pages.v[l], cu, kv_len, table, n)
-                    residual_rmsnorm(x, a, mixed, stream_out=x, weight=w[l], eps=eps)
-                y = layer(mixed)[0]
-                nxt = g.attn_norms[l + 1] if attn and l + 1 < self.nl else w[l + 1]
-                residual_rmsnorm(x, y, mixed, stream_out=x, weight=nxt, eps=eps)
+                batch = (positions, cu, kv_len, table, n)
+            mixed = self._through(x, batch)
             multi.append(x)
             self._advance(chunk)
         last = mixed[-1:].expand(self.rows, -1).contiguous()
         self.argmax(last, ids=self.row_ids, logits=self.plain_logits)
         self.last_finite = [bool(torch.isfinite(self.plain_logits[0]).all())]
         return [int(self.row_ids[0])], torch.cat(multi, 0)
+
+
+    def _through(self, x: torch.Tensor, batch=None, **kw) -> torch.Tensor:
+        """The rows x [n, H] through every layer, in place -> the normalised rows before the lm_head. `batch`: (positions, cu_rows, kv_len,
+        table, max_rows) of the attention, which also takes `kw`. Through the layers' prompt forms, where there are none by the verify
+        layers, as many rows at a time as those take."""
+        g, w, eps = self.graph, self.graph.norm_weights, self.graph.eps
+        mixed = torch.empty_like(x)
+        residual_rmsnorm(x, None, mixed, weight=(w if batch is None else g.attn_norms)[0], eps=eps)
+        for l in range(self.nl):
+            if batch is not None:
+                pages = self.cache.pages
+                a = g.attn[l](mixed, batch[0], pages.k[l], pages.v[l], *batch[1:], **pages.of_layer(l), **kw)
+                residual_rmsnorm(x, a, mixed, stream_out=x, weight=w[l], eps=eps)
+            if self.prompt_layers is not None:
+                y = self.prompt_layers[l](mixed)[0]
+            else:
+                y = torch.cat([g.layers[l](mixed[r:r + self.rows])[0] for r in range(0, x.shape[0], self.rows)])
+            nxt = g.attn_norms[l + 1] if batch is not None and l + 1 < self.nl else w[l + 1]
+            residual_rmsnorm(x, y, mixed, stream_out=x, weight=nxt, eps=eps)
+        return mixed
+
+    def take_back(self, n: int) -> None:
+        """The sequence's last n tokens are no longer its own (their rows in the cache are written over)."""
+        if not 0 <= n <= len(self.st.tokens):
+            raise ValueError(f"cannot take back {n} of {len(self.st.tokens)} tokens")
+        self.st.pos -= n
+        del self.st.tokens[len(self.st.tokens) - n:]
+        for c in self.st.attn.values():
+            c.pos = self.st.pos
+
+    def tree_step(self, tokens: list[int], parents: list[int]) -> tuple[TreeResult, torch.Tensor]:
+        """A greedy round over a tree: tokens[0] is the pending token, tokens[i] a draft behind row parents[i] < i (parents[0] is not
+        looked at), at most 64 rows, and with prompt_chunk at most so many. All rows go through the stack in one pass, each seeing the
+        sequence, its ancestors and itself; the branch that the stack's choices follow stays, moved up in the cache, and the position
+        advances by its rows. -> (the round, the final stream rows of the kept rows [n_accept + 1, H]). A row's choice may differ from
+        step()'s as far as another order of sums rounds another way."""
+        n = len(tokens)
+        if not 1 <= n <= TREE_ROWS or len(parents) != n:
+            raise ValueError(f"a tree has 1 to {TREE_ROWS} rows and a parent for each, got {n} and {len(parents)}")
+        if any(not 0 <= int(p) < i for i, p in enumerate(parents) if i):
+            raise ValueError("every row's parent must be a row before it")
+        if self.prompt_layers is not None and n > self.chunk:
+            raise ValueError(f"the prompt layers take {self.chunk} rows, the tree has {n}")
+        if self.cache is not None and any(0 < a.window < n for a in self.graph.attn):
+            raise ValueError(f"a layer's window must hold the tree's {n} rows")
+        if self._tree_head is None:
+            self._tree_head = LMHeadArgmax(self.lm_head, max_rows=TREE_ROWS, round_bf16=True, device=self.device)
+        rows = torch.tensor([[int(t) for t in tokens], [-1] + [int(p) for p in parents[1:]]], dtype=torch.int32).to(self.device)
+        x = gather_rows(self.embed, rows[0])
+        if self.cache is not None:
+            self.cache.place(self.st.pos, n)
+            cu, kv_len, table, _ = self.cache.rows(n)
+            masks, positions = tree_masks(rows[1], cu, kv_len, n)
+            mixed = self._through(x, (positions, cu, kv_len, table, n), tree=masks)
+        else:
+            cu = torch.tensor([0, n], dtype=torch.int32).to(self.device)
+            mixed = self._through(x)
+        logits = torch.empty((n, self.lm_head.n), dtype=torch.float32, device=self.device)
+        ids = torch.empty(n, dtype=torch.int32, device=self.device)
+        self._tree_head(mixed, ids=ids, logits=logits)
+        took = accept_tree(logits, rows[0], rows[1], cu, n)
+        if self.cache is not None:
+            pages = self.cache.pages
+            keep_rows(pages.k, pages.v, cu, kv_len, table, took, scales=pages.scales)
+        res = TreeResult.from_out(took[0].tolist())
+        self._advance([int(tokens[p]) for p in res.path])
+        return res, x[torch.tensor(res.path).to(self.device)]
+
+
+def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eos=(), on_token=None):
+    """Greedy decode after `prompt` by rounds over trees -> (tokens, nan, round_seconds, stats), as mtp_decode's.
+    tree_fn(pending, room, n_out) -> (drafts, parents): up to `room` drafts, each behind row parents[i] (0 the pending token, j + 1 draft
+    j). Where none fit, or it gives none, a round is the pending token alone. The drafts decide how many tokens a round emits, not
+    which (but for choices that another order of sums rounds another way). As after mtp_decode the stack's sequence is the prompt and
+    what was emitted but for the last token."""
+    out, step_s, nan = [], [], False
+    st = {"rounds": 0, "drafted": 0, "accepted": 0, "emitted_by_round": [], "verify_rows": 0}
+    nxt, _ = stack.prompt(prompt)
+    if not stack.last_finite[-1]:
+        return out, True, step_s, st
+    emitted, kept = [nxt[-1]], 1
+    most = TREE_ROWS - 1 if stack.prompt_layers is None else min(TREE_ROWS, stack.chunk) - 1
+    while True:
+        for i, tok in enumerate(emitted):
+            out.append(tok)
+            if on_token:
+                on_token(tok)
+            if tok in eos or len(out) == max_tokens:
+                if st["rounds"]:
+                    stack.take_back(kept - (i + 1))
+                return out, nan, step_s, st
+        if nan or stack.st.pos + 1 > stack.max_ctx:
+            return out, nan, step_s, st
+        t1 = time.perf_counter()
+        room = min(most, stack.max_ctx - stack.st.pos - 1)
+        drafts, parents = tree_fn(out[-1], room, len(out)) if room > 0 else ([], [])
+        if len(drafts) > room:
+            raise ValueError(f"{len(drafts)} drafts, there is room for {room}")
+        res, _ = stack.tree_step([out[-1], *drafts], [-1, *parents])
+        step_s.append(time.perf_counter() - t1)
+        emitted, kept, nan = res.tokens, len(res.path), bool(res.flags)
+        st["rounds"] += 1
+        st["drafted"] += len(drafts)
+        st["accepted"] += res.n_accept
+        st["verify_rows"] += 1 + len(drafts)
+        st["emitted_by_round"].append(res.n_emit)
 
 
 def mtp_decode(stack: MoEStack, head: mtp_mod.MTPHead, prompt: list[int], max_tokens: int, eos=(), on_token=None,

@@ -258,9 +258,9 @@ class MTPHead:
             kv_len, positions = base + (pos + S), base + torch.arange(pos, pos + S, dtype=torch.int32, device=h.device)
         args = (mixed, positions, a.pages.k[0], a.pages.v[0], cu, kv_len, table, S)
         if append_only:
-            a.layer.append(*args)
+            a.layer.append(*args, **a.pages.of_layer(0))
             return None
-        return hc_inject(h, a.layer(*args), inj)
+        return hc_inject(h, a.layer(*args, **a.pages.of_layer(0)), inj)
 
     def _step_rows(self, embedded, multi, r: _Rows, i: int, idx: torch.Tensor | None = None, pos: int = 0,
                    base: torch.Tensor | None = None):

@@ -174,7 +174,7 @@ class MTPStepGraph:
             pages, an = self.cache.pages, self.attn_norms
             residual_rmsnorm(self.x_in, None, self.attn_in, weight=an[0], eps=self.eps)
             for l, layer in enumerate(self.layers):
-                a = self.attn[l](self.attn_in, positions, pages.k[l], pages.v[l], cu, kv_len, table, self.rows)
+                a = self.attn[l](self.attn_in, positions, pages.k[l], pages.v[l], cu, kv_len, table, self.rows, **pages.of_layer(l))
                 residual_rmsnorm(self.streams[l], a, self.mixed[l], stream_out=self.attn_mid, weight=w[l], eps=self.eps)
                 layer(self.mixed[l], y=self.ys[l], ids=self.ids[l], weights=self.weights[l])
                 last = l + 1 == self.nl

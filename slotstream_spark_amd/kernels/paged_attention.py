@@ -148,7 +148,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if plan is None:
         plan = _plans.keep(key, _plan(q, k_pages, v_pages, cu_rows, kv_len, table, max_rows, window, sinks, scale, scales, tree))
     head, sizes, tail, nb, shape = plan
-    dev = check_device(q, k_pages, v_pages, cu_rows, kv_len, table, out, lse, scales, tree)
+    dev = check_device(q, k_pages, v_pages, cu_rows, kv_len, table, out, lse)
+    if ext:
+        check_device(q, scales, tree)
     q_at = q.data_ptr()
     if q_at % 16:
         raise ValueError("q needs 16-byte alignment")

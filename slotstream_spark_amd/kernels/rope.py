@@ -55,7 +55,9 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
             raise ValueError("factor must be finite and below 1e30")
         plan = _plans.keep(key, _plan(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, max_rows, axis, scales))
     row_strides, sizes, rot, axes, kind, shape = plan
-    dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out, scales)
+    dev = check_device(q, k, v, positions, inv_freq, k_pages, v_pages, cu_rows, kv_len, table, axis, out)
+    if scales is not None:
+        check_device(q, scales)
     q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if (q_at | k_at | v_at) % 16:
         raise ValueError("q, k and v need 16-byte alignment")

@@ -18,7 +18,7 @@ import torch
 
 from .. import _lib
 from ..kernels.kv_pages import move_pages
-from ..kernels.paged_attention import DIMS, PAGES, TYPES
+from ..kernels.paged_attention import DIMS, E4M3, PAGES, TYPES
 
 
 class KVPages:
@@ -26,18 +26,23 @@ class KVPages:
     page], zero at first. Up to `max_seqs` sequences of up to `max_tokens` tokens; table int32 [max_seqs, width] on the device, -1
     where a sequence holds no page. `length[s]` is the number of tokens that a sequence has room for and counts as its own.
     `resizes` counts the times that k and v became other tensors (a captured graph holds the ones it was captured with). A page given
-    back may be handed out at once: where sequences are worked on in several streams, their owners wait for each other first."""
+    back may be handed out at once: where sequences are worked on in several streams, their owners wait for each other first.
+
+    With dtype torch.float8_e4m3fn the cache is in 8 bits: `scales` uint8 [layers, n_pages, kv_heads, 2, page] has every token's powers of
+    two (rope_append writes them, paged_attention reads them), and moves with the pages; else it is None."""
 
     def __init__(self, layers: int, n_pages: int, kv_heads: int, dim: int, page: int = 64, max_seqs: int = 1,
                  max_tokens: int = 131072, dtype=torch.bfloat16, device="cuda"):
         if layers < 1 or n_pages < 1 or kv_heads < 1 or max_seqs < 1 or max_tokens < 1:
             raise ValueError("layers, n_pages, kv_heads, max_seqs and max_tokens must be positive")
-        if page not in PAGES or dim not in DIMS or dtype not in TYPES:
-            raise ValueError("pages hold 16, 32, 64, 128 or 256 tokens of 64, 128 or 256 bf16 or fp16 dimensions")
+        if page not in PAGES or dim not in DIMS or (dtype not in TYPES and dtype != E4M3):
+            raise ValueError("pages hold 16, 32, 64, 128 or 256 tokens of 64, 128 or 256 bf16, fp16 or e4m3 dimensions")
         self.layers, self.n_pages, self.kv_heads, self.dim, self.page = layers, n_pages, kv_heads, dim, page
         self.max_seqs, self.width = max_seqs, -(-max_tokens // page)
         self.k = torch.zeros((layers, n_pages, kv_heads, page, dim), dtype=dtype, device=device)
         self.v = torch.zeros((layers, n_pages, kv_heads, dim, page), dtype=dtype, device=device)
+        self.scales = (torch.zeros((layers, n_pages, kv_heads, 2, page), dtype=torch.uint8, device=device) if dtype == E4M3
+                       else None)
         self.table = torch.full((max_seqs, self.width), -1, dtype=torch.int32, device=device)
         self._table = np.full((max_seqs, self.width), -1, np.int32)
         self._refs = np.zeros(n_pages, np.int64)
@@ -78,8 +83,16 @@ class KVPages:
         self.table[seq].copy_(torch.from_numpy(self._table[seq]))
 
     def _move(self, src, dst, table=None) -> None:
-        move_pages(self.k, self.v, torch.tensor(src, dtype=torch.int32).to(self.k.device),
-                   torch.tensor(dst, dtype=torch.int32).to(self.k.device), table)
+        args = (self.k, self.v, torch.tensor(src, dtype=torch.int32).to(self.k.device),
+                torch.tensor(dst, dtype=torch.int32).to(self.k.device), table)
+        if self.scales is None:
+            move_pages(*args)
+        else:
+            move_pages(*args, scales=self.scales)
+
+    def of_layer(self, layer: int) -> dict:
+        """The keyword arguments that rope_append and paged_attention take for a layer's pages beside k[layer] and v[layer]."""
+        return {} if self.scales is None else {"scales": self.scales[layer]}
 
     # ------------------------------------------------------------------ sequences
     def new(self) -> int:
@@ -219,6 +232,8 @@ class KVPages:
             return out
 
         self.k, self.v = sized(self.k), sized(self.v)
+        if self.scales is not None:
+            self.scales = sized(self.scales)
         self.resizes += 1
         refs = np.zeros(n_pages, np.int64)
         refs[:keep] = self._refs[:keep]

@@ -30,9 +30,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int tile = (i * a.group + head % a.group) / a.packed, p0 = tile * a.packed, np = sr.n * a.group;
   const int lo = a.tree ? 0 : p0 / a.group, hi = a.tree ? sr.n - 1 : (min(p0 + a.packed, np) - 1) / a.group;
   const Seen sn = seen_tokens(sr.pos0 + lo, sr.pos0 + hi, sr.end, a.window, a.sinks);
-  const int sc = (sn.s_end + a.chunk - 1) / a.chunk, wc = max(sn.w_begin / a.chunk, sc);
-  const int used = sc + max((sn.end + a.chunk - 1) / a.chunk - wc, 0);
-  const int64_t row = (int64_t)(sr.r0 + i) * a.heads + head, rows = (int64_t)a.rows * a.heads;
+  const int chunk = a.share > 0 ? 64 * gp(a.meta)[0] : a.chunk;
+  const int sc = (sn.s_end + chunk - 1) / chunk, wc = max(sn.w_begin / chunk, sc);
+  const int used = sc + max((int)(((int64_t)sn.end + chunk - 1) / chunk) - wc, 0);
+  const int64_t row = (int64_t)(sr.r0 + i) * a.heads + head;
+  // Where the row's partial sums begin and how far those of the next chunk are.
+  const int64_t rows = a.share > 0 ? (int64_t)a.tiles * a.kv_heads * 128 : (int64_t)a.rows * a.heads;
+  const int packed = i * a.group + head % a.group;
+  const int64_t first = a.share > 0 ? ((int64_t)gp(a.meta)[1 + s] * a.tiles * a.kv_heads + (int64_t)tile * a.kv_heads + head / a.group) * 128 + packed % 128
+                                    : row;
   ss_f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float m = kNegInf, l = 0.f;
   auto add = [&](const ss_f32x4& x, float mk, float lk) {
@@ -46,7 +52,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   auto take = [&](int from, int to) {
 #pragma unroll 4
     for (int j = from; j < to; j += STEP) {
-      const int64_t at = j * rows + row;
+      const int64_t at = j * rows + first;
       const float mk = gp(a.pml)[2 * at], lk = gp(a.pml)[2 * at + 1];
       const ss_f32x4 x = *reinterpret_cast<const SS_G ss_f32x4*>(gp(a.po) + at * D + d4);
       add(x, mk, lk);
@@ -86,7 +92,7 @@ template <class T, int D>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
   constexpr int GROUPS = 256 / (D / 4);
-  if (a.slots > 16)
+  if ((a.share > 0 ? a.slots / a.seqs : a.slots) > 16)
     hipLaunchKernelGGL((attn_join_kernel<T, D, true>), dim3((unsigned)all), dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL((attn_join_kernel<T, D, false>), dim3((unsigned)((all + GROUPS - 1) / GROUPS)), dim3(256), 0, st, a);

@@ -34,6 +34,10 @@ struct AttnArgs {
   float scale; // of the scores, times log2(e)
   const uint8_t* scales;  // [n_pages][kv_heads][2][page] exponents of e4m3 keys and values (k, v then hold bytes), or null
   const uint64_t* tree;   // [rows] which of its sequence's rows a row sees, or null (causal)
+  // Shared chunks (many rows over e4m3 pages or of trees): `share` > 0 chunks for all sequences together, one size for all, by their
+  // lengths; `slots` then counts them over all sequences, po and pml are [slots][tiles][kv_heads][128 packed rows], and
+  int share;
+  int32_t* meta;  // [1 + seqs] has the size in units of 64 tokens and each sequence's first chunk, for the join
 };
 
 // ss_raise through a global pointer (a flat atomic would make every later wait of the wave one for all its LDS reads).
@@ -129,6 +133,51 @@ SS_DEV Seen seen_tokens(int pos_a, int pos_b, int end, int window, int sinks) {
   const int w = pos_a - window + 1;
   r.w_begin = w > 0 ? (w < r.end ? w : r.end) : 0;
   r.s_end = sinks < r.w_begin ? sinks : r.w_begin;
+  return r;
+}
+
+// ---------------------------------------------------------------- shared chunks
+// Chunk g of a call whose sequences share `a.share` chunks: units of 64 tokens, `size` of them a chunk, the least size (of two or
+// more) with which whole chunks number at most a.share; every sequence's last one may be short, so there are up to seqs more. A
+// wave works it out from all lengths. With `write` (one wave of the launch) the sequences' first chunks go to a.meta.
+struct Share {
+  int s, slot, size;  // the sequence, the chunk among its own; s < 0: there is no chunk g
+};
+SS_DEV Share find_share(const AttnArgs& a, int g, bool write) {
+  const int lane = threadIdx.x & 63;
+  const int64_t cap = (int64_t)a.width << a.page_shift;
+  auto units = [&](int s) {
+    if (s >= a.seqs || gp(a.cu)[s + 1] <= gp(a.cu)[s]) return 0u;
+    const int len = max(gp(a.kv_len)[s], 0);
+    return (uint32_t)(((int64_t)len < cap ? len : cap) + 63) / 64;
+  };
+  const uint32_t first = units(lane);
+  uint64_t total = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64)
+    total += ss_butterfly(s0 ? units(s0 + lane) : first, [](uint32_t x, uint32_t y) { return x + y; });
+  const uint32_t size = max((uint32_t)((total + a.share - 1) / a.share), 2u);
+  Share r = {-1, 0, (int)size};
+  int before = 0;
+  for (int s0 = 0; s0 < a.seqs && (write || r.s < 0); s0 += 64) {
+    const int mine = (int)(((s0 ? units(s0 + lane) : first) + size - 1) / size);
+    int upto = mine;
+    for (int d = 1; d < min(a.seqs, 64); d *= 2) {
+      const int o = __shfl_up(upto, d);
+      upto += lane >= d ? o : 0;
+    }
+    if (write && s0 + lane < a.seqs) a.meta[1 + s0 + lane] = before + upto - mine;
+    const uint64_t hit = __ballot(before + upto > g);
+    if (r.s < 0 && hit) {
+      const int l = __builtin_ctzll(hit);  // past the last sequence `upto` may be short: only a lane of one can be hit
+      r.s = s0 + l;
+      r.slot = g - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (write && lane == 0) a.meta[0] = (int)size;
+  r.s = __builtin_amdgcn_readfirstlane(r.s);
+  r.slot = __builtin_amdgcn_readfirstlane(r.slot);
+  r.size = __builtin_amdgcn_readfirstlane(r.size);
   return r;
 }
 

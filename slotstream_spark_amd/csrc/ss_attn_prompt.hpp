@@ -94,9 +94,23 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   b /= D / DV;
   const int kh = b % a.kv_heads;
   b /= a.kv_heads;
-  const int slot = b % a.slots;
+  int slot = b % a.slots;
   b /= a.slots;
-  const int s = b % a.seqs, turn = b / a.seqs;
+  constexpr bool SHARE = E8 || TREE;
+  const bool share = SHARE && a.share > 0;
+  int s, turn, chunk = a.chunk;
+  const int piece = slot;  // where its sums go
+  if (share) {
+    const Share sh = find_share(a, slot, blockIdx.x == 0 && w == 0);
+    if (sh.s < 0) return;  // whole workgroup, before any barrier
+    turn = b;
+    s = sh.s;
+    slot = sh.slot;
+    chunk = 64 * sh.size;
+  } else {
+    s = b % a.seqs;
+    turn = b / a.seqs;
+  }
   // The tiles that see most first; the last `a.rising` turns, which share CUs with the first ones, from the other end.
   const int tile = turn < a.tiles - a.rising ? a.tiles - 1 - turn : turn - (a.tiles - a.rising);
   const int page = 1 << a.page_shift;
@@ -111,12 +125,12 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int blk_lo = TREE ? sr.pos0 : sr.pos0 + p0 / a.group;
   const int blk_hi = TREE ? sr.pos0 + sr.n - 1 : sr.pos0 + (min(p0 + 128, np) - 1) / a.group;
   const Seen sn = seen_tokens(blk_lo, blk_hi, sr.end, a.window, a.sinks);
-  const int sc = (sn.s_end + a.chunk - 1) / a.chunk, wc = max(sn.w_begin / a.chunk, sc);
+  const int sc = (sn.s_end + chunk - 1) / chunk, wc = max(sn.w_begin / chunk, sc);
   int t_begin = 0, t_end = sn.end;
   if (a.slots > 1) {
     const int ch = slot < sc ? slot : wc + slot - sc;
-    t_begin = ch * a.chunk;
-    t_end = min(t_begin + a.chunk, sn.end);
+    t_begin = (int)min((int64_t)ch * chunk, (int64_t)sn.end);
+    t_end = (int)min((int64_t)t_begin + chunk, (int64_t)sn.end);
     if (t_begin >= t_end) return;
   }
   // The tiles of [t_begin, t_end) that some row sees: up to the first tokens' end, then from the window's begin on.
@@ -414,7 +428,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     float part[2] = {0.f, 0.f};
     // The operands of a product are read AHEAD products before it, those of the first value products beside the last of
     // the scores; PER scores of x are worked on beside each product of y.
-    constexpr int NK = ST * KS, PER = 16 * ST / NK, NV = DT * 2 * ST, AHEAD = E8 && TREE && D == 128 && TK == 64 ? 2 : 4, RING = AHEAD + 1;
+    constexpr int NK = ST * KS, PER = 16 * ST / NK, NV = DT * 2 * ST, AHEAD = 4, RING = AHEAD + 1;
     ss_u32x4 fr[RING];
     // Of e4m3 the places of the operands are worked out here from two (a place's 16-byte piece is 2 ks + h, and its swizzle, by exclusive or):
     // kept over the steps they would take 12 registers.
@@ -550,18 +564,20 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // no load into LDS outlives the wave
   __syncthreads();
   const bool fix = odd;
-  // This lane's column again, of e4m3 from nothing that is kept over the tiles.
-  int ln = lane;
-  if constexpr (E8) {
+  // This lane's column again, of e4m3 and of trees from nothing that is kept over the tiles.
+  int ln = lane, group = a.group;
+  if constexpr (SHARE) {
     uint32_t none = 0;
     asm volatile("" : "+v"(none));
+    asm volatile("" : "+s"(group));  // else the first division's reciprocal is kept
     ln = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
   }
-  const int ce = E8 ? ln & 31 : c, he = E8 ? ln >> 5 : h, pe = E8 ? p0 + 32 * w + ce : p, ie = E8 ? pe / a.group : i;
-  const bool ine = E8 ? pe < np : in;
+  const int ce = SHARE ? ln & 31 : c, he = SHARE ? ln >> 5 : h, pe = SHARE ? p0 + 32 * w + ce : p, ie = SHARE ? pe / group : i;
+  const bool ine = SHARE ? pe < np : in;
   l += other_half(l, he);
   const int64_t at = (int64_t)(sr.r0 + ie) * a.heads + kh * a.group + (pe - ie * a.group);
-  const int64_t pa = (int64_t)slot * a.rows * a.heads + at;
+  const int64_t pa = share ? (((int64_t)piece * a.tiles + tile) * a.kv_heads + kh) * 128 + (pe - p0)
+                           : (int64_t)slot * a.rows * a.heads + at;
   if (ine && a.slots > 1) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -638,7 +654,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
 // Tiles of 64 tokens where a page holds them, else of 32 (and of 256 dimensions always: registers).
 template <class T, int D, int DV, bool E8, bool TREE>
 void launch_prompt(const AttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * a.seqs * attn_prompt_parts(D, a.page_shift)));
+  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * (a.share > 0 ? 1 : a.seqs) * attn_prompt_parts(D, a.page_shift)));
   if (a.page_shift >= 6 && D < 256)
     hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, D < 256 ? 64 : 32, true, E8, TREE>), grid, dim3(256), 0, st, a);
   else if (a.page_shift >= 5)

@@ -5,6 +5,8 @@
 // that a set of rows is a 64-bit word.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "ss_attn.hpp"
 #include "ss_common.hpp"
 #include "ss_launch.hpp"
@@ -113,39 +115,46 @@ __global__ __launch_bounds__(256) void tree_argmax_kernel(TreeAcceptArgs a) {
   }
 }
 
-// A workgroup a sequence: four threads a row join its spans, then one wave walks the tree: from row 0, to the first row behind the
+// A workgroup a sequence: sixteen threads a row join its spans, then one wave walks the tree: from row 0, to the first row behind the
 // present one whose token is the present one's choice.
-__global__ __launch_bounds__(256) void tree_walk_kernel(TreeAcceptArgs a) {
+__global__ __launch_bounds__(1024) void tree_walk_kernel(TreeAcceptArgs a) {
   __shared__ uint64_t best[kTreeRows];
   const int tid = threadIdx.x, s = blockIdx.x;
   const TreeRows r = tree_rows(a.cu, s, a.rows, a.max_rows, a.err);
+  int p = -1, tok = -1;
+  if (tid > 0 && tid < r.n) {
+    p = gp(a.parents)[r.r0 + tid];
+    tok = gp(a.tokens)[r.r0 + tid];
+  }
   {
-    const int i = tid / 4;
+    const int i = tid / 16;
     uint64_t word = 0;
-    if (i < r.n)
-      for (int j = tid % 4; j < a.splits; j += 4) {
-        const uint64_t o = gp(a.part)[(int64_t)(r.r0 + i) * a.splits + j];
-        word = o > word ? o : word;
+    if (i < r.n) {
+      const uint64_t* part = a.part + (int64_t)(r.r0 + i) * a.splits;
+      for (int j = tid % 16; j < a.splits; j += 64) {  // four loads at a time; a span that is none is the first one again
+        uint64_t o[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[u] = gp(part)[j + 16 * u < a.splits ? j + 16 * u : 0];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) word = o[u] > word ? o[u] : word;
       }
+    }
     auto other = [&](uint64_t v, uint32_t hi, uint32_t lo) {
       const uint64_t o = (uint64_t)hi << 32 | lo;
       return o > v ? o : v;
     };
     word = other(word, ss_xor_lane<1>((uint32_t)(word >> 32)), ss_xor_lane<1>((uint32_t)word));
     word = other(word, ss_xor_lane<2>((uint32_t)(word >> 32)), ss_xor_lane<2>((uint32_t)word));
-    if (tid % 4 == 0) best[i] = word;
+    word = other(word, ss_xor_lane<4>((uint32_t)(word >> 32)), ss_xor_lane<4>((uint32_t)word));
+    word = other(word, ss_xor_lane<8>((uint32_t)(word >> 32)), ss_xor_lane<8>((uint32_t)word));
+    if (tid % 16 == 0) best[i] = word;
   }
   __syncthreads();
   if (tid >= 64) return;
   const int i = tid;
-  int p = -1, tok = -1;
-  if (i > 0 && i < r.n) {
-    p = gp(a.parents)[r.r0 + i];
-    tok = gp(a.tokens)[r.r0 + i];
-    if (p < 0 || p >= i) {
-      p = -1;
-      raise_bit(a.err, SS_ERR_BATCH);
-    }
+  if (i > 0 && i < r.n && (p < 0 || p >= i)) {
+    p = -1;
+    raise_bit(a.err, SS_ERR_BATCH);
   }
   const uint64_t mine = i < r.n ? best[i] : 0;
   const bool fine = mine != ~0ull;
@@ -173,26 +182,25 @@ __global__ __launch_bounds__(256) void tree_walk_kernel(TreeAcceptArgs a) {
   }
 }
 
-// A workgroup a sequence, layer and key head. Token base + d takes the row path[d]: paths rise, so every source lies at or behind
-// its place, and a thread that takes its bytes of the tokens in order, eight loads before eight stores, writes over none that it
-// has yet to read. Threads have 16 bytes of the keys, an element of each token's values, a byte of the exponents; no two share any.
-// Bound by latency and by how little of a line an element of the values is: 48 layers of one chat's branch take 9 us.
+// Token base + d takes the row path[d]: paths rise, so every source lies at or behind its place, and a thread that takes its part of the
+// tokens in order, eight loads before eight stores, writes over none that it has yet to read. The parts of a key head: an element
+// of each token's values (a thread a dimension), 16 bytes of the keys, a byte of the exponents; no two share any. A workgroup works a
+// sequence's branch out once and takes parts of all layers and key heads, `rounds` of them a thread.
+// Bound by latency for one sequence (48 layers of 4 key heads 4 us), and by the lines of the values, of which an element a token is moved:
+// 32 sequences of 48 layers, 8 key heads, 128 dimensions of e4m3 and pages of 64 tokens touch 100 MB of lines, read and written, in 59 us.
 template <class V, bool E8>
 __global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
   __shared__ int64_t src[kTreeRows], dst[kTreeRows];  // page and token in it: page << 8 | token
   __shared__ int count;
   const int tid = threadIdx.x, page = 1 << a.page_shift;
-  uint32_t b = blockIdx.x;
-  const int h = b % (uint32_t)a.kv_heads;
-  b /= (uint32_t)a.kv_heads;
-  const int layer = b % (uint32_t)a.layers, s = b / (uint32_t)a.layers;
+  const int s = blockIdx.x / (uint32_t)a.blocks, block = blockIdx.x - s * a.blocks;
   const int64_t cap = (int64_t)a.width * page;
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, cap, a.err);
   const int32_t* took = a.took + (int64_t)s * (4 + 2 * a.max_rows);
   if (tid < 64) {
     const int kept = gp(took)[0] + 1;
-    int at = -1;
-    if (tid < kept && tid < a.max_rows) at = gp(took)[4 + a.max_rows + tid];
+    int at = tid < a.max_rows ? gp(took)[4 + a.max_rows + tid] : -1;
+    if (tid >= kept) at = -1;
     int before = __shfl_up(at, 1);
     if (tid == 0) before = -1;
     // the branch as far as its rows rise and exist
@@ -223,9 +231,7 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
   __syncthreads();
   const int n = count;
   const int64_t one = (int64_t)a.kv_heads * page * a.dim;  // elements of a page
-  V* const kp = reinterpret_cast<V*>(a.k) + ((int64_t)layer * a.n_pages * one + (int64_t)h * page * a.dim);
-  V* const vp = reinterpret_cast<V*>(a.v) + ((int64_t)layer * a.n_pages * one + (int64_t)h * page * a.dim);
-  // item: its element type, the place of a token's part
+  // `base`: the part's first element in the layer; elements of a page and of a token of its kind
   auto move = [&](auto* base, int64_t per_page, int64_t per_token) {
     typedef typename std::remove_reference<decltype(*base)>::type E;
     for (int d0 = 0; d0 < n; d0 += 8) {
@@ -239,14 +245,18 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
     }
   };
   constexpr int EV = 16 / sizeof(V);  // elements of 16 bytes
-  const int kpieces = a.dim / EV;
-  for (int it = tid; it < a.dim + kpieces + (E8 ? 2 : 0); it += 256) {
-    if (it < a.dim)
-      move(vp + (int64_t)it * page, one, 1);
-    else if (it < a.dim + kpieces)
-      move(reinterpret_cast<ss_u32x4*>(kp) + (it - a.dim), one / EV, kpieces);
+  const int kpieces = a.dim / EV, parts = a.dim + kpieces + (E8 ? 2 : 0);
+  const int64_t all = (int64_t)parts * a.kv_heads * a.layers;
+  for (int64_t it = (int64_t)block * 256 + tid; it < all; it += (int64_t)a.blocks * 256) {
+    const int unit = (int)((uint64_t)it / (uint32_t)parts), part = (int)(it - (int64_t)unit * parts);
+    const int layer = (uint32_t)unit / (uint32_t)a.kv_heads, h = unit - layer * a.kv_heads;
+    const int64_t at = (int64_t)layer * a.n_pages * one + (int64_t)h * page * a.dim;
+    if (part < a.dim)
+      move(reinterpret_cast<V*>(a.v) + at + (int64_t)part * page, one, 1);
+    else if (part < a.dim + kpieces)
+      move(reinterpret_cast<ss_u32x4*>(reinterpret_cast<V*>(a.k) + at) + (part - a.dim), one / EV, kpieces);
     else
-      move(a.scales + (((int64_t)layer * a.n_pages * a.kv_heads + h) * 2 + (it - a.dim - kpieces)) * page, (int64_t)a.kv_heads * 2 * page, 1);
+      move(a.scales + (((int64_t)layer * a.n_pages * a.kv_heads + h) * 2 + (part - a.dim - kpieces)) * page, (int64_t)a.kv_heads * 2 * page, 1);
   }
 }
 
@@ -262,12 +272,16 @@ hipError_t launch_tree_accept(const TreeAcceptArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(tree_argmax_kernel, dim3((unsigned)((int64_t)a.rows * a.splits)), dim3(256), 0, st, a);
     if (const hipError_t e = hipGetLastError()) return e;
   }
-  hipLaunchKernelGGL(tree_walk_kernel, dim3((unsigned)a.seqs), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(tree_walk_kernel, dim3((unsigned)a.seqs), dim3(1024), 0, st, a);
   return hipGetLastError();
 }
 
-hipError_t launch_keep_rows(const KeepArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.layers * a.seqs * a.kv_heads));
+hipError_t launch_keep_rows(KeepArgs a, hipStream_t st) {
+  // A part a thread up to 8,192 workgroups, past which more of them change nothing: 32 sequences of 48 layers and 8 key heads of e4m3 take
+  // 59 us so and with 16,384, 63 with 4,096, 71 with 2,048, 104 with 512.
+  const int64_t parts = (int64_t)(a.dim + a.dim * a.size / 16 + (a.size == 1 ? 2 : 0)) * a.kv_heads * a.layers;
+  a.blocks = (int)std::min<int64_t>((parts + 255) / 256, std::max<int64_t>(8192 / a.seqs, 1));
+  const dim3 grid((unsigned)(a.blocks * a.seqs));
   if (a.size == 1)
     hipLaunchKernelGGL((keep_rows_kernel<uint8_t, true>), grid, dim3(256), 0, st, a);
   else

@@ -41,7 +41,8 @@ struct KeepArgs {
   int* err;
   int64_t n_pages;
   int layers, seqs, rows, max_rows, kv_heads, dim, page_shift, width, size;
+  int blocks;  // workgroups of a sequence (set by the launch)
 };
-hipError_t launch_keep_rows(const KeepArgs& a, hipStream_t st);
+hipError_t launch_keep_rows(KeepArgs a, hipStream_t st);
 
 }  // namespace ss

@@ -270,6 +270,11 @@ int check_apart(std::initializer_list<Span> written, std::initializer_list<Span>
 // 191 / 200 / 204 against 195 / 195 / 204 / 201; 8 of 16 on 2, 256 dimensions 33 / 43 / 56 / 69 against 42 / 45 / 48 / 52; 16
 // of 24 on 8, 64 dimensions 44 / 46 / 50 / 51 against 58 / 58 / 57 / 56.
 constexpr int kFewRows = 8;
+// Rows of partial sums (a row and head, or a column of a workgroup's tile) of a call.
+int64_t partial_rows(const ss::AttnArgs& a) {
+  if (a.slots <= 1) return 0;
+  return a.share > 0 ? (int64_t)a.slots * a.tiles * a.kv_heads * 128 : (int64_t)a.slots * a.rows * a.heads;
+}
 int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
   if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
   int shift = 0;
@@ -324,14 +329,23 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
     slots = std::min(slots, (std::min<int64_t>(a.sinks, cap) + chunk - 1) / chunk +
                                 (a.window + std::max(max_rows, kFewRows) + chunk - 2) / chunk + 1);
   if (*prompt && chunk >= seen) slots = 1;
+  // Over e4m3 pages and for trees the chunks are shared by the sequences' own lengths, which the kernel reads: as many for all
+  // together as CUs have places, so that the longest sequence does not hold up the launch.
+  if (*prompt && (e4m3 || tree) && a.window >= (1 << 30) && cap > 128) {
+    const int64_t want = 512 / std::max<int64_t>((int64_t)p->kv_heads * a.tiles * parts_of_dim, 1);
+    if (want >= 2 * std::max(p->seqs, 1)) {
+      a.share = (int)want;
+      slots = std::min<int64_t>(want + p->seqs, (int64_t)p->seqs * ((cap + 127) / 128));
+    }
+  }
   // Two workgroups fit a CU: of at most 512, the second 256 go to the CUs of the first, the lightest to the heaviest.
   const int64_t per_tile = units * slots * parts_of_dim, all = per_tile * a.tiles;
-  a.rising = *prompt && all > 256 && all <= 512 ? (int)((all - 256) / per_tile) : 0;
+  a.rising = *prompt && a.share == 0 && all > 256 && all <= 512 ? (int)((all - 256) / per_tile) : 0;
   a.slots = (int)slots;
   if (parts_of_dim * slots * a.tiles * p->kv_heads * p->seqs > INT32_MAX || (int64_t)p->seqs * max_rows * p->heads > INT32_MAX)
     return fail(SSMOE_EINVAL, "the call needs 2^31 workgroups or more: split it over sequences");
-  const int64_t parts = slots > 1 ? slots * p->rows * p->heads : 0;
-  *ws = (parts * p->dim * 4 + 255) / 256 * 256 + parts * 8;
+  const int64_t parts = partial_rows(a);
+  *ws = (parts * p->dim * 4 + 255) / 256 * 256 + parts * 8 + (a.share > 0 ? 4 * (1 + (int64_t)p->seqs) : 0);
   *out = a;
   return ok();
 }
@@ -1546,9 +1560,10 @@ int paged_attention(const ssmoe_paged_attention_args* p, const uint8_t* scales, 
   a.tree = tree;
   if (int rc = status_ptr(&a.err)) return rc;
   if (ws > 0) {
-    const int64_t parts = (int64_t)a.slots * p->rows * p->heads;
+    const int64_t parts = partial_rows(a);
     a.po = static_cast<float*>(p->ws);
     a.pml = reinterpret_cast<float*>(static_cast<char*>(p->ws) + (parts * p->dim * 4 + 255) / 256 * 256);
+    a.meta = reinterpret_cast<int32_t*>(a.pml + 2 * parts);
   }
   const bool fp16 = p->type == SSMOE_FP16;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -18,7 +18,9 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .paged_attention import DIMS, E4M3, PAGES, TREE_ROWS, TYPES, check_batch, check_device
+from .paged_attention import DIMS, E4M3, PAGES, TREE_ROWS, TYPES, Plans, check_batch, check_device
+
+_plans = Plans()
 
 
 def _check_tree(rows: int, cu_rows: torch.Tensor, max_rows: int, **ints) -> int:
@@ -64,24 +66,35 @@ def accept_tree(target: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     choice. A row with a logit that is not finite ends it before its choice (flag 1). Workspaces come from torch's allocator at each call.
     `out` overlaps nothing that the call reads. Capturable."""
     max_rows = int(max_rows)
+    key = (target.shape, target.dtype, target.is_contiguous(), tokens.shape, tokens.dtype, tokens.is_contiguous(), parents.shape,
+           parents.dtype, parents.is_contiguous(), cu_rows.shape, cu_rows.dtype, cu_rows.is_contiguous(), max_rows)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plans.keep(key, _accept_plan(target, tokens, parents, cu_rows, max_rows))
+    rows, vocab, seqs, nb, shape = plan
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=target.device)
+    elif out.dtype != torch.int32 or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous int32 {tuple(shape)}")
+    dev = check_device(target, tokens, parents, cu_rows, out)
+    ws = torch.empty(nb, dtype=torch.uint8, device=target.device) if nb else None
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().ssmoe_accept_tree(target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu_rows.data_ptr(), rows, seqs,
+                                                max_rows, vocab, _lib.ptr(ws), nb, out.data_ptr(), _lib.raw_stream(dev)))
+    return out
+
+
+def _accept_plan(target, tokens, parents, cu_rows, max_rows):
+    """Checks a call's shapes and types: (rows, vocab, seqs, workspace bytes, shape of out)."""
     if target.dim() != 2 or target.dtype != torch.float32 or not target.is_contiguous() or target.shape[1] < 1:
         raise ValueError("target must be contiguous fp32 [rows, vocab]")
     rows, vocab = target.shape
     seqs = _check_tree(rows, cu_rows, max_rows, tokens=tokens, parents=parents)
-    if out is None:
-        out = torch.empty((seqs, 4 + 2 * max_rows), dtype=torch.int32, device=target.device)
-    elif out.dtype != torch.int32 or tuple(out.shape) != (seqs, 4 + 2 * max_rows) or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous int32 {(seqs, 4 + 2 * max_rows)}")
-    dev = check_device(target, tokens, parents, cu_rows, out)
     L = _lib.lib()
     nb = L.ssmoe_accept_tree_workspace_bytes(rows, seqs, max_rows, vocab)
     if nb < 0:
         raise ValueError(L.ssmoe_last_error().decode(errors="replace"))
-    ws = torch.empty(nb, dtype=torch.uint8, device=target.device) if nb else None
-    with _lib.on_device(dev):
-        _lib.check(L.ssmoe_accept_tree(target.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu_rows.data_ptr(), rows, seqs,
-                                       max_rows, vocab, _lib.ptr(ws), nb, out.data_ptr(), _lib.raw_stream(dev)))
-    return out
+    return rows, vocab, seqs, nb, torch.Size((seqs, 4 + 2 * max_rows))
 
 
 def keep_rows(k: torch.Tensor, v: torch.Tensor, cu_rows: torch.Tensor, kv_len: torch.Tensor, table: torch.Tensor,

@@ -12,7 +12,8 @@ namespace {
 // groups of dim / 4 threads, 16 bytes each. WIDE: its workgroup's groups take the chunks by their number modulo the
 // number of groups, each with a running maximum, and the groups' sums are added in order; else one group takes all its
 // chunks and a workgroup has as many rows. Either way the order goes by the chunks' numbers alone.
-template <class T, int D, bool WIDE>
+// EXT: calls of trees or with shared chunks.
+template <class T, int D, bool WIDE, bool EXT>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int TD = D / 4, GROUPS = 256 / TD, STEP = WIDE ? GROUPS : 1;
   __shared__ __attribute__((aligned(16))) float part[WIDE ? GROUPS : 1][D];
@@ -28,17 +29,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   if (i >= sr.n) return;
   // The slots of the workgroup that had this row, as it counted them.
   const int tile = (i * a.group + head % a.group) / a.packed, p0 = tile * a.packed, np = sr.n * a.group;
-  const int lo = a.tree ? 0 : p0 / a.group, hi = a.tree ? sr.n - 1 : (min(p0 + a.packed, np) - 1) / a.group;
+  const bool tree = EXT && a.tree, share = EXT && a.share > 0;
+  const int lo = tree ? 0 : p0 / a.group, hi = tree ? sr.n - 1 : (min(p0 + a.packed, np) - 1) / a.group;
   const Seen sn = seen_tokens(sr.pos0 + lo, sr.pos0 + hi, sr.end, a.window, a.sinks);
-  const int chunk = a.share > 0 ? 64 * gp(a.meta)[0] : a.chunk;
+  const int chunk = share ? 64 * gp(a.meta)[0] : a.chunk;
   const int sc = (sn.s_end + chunk - 1) / chunk, wc = max(sn.w_begin / chunk, sc);
-  const int used = sc + max((int)(((int64_t)sn.end + chunk - 1) / chunk) - wc, 0);
+  const int used = sc + max((EXT ? (int)(((int64_t)sn.end + chunk - 1) / chunk) : (sn.end + chunk - 1) / chunk) - wc, 0);
   const int64_t row = (int64_t)(sr.r0 + i) * a.heads + head;
   // Where the row's partial sums begin and how far those of the next chunk are.
-  const int64_t rows = a.share > 0 ? (int64_t)a.tiles * a.kv_heads * 128 : (int64_t)a.rows * a.heads;
-  const int packed = i * a.group + head % a.group;
-  const int64_t first = a.share > 0 ? ((int64_t)gp(a.meta)[1 + s] * a.tiles * a.kv_heads + (int64_t)tile * a.kv_heads + head / a.group) * 128 + packed % 128
-                                    : row;
+  const int64_t rows = share ? (int64_t)a.tiles * a.kv_heads * 128 : (int64_t)a.rows * a.heads;
+  int64_t first = row;
+  if (share)
+    first = ((int64_t)gp(a.meta)[1 + s] * a.tiles * a.kv_heads + (int64_t)tile * a.kv_heads + head / a.group) * 128 +
+            (i * a.group + head % a.group) % 128;
   ss_f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float m = kNegInf, l = 0.f;
   auto add = [&](const ss_f32x4& x, float mk, float lk) {
@@ -88,20 +91,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // More than 16 chunks are joined by a workgroup a row: one row and 32 heads over 12,000 tokens 12.3 us a call with it, 18.9
 // without, over 51,000 24.4 and 39.8. Up to 16, where a batch brings the rows, by a group of threads a row: 32 sequences of 4
 // rows and 32 heads 186 us a call, 191 with a workgroup each.
-template <class T, int D>
+template <class T, int D, bool EXT>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
   constexpr int GROUPS = 256 / (D / 4);
   if ((a.share > 0 ? a.slots / a.seqs : a.slots) > 16)
-    hipLaunchKernelGGL((attn_join_kernel<T, D, true>), dim3((unsigned)all), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_join_kernel<T, D, true, EXT>), dim3((unsigned)all), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_join_kernel<T, D, false>), dim3((unsigned)((all + GROUPS - 1) / GROUPS)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_join_kernel<T, D, false, EXT>), dim3((unsigned)((all + GROUPS - 1) / GROUPS)), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
-template <class T>
+template <class T, bool EXT>
 hipError_t launch_join_of(const AttnArgs& a, int dim, hipStream_t st) {
-  return dim == 64 ? launch_join<T, 64>(a, st) : dim == 128 ? launch_join<T, 128>(a, st) : launch_join<T, 256>(a, st);
+  return dim == 64 ? launch_join<T, 64, EXT>(a, st) : dim == 128 ? launch_join<T, 128, EXT>(a, st) : launch_join<T, 256, EXT>(a, st);
 }
 
 }  // namespace
@@ -118,7 +121,8 @@ hipError_t launch_attn_few(const AttnArgs& a, int dim, bool fp16, hipStream_t st
 }
 
 hipError_t launch_attn_join(const AttnArgs& a, int dim, bool fp16, hipStream_t st) {
-  return fp16 ? launch_join_of<Fp16>(a, dim, st) : launch_join_of<Bf16>(a, dim, st);
+  if (a.tree || a.share > 0) return fp16 ? launch_join_of<Fp16, true>(a, dim, st) : launch_join_of<Bf16, true>(a, dim, st);
+  return fp16 ? launch_join_of<Fp16, false>(a, dim, st) : launch_join_of<Bf16, false>(a, dim, st);
 }
 
 }  // namespace ss

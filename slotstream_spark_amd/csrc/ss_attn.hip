@@ -37,11 +37,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int used = sc + max((EXT ? (int)(((int64_t)sn.end + chunk - 1) / chunk) : (sn.end + chunk - 1) / chunk) - wc, 0);
   const int64_t row = (int64_t)(sr.r0 + i) * a.heads + head;
   // Where the row's partial sums begin and how far those of the next chunk are.
-  const int64_t rows = share ? (int64_t)a.tiles * a.kv_heads * 128 : (int64_t)a.rows * a.heads;
+  const int64_t rows = share ? (int64_t)((np + 127) / 128) * a.kv_heads * 128 : (int64_t)a.rows * a.heads;
   int64_t first = row;
   if (share)
-    first = ((int64_t)gp(a.meta)[1 + s] * a.tiles * a.kv_heads + (int64_t)tile * a.kv_heads + head / a.group) * 128 +
-            (i * a.group + head % a.group) % 128;
+    first = ((int64_t)(gp(a.meta)[1 + s] + tile) * a.kv_heads + head / a.group) * 128 + (i * a.group + head % a.group) % 128;
   ss_f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float m = kNegInf, l = 0.f;
   auto add = [&](const ss_f32x4& x, float mk, float lk) {
@@ -95,7 +94,7 @@ template <class T, int D, bool EXT>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
   constexpr int GROUPS = 256 / (D / 4);
-  if ((a.share > 0 ? a.slots / a.seqs : a.slots) > 16)
+  if ((a.share > 0 ? a.slots / ((int64_t)a.seqs * a.tiles) : a.slots) > 16)  // of shared chunks as many as a row has if all are alike
     hipLaunchKernelGGL((attn_join_kernel<T, D, true, EXT>), dim3((unsigned)all), dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL((attn_join_kernel<T, D, false, EXT>), dim3((unsigned)((all + GROUPS - 1) / GROUPS)), dim3(256), 0, st, a);

@@ -34,8 +34,8 @@ struct AttnArgs {
   float scale; // of the scores, times log2(e)
   const uint8_t* scales;  // [n_pages][kv_heads][2][page] exponents of e4m3 keys and values (k, v then hold bytes), or null
   const uint64_t* tree;   // [rows] which of its sequence's rows a row sees, or null (causal)
-  // Shared chunks (many rows over e4m3 pages or of trees): `share` > 0 chunks for all sequences together, one size for all, by their
-  // lengths; `slots` then counts them over all sequences, po and pml are [slots][tiles][kv_heads][128 packed rows], and
+  // Shared chunks (many rows over e4m3 pages or of trees): `share` > 0 of them for the row tiles of all sequences together, of one size,
+  // by how many tiles and tokens each has; `slots` then counts them over all, po and pml are [slots][kv_heads][128 packed rows], and
   int share;
   int32_t* meta;  // [1 + seqs] has the size in units of 64 tokens and each sequence's first chunk, for the join
 };
@@ -137,46 +137,95 @@ SS_DEV Seen seen_tokens(int pos_a, int pos_b, int end, int window, int sinks) {
 }
 
 // ---------------------------------------------------------------- shared chunks
-// Chunk g of a call whose sequences share `a.share` chunks: units of 64 tokens, `size` of them a chunk, the least size (of two or
-// more) with which whole chunks number at most a.share; every sequence's last one may be short, so there are up to seqs more. A
-// wave works it out from all lengths. With `write` (one wave of the launch) the sequences' first chunks go to a.meta.
+// Chunk g of a call whose row tiles share at most `a.share` chunks: units of 64 tokens, `size` of them a chunk, two or more. (More than
+// the CUs have places for would wait for the first to end: with 150 in the place of 126 sixteen trees of up to 26 rows took 96 us, not 65.) A
+// sequence's chunks go by their place, the tiles of one place side by side. A wave works it out from all lengths. With `write` (one
+// wave of the launch) the sequences' first chunks go to a.meta.
+//
+// A chunk has `per` workgroups (key heads, parts of the dimensions). Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of
+// neighbours, so that the row tiles that read one chunk of the cache do so through one L2.
 struct Share {
-  int s, slot, size;  // the sequence, the chunk among its own; s < 0: there is no chunk g
+  int s, tile, slot, size;  // the sequence, the row tile, the chunk of its tokens; s < 0: nothing for this workgroup
+  int g, part;              // the chunk, the workgroup's number in it
 };
-SS_DEV Share find_share(const AttnArgs& a, int g, bool write) {
+SS_DEV Share find_share(const AttnArgs& a, int block, int per, bool write) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)a.width << a.page_shift;
-  auto units = [&](int s) {
-    if (s >= a.seqs || gp(a.cu)[s + 1] <= gp(a.cu)[s]) return 0u;
-    const int len = max(gp(a.kv_len)[s], 0);
-    return (uint32_t)(((int64_t)len < cap ? len : cap) + 63) / 64;
+  struct Size {
+    uint32_t units, tiles;
   };
-  const uint32_t first = units(lane);
+  auto size_of = [&](int s) {
+    Size r = {0, 0};
+    if (s >= a.seqs) return r;
+    const int from = gp(a.cu)[s], to = gp(a.cu)[s + 1], len = max(gp(a.kv_len)[s], 0);
+    const int n = min(min(to, a.rows) - min(max(from, 0), a.rows), a.max_rows);  // as seq_rows cuts them
+    if (n <= 0) return r;
+    r.units = (uint32_t)(((int64_t)len < cap ? len : cap) + 63) / 64;
+    r.tiles = (uint32_t)(n * a.group + 127) / 128;
+    return r;
+  };
+  auto sum = [](uint32_t x) {  // over the lanes; in a scalar register, as all that follows from it
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)ss_butterfly(x, [](uint32_t p, uint32_t q) { return p + q; }));
+  };
+  const Size first = size_of(lane);
   uint64_t total = 0;
-  for (int s0 = 0; s0 < a.seqs; s0 += 64)
-    total += ss_butterfly(s0 ? units(s0 + lane) : first, [](uint32_t x, uint32_t y) { return x + y; });
-  const uint32_t size = max((uint32_t)((total + a.share - 1) / a.share), 2u);
-  Share r = {-1, 0, (int)size};
+  uint32_t tiles = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    const Size z = s0 ? size_of(s0 + lane) : first;
+    total += sum(z.units * z.tiles);
+    tiles += sum(z.tiles);
+  }
+  // No size below total / share is enough, and total / (share - tiles) is, whatever the tiles' last chunks are (tiles are at most
+  // half of share). Between them the least one is looked for; of more than 64 sequences the latter is taken.
+  uint32_t size = max((uint32_t)((total + a.share - tiles - 1) / (a.share - tiles)), 2u);
+  if (a.seqs <= 64) {
+    uint32_t lo = max((uint32_t)((total + a.share - 1) / a.share), 2u);
+    while (lo < size) {
+      const uint32_t mid = (lo + size) / 2;
+      if (sum((first.units + mid - 1) / mid * first.tiles) <= (uint32_t)a.share)
+        size = mid;
+      else
+        lo = mid + 1;
+    }
+  }
+  uint32_t chunks = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    const Size z = s0 ? size_of(s0 + lane) : first;
+    chunks += sum((z.units + size - 1) / size * z.tiles);
+  }
+  const int all = (int)chunks * per, run = (all + 7) / 8, id = block % 8 * run + block / 8;
+  Share r = {-1, 0, 0, (int)size, -1, 0};
+  if (block / 8 < run && id < all) {
+    r.g = id / per;
+    r.part = id - r.g * per;
+  }
+  const int g = r.g;
+  if (g < 0 && !write) return r;
   int before = 0;
   for (int s0 = 0; s0 < a.seqs && (write || r.s < 0); s0 += 64) {
-    const int mine = (int)(((s0 ? units(s0 + lane) : first) + size - 1) / size);
+    const Size z = s0 ? size_of(s0 + lane) : first;
+    const int mine = (int)((z.units + size - 1) / size * z.tiles);
     int upto = mine;
     for (int d = 1; d < min(a.seqs, 64); d *= 2) {
       const int o = __shfl_up(upto, d);
       upto += lane >= d ? o : 0;
     }
     if (write && s0 + lane < a.seqs) a.meta[1 + s0 + lane] = before + upto - mine;
-    const uint64_t hit = __ballot(before + upto > g);
+    const uint64_t hit = g < 0 ? 0 : __ballot(before + upto > g);
     if (r.s < 0 && hit) {
       const int l = __builtin_ctzll(hit);  // past the last sequence `upto` may be short: only a lane of one can be hit
       r.s = s0 + l;
-      r.slot = g - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+      const int local = g - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+      const int tiles = __builtin_amdgcn_readlane((int)z.tiles, l);
+      r.slot = local / tiles;
+      r.tile = local - r.slot * tiles;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   if (write && lane == 0) a.meta[0] = (int)size;
   r.s = __builtin_amdgcn_readfirstlane(r.s);
   r.slot = __builtin_amdgcn_readfirstlane(r.slot);
+  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
   r.size = __builtin_amdgcn_readfirstlane(r.size);
   return r;
 }

@@ -55,6 +55,12 @@ SS_DEV void dma4(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(
 template <int OFF>  // bytes added to both addresses
 SS_DEV void dma16(const void* src, void* lds) { __builtin_amdgcn_global_load_lds(src, (lds_void*)lds, 16, OFF, 0); }
 
+// The same from a place that all lanes have and a lane's own offset.
+template <int OFF>
+SS_DEV void dma16_at(const void* src, uint32_t off, void* lds) {
+  __builtin_amdgcn_global_load_lds((const SS_G void*)((const SS_G char*)src + off), (lds_void*)lds, 16, OFF, 0);
+}
+
 // A barrier over LDS alone: it waits for no load or store in flight.
 SS_DEV void local_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -68,6 +74,13 @@ SS_DEV void wait_loads() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
   asm volatile("" ::: "memory");
+}
+
+// This lane's number, worked out anew: what a kernel derives from it then takes no register up to there.
+SS_DEV int fresh_lane() {
+  uint32_t none = 0;
+  asm volatile("" : "+v"(none));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
 }
 
 // Where the 16-byte piece p of a key row lies: at p ^ key_swizzle(row). The 16 rows of an operand read differ in bits 0, 1, 3
@@ -93,7 +106,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   constexpr int LI = SLOT / 1024;                            // load instructions of a slot
   // Column tiles whose scores are worked out at once: of four of e4m3, or two of 256 dimensions, the scores would take the registers
   // that there are, so the keys are read (and widened) once for each half.
-  constexpr int NB = E8 && (NT == 4 || (D == 256 && NT == 2)) ? NT / 2 : NT;
+  constexpr int NB = E8 && (NT == 4 || (TREE && D == 256 && NT == 2)) ? NT / 2 : NT;
   constexpr int RK = 64 / KC;                                // key rows of one (of values 16: a row is 64 bytes)
   constexpr int JH = 2, JD = D / JH;  // the waves' sums are joined in two halves of the dimensions, one where the keys were
   // Keys and queries in dynamic LDS: where all of it is static and leaves room for one workgroup a CU, the compiler takes 512
@@ -226,16 +239,31 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   // of G keys lie as close in a page as in the slot, so one address serves them with a constant added to both.
   constexpr auto swizzle = [](int row) { return E8 ? key_swizzle8<D>(row) : key_swizzle<D>(row); };
   const uint32_t koff = (lane / KC) * KROW + 16 * ((lane % KC) ^ swizzle(lane / KC));
-  const int vpiece = (lane & 3) ^ ((lane >> 4) & 3);
+  const int vpiece0 = (lane & 3) ^ ((lane >> 4) & 3);
   auto load_k = [&](int tt) {
     const int4 ids = *reinterpret_cast<const int4*>(&page_of[4 * tt]);
     const int id[4] = {ids.x, ids.y, ids.z, ids.w};
+    uint32_t ko = koff;
+    if constexpr (E8) {
+      const int ln = fresh_lane();
+      ko = (ln / KC) * KROW + 16 * ((ln % KC) ^ swizzle(ln / KC));
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t at = __builtin_amdgcn_readfirstlane(max(id[j], 0));
       const uint32_t tok = (t_begin + TT * tt + G * j) & (page - 1);
       const char* from = kbase + ((uint64_t)at * page_bytes + tok * KROW);
       uint8_t* to = kl + G * KROW * j;
+      if constexpr (E8) {
+        // The places go by one register (kept for every row group they would take 16).
+        dma16_at<0>(from, ko ^ (16 * swizzle(G * j)), to);
+        if constexpr (LI >= 8) dma16_at<1024>(from, ko ^ (16 * swizzle(G * j + RK)), to);
+        if constexpr (LI >= 16) {
+          dma16_at<2048>(from, ko ^ (16 * swizzle(G * j + 2 * RK)), to);
+          dma16_at<3 * 1024>(from, ko ^ (16 * swizzle(G * j + 3 * RK)), to);
+        }
+        continue;
+      }
       dma16<0>(from + (koff ^ (16 * swizzle(G * j))), to);
       if constexpr (LI >= 8) dma16<1024>(from + (koff ^ (16 * swizzle(G * j + RK))), to);
       if constexpr (LI >= 16) {
@@ -244,14 +272,15 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       }
     }
     if constexpr (E8) {  // the exponents of 4 tokens a lane, keys' and values' (the upper 32 lanes do the same again)
-      const int q = lane & 15, id = page_of[4 * tt + q / 4];
-      const int64_t at = ((int64_t)max(id, 0) * a.kv_heads + h) * 2 + ((lane >> 4) & 1);
+      const int ln = fresh_lane(), q = ln & 15, id = page_of[4 * tt + q / 4];
+      const int64_t at = ((int64_t)max(id, 0) * a.kv_heads + h) * 2 + ((ln >> 4) & 1);
       dma4(a.scales + at * page + ((t_begin + TT * tt + 4 * q) & (page - 1)), exp_slot[w]);
     }
   };
   auto load_v = [&](int tt) {
+    const int ln = E8 ? fresh_lane() : lane, vpiece = E8 ? (ln & 3) ^ ((ln >> 4) & 3) : vpiece0;
     const int id = page_of[4 * tt + vpiece], tok = (t_begin + TT * tt + G * vpiece) & (page - 1);
-    const char* at = vbase + ((uint64_t)(uint32_t)max(id, 0) * page_bytes + ((lane >> 2) * page + tok) * EB);
+    const char* at = vbase + ((uint64_t)(uint32_t)max(id, 0) * page_bytes + ((ln >> 2) * page + tok) * EB);
     const int64_t step = 16 * EB * page;
 #pragma unroll
     for (int n = 0; n < LI; n += 4) {
@@ -271,9 +300,11 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     return *reinterpret_cast<const ss_u32x4*>(vl + (16 * d + c) * 64 + 16 * (g ^ ((c >> 2) & 3)));
   };
   // Row m of the score tile t of unit u is token 16 (m / 4) + 8 u + 4 t + m % 4 of e4m3, so that a lane ends with tokens G g + 8 u + 4 t + 0..3.
-  auto kread8 = [&](int u, int t, int kp) {
-    const int row = 16 * (c >> 2) + 8 * u + 4 * t + (c & 3);
-    return *reinterpret_cast<const ss_u32x4*>(kl + row * KROW + 16 * ((4 * kp + g) ^ swizzle(row)));
+  // The swizzle is that of the row with u = t = 0, so all places are one (kat0) by exclusive or and a constant.
+  const int krow0 = 16 * (c >> 2) + (c & 3);
+  const uint32_t kat0 = krow0 * KROW + 16 * (g ^ swizzle(krow0));
+  auto kread8 = [&](uint32_t kat, int u, int t, int kp) {
+    return *reinterpret_cast<const ss_u32x4*>(kl + (kat ^ (64 * kp)) + (8 * u + 4 * t) * KROW);
   };
   bool any_odd = false;
   // The loop's first turn has no tile yet and only loads. A wave issues an instruction in some 5 cycles, so short calls go by
@@ -297,6 +328,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       if constexpr (E8) {
         const ss_u32x4 kexp = *reinterpret_cast<const ss_u32x4*>(&exp_slot[w][16 * (c >> 2)]);
         float by[4];
+        uint32_t kat = kat0;
+        asm volatile("" : "+v"(kat));
 #pragma unroll
         for (int t = 0; t < 4; ++t) by[t] = scale_of((kexp[t] >> (8 * (c & 3))) & 0xFFu);
 #pragma unroll
@@ -304,7 +337,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
           if constexpr (NT * D >= 256) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            const ss_u32x4 k8 = kread8(t / 2, t % 2, kp);
+            const ss_u32x4 k8 = kread8(kat, t / 2, t % 2, kp);
             const ss_u32x4 k0 = widen8(k8[0], k8[1], by[t]), k1 = widen8(k8[2], k8[3], by[t]);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
@@ -462,6 +495,9 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
   }
   wait_loads<0>();  // no load into LDS outlives the tiles (without tiles the queries are on their way)
 
+  const int lane_was = lane;
+  {
+  const int lane = E8 ? fresh_lane() : lane_was, c = lane & 15, g = lane >> 4, tid = 64 * w + lane;
   // The waves' sums, weighted by how far each wave's maximum is below the largest.
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -487,6 +523,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
       f[k] = mk == kNegInf ? 1.f : __builtin_amdgcn_exp2f(mk - big);
       sum += jl[WS * k + tid] * f[k];
     }
+    uint32_t group = a.group;
+    if constexpr (E8) asm volatile("" : "+s"(group));  // else the reciprocal of the queries' division is kept over the tiles
     const int p = p0 + tid, i = p / group;
     int64_t at = (int64_t)(sr.r0 + i) * a.heads + h * a.group + (p - i * a.group);
     if (a.slots > 1) {
@@ -572,6 +610,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
         *reinterpret_cast<uint2*>(a.out + at) = word;
       }
     }
+  }
   }
 }
 

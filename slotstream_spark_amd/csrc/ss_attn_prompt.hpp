@@ -90,29 +90,32 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
   int b = blockIdx.x;
-  const int dv = b % (D / DV) * DV;  // first output dimension
+  int dv = b % (D / DV) * DV;  // first output dimension
   b /= D / DV;
-  const int kh = b % a.kv_heads;
+  int kh = b % a.kv_heads;
   b /= a.kv_heads;
   int slot = b % a.slots;
   b /= a.slots;
   constexpr bool SHARE = E8 || TREE;
   const bool share = SHARE && a.share > 0;
-  int s, turn, chunk = a.chunk;
-  const int piece = slot;  // where its sums go
+  int s, tile, chunk = a.chunk;
+  int piece = 0;  // where its sums go
   if (share) {
-    const Share sh = find_share(a, slot, blockIdx.x == 0 && w == 0);
+    const Share sh = find_share(a, blockIdx.x, a.kv_heads * (D / DV), blockIdx.x == 0 && w == 0);
     if (sh.s < 0) return;  // whole workgroup, before any barrier
-    turn = b;
+    piece = sh.g;
+    kh = sh.part / (D / DV);
+    dv = sh.part % (D / DV) * DV;
     s = sh.s;
+    tile = sh.tile;
     slot = sh.slot;
     chunk = 64 * sh.size;
   } else {
     s = b % a.seqs;
-    turn = b / a.seqs;
+    // The tiles that see most first; the last `a.rising` turns, which share CUs with the first ones, from the other end.
+    const int turn = b / a.seqs;
+    tile = turn < a.tiles - a.rising ? a.tiles - 1 - turn : turn - (a.tiles - a.rising);
   }
-  // The tiles that see most first; the last `a.rising` turns, which share CUs with the first ones, from the other end.
-  const int tile = turn < a.tiles - a.rising ? a.tiles - 1 - turn : turn - (a.tiles - a.rising);
   const int page = 1 << a.page_shift;
   SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, (int64_t)a.width * page, a.err);
   sr.r0 = __builtin_amdgcn_readfirstlane(sr.r0);
@@ -576,7 +579,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const bool ine = SHARE ? pe < np : in;
   l += other_half(l, he);
   const int64_t at = (int64_t)(sr.r0 + ie) * a.heads + kh * a.group + (pe - ie * a.group);
-  const int64_t pa = share ? (((int64_t)piece * a.tiles + tile) * a.kv_heads + kh) * 128 + (pe - p0)
+  const int64_t pa = share ? ((int64_t)piece * a.kv_heads + kh) * 128 + (pe - p0)
                            : (int64_t)slot * a.rows * a.heads + at;
   if (ine && a.slots > 1) {
 #pragma unroll
@@ -654,7 +657,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
 // Tiles of 64 tokens where a page holds them, else of 32 (and of 256 dimensions always: registers).
 template <class T, int D, int DV, bool E8, bool TREE>
 void launch_prompt(const AttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.slots * a.tiles * a.kv_heads * (a.share > 0 ? 1 : a.seqs) * attn_prompt_parts(D, a.page_shift)));
+  const int64_t units = (int64_t)a.slots * a.kv_heads * attn_prompt_parts(D, a.page_shift);
+  const dim3 grid((unsigned)(a.share > 0 ? (units + 7) / 8 * 8 : units * a.tiles * a.seqs));
   if (a.page_shift >= 6 && D < 256)
     hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, D < 256 ? 64 : 32, true, E8, TREE>), grid, dim3(256), 0, st, a);
   else if (a.page_shift >= 5)

@@ -273,7 +273,7 @@ constexpr int kFewRows = 8;
 // Rows of partial sums (a row and head, or a column of a workgroup's tile) of a call.
 int64_t partial_rows(const ss::AttnArgs& a) {
   if (a.slots <= 1) return 0;
-  return a.share > 0 ? (int64_t)a.slots * a.tiles * a.kv_heads * 128 : (int64_t)a.slots * a.rows * a.heads;
+  return a.share > 0 ? (int64_t)a.slots * a.kv_heads * 128 : (int64_t)a.slots * a.rows * a.heads;
 }
 int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss::AttnArgs* out, int64_t* ws, bool* prompt) {
   if (!p) return fail(SSMOE_EINVAL, "args must be non-null");
@@ -329,13 +329,14 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
     slots = std::min(slots, (std::min<int64_t>(a.sinks, cap) + chunk - 1) / chunk +
                                 (a.window + std::max(max_rows, kFewRows) + chunk - 2) / chunk + 1);
   if (*prompt && chunk >= seen) slots = 1;
-  // Over e4m3 pages and for trees the chunks are shared by the sequences' own lengths, which the kernel reads: as many for all
-  // together as CUs have places, so that the longest sequence does not hold up the launch.
-  if (*prompt && (e4m3 || tree) && a.window >= (1 << 30) && cap > 128) {
-    const int64_t want = 512 / std::max<int64_t>((int64_t)p->kv_heads * a.tiles * parts_of_dim, 1);
-    if (want >= 2 * std::max(p->seqs, 1)) {
+  // Over e4m3 pages and for trees the chunks are shared by the sequences' own rows and lengths, which the kernel reads: as many for all
+  // together as CUs have places, so that the longest sequence does not hold up the launch, nor places stay empty for row tiles that
+  // a sequence of fewer rows has not.
+  if (*prompt && (e4m3 || tree) && a.window >= (1 << 30) && cap > 128 && cap <= (1 << 29)) {  // sums of units in 32 bits
+    const int64_t want = 512 / std::max<int64_t>(p->kv_heads * parts_of_dim, 1), row_tiles = (int64_t)std::max(p->seqs, 1) * a.tiles;
+    if (want >= 2 * row_tiles) {
       a.share = (int)want;
-      slots = std::min<int64_t>(want + p->seqs, (int64_t)p->seqs * ((cap + 127) / 128));
+      slots = std::min<int64_t>(want, row_tiles * ((cap + 127) / 128));
     }
   }
   // Two workgroups fit a CU: of at most 512, the second 256 go to the CUs of the first, the lightest to the heaviest.

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from slotstream_spark_amd import _lib
+from slotstream_spark_amd.kernels.kv_pages import move_pages
 from slotstream_spark_amd.kernels.paged_attention import paged_attention
 from slotstream_spark_amd.kernels.rope import rope_append
 from tests.paged_util import Batch, attention64, attention_bound, rope64
@@ -238,6 +239,29 @@ def test_append_values_at_the_edges():
         qkv[6, 6:] = math.nan
         qkv[7, 4:, :] = 1.875
     check_append([9], [20], 4, 2, 64, 16, 16, seed=4, big=big)
+
+
+@pytest.mark.parametrize("kv_heads,dim,page", [(1, 64, 16), (3, 64, 16), (2, 128, 64), (1, 256, 256)])
+def test_pages_move_with_their_scales(kv_heads, dim, page):
+    """Pages of one KB and of an odd number of them, ids outside the cache, a table that follows."""
+    g = torch.Generator().manual_seed(dim)
+    n, layers = 23, 3
+    k, v, sc = (torch.randint(0, 256, s, generator=g, dtype=torch.uint8) for s in (
+        (layers, n, kv_heads, page, dim), (layers, n, kv_heads, dim, page), (layers, n, kv_heads, 2, page)))
+    perm = torch.randperm(n, generator=g)
+    src, dst = perm[:9].to(torch.int32), perm[9:18].to(torch.int32)
+    table = torch.randint(-1, n, (5, 40), generator=g).to(torch.int32)
+    dk, dv, ds, dt = k.cuda().view(E4M3), v.cuda().view(E4M3), sc.cuda(), table.cuda()
+    move_pages(dk, dv, src.cuda(), dst.cuda(), dt, scales=ds)
+    to = {int(a): int(b) for a, b in zip(src, dst)}
+    for t, d in ((k, dk.view(torch.uint8)), (v, dv.view(torch.uint8)), (sc, ds)):
+        t[:, dst.long()] = t[:, src.long()].clone()
+        assert torch.equal(t, d.cpu())
+    assert torch.equal(dt.cpu(), torch.tensor([[to.get(p, p) for p in row] for row in table.tolist()], dtype=torch.int32))
+    assert _lib.device_error() == 0
+    move_pages(dk, dv, torch.tensor([n, 1], dtype=torch.int32).cuda(), torch.tensor([0, -1], dtype=torch.int32).cuda(), scales=ds)
+    assert _lib.device_error() == 32
+    assert torch.equal(sc, ds.cpu()) and torch.equal(k, dk.view(torch.uint8).cpu())
 
 
 def test_written_rows_are_read_back():

@@ -8,7 +8,7 @@ import torch
 from slotstream_spark_amd import _lib
 from slotstream_spark_amd.kernels.paged_attention import paged_attention
 from slotstream_spark_amd.kernels.tree import accept_tree, keep_rows, tree_masks
-from tests.paged_util import Batch
+from tests.paged_util import Batch, attention64, attention_bound
 from tests.tree_util import Batch8, accept64, as_int64, masks_of, random_parents, tree64, tree_bound
 
 pytestmark = pytest.mark.gpu
@@ -105,6 +105,39 @@ def test_long_cache_in_many_chunks(kind):
     check(b, trees(b), window=3000, sinks=70)
     b = make(kind, [8, 3], [9001, 5000], 8, 2, 128, 64, seed=6, width=400)
     check(b, trees(b))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("seqs", [3, 64, 65, 130])
+def test_many_sequences_share_the_chunks(kind, seqs):
+    """Rows and lengths of every size, none among them: the chunks are shared by all sequences' own."""
+    g = torch.Generator().manual_seed(seqs)
+    rows = [int(torch.randint(0, 21, (1,), generator=g)) for _ in range(seqs)]
+    rows[1] = 20
+    lens = [int(torch.randint(0, 700, (1,), generator=g)) if i % 5 else i % 40 for i in range(seqs)]
+    b = make(kind, rows, lens, 2, 1, 64, 16, seed=seqs)
+    check(b, trees(b))
+    if kind == "e4m3":                                            # and those of causal rows
+        out = paged_attention(*b.args(), scales=b.scales.cuda())
+        want, _ = attention64(b)
+        assert ((out.double().cpu() - want).abs() <= attention_bound(b)).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_shared_chunks_in_a_graph_follow_the_lengths(kind):
+    b = make(kind, [30, 12, 9], [2000, 900, 640], 8, 1, 64, 16, seed=12)
+    q, k, v, cu, kv_len, table, most = b.args()
+    sc = b.scales.cuda() if kind == "e4m3" else None
+    tree, out = as_int64(trees(b)).cuda(), torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        paged_attention(q, k, v, cu, kv_len, table, most, scales=sc, tree=tree, out=out)
+    for lens in ([2000, 900, 640], [30, 900, 9], [0, 0, 0], [2000, 12, 640]):
+        kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(9)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, paged_attention(q, k, v, cu, kv_len, table, most, scales=sc, tree=tree))
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])

@@ -611,7 +611,8 @@ int ssmoe_rope_append_e4m3(const ssmoe_rope_append_args* a, uint8_t* scales, voi
 /* ssmoe_paged_attention over e4m3 pages (scales non-null) and for rows of trees (tree non-null).
  * tree uint64 [rows]: row i sees the tokens before its sequence's rows and of those rows the ones whose bits are set in its word (bit
  * j: the sequence's row j; its own bit as any other); bits of rows that the sequence has not are not looked at. max_rows at most 64.
- * Under a window the row's position is that of as many rows behind the cache as it sees; the window must be at least max_rows.
+ * Under a window the row's position is that of as many rows behind the cache as it sees, one at least; the window must be at least
+ * max_rows.
  * Scores, sums and partial results are fp32; a probability is rounded once, with its token's power of two, before its product. */
 int64_t ssmoe_paged_attention_ext_workspace_bytes(const ssmoe_paged_attention_args* a, int e4m3, int tree); /* -1: refused */
 int ssmoe_paged_attention_ext(const ssmoe_paged_attention_args* a, const uint8_t* scales, const uint64_t* tree, void* stream);

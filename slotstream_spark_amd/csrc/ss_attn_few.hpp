@@ -179,10 +179,10 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     const int p = p0 + 16 * n + c, i = p / group;
     const bool in = p < np;
     if constexpr (TREE) {
-      if (w == 0 && g == 0) {  // a row's position: as many rows behind the cache as it sees
+      if (w == 0 && g == 0) {  // a row's position: as many rows behind the cache as it sees, one at least
         const uint64_t mine = in ? gp(a.tree)[sr.r0 + i] & (~0ull >> (64 - sr.n)) : 0;
         qmask[16 * n + c] = mine;
-        qpos[16 * n + c] = in ? sr.pos0 + __builtin_popcountll(mine) - 1 : -1;
+        qpos[16 * n + c] = in ? sr.pos0 + max(__builtin_popcountll(mine), 1) - 1 : -1;
       }
     } else {
       if (w == 0) qpos[16 * n + c] = in ? sr.pos0 + i : -1;

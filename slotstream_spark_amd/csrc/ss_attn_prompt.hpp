@@ -143,12 +143,12 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   // This lane's column.
   const int p = p0 + 32 * w + c, i = p / a.group;
   const bool in = p < np;
-  // Of a tree, a row's position is as many rows behind the cache as it sees.
+  // Of a tree, a row's position is as many rows behind the cache as it sees, one at least.
   const int qpos = in ? sr.pos0 + i : -1;
   if constexpr (TREE) {
     const uint64_t mine = in ? gp(a.tree)[sr.r0 + i] & (~0ull >> (64 - sr.n)) : 0;
     tree_mask[32 * w + c] = mine;
-    tree_pos[32 * w + c] = sr.pos0 + __builtin_popcountll(mine) - 1;
+    tree_pos[32 * w + c] = sr.pos0 + max(__builtin_popcountll(mine), 1) - 1;
   }
   auto bits_of = [&](int first) {  // of the tokens first .. first + 7 those that this lane's row sees
     const int col = TREE ? 32 * w + c : 0;

@@ -304,6 +304,14 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
   a.scale = p->scale * 1.44269504088896340736f;
   if ((int64_t)max_rows * a.group > (1 << 30)) return fail(SSMOE_EINVAL, "max_rows * heads / kv_heads must be at most 2^30");
   *prompt = p->max_rows > kFewRows;
+  // Over e4m3 pages and for trees the few-row kernel has more rows where their packed rows are few. A call in us, few against many rows,
+  // over 200 / 777 / 3,000 / 20,000 tokens: 8 trees of 20 packed rows (8 heads on 8, 128 dimensions) 9 / 15 / 26 / 130 against 16 / 21 /
+  // 31 / 131, over e4m3 9 / 15 / 20 / 79 against 16 / 21 / 30 / 109; of 64 14 / 23 / 32 / 172 against 18 / 24 / 35 / 133, of 256
+  // dimensions 14 / 32 / 51 / 265 against 19 / 26 / 40 / 153; of 128 (16 rows of 32 heads on 4) 13 / 31 / 40 / - against 18 / 26 / 34 / -.
+  if (e4m3 || tree) {
+    const int64_t packed = (int64_t)max_rows * a.group;
+    if (packed <= 32 || (packed <= 64 && p->dim < 256 && cap <= 4096) || (packed <= 128 && cap <= 512)) *prompt = false;
+  }
   a.packed = *prompt ? 128 : ss::attn_few_packed(p->dim, max_rows * a.group, e4m3);
   a.tiles = (max_rows * a.group + a.packed - 1) / a.packed;
   // tokens of a sequence that the call may read

@@ -194,8 +194,9 @@ class MoEStack:
         """A greedy round over a tree: tokens[0] is the pending token, tokens[i] a draft behind row parents[i] < i (parents[0] is not
         looked at), at most 64 rows, and with prompt_chunk at most so many. All rows go through the stack in one pass, each seeing the
         sequence, its ancestors and itself; the branch that the stack's choices follow stays, moved up in the cache, and the position
-        advances by its rows. -> (the round, the final stream rows of the kept rows [n_accept + 1, H]). A row's choice may differ from
-        step()'s as far as another order of sums rounds another way."""
+        advances by its rows. -> (the round, the final stream rows of the kept rows [n_accept + 1, H]). Sums go in another order than
+        step()'s, so a row's stream may differ by roundings from that of a one-token step, and where a router's or the lm_head's choice is that
+        near, so does the choice."""
         n = len(tokens)
         if not 1 <= n <= TREE_ROWS or len(parents) != n:
             raise ValueError(f"a tree has 1 to {TREE_ROWS} rows and a parent for each, got {n} and {len(parents)}")
@@ -233,7 +234,7 @@ def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eo
     """Greedy decode after `prompt` by rounds over trees -> (tokens, nan, round_seconds, stats), as mtp_decode's.
     tree_fn(pending, room, n_out) -> (drafts, parents): up to `room` drafts, each behind row parents[i] (0 the pending token, j + 1 draft
     j). Where none fit, or it gives none, a round is the pending token alone. The drafts decide how many tokens a round emits, not
-    which (but for choices that another order of sums rounds another way). As after mtp_decode the stack's sequence is the prompt and
+    which (but for a router's or the lm_head's choices that another order of sums rounds another way). As after mtp_decode the stack's sequence is the prompt and
     what was emitted but for the last token."""
     out, step_s, nan = [], [], False
     st = {"rounds": 0, "drafted": 0, "accepted": 0, "emitted_by_round": [], "verify_rows": 0}

@@ -133,7 +133,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cu_rows[-1] are left as they were in `out` and `lse`, which must not overlap each other nor anything that the call reads.
     `scales`: the pages are of e4m3 numbers. `tree`: row i sees the tokens before its sequence's rows and the rows j of it with bit j
     of tree[i] (tree_masks' words: itself and its ancestors), at most 64 rows a sequence; its position under a window, which must be
-    at least max_rows, is that of as many rows as it sees. A tree's rows have no bits of their own: the order of its sums goes by where
+    at least max_rows, is that of as many rows as it sees, one at least. A tree's rows have no bits of their own: the order of its sums goes by where
     its tokens lie, so a row of a tree and the same token decoded alone agree as far as fp32 sums do.
     Capturable; workspaces come from torch's allocator at each call, so calls and captured graphs never share one."""
     max_rows, window, sinks = int(max_rows), int(window), int(sinks)

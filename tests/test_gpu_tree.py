@@ -88,6 +88,22 @@ def test_any_words(kind, rows):
     check(b, words, window=77, sinks=9)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [4, 40])
+def test_windows_that_begin_at_the_edges_of_tiles(kind, rows):
+    """The first token in sight is the last of a tile of 32 or 64, the first of the next, or beside them; rows that see none of the tree
+    among the others; pages before the window are not held, and nothing is raised for them."""
+    window = 70
+    lens = [rows + window + d for d in (30, 31, 32, 33, 62, 63, 64, 65, 66, 127, 128, 129)]
+    b = make(kind, [rows] * len(lens), lens, 4, 2, 64, 16, seed=rows)
+    words = trees(b)
+    for s in range(len(lens)):
+        words[s * rows + 2] = 0
+        first = lens[s] - rows - window + 1                      # the first token that row 0 (and a row without bits) sees
+        b.table[s, :first // 16] = -1
+    check(b, words, window=window)
+
+
 def test_a_chain_is_the_causal_rows():
     """In a chain every row sees what a causal row sees. Its values agree with the causal call's to the roundings of both."""
     for dim, rows in ((64, 5), (128, 20), (256, 8)):

@@ -87,7 +87,7 @@ def tree64(b, words, window=0, sinks=0, scale=None, absolute=False):
         k, v = b.k[ids, :, off].double(), b.v[ids, :, :, off].double()
         for i in range(n):
             word = words[r] & ((1 << n) - 1)
-            p = base + bin(word).count("1") - 1
+            p = base + max(bin(word).count("1"), 1) - 1
             see = torch.tensor([(t < base and (not window or p - t < window or t < sinks))
                                 or (t >= base and (word >> (t - base)) & 1 == 1) for t in held], dtype=torch.bool)
             if see.any():

@@ -61,13 +61,20 @@ SS_DEV float other_half(float v, bool upper) {
 
 // Where the 16-byte piece c of row r lies in LDS: at c ^ swizzle(r). A row has D / 8 pieces (keys) or TK / 8 (values), and 16
 // rows that one read touches at the same piece fall on 16 different places of the 256 bytes that the banks cover.
-template <int D>
+// E8: rows are written by lanes that have every other piece of a row, eight lanes beside each other at once, 128 bytes wide: their
+// places differ in the lowest bit between the two halves of 256 bytes (kodd for the pieces of a long row, else in the
+// swizzle). Without, a write took twice its cycles (11 % of the cycles of a prompt, most of it behind its products: 502 -> 500 us).
+template <int D, bool E8>
 SS_DEV constexpr int kswizzle(int row) {
-  return D == 64 ? (row >> 1) & 7 : row & 15;
+  return D == 64 ? ((row >> 1) & 7) ^ (E8 ? row & 1 : 0) : row & 15;
 }
-template <int TK>
+template <int TK, bool E8>
 SS_DEV constexpr int vswizzle(int row) {
-  return TK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+  return TK == 64 ? ((row >> 1) & 7) ^ (E8 ? row & 1 : 0) : ((row >> 2) & 3) ^ (E8 ? (row >> 1) & 1 : 0);
+}
+template <int D, bool E8>
+SS_DEV constexpr int kodd(int piece) {
+  return E8 && D > 64 ? (piece >> 3) & 1 : 0;
 }
 
 // D: dimensions; DV: those of the output that one workgroup has (of 256 it has half, and its scores are computed twice: the
@@ -189,8 +196,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   // the swizzle bits of those rows.
   constexpr int RK = 64 / KC, RV = 64 / VC;
   const int krow0 = w * KI * RK + lane / KC, vrow0 = w * VI * RV + lane / VC;
-  const uint32_t koff0 = (ONE ? krow0 : krow0 % 16) * KROW + 16 * ((lane % KC) ^ kswizzle<D>(krow0));
-  const int vpiece0 = (lane % VC) ^ vswizzle<TK>(vrow0);
+  const uint32_t koff0 = (ONE ? krow0 : krow0 % 16) * KROW + 16 * ((lane % KC) ^ kswizzle<D, E8>(krow0));
+  const int vpiece0 = (lane % VC) ^ vswizzle<TK, E8>(vrow0);
   const uint32_t voff0 = (uint32_t)vrow0 * page * 2 + 16 * (ONE ? vpiece0 : vpiece0 & 1);
   struct Tile {
     int t;          // its first token
@@ -216,16 +223,16 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int q = 1; q < NP; ++q) id = j == q ? r.ids[q] : id;
       const char* at = kbase + id * page_bytes + (((r.t + 16 * j) & (page - 1)) + n * RK) * KROW;
-      dma16(at + (koff0 ^ (16 * kswizzle<D>(n * RK))), kl + (w * KI + n) * 1024);
+      dma16(at + (koff0 ^ (16 * kswizzle<D, E8>(n * RK))), kl + (w * KI + n) * 1024);
     }
   };
   auto load_v = [&](const Tile& r, uint8_t* vl, int n) {
     {
       if constexpr (ONE) {
         const char* at = vbase + r.ids[0] * page_bytes + ((r.t & (page - 1)) + n * RV * page) * 2;
-        dma16(at + (voff0 ^ (16 * vswizzle<TK>(n * RV))), vl + (w * VI + n) * 1024);
+        dma16(at + (voff0 ^ (16 * vswizzle<TK, E8>(n * RV))), vl + (w * VI + n) * 1024);
       } else {
-        const int j = (vpiece0 ^ vswizzle<TK>(n * RV)) / 2;
+        const int j = (vpiece0 ^ vswizzle<TK, E8>(n * RV)) / 2;
         int id = r.ids[0];
 #pragma unroll
         for (int q = 1; q < NP; ++q) id = j == q ? r.ids[q] : id;
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int KT = 4096 / D, VT = 4096 / TK;
   const int kpiece = K8 < 256 ? tid % K8 : tid, vpiece = V8 < 256 ? tid % V8 : tid;
   const int ktok = kpiece / (D / 16), kpc = kpiece % (D / 16), vdim = vpiece / (TK / 16), vtok = 16 * (vpiece % (TK / 16));
-  const uint32_t kput = ktok * KROW + 16 * ((2 * kpc) ^ kswizzle<D>(ktok)), vput = vdim * VROW + 16 * ((vtok / 8) ^ vswizzle<TK>(vdim));
+  const uint32_t kput = ktok * KROW + 16 * ((2 * kpc) ^ kodd<D, E8>(2 * kpc) ^ kswizzle<D, E8>(ktok)), vput = vdim * VROW + 16 * ((vtok / 8) ^ vswizzle<TK, E8>(vdim));
   const uint32_t kget = ktok * D + 16 * kpc, vget = (uint32_t)vdim * page + vtok;
   auto page_at = [&](const Tile& r, int token) {
     int id = r.ids[0];
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
 
   // Where this lane reads: K row of score row c, V row of dimension c.
   const int krow = 16 * (c / 16) + 8 * ((c / 4) % 2) + 4 * ((c / 8) % 2) + c % 4;
-  const int kswz = kswizzle<D>(krow), vswz = vswizzle<TK>(c);
+  const int kswz = kswizzle<D, E8>(krow), vswz = vswizzle<TK, E8>(c);
   const uint32_t kat0 = krow * KROW + 16 * (h ^ kswz), vat0 = c * VROW + 16 * (h ^ vswz);
 
   auto sees = [&](int tok, bool held) { return held && tok <= qpos && (tok > qpos - a.window || tok < a.sinks); };
@@ -312,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int plain_a = blk_hi - a.window + 1, plain_b = (TREE ? blk_lo - 1 : blk_lo) - TK + 1;
   auto plain = [&](const Tile& r) { return r.t >= plain_a && r.t <= plain_b && r.held == kAll; };
   auto kread = [&](const uint8_t* kl, int f) {
-    return *reinterpret_cast<const ss_u32x4*>(kl + (krow + 32 * (f / KS)) * KROW + 16 * ((2 * (f % KS) + h) ^ kswz));
+    return *reinterpret_cast<const ss_u32x4*>(kl + (krow + 32 * (f / KS)) * KROW + 16 * ((2 * (f % KS) + h) ^ kodd<D, E8>(2 * (f % KS)) ^ kswz));
   };
   auto vread = [&](const uint8_t* vl, int d, int nk) {
     return *reinterpret_cast<const ss_u32x4*>(vl + (c + 32 * d) * VROW + 16 * ((2 * nk + h) ^ vswz));
@@ -402,6 +409,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   // the next tile (in kl) are worked out into y: the matrix unit has them while the exponentials take the vector unit.
   // The loads of the keys of rk (to kn) and the values of rv (to vn) go out one at a time beside the products: all at once
   // they hold up the wave for as long as the memory path takes them in.
+  // The order of the instructions is kept by pairs of products, of e4m3 by four (491 -> 484 us for a prompt; by eight 497).
   // Of e4m3 they come into registers, the keys at the start, the values later, and go into their stages beside the value products.
   auto step = [&](const Tile& r, const uint8_t* kl, uint8_t* vl, f32x16 (&x)[ST], f32x16 (&y)[ST], const Tile& rk,
                   uint8_t* kn, const Tile& rv, uint8_t* vn, const float* vb, float* vbn) {
@@ -429,6 +437,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     }
     ss_u32x4 pf[ST][2];
     float part[2] = {0.f, 0.f};
+    ss_f32x4 by;
     // The operands of a product are read AHEAD products before it, those of the first value products beside the last of
     // the scores; PER scores of x are worked on beside each product of y.
     constexpr int NK = ST * KS, PER = 16 * ST / NK, NV = DT * 2 * ST, AHEAD = 4, RING = AHEAD + 1;
@@ -440,7 +449,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
     auto fetch = [&](int f) {
       if constexpr (E8) {
         if (f < NK)
-          fr[f % RING] = *reinterpret_cast<const ss_u32x4*>(kl + (kat ^ (32 * (f % KS))) + 32 * (f / KS) * KROW);
+          fr[f % RING] = *reinterpret_cast<const ss_u32x4*>(kl + (kat ^ (16 * ((2 * (f % KS)) ^ kodd<D, E8>(2 * (f % KS))))) + 32 * (f / KS) * KROW);
         else if (f < NK + NV)
           fr[f % RING] = *reinterpret_cast<const ss_u32x4*>(vl + (vat ^ (32 * ((f - NK) % (2 * ST)))) + 32 * ((f - NK) / (2 * ST)) * VROW);
       } else if (f < NK) {
@@ -468,9 +477,9 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
           part[q / 2 % 2] += q1;  // the sum has the weights as they are, the product rounded once to the element type
           if constexpr (E8) {
             asm volatile("" : "+v"(part[q / 2 % 2]));  // summed here: put off, the additions keep every weight in a register
-            const float2 by = *reinterpret_cast<const float2*>(vb + 32 * n + 16 * (e / 8) + 8 * h + e % 8);
-            q0 *= by.x;
-            q1 *= by.y;
+            if (e % 4 == 0) by = *reinterpret_cast<const ss_f32x4*>(vb + 32 * n + 16 * (e / 8) + 8 * h + e % 8);
+            q0 *= by[e % 4];
+            q1 *= by[e % 4 + 1];
           }
           pf[n][e / 8][(e % 8) / 2] = T::pack(q0, q1);
         }
@@ -486,7 +495,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
         else if (f / EVERY < KI + VI)
           load_v(rv, vn, f / EVERY - KI);
       }
-      if (f % 2) __builtin_amdgcn_sched_barrier(0);
+      if (E8 ? f % 4 == 3 : f % 2) __builtin_amdgcn_sched_barrier(0);
     }
     l += part[0] + part[1];
     top = y[0][0];
@@ -507,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
             put_v8(next, vn, vbn, at - KN);
         }
       }
-      if (f % 2) __builtin_amdgcn_sched_barrier(0);
+      if (E8 ? f % 4 == 3 : f % 2) __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto sync = [&]() {

@@ -182,21 +182,38 @@ __global__ __launch_bounds__(1024) void tree_walk_kernel(TreeAcceptArgs a) {
   }
 }
 
-// Token base + d takes the row path[d]: paths rise, so every source lies at or behind its place, and a thread that takes its part of the
-// tokens in order, eight loads before eight stores, writes over none that it has yet to read. The parts of a key head: an element
-// of each token's values (a thread a dimension), 16 bytes of the keys, a byte of the exponents; no two share any. A workgroup works a
-// sequence's branch out once and takes parts of all layers and key heads, `rounds` of them a thread.
-// Bound by latency for one sequence (48 layers of 4 key heads 4 us), and by the lines of the values, of which an element a token is moved:
-// 32 sequences of 48 layers, 8 key heads, 128 dimensions of e4m3 and pages of 64 tokens touch 100 MB of lines, read and written, in 59 us.
+// Token base + d takes the row path[d]. Paths rise, so every source lies at or behind its place. A thread has one of three kinds of
+// parts of a layer and key head, and no two share any:
+//   a dimension of the values: 8 tokens at multiples of 8 are a piece of 8 or 16 bytes, which is read whole, gets the moved tokens'
+//     elements and is written whole (the others as they were): stores of single elements are as many requests as elements;
+//   16 bytes of the keys, or a byte of the exponents, of each token: eight loads before eight stores.
+// Either way pieces and tokens go by their order, so nothing is written over that is yet to be read. A workgroup works a sequence's
+// branch out once and takes parts of all layers and key heads; a wave's parts are of one kind.
+// Bound by latency for one sequence (48 layers of 4 key heads 4.5 us), and by the lines of the values, of which an element a token is
+// moved: 32 sequences of 48 layers, 8 key heads, 128 dimensions of e4m3 and pages of 64 tokens read 119 MB of lines and write 56 MB, of
+// 32 bytes at least each, in 51 us (stored an element at a time 57).
 template <class V, bool E8>
 __global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
+  constexpr int EV = 16 / sizeof(V), W = 2 * sizeof(V);  // elements of 16 bytes; words of 8 elements
+  constexpr int kPieces = kTreeRows / 8 + 1;
   __shared__ int64_t src[kTreeRows], dst[kTreeRows];  // page and token in it: page << 8 | token
+  // Of the values' pieces that hold the branch: element places in a dimension's pages of what their tokens take (-1: stay), the
+  // pieces' own and the bits of the tokens that move.
+  __shared__ __attribute__((aligned(16))) int64_t take[8 * kPieces], into[kPieces];
+  __shared__ uint32_t moved[kPieces][W];
   __shared__ int count;
   const int tid = threadIdx.x, page = 1 << a.page_shift;
   const int s = blockIdx.x / (uint32_t)a.blocks, block = blockIdx.x - s * a.blocks;
-  const int64_t cap = (int64_t)a.width * page;
+  const int64_t cap = (int64_t)a.width * page, one = (int64_t)a.kv_heads * page * a.dim;  // `one`: elements of a page
   const SeqRows sr = seq_rows(a.cu, a.kv_len, s, a.rows, a.max_rows, cap, a.err);
   const int32_t* took = a.took + (int64_t)s * (4 + 2 * a.max_rows);
+  const int skew = sr.pos0 & 7;  // of the first row in its piece
+  if (tid < 8 * kPieces) take[tid] = -1;
+  if (tid < kPieces) {
+    into[tid] = -1;
+    for (int i = 0; i < W; ++i) moved[tid][i] = 0;
+  }
+  __syncthreads();
   if (tid < 64) {
     const int kept = gp(took)[0] + 1;
     int at = tid < a.max_rows ? gp(took)[4 + a.max_rows + tid] : -1;
@@ -224,13 +241,43 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
         return id < 0 ? (int64_t)-1 : (int64_t)id << 8 | (t & (page - 1));
       };
       const int64_t x = at == tid ? -1 : place(sr.pos0 + at), y = at == tid ? -1 : place(sr.pos0 + tid);
-      src[tid] = x < 0 || y < 0 ? -1 : x;  // rows in their places, or without one, stay
+      const bool moves = x >= 0 && y >= 0;  // rows in their places, or without one, stay
+      src[tid] = moves ? x : -1;
       dst[tid] = y;
+      if (moves) {
+        const int j = skew + tid;
+        take[j] = (x >> 8) * one + (x & 255);
+        into[j / 8] = (y >> 8) * one + (y & 255 & ~7);  // the same of every token of the piece
+        atomicOr(&moved[j / 8][j % 8 * sizeof(V) / 4], (E8 ? 0xFFu : 0xFFFFu) << (8 * (j * sizeof(V) % 4)));
+      }
     }
   }
   __syncthreads();
-  const int n = count;
-  const int64_t one = (int64_t)a.kv_heads * page * a.dim;  // elements of a page
+  const int n = __builtin_amdgcn_readfirstlane(count), last = n > 0 ? (skew + n - 1) / 8 : -1;
+  auto values = [&](V* base) {
+    for (int b = 0; b <= last; ++b) {
+      const int64_t to = into[b];
+      if (__builtin_amdgcn_readfirstlane((int)(to >> 32)) < 0) continue;
+      uint32_t x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t from = take[8 * b + u];
+        x[u] = 0;
+        if (__builtin_amdgcn_readfirstlane((int)(from >> 32)) >= 0) x[u] = gp(base)[from];
+      }
+      typedef uint32_t Piece __attribute__((ext_vector_type(W)));
+      SS_G Piece* const at = (SS_G Piece*)(base + to);
+      Piece w = *at;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const uint32_t m = moved[b][i];
+        const uint32_t v = E8 ? x[4 * i % 8] | x[(4 * i + 1) % 8] << 8 | x[(4 * i + 2) % 8] << 16 | x[(4 * i + 3) % 8] << 24
+                              : x[2 * i % 8] | x[(2 * i + 1) % 8] << 16;
+        w[i] = (w[i] & ~m) | v;
+      }
+      *at = w;
+    }
+  };
   // `base`: the part's first element in the layer; elements of a page and of a token of its kind
   auto move = [&](auto* base, int64_t per_page, int64_t per_token) {
     typedef typename std::remove_reference<decltype(*base)>::type E;
@@ -244,19 +291,24 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
         if (d0 + u < n && src[d0 + u] >= 0) *(SS_G E*)(base + (dst[d0 + u] >> 8) * per_page + (dst[d0 + u] & 255) * per_token) = x[u];
     }
   };
-  constexpr int EV = 16 / sizeof(V);  // elements of 16 bytes
-  const int kpieces = a.dim / EV, parts = a.dim + kpieces + (E8 ? 2 : 0);
-  const int64_t all = (int64_t)parts * a.kv_heads * a.layers;
-  for (int64_t it = (int64_t)block * 256 + tid; it < all; it += (int64_t)a.blocks * 256) {
-    const int unit = (int)((uint64_t)it / (uint32_t)parts), part = (int)(it - (int64_t)unit * parts);
-    const int layer = (uint32_t)unit / (uint32_t)a.kv_heads, h = unit - layer * a.kv_heads;
-    const int64_t at = (int64_t)layer * a.n_pages * one + (int64_t)h * page * a.dim;
-    if (part < a.dim)
-      move(reinterpret_cast<V*>(a.v) + at + (int64_t)part * page, one, 1);
-    else if (part < a.dim + kpieces)
-      move(reinterpret_cast<ss_u32x4*>(reinterpret_cast<V*>(a.k) + at) + (part - a.dim), one / EV, kpieces);
-    else
-      move(a.scales + (((int64_t)layer * a.n_pages * a.kv_heads + h) * 2 + (part - a.dim - kpieces)) * page, (int64_t)a.kv_heads * 2 * page, 1);
+  // Numbers of parts fit 31 bits (the entry point's bound).
+  const uint32_t units = (uint32_t)(a.layers * a.kv_heads), nv = units * a.dim, kpieces = a.dim / EV, nk = units * kpieces;
+  const uint32_t all = nv + (nk + 63) / 64 * 64 + (E8 ? 2 * units : 0);
+  auto first = [&](uint32_t unit) {  // element of the unit's first page
+    const uint32_t layer = unit / (uint32_t)a.kv_heads, h = unit - layer * a.kv_heads;
+    return (int64_t)layer * a.n_pages * one + (int64_t)(h * (uint32_t)page) * a.dim;
+  };
+  const int dsh = 31 - __builtin_clz(a.dim), ksh = 31 - __builtin_clz(kpieces);
+  for (uint32_t it = block * 256 + tid; it < all; it += a.blocks * 256) {
+    if (it < nv) {
+      values(reinterpret_cast<V*>(a.v) + first(it >> dsh) + (int64_t)(it & (a.dim - 1)) * page);
+    } else if (it - nv < (nk + 63) / 64 * 64) {
+      const uint32_t i = it - nv;
+      if (i < nk) move(reinterpret_cast<ss_u32x4*>(reinterpret_cast<V*>(a.k) + first(i >> ksh)) + (i & (kpieces - 1)), one / EV, kpieces);
+    } else {
+      const uint32_t i = it - nv - (nk + 63) / 64 * 64, layer = (i >> 1) / (uint32_t)a.kv_heads, h = (i >> 1) - layer * a.kv_heads;
+      move(a.scales + (((int64_t)layer * a.n_pages * a.kv_heads + h) * 2 + (i & 1)) * page, (int64_t)a.kv_heads * 2 * page, 1);
+    }
   }
 }
 
@@ -278,8 +330,8 @@ hipError_t launch_tree_accept(const TreeAcceptArgs& a, hipStream_t st) {
 
 hipError_t launch_keep_rows(KeepArgs a, hipStream_t st) {
   // A part a thread up to 8,192 workgroups, past which more of them change nothing: 32 sequences of 48 layers and 8 key heads of e4m3 take
-  // 59 us so and with 16,384, 63 with 4,096, 71 with 2,048, 104 with 512.
-  const int64_t parts = (int64_t)(a.dim + a.dim * a.size / 16 + (a.size == 1 ? 2 : 0)) * a.kv_heads * a.layers;
+  // 54 us so and with 16,384, 57 with 4,096, 62 with 2,048, 60 with 512.
+  const int64_t parts = (int64_t)(a.dim + a.dim * a.size / 16 + (a.size == 1 ? 2 : 0)) * a.kv_heads * a.layers + 63;
   a.blocks = (int)std::min<int64_t>((parts + 255) / 256, std::max<int64_t>(8192 / a.seqs, 1));
   const dim3 grid((unsigned)(a.blocks * a.seqs));
   if (a.size == 1)

@@ -1737,7 +1737,7 @@ int ssmoe_keep_rows(void* k, void* v, uint8_t* scales, int layers, int64_t n_pag
   if (bytes != 1 && bytes != 2) return fail(SSMOE_EINVAL, "bytes of an element must be 1 (e4m3) or 2, got %d", bytes);
   if (max_rows > ss::kTreeRows) return fail(SSMOE_EINVAL, "a tree has at most %d rows of a sequence, max_rows is %d", ss::kTreeRows, max_rows);
   const int64_t one = (int64_t)kv_heads * page * dim;
-  if (n_pages > INT64_MAX / 4 / one / layers || (int64_t)layers * kv_heads > INT32_MAX / std::max(seqs, 1))
+  if (n_pages > INT64_MAX / 4 / one / layers || (int64_t)layers * kv_heads > std::min((int64_t)1 << 22, (int64_t)INT32_MAX / std::max(seqs, 1)))
     return fail(SSMOE_EINVAL, "too many layers and sequences for one call");
   if (rows == 0 || seqs == 0) return ok();
   if (!k || !v || !cu_rows || !kv_len || !table || !accepted || (bytes == 1 && !scales))

@@ -377,6 +377,14 @@ def test_keep_paths(kind):
     check_keep(kind, [20, 5, 1, 0, 4, 6], [33, 40, 9, 12, 60, 4], 2, 64, 16, 2, paths=paths)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_keep_from_every_place(kind, page):
+    """Long branches (every other row, all but one, the last ones) that begin at each of eight places beside each other."""
+    paths = [list(range(0, 64, 2)), [0, 1, 2] + list(range(4, 64)), [0] + list(range(50, 64)), list(range(0, 40, 3))] * 2
+    check_keep(kind, [64, 64, 64, 40] * 2, [64 + 250 + i for i in range(8)], 1, 64, page, 2, paths=paths)
+
+
 def test_keep_follows_a_bad_path_up_to_its_fault():
     check_keep("bf16", [6, 6, 6], [20, 20, 20], 1, 64, 16, 1, paths=[[0, 2, 2, 4], [0, 3, 9], [0, 4, 1]], error=ERR_BATCH)
 

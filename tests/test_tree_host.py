@@ -178,7 +178,7 @@ def test_pages_in_8_bits():
         KVPages(1, 2, 1, 64, 16, dtype=torch.float8_e5m2, device="cpu")
 
 
-def test_keep_rows_bounds_its_parts(L):
+def test_keep_rows_bounds_its_parts(L):  # noqa: F811
     """A thread's part is counted in 31 bits: more layers and key heads than that are refused."""
     for layers, heads, page, seqs in ((1 << 22, 2, 16, 2), (1 << 21, 4, 16, 1), (1 << 20, 4, 16, 1 << 10)):
         assert L.ssmoe_keep_rows(M, 1 << 50, None, layers, 1, heads, page, 64, 2, 3, 4, 5, 8, 6, 16, seqs, 8, None) == EINVAL

@@ -167,6 +167,27 @@ SS_DEV Share find_share(const AttnArgs& a, int block, int per, bool write) {
   auto sum = [](uint32_t x) {  // over the lanes; in a scalar register, as all that follows from it
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)ss_butterfly(x, [](uint32_t p, uint32_t q) { return p + q; }));
   };
+  // One sequence: no sums over the lanes (a tree of 12 rows over 777 tokens 16.2 -> 15.6 us).
+  if (a.seqs == 1) {
+    const Size z = size_of(0);
+    const uint32_t units = __builtin_amdgcn_readfirstlane(z.units), tiles = max(__builtin_amdgcn_readfirstlane(z.tiles), 1);
+    const uint32_t most = (uint32_t)a.share / tiles;  // chunks of a tile
+    const uint32_t size = max((units + most - 1) / most, 2u), chunks = (units + size - 1) / size;
+    const int all = (int)(chunks * tiles) * per, run = (all + 7) / 8, id = block % 8 * run + block / 8;
+    if (write && lane == 0) {
+      a.meta[0] = (int)size;
+      a.meta[1] = 0;
+    }
+    Share r = {-1, 0, 0, (int)size, -1, 0};
+    if (block / 8 < run && id < all) {
+      r.g = id / per;
+      r.part = id - r.g * per;
+      r.s = 0;
+      r.slot = r.g / (int)tiles;
+      r.tile = r.g - r.slot * (int)tiles;
+    }
+    return r;
+  }
   const Size first = size_of(lane);
   uint64_t total = 0;
   uint32_t tiles = 0;

@@ -1,7 +1,7 @@
 // Attention of prompt chunks over a paged cache: many rows of a sequence, so that the work is the two matrix products,
 // 4 dim FLOP per (row, token) and head.
 //
-// The rows of a sequence times the heads of a key head are one packed axis, as in ss_attn.hip: a chunk's tiles hold
+// The rows of a sequence times the heads of a key head are one packed axis, as in ss_attn_few.hpp: a chunk's tiles hold
 // rows of nearly one position, and a key head's tokens are read once for all its heads. A workgroup has 128 packed rows,
 // 32 a wave as the columns of v_mfma_f32_32x32x16, and goes over the tokens in tiles of TK:
 //   S^T = K Q^T, queries in registers; A row m = 8 b + 4 h + r of a 32-token tile is token 16 (b / 2) + 8 h + 4 (b % 2) + r, so
@@ -16,11 +16,23 @@
 //
 // The running maximum is raised only when a score passes it by 2^kLazy: until then probabilities are up to 2^kLazy, exact
 // all the same, and the sums are not touched. Masks are worked out only in tiles that some row of the wave does not see
-// whole, where values at unseen places are also kept out of the products (as in ss_attn.hip).
+// whole, where values at unseen places are also kept out of the products (as in ss_attn_few.hpp).
+//
+// Pages of e4m3 numbers (E8) are widened on their way to LDS, once for the workgroup's 128 columns: a thread takes 16 codes of a key or of a
+// dimension's values into registers one step ahead and writes 16 bfloat16 into the stage beside the value products. Keys have their powers of
+// two then; the values' go to the weights (see ss_attn_few.hpp), from LDS beside the stage.
+//
+// Trees (TREE): as in ss_attn_few.hpp; a workgroup's tiles before the sequence's rows are plain, so the masks are read in one or two.
+//
+// Over e4m3 and for trees without a window the workgroups share the call's tokens by the sequences' own lengths and row tiles (find_share): 512
+// in all, two a CU, chunks of one size, neighbours on one XCD where they read one chunk.
 //
 // Bound by the matrix units and what runs beside them: a tile of 64 tokens and 128 dimensions is 32 products (1,024 cycles of a
 // SIMD) beside some 290 other instructions, 32 exponentials among them. 8,191 rows of 32 heads under a window of 4,096 (551
 // GFLOP) take 560-620 us, 0.89 to 0.98 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
+// Of e4m3 4,095 rows after 4,905 tokens (466 GFLOP) take 482 to 540 us, 0.86 to 0.97 PFLOP/s, the matrix units busy 48 % of the cycles: a tile
+// has 32 conversions and 32 products of weights more. Trees: 16 of up to 26 rows, 32 heads on 4, up to 8,000 tokens (169 MB, 24 GFLOP, 38
+// with the columns that no row has) 53 us; 4 of 64 rows over 50,000 tokens of e4m3 and 8 key heads (417 MB, 209 GFLOP) 245 to 254 us, 45 % busy.
 #pragma once
 #include <hip/hip_runtime.h>
 

@@ -12,6 +12,9 @@
 // Bound by memory on prompts: 8,190 rows of 16 + 2 + 2 heads of 256 dimensions, a quarter of them turned by three axes, 168 MB
 // in 39 us from memory (4.3 TB/s; a copy reaches 4.9); 64 single tokens of 32 + 4 + 4 heads of 128 take 6 to 7 us, most of it
 // the chain of a row's place, its page, its angles and its rows. With every wave working out its own angles 8.8.
+// Into pages of e4m3 numbers (E8) a row's largest magnitude is found first, over the lanes that have its elements in registers already, so each
+// byte is still read and written once: the prompt writes 76 MB where 16 bits take 92 (160 MB both ways) in 34 to 36 us, the single
+// tokens take 9.1, the maximum's exchanges one more link of the chain.
 #include <hip/hip_runtime.h>
 
 #include "ss_attn.hpp"

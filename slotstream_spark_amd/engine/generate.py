@@ -13,6 +13,9 @@ stack verifies pending + drafts in one pass, the host walks the rows with the pl
 first 1 + good rows (rollback cuts the position and the token list; the MoE stack records no recurrent state) and
 feeds the kept tokens with their final stream rows (the head's `multi`, hc = 1 here) to the head. Near the context end
 (fewer than DEPTH drafts fit) the loop switches for good to plain steps.
+
+tree_decode is the loop over trees of drafts: a round (MoEStack.tree_step) verifies all rows of a tree in one pass, accepts the branch that the
+stack's choices follow on the device and moves its keys and values up. It has no counterpart in the reference, whose drafts are a chain.
 """
 from __future__ import annotations
 

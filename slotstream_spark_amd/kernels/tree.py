@@ -102,7 +102,8 @@ def keep_rows(k: torch.Tensor, v: torch.Tensor, cu_rows: torch.Tensor, kv_len: t
     """Token kv_len - rows + d of every sequence := its token kv_len - rows + path[d], for d up to n_accept, in all layers: k [layers,
     n_pages, kv_heads, page, dim], v [layers, n_pages, kv_heads, dim, page], of e4m3 with scales uint8 [layers, n_pages, kv_heads, 2,
     page]. cu_rows, kv_len and table are the round's; accepted int32 [seqs, 4 + 2 max_rows] is accept_tree's result. What lies behind the
-    moved tokens is not to be read any more. Rows of pages that others hold too are not to be moved (KVPages.extend copies those).
+    moved tokens is not to be read any more. Rows of pages that others hold too are not to be moved (KVPages.extend copies those); values are
+    written in whole pieces of 8 tokens, the others of a piece as they were, so nothing else may write to these pages meanwhile.
     A path that does not rise, or names no row of the sequence, is followed up to there and raises SSMOE_ERR_BATCH in the device
     status. Capturable."""
     if k.dim() != 5 or v.dim() != 5:

@@ -12,8 +12,8 @@ namespace {
 // groups of dim / 4 threads, 16 bytes each. WIDE: its workgroup's groups take the chunks by their number modulo the
 // number of groups, each with a running maximum, and the groups' sums are added in order; else one group takes all its
 // chunks and a workgroup has as many rows. Either way the order goes by the chunks' numbers alone.
-// EXT: calls of trees or with shared chunks.
-template <class T, int D, bool WIDE, bool EXT>
+// EXT: calls of trees or with shared chunks. DEEP: a group's loads of eight chunks go out together, those past its last one anew.
+template <class T, int D, bool WIDE, bool EXT, bool DEEP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int TD = D / 4, GROUPS = 256 / TD, STEP = WIDE ? GROUPS : 1;
   __shared__ __attribute__((aligned(16))) float part[WIDE ? GROUPS : 1][D];
@@ -76,6 +76,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     o = ss_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) add(*reinterpret_cast<const ss_f32x4*>(&part[j][d4]), part_m[j], part_l[j]);
+  } else if constexpr (DEEP) {
+    constexpr int U = 8;
+    for (int j = 0; j < used; j += U) {
+      float mk[U], lk[U];
+      ss_f32x4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = min(j + u, used - 1) * rows + first;
+        mk[u] = gp(a.pml)[2 * at];
+        lk[u] = gp(a.pml)[2 * at + 1];
+        x[u] = *reinterpret_cast<const SS_G ss_f32x4*>(gp(a.po) + at * D + d4);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u < used) add(x[u], mk[u], lk[u]);
+    }
   } else {
     take(0, used);
   }
@@ -90,14 +106,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // More than 16 chunks are joined by a workgroup a row: one row and 32 heads over 12,000 tokens 12.3 us a call with it, 18.9
 // without, over 51,000 24.4 and 39.8. Up to 16, where a batch brings the rows, by a group of threads a row: 32 sequences of 4
 // rows and 32 heads 186 us a call, 191 with a workgroup each.
+// Where those are at most a wave for each SIMD of 256 CUs, eight chunks are loaded at a time: then no other wave's loads fill the time. A call in us,
+// so and without: one token after 777 8.8 and 9.2, a tree of 12 rows over 777 14.8 and 15.2, 8 sequences of 3 rows of 256 dimensions
+// 24.4 and 24.8; but 3 prompts of 333 rows 84.5 and 82.6, 16 trees of 26 rows 64.1 and 63.6.
 template <class T, int D, bool EXT>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   const int64_t all = (int64_t)a.seqs * a.max_rows * a.heads;
   constexpr int GROUPS = 256 / (D / 4);
+  const dim3 rows((unsigned)((all + GROUPS - 1) / GROUPS));
   if ((a.share > 0 ? a.slots / ((int64_t)a.seqs * a.tiles) : a.slots) > 16)  // of shared chunks as many as a row has if all are alike
-    hipLaunchKernelGGL((attn_join_kernel<T, D, true, EXT>), dim3((unsigned)all), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_join_kernel<T, D, true, EXT, false>), dim3((unsigned)all), dim3(256), 0, st, a);
+  else if (rows.x <= 256)
+    hipLaunchKernelGGL((attn_join_kernel<T, D, false, EXT, true>), rows, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_join_kernel<T, D, false, EXT>), dim3((unsigned)((all + GROUPS - 1) / GROUPS)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_join_kernel<T, D, false, EXT, false>), rows, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -252,7 +252,7 @@ SS_DEV Share find_share(const AttnArgs& a, int block, int per, bool write) {
 }
 
 // ---------------------------------------------------------------- pages of e4m3 numbers
-// A token's keys (its values) are its e4m3 numbers times 2^(s - 127), s a byte of 1 to 254: a power of two, so that a key
+// A token's keys (its values) are its e4m3 numbers times 2^(s - 127), s a byte of 1 to 247: a power of two, so that a key
 // times its scale is a bfloat16 as it is (3 bits of mantissa), and the conversion instruction applies it on the way. 255 is read
 // as 254: what an unseen place holds stays finite.
 SS_DEV float scale_of(uint32_t s) { return ss_uf(min(s, 254u) << 23); }

@@ -308,9 +308,24 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
   // over 200 / 777 / 3,000 / 20,000 tokens: 8 trees of 20 packed rows (8 heads on 8, 128 dimensions) 9 / 15 / 26 / 130 against 16 / 21 /
   // 31 / 131, over e4m3 9 / 15 / 20 / 79 against 16 / 21 / 30 / 109; of 64 14 / 23 / 32 / 172 against 18 / 24 / 35 / 133, of 256
   // dimensions 14 / 32 / 51 / 265 against 19 / 26 / 40 / 153; of 128 (16 rows of 32 heads on 4) 13 / 31 / 40 / - against 18 / 26 / 34 / -.
+  // Where a table is one chunk of few rows there is no join, as long as the workgroups find places at once: 8 trees of 40 rows, 32 heads on
+  // 4 of 128 dimensions, over 300 / 500 tokens 17 / 20 against 26 / 29, over e4m3 16 / 17 against 27 / 31; 32 trees of 24 rows 32 / 37
+  // against 32 / 35, over e4m3 27 / 29 against 34 / 36; 32 of 40 rows 48 / 54 against 22 / 28. 24 heads on 8 of 64, 32 trees of 40 rows 19 /
+  // 21 against 18 / 27, of 64 28 / 32 against 19 / 23; 16 on 2 of 256 over 300, 8 of 40 rows 18 against 28, 32 of 40 51 against 29. (The
+  // other way: one tree of 24 rows over 500, 32 heads on 8, 16.8 against 15.1.)
+  const int64_t units = (int64_t)p->seqs * p->kv_heads, packed = (int64_t)max_rows * a.group;
+  auto few_chunk = [&](int64_t seen) {
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(16 * units, 512), 4096);
+    int64_t chunk = (seen * units + 255) / 256;
+    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), most);
+    if (cap <= 4096 && (cap - chunk) * std::max(p->dim, 128) <= 512 * 128) chunk = (cap + 127) / 128 * 128;
+    return chunk;
+  };
   if (e4m3 || tree) {
-    const int64_t packed = (int64_t)max_rows * a.group;
-    if (packed <= 32 || (packed <= 64 && p->dim < 256 && cap <= 4096) || (packed <= 128 && cap <= 512)) *prompt = false;
+    if (packed <= 32 || (packed <= 64 && p->dim < 256 && cap <= 4096)) *prompt = false;
+    if (units * packed <= 32768 && units * packed * p->dim <= (e4m3 ? 6 << 19 : 5 << 19) &&
+        ((packed <= 128 && cap <= 512) || (cap <= 768 && few_chunk(cap) >= cap)))
+      *prompt = false;
   }
   a.packed = *prompt ? 128 : ss::attn_few_packed(p->dim, max_rows * a.group, e4m3);
   a.tiles = (max_rows * a.group + a.packed - 1) / a.packed;
@@ -319,17 +334,13 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
   if (a.window < (1 << 30))
     seen = std::min<int64_t>(cap, (int64_t)a.window + std::max(max_rows, kFewRows) + a.sinks);
   int64_t chunk = cap, slots = 1;
-  const int64_t units = (int64_t)p->seqs * p->kv_heads;
   const int parts_of_dim = ss::attn_prompt_parts(p->dim, shift);
   if (*prompt) {
     const int64_t want = 512 / std::max<int64_t>(units * a.tiles * parts_of_dim, 1);
     if (want > 1 && seen > 512) chunk = std::max<int64_t>((seen + want - 1) / want, 512);
     chunk = (chunk + 127) / 128 * 128;
   } else {
-    const int64_t most = std::min<int64_t>(std::max<int64_t>(16 * units, 512), 4096);
-    chunk = (seen * units + 255) / 256;
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), most);
-    if (cap <= 4096 && (cap - chunk) * std::max(p->dim, 128) <= 512 * 128) chunk = (cap + 127) / 128 * 128;
+    chunk = few_chunk(seen);
   }
   a.chunk = (int)chunk;
   slots = (cap + chunk - 1) / chunk;

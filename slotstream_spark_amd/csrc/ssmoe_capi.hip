@@ -308,6 +308,8 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
   // over 200 / 777 / 3,000 / 20,000 tokens: 8 trees of 20 packed rows (8 heads on 8, 128 dimensions) 9 / 15 / 26 / 130 against 16 / 21 /
   // 31 / 131, over e4m3 9 / 15 / 20 / 79 against 16 / 21 / 30 / 109; of 64 14 / 23 / 32 / 172 against 18 / 24 / 35 / 133, of 256
   // dimensions 14 / 32 / 51 / 265 against 19 / 26 / 40 / 153; of 128 (16 rows of 32 heads on 4) 13 / 31 / 40 / - against 18 / 26 / 34 / -.
+  // Over e4m3 of 64 dimensions 36 to 60 packed rows (24 heads on 8) are few at any length: over 12,000 tokens 16 / 48 sequences 69 to 72 / 182 to
+  // 185 against 88 / 275 to 286 (of 16 bits 83 to 96 / 243 to 250 against 84 / 284).
   // Where a table is one chunk of few rows there is no join, as long as the workgroups find places at once: 8 trees of 40 rows, 32 heads on
   // 4 of 128 dimensions, over 300 / 500 tokens 17 / 20 against 26 / 29, over e4m3 16 / 17 against 27 / 31; 32 trees of 24 rows 32 / 37
   // against 32 / 35, over e4m3 27 / 29 against 34 / 36; 32 of 40 rows 48 / 54 against 22 / 28. 24 heads on 8 of 64, 32 trees of 40 rows 19 /
@@ -322,7 +324,7 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
     return chunk;
   };
   if (e4m3 || tree) {
-    if (packed <= 32 || (packed <= 64 && p->dim < 256 && cap <= 4096)) *prompt = false;
+    if (packed <= 32 || (packed <= 64 && p->dim < 256 && (cap <= 4096 || (e4m3 && p->dim == 64)))) *prompt = false;
     if (units * packed <= 32768 && units * packed * p->dim <= (e4m3 ? 6 << 19 : 5 << 19) &&
         ((packed <= 128 && cap <= 512) || (cap <= 768 && few_chunk(cap) >= cap)))
       *prompt = false;

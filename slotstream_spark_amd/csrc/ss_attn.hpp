@@ -288,7 +288,7 @@ SS_DEV uint32_t tree_sees(int first, int base, int end, uint64_t mask, int pos, 
   return r & (left >= 8 ? 0xFFu : left <= 0 ? 0u : (1u << left) - 1);
 }
 
-int attn_prompt_parts(int dim, int page_shift);
+int attn_prompt_parts(int dim, int page_shift, bool e4m3);
 hipError_t launch_attn_prompt(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 hipError_t launch_attn_prompt_tree(const AttnArgs& a, int dim, bool fp16, hipStream_t st);
 hipError_t launch_attn_prompt_e4m3(const AttnArgs& a, int dim, hipStream_t st);

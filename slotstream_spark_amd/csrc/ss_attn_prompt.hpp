@@ -211,14 +211,28 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const uint32_t koff0 = (ONE ? krow0 : krow0 % 16) * KROW + 16 * ((lane % KC) ^ kswizzle<D, E8>(krow0));
   const int vpiece0 = (lane % VC) ^ vswizzle<TK, E8>(vrow0);
   const uint32_t voff0 = (uint32_t)vrow0 * page * 2 + 16 * (ONE ? vpiece0 : vpiece0 & 1);
+  // Of e4m3 a thread needs the pages of its own tokens, which lie in LDS, a copy and a ring of four tiles for each wave (three are in use).
+  constexpr bool OWN = E8 && !ONE;
+  __shared__ int32_t own_ids[OWN ? 4 : 1][4][4];
   struct Tile {
-    int t;          // its first token
-    int ids[NP];    // its pages, 0 where there is none
-    uint32_t held;  // bit j: page j is there
+    int t;                   // its first token
+    int ids[OWN ? 1 : NP];   // its pages, 0 where there is none; of own_ids its place in the ring
+    uint32_t held;           // bit j: page j is there
   };
+  int ring = 0;
   auto tile_at = [&](int t) {
     Tile r;
     r.t = t;
+    if constexpr (OWN) {
+      const int at = t >> a.page_shift;  // a tile's first token is a multiple of its size, so its entries are in one register
+      if (__builtin_expect((uint32_t)(at - first_entry) >= 64u, 0)) page_id(t, 0);
+      const int mine = __shfl(entries, (((t + 16 * (lane % NP)) >> a.page_shift) - first_entry) & 63);
+      r.held = (uint32_t)__ballot(mine >= 0) & ((1u << NP) - 1);
+      r.ids[0] = ring;
+      if (lane < NP) own_ids[w][ring][lane] = max(mine, 0);
+      ring = (ring + 1) & 3;
+      return r;
+    }
     r.held = 0;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
@@ -267,14 +281,12 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   const int ktok = kpiece / (D / 16), kpc = kpiece % (D / 16), vdim = vpiece / (TK / 16), vtok = 16 * (vpiece % (TK / 16));
   const uint32_t kput = ktok * KROW + 16 * ((2 * kpc) ^ kodd<D, E8>(2 * kpc) ^ kswizzle<D, E8>(ktok)), vput = vdim * VROW + 16 * ((vtok / 8) ^ vswizzle<TK, E8>(vdim));
   const uint32_t kget = ktok * D + 16 * kpc, vget = (uint32_t)vdim * page + vtok;
-  auto page_at = [&](const Tile& r, int token) {
-    int id = r.ids[0];
-    if constexpr (!ONE) {
-#pragma unroll
-      for (int q = 1; q < NP; ++q) id = token / 16 == q ? r.ids[q] : id;
-    }
-    return id;
+  auto own_tid = [&] {  // the thread's number worked out anew, so that no place that follows from it is kept over the tiles
+    uint32_t none = 0;
+    asm volatile("" : "+v"(none));
+    return 64 * w + (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
   };
+  auto page_at = [&](const Tile& r, int token) { return OWN ? own_ids[w][r.ids[0]][token / 16] : r.ids[0]; };
   const uint8_t* exps = E8 ? a.scales + (int64_t)kh * 2 * page : nullptr;
   const int64_t exp_bytes = (int64_t)a.kv_heads * 2 * page;
   auto fetch_k8 = [&](const Tile& r, Fetched& f, int n) {
@@ -283,23 +295,26 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
       f.k[n] = *(const SS_G ss_u32x4*)(gp(kbase + r.ids[0] * page_bytes + (int64_t)(at + n * KT) * D) + kget);
       f.kexp[n] = gp(exps + r.ids[0] * exp_bytes + at + n * KT)[(uint32_t)ktok];
     } else {
+      const int piece = own_tid() % min(K8, 256), ktok = piece / (D / 16), kpc = piece % (D / 16);
       const int tok = ktok + n * KT, id = page_at(r, tok), at = (r.t + tok) & (page - 1);
-      f.k[n] = *(const SS_G ss_u32x4*)(kbase + id * page_bytes + at * D + 16 * kpc);
-      f.kexp[n] = gp(exps)[id * exp_bytes + at];
+      f.k[n] = *(const SS_G ss_u32x4*)(kbase + (uint64_t)(uint32_t)id * (uint32_t)page_bytes + (uint32_t)(at * D + 16 * kpc));
+      f.kexp[n] = gp(exps)[(uint64_t)(uint32_t)id * (uint32_t)exp_bytes + at];
     }
   };
   auto fetch_v8 = [&](const Tile& r, Fetched& f, int n) {
+    const int self = ONE ? tid : own_tid();
+    const int vpiece = self % min(V8, 256), vdim = vpiece / (TK / 16), vtok = 16 * (vpiece % (TK / 16));
     if constexpr (ONE)
       f.v[n] = *(const SS_G ss_u32x4*)(gp(vbase + r.ids[0] * page_bytes + (r.t & (page - 1)) + n * VT * page) + vget);
     else
-      f.v[n] = *(const SS_G ss_u32x4*)(vbase + page_at(r, vtok) * page_bytes + (int64_t)(vdim + n * VT) * page +
-                                       ((r.t + vtok) & (page - 1)));
+      f.v[n] = *(const SS_G ss_u32x4*)(vbase + (uint64_t)(uint32_t)page_at(r, vtok) * (uint32_t)page_bytes +
+                                       (uint32_t)((vdim + n * VT) * page + ((r.t + vtok) & (page - 1))));
     if (n == 0) {
-      const int one = tid % TK;
+      const int one = self % TK;
       if constexpr (ONE)
         f.vexp = gp(exps + r.ids[0] * exp_bytes + page + (r.t & (page - 1)))[(uint32_t)one];
       else
-        f.vexp = gp(exps)[page_at(r, one) * exp_bytes + page + ((r.t + one) & (page - 1))];
+        f.vexp = gp(exps)[(uint64_t)(uint32_t)page_at(r, one) * (uint32_t)exp_bytes + page + ((r.t + one) & (page - 1))];
     }
   };
   auto put_k8 = [&](const Fetched& f, uint8_t* kl, int n) {
@@ -675,13 +690,19 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
   }
 }
 
-// Tiles of 64 tokens where a page holds them, else of 32 (and of 256 dimensions always: registers).
+// Tiles of 64 tokens where a page holds them, and over e4m3, whose threads look their pages up; else of 32 (and of 256 dimensions always:
+// registers). Of e4m3 on pages of 16 / 32, and in tiles of 32 as of 16 bits: 4 trees of 64 rows over 50,000 tokens 295 / 290 and 334 / 298 us, 4,095
+// rows after 4,905 tokens of 64 dimensions 417 / 377 and 434 / 408, of 128 574 / 545 and 579 / 534; of 256 on pages of 16 with the output in
+// halves 773, in quarters 1,311.
 template <class T, int D, int DV, bool E8, bool TREE>
 void launch_prompt(const AttnArgs& a, hipStream_t st) {
-  const int64_t units = (int64_t)a.slots * a.kv_heads * attn_prompt_parts(D, a.page_shift);
+  const int64_t units = (int64_t)a.slots * a.kv_heads * attn_prompt_parts(D, a.page_shift, E8);
   const dim3 grid((unsigned)(a.share > 0 ? (units + 7) / 8 * 8 : units * a.tiles * a.seqs));
-  if (a.page_shift >= 6 && D < 256)
-    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, D < 256 ? 64 : 32, true, E8, TREE>), grid, dim3(256), 0, st, a);
+  constexpr int TK = D < 256 ? 64 : 32;
+  if (a.page_shift >= (D < 256 ? 6 : 5))
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, TK, true, E8, TREE>), grid, dim3(256), 0, st, a);
+  else if constexpr (E8)
+    hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, TK, false, E8, TREE>), grid, dim3(256), 0, st, a);
   else if (a.page_shift >= 5)
     hipLaunchKernelGGL((attn_prompt_kernel<T, D, DV, 32, true, E8, TREE>), grid, dim3(256), 0, st, a);
   else

@@ -336,7 +336,7 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
   if (a.window < (1 << 30))
     seen = std::min<int64_t>(cap, (int64_t)a.window + std::max(max_rows, kFewRows) + a.sinks);
   int64_t chunk = cap, slots = 1;
-  const int parts_of_dim = ss::attn_prompt_parts(p->dim, shift);
+  const int parts_of_dim = ss::attn_prompt_parts(p->dim, shift, e4m3);
   if (*prompt) {
     const int64_t want = 512 / std::max<int64_t>(units * a.tiles * parts_of_dim, 1);
     if (want > 1 && seen > 512) chunk = std::max<int64_t>((seen + want - 1) / want, 512);

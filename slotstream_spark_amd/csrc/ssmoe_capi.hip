@@ -313,8 +313,9 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
   // Where a table is one chunk of few rows there is no join, as long as the workgroups find places at once: 8 trees of 40 rows, 32 heads on
   // 4 of 128 dimensions, over 300 / 500 tokens 17 / 20 against 26 / 29, over e4m3 16 / 17 against 27 / 31; 32 trees of 24 rows 32 / 37
   // against 32 / 35, over e4m3 27 / 29 against 34 / 36; 32 of 40 rows 48 / 54 against 22 / 28. 24 heads on 8 of 64, 32 trees of 40 rows 19 /
-  // 21 against 18 / 27, of 64 28 / 32 against 19 / 23; 16 on 2 of 256 over 300, 8 of 40 rows 18 against 28, 32 of 40 51 against 29. (The
-  // other way: one tree of 24 rows over 500, 32 heads on 8, 16.8 against 15.1.)
+  // 21 against 18 / 27, of 64 28 / 32 against 19 / 23; 16 on 2 of 256 over 300, 8 of 40 rows 18 against 28, 32 of 40 51 against 29. A
+  // prompt of 80 / 300 / 500 rows over e4m3, 32 on 4 of 128, 10 / 14 / 16 against 16 / 22 / 30. (The other way: one tree of 24 rows over 500, 32
+  // heads on 8, 16.8 against 15.1.)
   const int64_t units = (int64_t)p->seqs * p->kv_heads, packed = (int64_t)max_rows * a.group;
   auto few_chunk = [&](int64_t seen) {
     const int64_t most = std::min<int64_t>(std::max<int64_t>(16 * units, 512), 4096);

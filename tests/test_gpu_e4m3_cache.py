@@ -58,6 +58,13 @@ def test_window_and_first_tokens(window, sinks, rows):
         check(Batch8([rows] * 4, [rows, 60, 129, 700], 6, 2, dim, page, seed=window + rows), window, sinks)
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (16, 2), (5, 1)])
+def test_prompts_over_short_tables(dim, page, heads, kv_heads):
+    check(Batch8([300, 1, 80], [300, 33, 200], heads, kv_heads, dim, page, seed=dim + page))
+    check(Batch8([500], [500], heads, kv_heads, dim, page, seed=dim))
+
+
 def test_sequences_without_rows_or_tokens():
     b = Batch8([0, 2, 1, 0, 3], [0, 50, 0, 20, 2], 4, 2, 64, 16)
     out = check(b)

@@ -321,13 +321,26 @@ int plan_attention(const ssmoe_paged_attention_args* p, bool e4m3, bool tree, ss
     const int64_t most = std::min<int64_t>(std::max<int64_t>(16 * units, 512), 4096);
     int64_t chunk = (seen * units + 255) / 256;
     chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), most);
-    if (cap <= 4096 && (cap - chunk) * std::max(p->dim, 128) <= 512 * 128) chunk = (cap + 127) / 128 * 128;
+    // A table that is not much more than a chunk is one, without a join. Over e4m3 the further tokens cost less, and beside the join of many
+    // columns least (but up to 8 causal rows have the bits of single ones, so their chunks do not go by the rows). Trees over e4m3 so and with
+    // 512: 8 of 24 rows, 32 heads on 4 of 128, over 600 / 760 / 1,000 / 1,200 tokens 16 / 16 / 18 / 20 and 29 / 30 / 32 / 32; one of 12 over 760
+    // 13.9 and 16.2; 8 of 64 rows, 24 on 8 of 64, over 1,000 22 and 29; 8 of 24, 16 on 2 of 256, over 450 20 and 27. 1,024 for few columns: one
+    // of 12 rows, 32 on 8, over 1,000 16.0 and 14.2; for 36 packed rows of 64 dimensions, 8 sequences, 19.5 and 17.0. Over 16 bits there is
+    // no gain (one of 64 rows over 760 20.9 and 18.2, 8 of 12 on 8 over 1,000 25 and 21).
+    int64_t span = 512;
+    if (e4m3 && (tree || p->max_rows > kFewRows)) {
+      if (units * packed >= (p->dim == 64 ? 4096 : p->dim == 128 ? 2048 : 1024))
+        span = 1024;
+      else if (p->dim == 128 || (p->dim == 64 && packed <= 16))
+        span = 768;
+    }
+    if (cap <= 4096 && (cap - chunk) * std::max(p->dim, 128) <= span * 128) chunk = (cap + 127) / 128 * 128;
     return chunk;
   };
   if (e4m3 || tree) {
     if (packed <= 32 || (packed <= 64 && p->dim < 256 && (cap <= 4096 || (e4m3 && p->dim == 64)))) *prompt = false;
     if (units * packed <= 32768 && units * packed * p->dim <= (e4m3 ? 6 << 19 : 5 << 19) &&
-        ((packed <= 128 && cap <= 512) || (cap <= 768 && few_chunk(cap) >= cap)))
+        ((packed <= 128 && cap <= 512) || (cap <= (e4m3 ? 1408 : 768) && few_chunk(cap) >= cap)))
       *prompt = false;
   }
   a.packed = *prompt ? 128 : ss::attn_few_packed(p->dim, max_rows * a.group, e4m3);

@@ -602,7 +602,7 @@ int ssmoe_move_pages(void* k, void* v, int layers, int64_t n_pages, int64_t page
 /* Pages of e4m3 numbers (OCP, no infinities): keys [n_pages][kv_heads][page][dim] and values [n_pages][kv_heads][dim][page] of a byte
  * each, and scales uint8 [n_pages][kv_heads][2][page]: token t's keys are its numbers times 2^(scales[..][0][t] - 127), its
  * values times 2^(scales[..][1][t] - 127). Written by ssmoe_rope_append_e4m3, which takes the least exponent from -126 on with which
- * no number is over 448 and rounds once from fp32; a power of two costs e4m3 no precision. Elements that are infinite or NaN are left out of
+ * no number is over 448 (of keys turned in 64 bits) and rounds once from fp32; a power of two costs e4m3 no precision. Elements that are infinite or NaN are left out of
  * that choice and kept as NaN (both signs of it read as NaN). Bytes are 1 to 247; what others read as
  * is not defined. Queries and rows are SSMOE_BF16 (fp16 has no exponents for a probability times such a scale). Batches, windows
  * and what unseen places may hold as above. scales 16-byte aligned, apart from what a call writes beside it. */

@@ -27,7 +27,7 @@ namespace {
 
 // ---------------------------------------------------------------- rows as e4m3 numbers
 // A vector x of a token and head is kept as e4m3 numbers of x 2^-e, rounded once from fp32, and the byte e + 127: e the least exponent
-// with max |x| <= 448 2^e, from -126 on. What is not finite is left out of the maximum and kept as NaN.
+// with max |x| <= 448 2^e, from -126 on, of a key turned in 64 bits. What is not finite is left out of the maximum and kept as NaN.
 SS_DEV float finite_abs(float x) {
   const float y = fabsf(x);
   return y < __builtin_inff() ? y : 0.f;
@@ -38,12 +38,35 @@ SS_DEV uint32_t exponent8(float top) {
   const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   return (uint32_t)max(e, 1);
 }
+// How far an fp32 maximum of turned elements may be from the one in 64 bits, in units of its last place at 1.75 2^n. Where both of a pair
+// are at most y, (|p| + |q|) factor <= 2 y. A cosine is off by 2 pi 2^-26 for its angle and 4 2^-24 for itself, times factor by 2^-24; the
+// products and their sum by 2^-24 each: 2 (0.94 + 2.4 + 0.6) 10^-7 + 1.8 10^-7 = 9.7 10^-7 of y, 15 units.
+constexpr uint32_t kNear = 32;
 // x 2^-e for the byte of e, NaN where x is not finite.
 SS_DEV float scaled8(float x, float by) { return fabsf(x) < __builtin_inff() ? x * by : __builtin_nanf(""); }
 SS_DEV float inverse8(uint32_t byte) { return ss_uf((254u - byte) << 23); }
 SS_DEV uint32_t pack8(float a, float b, float c, float d) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+}
+// Sine and cosine of a part of a turn in 64 bits: less its quarters it is at most pi / 4, where the series up to x^19 and x^18 are off by
+// less than 10^-19. A loop over a table: as straight code (the library's sincospi) it takes more scalar registers than there are.
+__constant__ const double kSeries[10][2] = {  // 1 / (2 n + 1)!, 1 / (2 n)!
+    {1., 1.}, {1. / 6, 1. / 2}, {1. / 120, 1. / 24}, {1. / 5040, 1. / 720}, {1. / 362880, 1. / 40320},
+    {1. / 39916800, 1. / 3628800}, {1. / 6227020800, 1. / 479001600}, {1. / 1307674368000, 1. / 87178291200},
+    {1. / 355687428096000, 1. / 20922789888000}, {1. / 121645100408832000, 1. / 6402373705728000}};
+SS_DEV void turn64(double part, double* sn, double* cs) {
+  const double quarters = __builtin_rint(4. * part), x = (part - 0.25 * quarters) * 6.28318530717958647693, z = -x * x;
+  double s = 0., c = 0.;
+#pragma unroll 1
+  for (int n = 9; n >= 0; --n) {
+    s = __builtin_fma(s, z, kSeries[n][0]);
+    c = __builtin_fma(c, z, kSeries[n][1]);
+  }
+  s *= x;
+  const int k = (int)quarters & 3;  // of -2 .. 2
+  *sn = k == 0 ? s : k == 1 ? c : k == 2 ? -s : -c;
+  *cs = k == 0 ? c : k == 1 ? -s : k == 2 ? -c : s;
 }
 // The maximum over the lanes l ^ 1, ..., l ^ (n - 1), n = 4, 8, 16 or 32.
 SS_DEV float max_over(float v, int n) {
@@ -62,7 +85,7 @@ SS_DEV float max_over(float v, int n) {
 // Key and value rows of the 8 positions from `first` on, into page `id` at `off`.
 template <class T>
 SS_DEV void append_e4m3(const RopeArgs& a, const SeqRows& sr, int first, int id, int off, int h0, int stride, const float* cs_of,
-                        const float* sn_of) {
+                        const float* sn_of, const double* turn_of) {
   if (id < 0) return;
   const int lane = threadIdx.x & 63, D = a.dim, page = 1 << a.page_shift, half = a.rot / 2, chunks = a.rot / 16;
   const int lo = max(sr.pos0 - first, 0), hi = min(sr.pos0 + sr.n - first, 8), rows = hi - lo;  // the call's tokens of the 8
@@ -104,7 +127,39 @@ SS_DEV void append_e4m3(const RopeArgs& a, const SeqRows& sr, int first, int id,
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, finite_abs(y[e]));
-    const uint32_t byte = exponent8(max_over(top, L));
+    top = max_over(top, L);
+    uint32_t byte = exponent8(top);
+    // The exponent is that of the rows turned in 64 bits. Where the maximum is that near to 448 2^n, the turned elements that may pass it are
+    // turned again: elements of 448 2^n itself under small angles (27 of 39 million keys had the next smaller byte without).
+    const uint32_t bits = ss_fu(top), edge = (bits & 0x7F800000u) | 0x600000u;
+    const bool near = bits + kNear >= edge && bits <= edge + kNear;
+    if (__builtin_expect(__any(near), 0)) {
+      // The elements that may: all at once their comparisons would take more scalar registers than there are.
+      const uint32_t least = near ? (turn ? edge - kNear : edge + 1) : ~0u;
+      uint32_t which = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        which |= ss_fu(finite_abs(y[e])) >= least ? 1u << e : 0u;
+        asm volatile("" : "+v"(which));
+      }
+      bool over = !turn && which;
+      if (!turn) which = 0;
+      which = a.adjacent ? which | which >> 1 : which | which >> 8;  // by frequencies, in the even bits of adjacent pairs
+      which &= a.adjacent ? 0x5555u : 0xFFu;
+#pragma unroll 1
+      while (which) {
+        const int f = __builtin_ctz(which) >> (a.adjacent ? 1 : 0), freq = 8 * j + f;
+        which &= which - 1;
+        double sn, cs;
+        turn64(turn_of[rr * half + freq], &sn, &cs);
+        sn *= a.factor;
+        cs *= a.factor;
+        const double p = T::widen(gp(src)[a.adjacent ? 2 * freq : freq]), q = T::widen(gp(src)[a.adjacent ? 2 * freq + 1 : half + freq]);
+        over |= fmax(fabs(p * cs - q * sn), fabs(q * cs + p * sn)) > (double)ss_uf(edge);
+      }
+      const int e = (int)(bits >> 23) - 8 + (max_over(over ? 1.f : 0.f, L) > 0.f ? 1 : 0);
+      if (near) byte = (uint32_t)max(e, 1);
+    }
     const float by = inverse8(byte);
 #pragma unroll
     for (int e = 0; e < 16; ++e) y[e] = scaled8(y[e], by);
@@ -162,11 +217,13 @@ SS_DEV void append_e4m3(const RopeArgs& a, const SeqRows& sr, int first, int id,
   }
 }
 
+// Five waves a SIMD with E8 (the compiler would take 99 registers and leave four: 8,190 rows 45.0 us a call for 44.5).
 // E8: the cache's pages are e4m3 numbers with exponents; keys and values then go in two parts of their own, in units of a wave
 // behind the query heads: of keys 16 elements of a row a lane, of values 8 rows by 8 dimensions.
 template <class T, bool E8>
-__global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
+__global__ __launch_bounds__(256, E8 ? 5 : 1) void rope_append_kernel(RopeArgs a) {
   __shared__ __attribute__((aligned(16))) float cs_of[8 * 128], sn_of[8 * 128];  // [8 positions][rot / 2]
+  __shared__ double turn_of[E8 ? 8 * 128 : 1];                                   // the angles' parts of a turn, as they are
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups are dealt to the 8 XCDs in turn; each XCD takes a run of neighbours, whose 16-byte parts of a line of values then
   // meet in one L2 (8,190 rows of 40 heads of 128: 53 us in launch order, 49 so; 64 sequences of 4 rows 10.2 and 9.3; 8,190 rows
@@ -208,8 +265,10 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
     else
       raise_bit(a.err, SS_ERR_BATCH);
     const double turns = (double)p * (gp(a.inv_freq)[f] * 0.15915494309189533577);
+    const double part = turns - __builtin_rint(turns);
+    if constexpr (E8) turn_of[it] = part;
     float sn, cs;
-    sincospif(2.f * (float)(turns - __builtin_rint(turns)), &sn, &cs);
+    sincospif(2.f * (float)part, &sn, &cs);
     cs_of[it] = cs * a.factor;
     sn_of[it] = sn * a.factor;
   }
@@ -299,7 +358,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
     }
   }
   if constexpr (E8) {
-    append_e4m3<T>(a, sr, first, id, off, h0, stride, cs_of, sn_of);
+    append_e4m3<T>(a, sr, first, id, off, h0, stride, cs_of, sn_of, turn_of);
     return;
   }
   // Value rows.

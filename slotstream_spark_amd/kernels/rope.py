@@ -39,8 +39,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     each other and the inputs nowhere. Rows past cu_rows[-1] are left as they were.
 
     `scales` uint8 [n_pages, kv_heads, 2, page]: the pages are of e4m3 numbers, q, k and v bf16. A token's and head's keys (values) are
-    kept as x 2^-e rounded once, e the least exponent from -126 on with which none is over 448, and scales[.., 0 (1), t] = e + 127. An
-    infinity or NaN is left out of that choice and kept as NaN. scales is written as the pages are, and overlaps nothing either."""
+    kept as x 2^-e rounded once from fp32, e the least exponent from -126 on with which none is over 448 (of keys turned in 64 bits), and
+    scales[.., 0 (1), t] = e + 127. An infinity or NaN is left out of that choice and kept as NaN. scales is written as the pages are, and overlaps nothing either."""
     max_rows = int(max_rows)
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, positions.shape,
            positions.dtype, positions.is_contiguous(), inv_freq.shape, inv_freq.dtype, inv_freq.is_contiguous(), k_pages.shape,

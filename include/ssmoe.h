@@ -642,6 +642,7 @@ int ssmoe_accept_tree(const float* target, const int32_t* tokens, const int32_t*
  * (`bytes` of an element: 2, or 1 with scales [layers][n_pages][kv_heads][2][page]) the token kv_len - rows + d of a sequence becomes
  * its token kv_len - rows + path[d], path the branch's rows in `accepted` (ssmoe_accept_tree's out), d up to n_accept. Tokens past them hold
  * what they held or a moved row's copy. A path that does not rise or names no row of the sequence is followed up to there (SSMOE_ERR_BATCH).
+ * `rows` bounds the entries of cu_rows, which may begin past 0 (the rows of a larger batch); nothing else goes by it.
  * Values are written in whole pieces of 8 tokens, the others as they were: nothing else may write to these pages meanwhile. At most 2^22
  * layers and key heads together (their product). */
 int ssmoe_keep_rows(void* k, void* v, uint8_t* scales, int layers, int64_t n_pages, int kv_heads, int page, int dim, int bytes,

@@ -101,9 +101,10 @@ def keep_rows(k: torch.Tensor, v: torch.Tensor, cu_rows: torch.Tensor, kv_len: t
               accepted: torch.Tensor, scales: torch.Tensor | None = None) -> None:
     """Token kv_len - rows + d of every sequence := its token kv_len - rows + path[d], for d up to n_accept, in all layers: k [layers,
     n_pages, kv_heads, page, dim], v [layers, n_pages, kv_heads, dim, page], of e4m3 with scales uint8 [layers, n_pages, kv_heads, 2,
-    page]. cu_rows, kv_len and table are the round's; accepted int32 [seqs, 4 + 2 max_rows] is accept_tree's result. What lies behind the
-    moved tokens is not to be read any more. Rows of pages that others hold too are not to be moved (KVPages.extend copies those); values are
-    written in whole pieces of 8 tokens, the others of a piece as they were, so nothing else may write to these pages meanwhile.
+    page]. cu_rows, kv_len and table are the round's (cu_rows[m:], kv_len[m:] and table[m:] of a larger batch among them); accepted int32
+    [seqs, 4 + 2 max_rows] is accept_tree's result. What lies behind the moved tokens is not to be read any more. Rows of pages that others
+    hold too are not to be moved (KVPages.extend copies those); values are written in whole pieces of 8 tokens, the others of a piece as
+    they were, so nothing else may write to these pages meanwhile.
     A path that does not rise, or names no row of the sequence, is followed up to there and raises SSMOE_ERR_BATCH in the device
     status. Capturable."""
     if k.dim() != 5 or v.dim() != 5:
@@ -125,8 +126,9 @@ def keep_rows(k: torch.Tensor, v: torch.Tensor, cu_rows: torch.Tensor, kv_len: t
             or accepted.shape[1] % 2 or not 6 <= accepted.shape[1] <= 4 + 2 * TREE_ROWS:
         raise ValueError(f"accepted must be contiguous int32 [{seqs}, 4 + 2 max_rows]")
     max_rows = (accepted.shape[1] - 4) // 2
+    most = 2 ** 31 - 1   # rows of the call: nothing is at a row's number, and the views cu_rows[m:] of a batch begin anywhere
     dev = check_device(k, v, cu_rows, kv_len, table, accepted, scales)
     with _lib.on_device(dev):
         _lib.check(_lib.lib().ssmoe_keep_rows(
             k.data_ptr(), v.data_ptr(), _lib.ptr(scales), layers, n, h, page, dim, k.element_size(), cu_rows.data_ptr(),
-            kv_len.data_ptr(), table.data_ptr(), width, accepted.data_ptr(), seqs * max_rows, seqs, max_rows, _lib.raw_stream(dev)))
+            kv_len.data_ptr(), table.data_ptr(), width, accepted.data_ptr(), most, seqs, max_rows, _lib.raw_stream(dev)))

@@ -192,6 +192,12 @@ class MoEStack:
         del self.st.tokens[len(self.st.tokens) - n:]
         for c in self.st.attn.values():
             c.pos = self.st.pos
+        self._give_up()
+
+    def _give_up(self) -> None:
+        """The pages' count of the sequence's tokens becomes the position: evict() goes by it, and a tree is up to 64 rows, not `rows`."""
+        if self.cache is not None:
+            self.cache.pages.truncate(self.cache.seq, self.st.pos)
 
     def tree_step(self, tokens: list[int], parents: list[int]) -> tuple[TreeResult, torch.Tensor]:
         """A greedy round over a tree: tokens[0] is the pending token, tokens[i] a draft behind row parents[i] < i (parents[0] is not
@@ -230,6 +236,7 @@ class MoEStack:
             keep_rows(pages.k, pages.v, cu, kv_len, table, took, scales=pages.scales)
         res = TreeResult.from_out(took[0].tolist())
         self._advance([int(tokens[p]) for p in res.path])
+        self._give_up()
         return res, x[torch.tensor(res.path).to(self.device)]
 
 

@@ -1,0 +1,61 @@
+"""Rounds over trees as a stack runs them."""
+import pytest
+import torch
+
+from slotstream_spark_amd import _lib
+from slotstream_spark_amd.engine.generate import MoEStack, tree_decode
+from slotstream_spark_amd.engine.step import MoEWeights
+from slotstream_spark_amd.memory.kv_pages import KVPages
+from slotstream_spark_amd.memory.synth import attention_layer, head_weights, normal_bf16
+from tests.test_gpu_attention_layer import D, H, K, NL, V, parts  # noqa: F401  (parts is a fixture)
+from tests.test_gpu_tree_stack import PROMPT, stack_of
+from tests.tree_util import E4M3
+
+pytestmark = pytest.mark.gpu
+
+
+def windowed(parts, window, dtype=torch.bfloat16, prompt_chunk=0, max_tokens=320, pages=22):  # noqa: F811
+    pool, lws, lm = parts
+    mw = [MoEWeights(w.router_w, w.sh_gate, w.sh_up, w.sh_down, w.sh_g) for w in lws[:NL]]
+    norms = [normal_bf16((H,), 0.1, 950 + l).float().add(1).to(torch.bfloat16) for l in range(NL + 1)]
+    return MoEStack(pool, mw, lm, head_weights(H, 1, 32, V, seed=921).embed, depth=D, norm_weights=norms, top_k=K,
+                    attn=[attention_layer(H, 16, 4, 64, 960 + l, window=window, sinks=2) for l in range(NL)], attn_norms=norms[:NL],
+                    pages=KVPages(NL, pages, 4, 64, 16, max_tokens=max_tokens, dtype=dtype), prompt_chunk=prompt_chunk)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("size", [40, 48])
+def test_pages_given_back_between_rounds(parts, dtype, size):  # noqa: F811
+    """Trees much larger than the rows they leave, under a window that just holds them: a loop that gives pages back before each round by the
+    stack's own recipe emits what one emits that keeps them, sees no missing page, and holds fewer."""
+    window, n, outs, free = 48, 100, [], []
+    for evict in (False, True):
+        stack, held = windowed(parts, window, dtype), []
+
+        def tree_fn(pending, room, n_out):
+            if evict:
+                stack.cache.pages.evict(stack.cache.seq, window, 2, back=stack.rows)
+            held.append(stack.cache.pages.free_pages)
+            m = min(room, size - 1)
+            return [(pending + 3 * i) % V for i in range(m)], [(i - 1) // 4 if i else 0 for i in range(m)]
+
+        out, nan, _, st = tree_decode(stack, PROMPT, n, tree_fn)
+        assert _lib.device_error() == 0
+        assert len(out) == n and not nan and st["rounds"] > n // 4 and st["drafted"] >= 20 * st["rounds"]
+        assert stack.st.pos == len(PROMPT) + n - 1
+        outs.append(out)
+        free.append(held[-1])
+    assert outs[0] == outs[1] and free[1] > free[0]
+
+
+def test_a_sequence_has_the_tokens_that_rounds_left(parts):  # noqa: F811
+    """After a round, and after tokens were taken back, the pages' own count is the stack's position."""
+    stack = stack_of(parts, torch.bfloat16)
+    pages, seq = stack.cache.pages, stack.cache.seq
+    stack.prompt(PROMPT)
+    res, _ = stack.tree_step([5] + [7] * 40, [-1] + [0] * 40)
+    assert pages.length[seq] == stack.st.pos == len(PROMPT) + len(res.path)
+    assert sum(p >= 0 for p in pages.table[seq].tolist()) == -(-stack.st.pos // pages.page)
+    stack.take_back(3)
+    assert pages.length[seq] == stack.st.pos == len(stack.st.tokens) == len(PROMPT) + len(res.path) - 3
+    assert _lib.device_error() == 0

@@ -184,6 +184,12 @@ class MoEStack:
             residual_rmsnorm(x, y, mixed, stream_out=x, weight=nxt, eps=eps)
         return mixed
 
+    @property
+    def tree_rows(self) -> int:
+        """The most rows that a tree may have: the mask's bits, the prompt layers' rows, and every layer's window."""
+        most = TREE_ROWS if self.prompt_layers is None else min(TREE_ROWS, self.chunk)
+        return min([most] + [a.window for a in (self.graph.attn or []) if a.window > 0])
+
     def take_back(self, n: int) -> None:
         """The sequence's last n tokens are no longer its own (their rows in the cache are written over)."""
         if not 0 <= n <= len(self.st.tokens):
@@ -252,7 +258,6 @@ def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eo
     if not stack.last_finite[-1]:
         return out, True, step_s, st
     emitted, kept = [nxt[-1]], 1
-    most = TREE_ROWS - 1 if stack.prompt_layers is None else min(TREE_ROWS, stack.chunk) - 1
     while True:
         for i, tok in enumerate(emitted):
             out.append(tok)
@@ -265,7 +270,7 @@ def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eo
         if nan or stack.st.pos + 1 > stack.max_ctx:
             return out, nan, step_s, st
         t1 = time.perf_counter()
-        room = min(most, stack.max_ctx - stack.st.pos - 1)
+        room = min(stack.tree_rows - 1, stack.max_ctx - stack.st.pos - 1)
         drafts, parents = tree_fn(out[-1], room, len(out)) if room > 0 else ([], [])
         if len(drafts) > room:
             raise ValueError(f"{len(drafts)} drafts, there is room for {room}")

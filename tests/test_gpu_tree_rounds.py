@@ -59,3 +59,20 @@ def test_a_sequence_has_the_tokens_that_rounds_left(parts):  # noqa: F811
     stack.take_back(3)
     assert pages.length[seq] == stack.st.pos == len(stack.st.tokens) == len(PROMPT) + len(res.path) - 3
     assert _lib.device_error() == 0
+
+
+def test_drafts_up_to_the_room_under_a_window(parts):  # noqa: F811
+    """A tree's rows must fit every layer's window: the room that a drafter is told is one that a round takes."""
+    stack, rooms = windowed(parts, 20), []
+
+    def tree_fn(pending, room, n_out):
+        rooms.append(room)
+        return [pending] * room, [0] * room
+
+    out, nan, _, _ = tree_decode(stack, PROMPT, 12, tree_fn)
+    assert len(out) == 12 and not nan and set(rooms) == {19} and _lib.device_error() == 0
+    with pytest.raises(ValueError, match="window"):
+        stack.tree_step([1] * 21, [-1] + [0] * 20)
+    one, drafted = windowed(parts, 1), []
+    out, _, _, st = tree_decode(one, PROMPT, 5, lambda *a: drafted.append(a) or ([], []))
+    assert len(out) == 5 and st["rounds"] == 4 and not drafted and _lib.device_error() == 0

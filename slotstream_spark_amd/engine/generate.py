@@ -263,7 +263,7 @@ def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eo
             out.append(tok)
             if on_token:
                 on_token(tok)
-            if tok in eos or len(out) == max_tokens:
+            if tok in eos or len(out) >= max_tokens:
                 if st["rounds"]:
                     stack.take_back(kept - (i + 1))
                 return out, nan, step_s, st

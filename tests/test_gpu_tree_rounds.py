@@ -3,11 +3,11 @@ import pytest
 import torch
 
 from slotstream_spark_amd import _lib
-from slotstream_spark_amd.engine.generate import MoEStack, tree_decode
+from slotstream_spark_amd.engine.generate import MoEStack, mtp_decode, tree_decode
 from slotstream_spark_amd.engine.step import MoEWeights
 from slotstream_spark_amd.memory.kv_pages import KVPages
 from slotstream_spark_amd.memory.synth import attention_layer, head_weights, normal_bf16
-from tests.test_gpu_attention_layer import D, H, K, NL, V, parts  # noqa: F401  (parts is a fixture)
+from tests.test_gpu_attention_layer import D, H, K, NL, V, make_head, parts  # noqa: F401  (parts is a fixture)
 from tests.test_gpu_tree_stack import PROMPT, stack_of
 from tests.tree_util import E4M3
 
@@ -76,3 +76,14 @@ def test_drafts_up_to_the_room_under_a_window(parts):  # noqa: F811
     one, drafted = windowed(parts, 1), []
     out, _, _, st = tree_decode(one, PROMPT, 5, lambda *a: drafted.append(a) or ([], []))
     assert len(out) == 5 and st["rounds"] == 4 and not drafted and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [0, -1, 1])
+def test_no_token_asked_for(parts, n):  # noqa: F811
+    """The prompt's own token comes first in either loop, and a loop that is asked for no more ends with it."""
+    stack, head = stack_of(parts, torch.bfloat16), make_head(parts, 1)
+    want, _, _, _ = mtp_decode(stack, head, PROMPT, n)
+    stack.reset()
+    out, nan, _, st = tree_decode(stack, PROMPT, n, lambda p, room, k: ([1], [0]))
+    assert out == want and len(out) == 1 and not nan and st["rounds"] == 0
+    assert stack.st.pos == stack.cache.pos == len(PROMPT)

@@ -250,8 +250,9 @@ def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eo
     """Greedy decode after `prompt` by rounds over trees -> (tokens, nan, round_seconds, stats), as mtp_decode's.
     tree_fn(pending, room, n_out) -> (drafts, parents): up to `room` drafts, each behind row parents[i] (0 the pending token, j + 1 draft
     j). Where none fit, or it gives none, a round is the pending token alone. The drafts decide how many tokens a round emits, not
-    which (but for a router's or the lm_head's choices that another order of sums rounds another way). As after mtp_decode the stack's sequence is the prompt and
-    what was emitted but for the last token."""
+    which (but for a router's or the lm_head's choices that another order of sums rounds another way). As after mtp_decode the stack's
+    sequence is the prompt and what was emitted but for the last token; where a row that is not finite ended the loop (`nan`) that one has
+    been run too, and the sequence ends with it."""
     out, step_s, nan = [], [], False
     st = {"rounds": 0, "drafted": 0, "accepted": 0, "emitted_by_round": [], "verify_rows": 0}
     nxt, _ = stack.prompt(prompt)
@@ -266,7 +267,7 @@ def tree_decode(stack: MoEStack, prompt: list[int], max_tokens: int, tree_fn, eo
             if tok in eos or len(out) >= max_tokens:
                 if st["rounds"]:
                     stack.take_back(kept - (i + 1))
-                return out, nan, step_s, st
+                return out, False, step_s, st   # a row that was not finite came after
         if nan or stack.st.pos + 1 > stack.max_ctx:
             return out, nan, step_s, st
         t1 = time.perf_counter()

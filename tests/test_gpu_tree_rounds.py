@@ -8,7 +8,7 @@ from slotstream_spark_amd.engine.step import MoEWeights
 from slotstream_spark_amd.memory.kv_pages import KVPages
 from slotstream_spark_amd.memory.synth import attention_layer, head_weights, normal_bf16
 from tests.test_gpu_attention_layer import D, H, K, NL, V, make_head, parts  # noqa: F401  (parts is a fixture)
-from tests.test_gpu_tree_stack import PROMPT, stack_of
+from tests.test_gpu_tree_stack import PROMPT, branching, plain, stack_of
 from tests.tree_util import E4M3
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +87,60 @@ def test_no_token_asked_for(parts, n):  # noqa: F811
     out, nan, _, st = tree_decode(stack, PROMPT, n, lambda p, room, k: ([1], [0]))
     assert out == want and len(out) == 1 and not nan and st["rounds"] == 0
     assert stack.st.pos == stack.cache.pos == len(PROMPT)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("prompt_chunk", [0, 32])
+def test_a_row_that_is_not_finite_ends_the_loop(parts, dtype, prompt_chunk):  # noqa: F811
+    """A token whose embedding is NaN, drafted and accepted in the middle of a branch, or pending: its row's choice is not emitted, the loop
+    ends, and the sequence is the prompt and all that was emitted (the last token's row has been run, as at mtp_decode's end)."""
+    stack = stack_of(parts, dtype, prompt_chunk)
+    tree_fn = branching(plain(stack)[0])
+    stack.reset()
+    want, _, _, st = tree_decode(stack, PROMPT, 24, tree_fn)
+    ends, at = [], 1
+    for n in st["emitted_by_round"]:
+        ends.append(at)
+        at += n
+    ran = 0
+    for i in (next(i for i in range(ends[1], 20) if want.index(want[i]) == i and i + 1 not in ends), ends[3] - 1):
+        if want.index(want[i]) != i or want[i] in PROMPT:
+            continue
+        ran += 1
+        bad = stack_of(parts, dtype, prompt_chunk)
+        bad.embed = bad.embed.clone()
+        bad.embed[want[i]] = float("nan")
+        out, nan, _, st = tree_decode(bad, PROMPT, 24, tree_fn)
+        assert nan and out == want[:i + 1], (i, out, want)
+        assert bad.st.tokens == PROMPT + out and bad.st.pos == bad.cache.pos == bad.cache.pages.length[bad.cache.seq] == len(bad.st.tokens)
+        assert _lib.device_error() == 0
+        bad.reset()
+        res, rows = (bad.prompt(PROMPT), bad.tree_step([want[i], 3, 4], [-1, 0, 0]))[1]
+        assert (res.n_accept, res.n_emit, res.flags, res.path) == (0, 0, 1, [0]) and torch.isnan(rows[0]).any()
+    assert ran
+
+
+def test_an_end_before_a_row_that_is_not_finite(parts):  # noqa: F811
+    """A round whose branch ends at a row that is not finite, behind a token that ends the sequence or is the last one asked for: the loop ends
+    with that token, and nothing that it emits came after such a row."""
+    stack = stack_of(parts, torch.bfloat16)
+    tree_fn = branching(plain(stack)[0])
+    stack.reset()
+    want, _, _, st = tree_decode(stack, PROMPT, 24, tree_fn)
+    at, found = 1, None
+    for n in st["emitted_by_round"]:                         # a round of three tokens or more, the third of them a new one
+        if found is None and n >= 3 and want.index(want[at + 1]) == at + 1 and want[at + 1] not in PROMPT:
+            found = at
+        at += n
+    assert found is not None
+    bad = stack_of(parts, torch.bfloat16)
+    bad.embed = bad.embed.clone()
+    bad.embed[want[found + 1]] = float("nan")
+    out, nan, _, _ = tree_decode(bad, PROMPT, 24, tree_fn)
+    assert nan and out == want[:found + 2]
+    for kw in (dict(max_tokens=found + 2), dict(max_tokens=found + 1), dict(max_tokens=24, eos=(want[found + 1],))):
+        bad.reset()
+        out, nan, _, _ = tree_decode(bad, PROMPT, tree_fn=tree_fn, **kw)
+        assert out == want[:min(kw["max_tokens"], found + 2)] and not nan
+        assert bad.st.tokens == PROMPT + out[:-1] and bad.st.pos == bad.cache.pos == bad.cache.pages.length[bad.cache.seq] == len(PROMPT) + len(out) - 1
+    assert _lib.device_error() == 0

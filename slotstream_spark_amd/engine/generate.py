@@ -203,7 +203,8 @@ class MoEStack:
     def _give_up(self) -> None:
         """The pages' count of the sequence's tokens becomes the position: evict() goes by it, and a tree is up to 64 rows, not `rows`."""
         if self.cache is not None:
-            self.cache.pages.truncate(self.cache.seq, self.st.pos)
+            pages, seq = self.cache.pages, self.cache.seq
+            pages.truncate(seq, min(self.st.pos, pages.length[seq]))
 
     def tree_step(self, tokens: list[int], parents: list[int]) -> tuple[TreeResult, torch.Tensor]:
         """A greedy round over a tree: tokens[0] is the pending token, tokens[i] a draft behind row parents[i] < i (parents[0] is not
@@ -223,6 +224,13 @@ class MoEStack:
             raise ValueError(f"a layer's window must hold the tree's {n} rows")
         if self._tree_head is None:
             self._tree_head = LMHeadArgmax(self.lm_head, max_rows=TREE_ROWS, round_bf16=True, device=self.device)
+        try:
+            return self._tree_round(tokens, parents)
+        finally:
+            self._give_up()
+
+    def _tree_round(self, tokens: list[int], parents: list[int]) -> tuple[TreeResult, torch.Tensor]:
+        n = len(tokens)
         rows = torch.tensor([[int(t) for t in tokens], [-1] + [int(p) for p in parents[1:]]], dtype=torch.int32).to(self.device)
         x = gather_rows(self.embed, rows[0])
         if self.cache is not None:
@@ -242,7 +250,6 @@ class MoEStack:
             keep_rows(pages.k, pages.v, cu, kv_len, table, took, scales=pages.scales)
         res = TreeResult.from_out(took[0].tolist())
         self._advance([int(tokens[p]) for p in res.path])
-        self._give_up()
         return res, x[torch.tensor(res.path).to(self.device)]
 
 

@@ -1,4 +1,5 @@
-"""Rounds over trees as a stack runs them."""
+"""Rounds over trees as a stack runs them: windows whose pages are given back between the rounds, rows that are not finite, the loop's ends,
+and every kept row against one-token steps."""
 import pytest
 import torch
 
@@ -7,7 +8,7 @@ from slotstream_spark_amd.engine.generate import MoEStack, mtp_decode, tree_deco
 from slotstream_spark_amd.engine.step import MoEWeights
 from slotstream_spark_amd.memory.kv_pages import KVPages
 from slotstream_spark_amd.memory.synth import attention_layer, head_weights, normal_bf16
-from tests.test_gpu_attention_layer import D, H, K, NL, V, make_head, parts  # noqa: F401  (parts is a fixture)
+from tests.test_gpu_attention_layer import D, E, H, K, NL, V, make_head, parts  # noqa: F401  (parts is a fixture)
 from tests.test_gpu_tree_stack import PROMPT, branching, plain, stack_of
 from tests.tree_util import E4M3
 
@@ -154,3 +155,89 @@ def test_an_end_before_a_row_that_is_not_finite(parts):  # noqa: F811
         assert out == want[:min(kw["max_tokens"], found + 2)] and not nan
         assert bad.st.tokens == PROMPT + out[:-1] and bad.st.pos == bad.cache.pos == bad.cache.pages.length[bad.cache.seq] == len(PROMPT) + len(out) - 1
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("routed", ["freely", "alike"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("prompt_chunk", [0, 32])
+def test_kept_rows_of_every_round(parts, dtype, prompt_chunk, routed):  # noqa: F811
+    """Every kept row of every round, deep ones and those behind moved branches among them, against a one-token step of a stack that is fed
+    what the rounds kept.
+
+    A row's stream is off by bf16's half step (2^-8) for each of a layer's two residual sums and what they carry on: 2^-6 of it after two
+    layers. Over e4m3 a key or value that is 2^-8 of itself off falls on the next code in one of 2^5 (a step is 2^-3 at most), 2^-5.5 in
+    the mean square of what the attention adds: 2^-5 in all. A choice (of the lm_head, of a router) that differs was that near: four times
+    that of the logits' spread. Routed alike nothing else may differ, so every kept row is compared, whatever was chosen. Routed freely, a
+    row whose experts differ ends its round; the plain stack's cache is then made the rounds' own before the next."""
+    bias = None
+    if routed == "alike":
+        bias = torch.zeros(E, device="cuda")
+        bias[5:5 + K] = 1000.0
+    far = 2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -5
+    ref, stack = stack_of(parts, dtype, prompt_chunk, bias=bias), stack_of(parts, dtype, prompt_chunk, bias=bias)
+    n = 40
+    own, _, _, _ = tree_decode(stack, PROMPT, n + 5, lambda p, room, k: ([], []))
+    tree_fn, seen = branching(own), []
+    stack.reset()
+
+    class Watched:
+        def __init__(self, layer):
+            self.layer = layer
+
+        def __call__(self, x, **kw):
+            got = self.layer(x, **kw)
+            seen.append(got[1].clone())
+            return got
+
+    def same_cache():
+        a, b = ref.cache, stack.cache
+        for w in range(-(-stack.st.pos // a.pages.page)):
+            x, y = int(a.table[0, w]), int(b.table[0, w])
+            for s, t in ((a.pages.k, b.pages.k), (a.pages.v, b.pages.v)) + (((a.pages.scales, b.pages.scales),) if dtype == E4M3 else ()):
+                s.view(torch.uint8)[:, x] = t.view(torch.uint8)[:, y]
+
+    assert stack.prompt(PROMPT)[0][-1] == ref.prompt(PROMPT)[0][-1] == own[0]
+    out, kept_rows, compared, deep, after, moved, apart = own[:1], 0, 0, 0, 0, False, False
+    watched = "layers" if prompt_chunk == 0 else "prompt_layers"
+    holder = stack.graph if prompt_chunk == 0 else stack
+    layers = getattr(holder, watched)
+    while len(out) < n:
+        if apart:
+            same_cache()
+            apart = False
+        drafts, par = tree_fn(out[-1], 63, len(out))
+        seen.clear()
+        setattr(holder, watched, [Watched(x) for x in layers])
+        res, rows = stack.tree_step([out[-1], *drafts], [-1, *par])
+        setattr(holder, watched, layers)
+        per = len(seen) // NL
+        ids = [torch.cat(seen[l * per:(l + 1) * per]) for l in range(NL)]
+        kept = [([out[-1]] + drafts)[r] for r in res.path]
+        assert res.flags == 0 and kept[1:] == res.tokens[:-1] and res.n_emit == len(kept)
+        kept_rows += len(kept)
+        for j, tok in enumerate(kept):
+            nxt, multi = ref.forward([tok])
+            for l in range(0 if apart else NL):
+                if set(ids[l][res.path[j]].tolist()) != set(ref.graph.ids[l, 0].tolist()):
+                    assert routed == "freely"
+                    x = (ref.graph.mixed[l][0].float() @ parts[1][l].router_w.float().t()).sort(descending=True)[0]
+                    assert x[K - 1] - x[K] <= 4 * far * x.std(), (len(out), j, l)
+                    apart = True
+                    break
+            if apart:
+                continue
+            assert (rows[j].float() - multi[0].float()).norm() <= far * multi[0].float().norm(), (len(out), j)
+            compared += 1
+            deep += j >= 2
+            after += moved
+            if res.tokens[j] != nxt[0]:
+                x = ref.plain_logits[0]
+                assert x[nxt[0]] - x[res.tokens[j]] <= 4 * far * x.std(), (len(out), j)
+        moved |= res.path != list(range(len(res.path)))
+        out += res.tokens
+    assert ref.st.tokens == stack.st.tokens and _lib.device_error() == 0
+    print(f"[rounds] {routed} kept={kept_rows} compared={compared} deep={deep} after={after}", flush=True)
+    if routed == "alike":
+        assert compared == kept_rows and deep >= 8 and after >= 20
+    else:
+        assert compared >= 12 and deep >= 2 and after >= 8

@@ -29,8 +29,8 @@
 //
 // Bound by the matrix units and what runs beside them: a tile of 64 tokens and 128 dimensions is 32 products (1,024 cycles of a
 // SIMD) beside some 290 other instructions, 32 exponentials among them. 8,191 rows of 32 heads under a window of 4,096 (551
-// GFLOP) take 560-620 us, 0.89 to 0.98 PFLOP/s; an 8,192^3 bf16 product of the library reaches 1.23 on this card.
-// Of e4m3 4,095 rows after 4,905 tokens (466 GFLOP) take 482 to 531 us, 0.88 to 0.97 PFLOP/s, the matrix units busy 48 % of the cycles: a tile
+// GFLOP) take 560-620 us, 0.89 to 0.98 PFLOP/s; an 8,192^3 bf16 product a b^T of the library reaches 1.61 on this card, a b 1.38.
+// Of e4m3 4,095 rows after 4,905 tokens (466 GFLOP) take 477 to 531 us, 0.88 to 0.98 PFLOP/s, the matrix units busy 48 % of the cycles: a tile
 // has 32 conversions and 32 products of weights more. Trees: 16 of up to 26 rows, 32 heads on 4, up to 8,000 tokens (169 MB, 24 GFLOP, 38
 // with the columns that no row has) 53 us; 4 of 64 rows over 50,000 tokens of e4m3 and 8 key heads (417 MB, 209 GFLOP) 249 us, 45 % busy.
 #pragma once
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a) {
           float q0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], a.scale, -mu));
           float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e + 1], a.scale, -mu));
           part[q / 2 % 2] += q0;
-          part[q / 2 % 2] += q1;  // the sum has the weights as they are, the product rounded once to the element type
+          part[q / 2 % 2] += q1;  // the sum has the weights as they are, the product rounded once to the element type that the matrix unit takes
           if constexpr (E8) {
             asm volatile("" : "+v"(part[q / 2 % 2]));  // summed here: put off, the additions keep every weight in a register
             if (e % 4 == 0) by = *reinterpret_cast<const ss_f32x4*>(vb + 32 * n + 16 * (e / 8) + 8 * h + e % 8);

@@ -27,7 +27,8 @@ namespace {
 
 // ---------------------------------------------------------------- rows as e4m3 numbers
 // A vector x of a token and head is kept as e4m3 numbers of x 2^-e, rounded once from fp32, and the byte e + 127: e the least exponent
-// with max |x| <= 448 2^e, from -126 on, of a key turned in 64 bits. What is not finite is left out of the maximum and kept as NaN.
+// with max |x| <= 448 2^e, from -126 on, of a key turned in 64 bits. The numbers are of keys turned in fp32: off by 2^-20 of the largest,
+// beside a code's half step of 2^-4. What is not finite is left out of the maximum and kept as NaN.
 SS_DEV float finite_abs(float x) {
   const float y = fabsf(x);
   return y < __builtin_inff() ? y : 0.f;

@@ -258,7 +258,9 @@ int check_apart(std::initializer_list<Span> written, std::initializer_list<Span>
 // tokens off a workgroup (256 of 256 dimensions) it is not worth the join: a call on a table of 256 / 512 / 768 tokens, whole
 // against split, takes 6.0 / 7.7 / 9.5 against 7.8 / 7.9 / 8.7 us (one row of 32 heads on 4, 128 dimensions, in a graph; the
 // host saves 3 us besides), 7.6 / 10.2 / 12.8 against 8.8 / 9.0 / 9.7 (16 on 2, 256 dimensions), 16 sequences of 768 / 1,024
-// tokens 11.7 / 14.1 against 14.5 / 17.2. It goes by seqs, kv_heads, dim and the table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call. With 256 /
+// tokens 11.7 / 14.1 against 14.5 / 17.2. In causal calls of up to kFewRows rows, over either kind of page, it goes by seqs, kv_heads, dim, the window and
+// the table's width alone, so a row's chunks, and with them its bits, do not depend on the other rows of a call. (Trees and longer calls over
+// e4m3 have no such promise: there the chunk also goes by the packed rows, see few_chunk.) With 256 /
 // 512 / 1024 / 2048 workgroups, kernel and join in us: one sequence of 131,072 tokens 50 / 49 / 49 / 52; eight of 6,145
 // with three rows at 256 dimensions 25 / 30 / 37 / 37; 32 with four rows under a window of 1,024 21 / 25 / 20 / 21.
 // Many rows: the tokens are split only where the row tiles alone would leave CUs without work (two workgroups fit a CU): three

@@ -126,7 +126,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     scales: torch.Tensor | None = None, tree: torch.Tensor | None = None) -> torch.Tensor:
     """q [rows, heads, dim] -> [rows, heads, dim] of q's type. `max_rows` bounds the rows of one sequence. window 0: every
     token up to the row's own; else the last `window` of them and the first `sinks`. scale: 1 / sqrt(dim) unless given. One kernel
-    for the call, chosen by max_rows (up to 8 or more): single tokens in a batch with a prompt go through the prompt's, without
+    for the call: that of few rows up to a max_rows of 8 (over e4m3 pages and for trees also where max_rows times the heads of a key head is
+    small or the table short), else that of many: single tokens in a batch with a prompt go through the prompt's, without
     the split over their length and the bits of a call of few rows. Two calls over one q and `out`, with cu_rows[:m + 1] and
     cu_rows[m:], serve them apart (rows outside a call's cu_rows are left alone).
     `lse` fp32 [rows, heads] receives ln sum_j exp(scale q_i . k_j). A row that sees nothing is 0, its lse -inf; rows past

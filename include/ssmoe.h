@@ -568,7 +568,7 @@ int ssmoe_rope_append(const ssmoe_rope_append_args* a, void* stream);
  * apart from each other and from all that the call reads. Scores, maxima, sums and
  * partial results are fp32; a probability is rounded to the element type before its product with the values. What the
  * cache holds at tokens that a row does not see does not reach it, infinities and NaN included. Probabilities are up to 2^8 before they are
- * divided by their sum: bf16 values of 2^119 and more may come out infinite.
+ * divided by their sum: bf16 values of 2^119 and more may come out infinite or NaN.
  * Calls with max_rows <= 8 (decoding, verification): the bits of a row depend on its sequence's tokens, seqs, kv_heads and
  * the width of the table, not on the other rows of the call. With more, all of the call's sequences take the many-row form, single
  * tokens among them: split over their length only as far as the row tiles of all sequences at max_rows leave CUs without work.

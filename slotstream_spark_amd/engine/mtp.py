@@ -35,6 +35,7 @@ from ..kernels.head_ops import (EPI_ADD, EPI_INJECT, EPI_SIGMOID, EPI_SILU_DIV, 
                                 head_gemv, lin_epi, rmsnorm)
 from ..memory.kv_pages import KVPages
 from .attention import AttentionLayer, SeqCache
+from .step import capturing
 from .verify import MoEVerifyLayer
 
 MAP_ROW = 48   # the head's layer index in the 49-row expert map (engine/mtp.py:38)
@@ -430,7 +431,7 @@ class DraftGraph:
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with capturing(g):
             self._body()
         self.graph = g
         self._resizes = self.head.cache.pages.resizes if self.head.attn is not None else 0

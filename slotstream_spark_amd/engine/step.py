@@ -20,6 +20,8 @@ are outside the path, so the caller supplies the drafts of the next round, as `d
 """
 from __future__ import annotations
 
+import contextlib
+import gc
 from dataclasses import dataclass
 
 import torch
@@ -61,6 +63,20 @@ def residual_rmsnorm(resid: torch.Tensor, y: torch.Tensor | None, mixed: torch.T
     _lib.check(_lib.lib().ssmoe_residual_rmsnorm(
         resid.data_ptr(), _lib.ptr(y), _lib.ptr(weight), float(eps), resid.shape[0], resid.shape[1],
         _lib.ptr(stream_out), mixed.data_ptr(), torch.cuda.current_stream(resid.device).cuda_stream))
+
+
+@contextlib.contextmanager
+def capturing(graph: torch.cuda.CUDAGraph, **kw):
+    """torch.cuda.graph with Python's cyclic collector off. Garbage that holds another graph (a stack that something it holds refers to) must
+    not be freed here: the end of a graph waits for the device, a capture forbids that, and the failure ends the process."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, **kw):
+            yield
+    finally:
+        if on:
+            gc.enable()
 
 
 class MTPStepGraph:
@@ -214,7 +230,7 @@ class MTPStepGraph:
             self._body()                           # first launches outside the capture (module loads, workspaces)
         self.stream.synchronize()
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph, stream=self.stream):
+        with capturing(self.graph, stream=self.stream):
             self._body()
         self._resizes = self.cache.pages.resizes if self.cache is not None else 0
 

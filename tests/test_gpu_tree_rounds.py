@@ -57,8 +57,6 @@ def test_a_sequence_has_the_tokens_that_rounds_left(parts):  # noqa: F811
     res, _ = stack.tree_step([5] + [7] * 40, [-1] + [0] * 40)
     assert pages.length[seq] == stack.st.pos == len(PROMPT) + len(res.path)
     assert sum(p >= 0 for p in pages.table[seq].tolist()) == -(-stack.st.pos // pages.page)
-    through = stack._through
-
     def fails(*a, **kw):
         raise RuntimeError("no pass")
 
@@ -66,7 +64,7 @@ def test_a_sequence_has_the_tokens_that_rounds_left(parts):  # noqa: F811
     with pytest.raises(RuntimeError, match="no pass"):
         stack.tree_step([5] + [7] * 40, [-1] + [0] * 40)
     assert pages.length[seq] == stack.st.pos == len(stack.st.tokens) == len(PROMPT) + len(res.path)
-    stack._through = through
+    del stack._through                                      # the class's own again (put back by value it would hold the stack itself)
     stack.take_back(3)
     assert pages.length[seq] == stack.st.pos == len(stack.st.tokens) == len(PROMPT) + len(res.path) - 3
     assert _lib.device_error() == 0
